@@ -22,7 +22,7 @@ LIB = os.path.join(HERE, "libb200moe.so")
 EXT = os.path.join(HERE, "cinfer_ascendc" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 CU_SOURCES = ["host_util.cu", "fp4_dequant.cu", "grouped_gemv.cu", "grouped_gemm.cu", "grouped_gemm_packed.cu", "moe_aux.cu",
-              "ep_exchange.cu"]
+              "ep_exchange.cu", "fp8_quantize.cu", "grouped_gemm_fp8_block.cu", "moe_balance.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC"]
 

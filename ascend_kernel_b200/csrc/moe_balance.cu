@@ -1,0 +1,428 @@
+// Balance loss of the MoE router, the pairs per expert, and the loss's gradient.
+//
+// The tokens form sequences (a list of cumulative ends; without one, a single sequence).  For sequence s with T_s tokens that the
+// mask leaves, p_t the softmax of a token's logits and c_se the number of its (token, j) pairs on expert e:
+//
+//   loss_s = E / (k T_s) sum_e c_se (1 / T_s sum_t p_te)                     (1 where the load is even)
+//   d loss_s / d logit_te = p_te / T_s (F_se - sum_j F_sj p_tj),   F_se = E c_se / (k T_s) - 1
+//
+// (the 1 cancels in the difference; taking it out first keeps the digits that an almost even load leaves).  The counts are piecewise
+// constant and have no gradient.
+//
+// Forward: a CTA takes a range of tokens, a warp a token at a time, its lanes adding the probabilities of their experts up in
+// registers; what a CTA has of a sequence goes to row (range + sequence) of the scratch (going on by a range or by a sequence
+// raises that sum by one, so no two pieces share a row), and a second kernel adds a sequence's rows in their order: no
+// floating-point atomics, the same bits each time.  Backward: a warp per token, the softmax again from the logits.  Both read the
+// logits once and are bound by that.
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace b200moe {
+namespace mb {
+
+constexpr int kWarps = 16, kThreads = kWarps * 32;
+constexpr int kMaxTopK = 32;
+
+template <class T>
+struct Logit;
+template <>
+struct Logit<__nv_bfloat16> {
+    static constexpr int kVec = 8;
+    template <int VEC>
+    static __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&v)[VEC]) {
+        if constexpr (VEC == 8) {
+            const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[2 * i] = __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+            }
+        } else {
+            v[0] = __bfloat162float(*p);
+        }
+    }
+    template <int VEC>
+    static __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&v)[VEC]) {
+        if constexpr (VEC == 8)
+            *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                                                      pack_bf16x2(v[6], v[7]));
+        else
+            *p = __float2bfloat16_rn(v[0]);
+    }
+};
+template <>
+struct Logit<float> {
+    static constexpr int kVec = 4;
+    template <int VEC>
+    static __device__ __forceinline__ void load(const float* p, float (&v)[VEC]) {
+        if constexpr (VEC == 4) {
+            const float4 q = __ldg(reinterpret_cast<const float4*>(p));
+            v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+        } else {
+            v[0] = __ldg(p);
+        }
+    }
+    template <int VEC>
+    static __device__ __forceinline__ void store(float* p, const float (&v)[VEC]) {
+        if constexpr (VEC == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        else *p = v[0];
+    }
+};
+
+struct Args {
+    const void* logits;
+    const int32_t* idx;
+    const int64_t* seq_list;  // cumulative ends, or NULL: one sequence of all tokens
+    const uint8_t* mask;      // NULL: every token counts
+    int T, E, k, S, chunk;    // chunk: tokens a CTA takes
+    int pitch;                // floats of a scratch row: E rounded up to 4
+    float* psum;              // [rows][pitch]
+    int32_t* csum;            // [rows][pitch]
+    int32_t* nsum;            // [rows]
+};
+
+// [a, b) of sequence s, inside the tokens whatever the list holds
+__device__ __forceinline__ int seq_end(const Args& a, int s) {
+    if (a.seq_list == nullptr) return a.T;
+    const long long v = __ldg(a.seq_list + s);
+    return (int)(v < 0 ? 0 : (v > a.T ? a.T : v));
+}
+__device__ __forceinline__ int seq_start(const Args& a, int s) { return s == 0 ? 0 : seq_end(a, s - 1); }
+// the first sequence that ends behind token t (a.S if none does)
+__device__ __forceinline__ int seq_of(const Args& a, int t) {
+    if (a.seq_list == nullptr) return 0;
+    int lo = 0, hi = a.S;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (seq_end(a, mid) > t) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// A token's probabilities: lane l holds experts (c * 32 + l) * VEC + j.  A row of nothing but -infinity has none (all 0), a NaN or
+// +infinity makes the row NaN.
+template <class T, int VEC, int CHUNKS>
+__device__ __forceinline__ void softmax_row(const T* row, int E, float (&p)[CHUNKS][VEC]) {
+    const int lane = threadIdx.x & 31;
+    float m = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+        const int e = (c * 32 + lane) * VEC;
+        if (e < E) {
+            Logit<T>::template load<VEC>(row + e, p[c]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) p[c][j] = -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) m = fmaxf(m, p[c][j]);
+    }
+    m = warp_max(m);
+    float sum = 0.f;
+    // (a difference first: logits of the type's lowest value times log2(e) would overflow)
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            p[c][j] = exp2f((p[c][j] - base) * 1.44269504f);
+            sum += p[c][j];
+        }
+    sum = warp_sum(sum);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) p[c][j] *= inv;
+}
+
+template <class T, int VEC, int CHUNKS>
+__global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
+    extern __shared__ float smem[];  // [kWarps][pitch] probabilities, [pitch] counts, 1 number of tokens
+    int* hist = reinterpret_cast<int*>(smem + kWarps * a.pitch);
+    int* n_tokens = hist + a.pitch;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int t0 = blockIdx.x * a.chunk, t1 = min(t0 + a.chunk, a.T);
+    const T* logits = static_cast<const T*>(a.logits);
+    for (int s = seq_of(a, t0); s < a.S; ++s) {
+        const int start = seq_start(a, s);
+        if (start >= t1) break;
+        const int lo = max(start, t0), hi = min(seq_end(a, s), t1);
+        if (lo >= hi) continue;
+        for (int e = threadIdx.x; e <= a.pitch; e += kThreads) hist[e] = 0;  // (and the number of tokens behind them)
+        __syncthreads();
+        float acc[CHUNKS][VEC] = {};
+        int n = 0;
+        for (int t = lo + warp; t < hi; t += kWarps) {
+            if (a.mask != nullptr && __ldg(a.mask + t) == 0) continue;
+            ++n;
+            if (lane < a.k) {
+                const int e = __ldg(a.idx + (size_t)t * a.k + lane);
+                if ((unsigned)e < (unsigned)a.E) atomicAdd(&hist[e], 1);
+            }
+            float p[CHUNKS][VEC];
+            softmax_row<T, VEC, CHUNKS>(logits + (size_t)t * a.E, a.E, p);
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) acc[c][j] += p[c][j];
+        }
+        if (lane == 0 && n) atomicAdd(n_tokens, n);
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const int e = (c * 32 + lane) * VEC + j;
+                if (e < a.pitch) smem[warp * a.pitch + e] = acc[c][j];
+            }
+        __syncthreads();
+        const size_t row = (size_t)blockIdx.x + s;
+        for (int e = threadIdx.x; e < a.pitch; e += kThreads) {
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) sum += smem[w * a.pitch + e];
+            a.psum[row * a.pitch + e] = sum;
+            a.csum[row * a.pitch + e] = hist[e];
+        }
+        if (threadIdx.x == 0) a.nsum[row] = *n_tokens;
+        __syncthreads();
+    }
+    grid_dep_launch();
+}
+
+// A CTA per sequence: its rows of the scratch in their order.  A warp takes 128 experts of every n-th row; what the warps have is
+// added in their order.
+constexpr int kJoinThreads = 1024;
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a, float* __restrict__ loss, long long* __restrict__ counts,
+                                                            float* __restrict__ load, float* __restrict__ inv_n, int* findings) {
+    __shared__ alignas(16) float s_p[32 * 128];
+    __shared__ alignas(16) int s_c[32 * 128];
+    __shared__ float s_loss[32];
+    __shared__ int s_n;
+    const int s = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int start = seq_start(a, s), end = seq_end(a, s);
+    if (threadIdx.x == 0) {
+        s_n = 0;
+        const long long given = a.seq_list ? a.seq_list[s] : a.T;
+        if (findings != nullptr && (given != end || end < start)) {  // (kept until the caller clears them)
+            if (atomicCAS(findings, 0, kDevBadGroupList) == 0) findings[1] = s;
+        }
+    }
+    __syncthreads();
+    const int groups = (a.pitch + 127) / 128, rows_at_once = 32 / groups;  // pitch <= 1024
+    const int e = (warp % groups) * 128 + lane * 4, r0 = warp / groups;
+    float4 p = make_float4(0.f, 0.f, 0.f, 0.f);
+    int4 c = make_int4(0, 0, 0, 0);
+    int n = 0;
+    grid_dep_wait();
+    if (end > start && r0 < rows_at_once) {
+        const int last = (end - 1) / a.chunk;
+#pragma unroll 4
+        for (int r = start / a.chunk + r0; r <= last; r += rows_at_once) {
+            const size_t row = (size_t)r + s;
+            if (e < a.pitch) {
+                const float4 q = __ldcg(reinterpret_cast<const float4*>(a.psum + row * a.pitch + e));
+                const int4 d = __ldcg(reinterpret_cast<const int4*>(a.csum + row * a.pitch + e));
+                p.x += q.x; p.y += q.y; p.z += q.z; p.w += q.w;
+                c.x += d.x; c.y += d.y; c.z += d.z; c.w += d.w;
+            }
+            if (e == 0) n += __ldcg(a.nsum + row);
+        }
+    }
+    if (e == 0 && n) atomicAdd(&s_n, n);
+    reinterpret_cast<float4*>(s_p)[warp * 32 + lane] = p;
+    reinterpret_cast<int4*>(s_c)[warp * 32 + lane] = c;
+    __syncthreads();
+    const double tokens = s_n, pairs = tokens * a.k;
+    double part = 0.;
+    if ((int)threadIdx.x < a.E) {
+        const int at = (threadIdx.x >> 7) * 128 + (threadIdx.x & 127);
+        double sum = 0.;
+        long long count = 0;
+        for (int r = 0; r < rows_at_once; ++r) {
+            sum += s_p[r * groups * 128 + at];
+            count += s_c[r * groups * 128 + at];
+        }
+        const size_t o = (size_t)s * a.E + threadIdx.x;
+        counts[o] = count;
+        load[o] = s_n ? (float)((count * (double)a.E - pairs) / pairs) : 0.f;
+        if (s_n) part = (double)count * sum;
+    }
+    // (sums of positive terms: fp32 from here on)
+    float v = warp_sum(s_n ? (float)(part / (pairs * tokens) * a.E) : 0.f);
+    if (lane == 0) s_loss[warp] = v;
+    __syncthreads();
+    if (warp == 0) {
+        v = warp_sum(s_loss[lane]);
+        if (lane == 0) {
+            loss[s] = v;
+            inv_n[s] = s_n ? 1.f / (float)s_n : 0.f;
+        }
+    }
+}
+
+template <class T, int VEC, int CHUNKS>
+__global__ void __launch_bounds__(256) backward_kernel(const Args a, const float* __restrict__ load, const float* __restrict__ inv_n,
+                                                       const float* __restrict__ grad, T* __restrict__ out) {
+    const int lane = threadIdx.x & 31, t = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (t >= a.T) return;
+    const int s = seq_of(a, t);
+    T* dst = out + (size_t)t * a.E;
+    float p[CHUNKS][VEC];
+    // a token of no sequence, or one that the mask takes out, has no part in any loss (what its logits hold is not read)
+    if (s >= a.S || t < seq_start(a, s) || (a.mask != nullptr && __ldg(a.mask + t) == 0)) {
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            const int e = (c * 32 + lane) * VEC;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) p[c][j] = 0.f;
+            if (e < a.E) Logit<T>::template store<VEC>(dst + e, p[c]);
+        }
+        return;
+    }
+    const float g = __ldg(grad + s) * __ldg(inv_n + s);
+    softmax_row<T, VEC, CHUNKS>(static_cast<const T*>(a.logits) + (size_t)t * a.E, a.E, p);
+    const float* f = load + (size_t)s * a.E;
+    float fv[CHUNKS][VEC], mean = 0.f;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+        const int e = (c * 32 + lane) * VEC;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            fv[c][j] = e < a.E ? __ldg(f + e + j) : 0.f;  // (VEC divides E)
+            mean = fmaf(fv[c][j], p[c][j], mean);
+        }
+    }
+    mean = warp_sum(mean);
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+        const int e = (c * 32 + lane) * VEC;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) p[c][j] *= g * (fv[c][j] - mean);
+        if (e < a.E) Logit<T>::template store<VEC>(dst + e, p[c]);
+    }
+}
+
+// Tokens a CTA of the forward pass takes: about two CTAs a multiprocessor, a token a warp at least.
+static int chunk_of(int64_t T) {
+    const int64_t ctas = 2LL * 148;  // (not the device's own number: the scratch size is a function of the sizes alone)
+    int64_t c = (T + ctas - 1) / ctas;
+    return (int)(c < kWarps ? kWarps : c);
+}
+static int64_t scratch_rows(int64_t T, int64_t S) { return (T + chunk_of(T) - 1) / chunk_of(T) + S; }
+static int pitch_of(int64_t E) { return (int)((E + 3) & ~3LL); }
+
+static bool sizes_ok(int64_t T, int64_t E, int64_t k, int64_t S) {
+    return T >= 0 && E > 0 && E <= 1024 && k > 0 && k <= kMaxTopK && k <= E && S > 0 && S <= 65535 && T * k <= 0x3FFFFFFFLL;
+}
+
+// Calls fn<VEC, CHUNKS> with the widest loads that E and the pointers allow and as many of them as E needs.
+template <class T, class F>
+static void pick(int E, bool aligned, F&& fn) {
+    constexpr int V = Logit<T>::kVec;
+    if (aligned && E % V == 0) {
+        const int c = (E + 32 * V - 1) / (32 * V);
+        if (c <= 1) fn(std::integral_constant<int, V>(), std::integral_constant<int, 1>());
+        else if (c <= 2) fn(std::integral_constant<int, V>(), std::integral_constant<int, 2>());
+        else if (c <= 4) fn(std::integral_constant<int, V>(), std::integral_constant<int, 4>());
+        else fn(std::integral_constant<int, V>(), std::integral_constant<int, 8>());
+    } else {
+        const int c = (E + 31) / 32;
+        if (c <= 4) fn(std::integral_constant<int, 1>(), std::integral_constant<int, 4>());
+        else if (c <= 16) fn(std::integral_constant<int, 1>(), std::integral_constant<int, 16>());
+        else fn(std::integral_constant<int, 1>(), std::integral_constant<int, 32>());
+    }
+}
+
+}  // namespace mb
+}  // namespace b200moe
+
+using namespace b200moe;
+
+extern "C" size_t b200moe_moe_balance_scratch_bytes(int64_t n_tokens, int64_t n_experts, int64_t n_seqs) {
+    if (!mb::sizes_ok(n_tokens, n_experts, 1, n_seqs)) return 0;
+    return (size_t)mb::scratch_rows(n_tokens, n_seqs) * (8u * (size_t)mb::pitch_of(n_experts) + 4u);
+}
+
+extern "C" int b200moe_moe_balance_loss(const void* logits, int logits_fp32, const int32_t* idx, const int64_t* seq_list,
+                                        const uint8_t* token_mask, int64_t n_tokens, int64_t n_experts, int64_t top_k, int64_t n_seqs,
+                                        float* loss, int64_t* counts, float* load, float* inv_tokens, void* scratch,
+                                        size_t scratch_bytes, int32_t* findings, void* stream) {
+    if (!mb::sizes_ok(n_tokens, n_experts, top_k, n_seqs) || (!seq_list && n_seqs != 1)) return B200MOE_ERR_SHAPE;
+    if (logits_fp32 != 0 && logits_fp32 != 1) return B200MOE_ERR_ARGUMENT;
+    if ((n_tokens > 0 && (!logits || !idx)) || !loss || !counts || !load || !inv_tokens) return B200MOE_ERR_NULL_POINTER;
+    if (!scratch || scratch_bytes < b200moe_moe_balance_scratch_bytes(n_tokens, n_experts, n_seqs)) return B200MOE_ERR_WORKSPACE;
+    if (!aligned16(scratch)) return B200MOE_ERR_ALIGNMENT;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    mb::Args a;
+    a.logits = logits;
+    a.idx = idx;
+    a.seq_list = seq_list;
+    a.mask = token_mask;
+    a.T = (int)n_tokens; a.E = (int)n_experts; a.k = (int)top_k; a.S = (int)n_seqs;
+    a.chunk = mb::chunk_of(n_tokens);
+    a.pitch = mb::pitch_of(n_experts);
+    const size_t cells = (size_t)mb::scratch_rows(n_tokens, n_seqs) * a.pitch;
+    a.psum = static_cast<float*>(scratch);
+    a.csum = reinterpret_cast<int32_t*>(a.psum + cells);
+    a.nsum = a.csum + cells;
+    if (a.T > 0) {
+        const unsigned grid = (unsigned)((a.T + a.chunk - 1) / a.chunk);
+        const size_t smem = (size_t)(mb::kWarps + 1) * a.pitch * 4 + 4;
+        cudaError_t err = cudaSuccess;
+        const auto run = [&](auto vec, auto chunks, auto zero) {
+            auto* k = mb::forward_kernel<decltype(zero), decltype(vec)::value, decltype(chunks)::value>;
+            if (smem > 48 * 1024) err = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
+            if (err == cudaSuccess) {
+                k<<<grid, mb::kThreads, smem, st>>>(a);
+                err = cudaGetLastError();
+            }
+        };
+        if (logits_fp32) mb::pick<float>(a.E, aligned16(logits), [&](auto v, auto c) { run(v, c, float()); });
+        else mb::pick<__nv_bfloat16>(a.E, aligned16(logits), [&](auto v, auto c) { run(v, c, __nv_bfloat16()); });
+        B200MOE_CUDA_TRY(err);
+    }
+    B200MOE_CUDA_TRY(launch_dependent(mb::join_kernel, (unsigned)a.S, mb::kJoinThreads, 0, st, a, loss,
+                                      reinterpret_cast<long long*>(counts), load, inv_tokens, findings));
+    return B200MOE_OK;
+}
+
+extern "C" int b200moe_moe_balance_loss_grad(const void* logits, int logits_fp32, const int64_t* seq_list, const uint8_t* token_mask,
+                                             const float* load, const float* inv_tokens, const float* grad_loss, int64_t n_tokens,
+                                             int64_t n_experts, int64_t n_seqs, void* grad_logits, void* stream) {
+    if (!mb::sizes_ok(n_tokens, n_experts, 1, n_seqs) || (!seq_list && n_seqs != 1)) return B200MOE_ERR_SHAPE;
+    if (logits_fp32 != 0 && logits_fp32 != 1) return B200MOE_ERR_ARGUMENT;
+    if (n_tokens == 0) return B200MOE_OK;
+    if (!logits || !load || !inv_tokens || !grad_loss || !grad_logits) return B200MOE_ERR_NULL_POINTER;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    mb::Args a = {};
+    a.logits = logits;
+    a.seq_list = seq_list;
+    a.mask = token_mask;
+    a.T = (int)n_tokens; a.E = (int)n_experts; a.S = (int)n_seqs;
+    const unsigned grid = (unsigned)((n_tokens + 7) / 8);
+    const bool aligned = aligned16(logits) && aligned16(grad_logits);
+    const auto run = [&](auto vec, auto chunks, auto zero) {
+        using T = decltype(zero);
+        mb::backward_kernel<T, decltype(vec)::value, decltype(chunks)::value>
+            <<<grid, 256, 0, st>>>(a, load, inv_tokens, grad_loss, static_cast<T*>(grad_logits));
+    };
+    if (logits_fp32) mb::pick<float>(a.E, aligned, [&](auto v, auto c) { run(v, c, float()); });
+    else mb::pick<__nv_bfloat16>(a.E, aligned, [&](auto v, auto c) { run(v, c, __nv_bfloat16()); });
+    B200MOE_CUDA_TRY(cudaGetLastError());
+    return B200MOE_OK;
+}

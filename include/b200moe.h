@@ -296,6 +296,52 @@ int b200moe_moe_route(const void* logits, int64_t n_tokens, int64_t n_experts, i
 int b200moe_moe_regroup_index(const int64_t* recv_counts, int64_t world, int64_t e_local, int32_t* pos, int32_t* inv,
                               int64_t* local_counts, void* stream);
 
+/* ---- experts and rows in 8-bit floats, one scale per block of 128 ---------------------------------------------------
+ * (No reference counterpart: its fp8 format is weight-only, x stays bf16.  The weights are that same format.) */
+/* Rows of bf16 -> e4m3 with one fp32 scale per 128 elements (the last block of a row may be shorter).  Row i of the result is row
+ * index[i] of x [n_src, K], or row i where index is NULL (then n_rows <= n_src); an index outside x gives a row of zeros.
+ *   a = max(2^-100, largest magnitude of the block), scale = a / 448, code = e4m3(x * 448 / a), round to nearest even;
+ * a block that holds an infinity or a NaN gets scale NaN and codes 0.  codes [n_rows, K] bytes, scale fp32 [n_rows, ceil(K / 128)].
+ * K % 16 == 0; x and codes aligned to 16 bytes. */
+int b200moe_fp8_quantize_rows(const void* x, const int32_t* index, void* codes, float* scale, int64_t n_src, int64_t n_rows,
+                              int64_t K, void* stream);
+
+/* Grouped GEMM on such rows and weights:
+ *   y[m, n] = sum over blocks kb of 128 k:  x_scale[m, kb] * weight_scale[g, kb, n / 128] * sum_{k in kb} x[m, k] * w[g, k, n]
+ * x e4m3 [M, K], x_scale fp32 [M, ceil(K / 128)], weight e4m3 [G, K, N], weight_scale fp32 [G, ceil(K / 128), ceil(N / 128)]; e4m3 is
+ * the format's own (0x7F and 0xFF are NaN, which b200moe_grouped_gemm reads as +-480).  Sums in fp32, scales applied in fp32.
+ * gate_up_silu == 0: out bf16 [M, N], out_scale unused.  gate_up_silu == 1: N = 2 I with the gate columns first, N % 256 == 0;
+ * silu(gate) * up in fp32, quantised as b200moe_fp8_quantize_rows does: out e4m3 [M, I], out_scale fp32 [M, I / 128].
+ * K % 16 == 0 and N % 16 == 0; x, weight and out aligned to 16 bytes.  Rows of no expert are left as they were.
+ * The workspace belongs to the call until it has completed on the stream, and the next call may have another (calls that overlap must).
+ * findings: NULL, or two int32 in device memory that keep the first (code, detail) of the status words of any call until the
+ * caller zeroes them. */
+size_t b200moe_grouped_gemm_fp8_block_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, int gate_up_silu);
+int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scale, const void* weight, const float* weight_scale,
+                                   const int64_t* group_list, void* out, float* out_scale, int64_t M, int64_t K, int64_t N, int64_t G,
+                                   int group_list_type, int gate_up_silu, void* workspace, size_t workspace_bytes, int32_t* findings,
+                                   void* stream);
+
+/* Balance loss of the router (for training it; no reference counterpart).  logits [T, E] bf16 or fp32 (logits_fp32), idx int32 [T, top_k]
+ * the experts of each token as b200moe_moe_route returns them (an entry outside 0 .. E - 1 is a pair that was dropped: it counts on no
+ * expert).  seq_list int64 [n_seqs]: cumulative token ends of the sequences (tokens behind the last belong to none), or NULL with
+ * n_seqs 1: one sequence of all tokens.  token_mask bytes [T] or NULL: 0 takes a token out (its logits are not read).  For sequence s
+ * with T_s tokens left, p the softmax of a token's logits (all 0 where every logit is -infinity), c_se the pairs on expert e:
+ *   loss[s] = E / (top_k T_s) sum_e c_se (1 / T_s sum_t p_te),  0 where T_s is 0
+ * counts int64 [n_seqs, E] = c.  load fp32 [n_seqs, E] = E c / (top_k T_s) - 1 and inv_tokens fp32 [n_seqs] = 1 / T_s (0 where T_s is 0)
+ * are what b200moe_moe_balance_loss_grad takes with the gradient of the losses grad_loss fp32 [n_seqs]:
+ *   grad_logits [T, E] (of the logits' type) = grad_loss[s] inv_tokens[s] p_te (load[s, e] - sum_j load[s, j] p_tj), 0 for a token of no sequence.
+ * Sums have a fixed order.  A seq_list that falls or leaves 0 .. T is cut to that range and leaves code 1 with the sequence's number
+ * in findings (as above; may be NULL).  E <= 1024, top_k <= 32, n_seqs <= 65535, T * top_k < 2^30. */
+size_t b200moe_moe_balance_scratch_bytes(int64_t n_tokens, int64_t n_experts, int64_t n_seqs);
+int b200moe_moe_balance_loss(const void* logits, int logits_fp32, const int32_t* idx, const int64_t* seq_list,
+                             const uint8_t* token_mask, int64_t n_tokens, int64_t n_experts, int64_t top_k, int64_t n_seqs, float* loss,
+                             int64_t* counts, float* load, float* inv_tokens, void* scratch, size_t scratch_bytes, int32_t* findings,
+                             void* stream);
+int b200moe_moe_balance_loss_grad(const void* logits, int logits_fp32, const int64_t* seq_list, const uint8_t* token_mask,
+                                  const float* load, const float* inv_tokens, const float* grad_loss, int64_t n_tokens,
+                                  int64_t n_experts, int64_t n_seqs, void* grad_logits, void* stream);
+
 /* ---- expert-parallel token exchange over NVLink peer memory ----------------------------------
  * (No reference counterpart: the reference ships the two operators only; chitu exchanges tokens
  * with its own collectives.  These entry points are the exchange steps of the benchmark's MoE layer
