@@ -90,6 +90,10 @@ int sm_count();
 // swizzle128: 128-byte swizzle (box_cols * elem_bytes must be 128), else no swizzle.
 int make_tensor_map_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t rows, uint64_t cols,
                        uint32_t box_rows, uint32_t box_cols, bool swizzle128);
+// 3-D tensor of bytes [outer, rows, cols], box [1, box_rows, box_cols]: what a box holds outside the tensor is zero, also behind the
+// last row of a slice that another slice follows.  128-byte swizzle.
+int make_tensor_map_3d_u8(CUtensorMap* out, const void* base, uint64_t outer, uint64_t rows, uint64_t cols, uint32_t box_rows,
+                          uint32_t box_cols);
 
 // ---- small device utilities ---------------------------------------------------------------
 __device__ __forceinline__ float bf16_bits_to_float(uint32_t b) { return __uint_as_float(b << 16); }

@@ -3,103 +3,646 @@
 //   y[m, n] = sum over blocks kb of 128 k:  x_scale[m, kb] * weight_scale[g, kb, n / 128] * sum_{k in kb} x[m, k] * w[g, k, n]
 //
 // x e4m3 [M, K] with fp32 scales per row and 128 k, weights e4m3 [G, K, N] with fp32 scales per 128 x 128.
-#include <cuda_fp8.h>
+//
+// Persistent kernel on pairs of CTAs.  The operands are swapped: the 256 lanes of a pair's MMA (tcgen05 kind::f8f6f4, M = 256) are
+// weight columns, 128 to a CTA, and its N extent is the tile's token rows rounded up to 32 (32 .. 256), so an expert with 130 rows costs
+// 160 columns, and a decode step's few rows cost 32.  The weights enter as they are stored: a TMA box of 128 k x 128 columns is
+// the MN-major A operand.  The rows of x are split between the two CTAs' shared memory and read by both.
+//
+// An arbitrary fp32 scale cannot ride in the MMA, so a block of 128 k is a sum of its own: the MMA warps write it to one
+// of 2 .. 4 tensor-memory buffers, and the epilogue warps add it, times scale, to the tile's sums in their registers (one fused
+// multiply-add per two elements; a lane's 4 weight columns x 2 tokens of each 8 x 8 patch need one 16-byte read of scales per 16 tokens).
+// Blocks being independent, two warps issue them in turn: a block's MMAs last about as many cycles as it has token rows, fewer
+// than the waits, four issues and the commit cost one warp.
+//
+// Gate/up: CTA 0 of the pair holds 128 gate columns and CTA 1 the up columns of the same indices.  At the end of a tile each
+// sends the other half of its sums through distributed shared memory, and both finish half of the tokens: silu(gate) * up in fp32,
+// the largest magnitude over the 128 columns, e4m3.
+//
+// Warp roles (12 warps): 0 loads (and, in the pair's first CTA, tile tickets); 1 and 2 MMA issue (first CTA); 3 scales;
+// 4 - 11 epilogue.  The shared-memory ring holds as many stages as the call's widest tile leaves room for.  Every wait is bounded.
+//
+// Few tiles: the k range is split into parts whose fp32 sums go to the workspace, and a second kernel adds them in their order.
+#include <algorithm>
 
 #include "common.cuh"
 #include "fp8_block.cuh"
+#include "ptx.cuh"
+#include "tile_ring.h"
 
 namespace b200moe {
 namespace fb {
 
+constexpr int kThreads = 384;
+constexpr int kWarpLoad = 0, kWarpMma0 = 1, kWarpScale = 3, kWarpEpi0 = 4, kEpiWarps = 8;
+constexpr int kMaxR = 256;             // token rows of a tile
+constexpr int kABytes = 128 * 128;     // a CTA's weights of a stage
+constexpr int kMaxSlots = 12, kMaxBufs = 4, kScaleSlots = 8;
+constexpr uint32_t kTmemCols = 512;
+constexpr int kStripBytes = 1024;      // of an epilogue warp
+constexpr int kBigBox = 64, kSmallBox = 16;
+constexpr int kScaleRingBytes = kScaleSlots * kMaxR * 4;
+constexpr int kTopWords = kMaxR / 2 * 4;   // gate/up: magnitudes of a tile, [the CTA's tokens][4 warps]
+constexpr int kTopBytes = 2 * kTopWords * 4;  // of two tiles in turn
+constexpr int kBarrierBytes = 2048;
+constexpr int kFixedBytes = 1024 + kBarrierBytes + kScaleRingBytes + kEpiWarps * kStripBytes + kTopBytes + 2 * (kMaxExperts + 4) * 4;
+constexpr int kSmemBytes = 227 * 1024;
+constexpr int kRingBytes = kSmemBytes - kFixedBytes;  // stages, and the gate/up exchange
+static_assert(kRingBytes - kMaxR * 256 >= 4 * (kABytes + kMaxR / 2 * 128), "stages");
+
 struct Args {
-    const uint8_t* x;
     const float* x_scale;
-    const uint8_t* weight;
     const float* w_scale;
     const int64_t* group_list;
     void* out;
     float* out_scale;
+    float* parts;      // [max_parts][M][N], or NULL
+    int max_parts;
     int M, K, N, G, gl_type, KB, NB;
     int* status;
     int* findings;
 };
+// words of the workspace's first 256 bytes behind the status words
+constexpr int kWordTicket = 2, kWordParts = 8, kWordRows = 9;
 
-__device__ __forceinline__ float e4m3_to_float(uint32_t code) {
-    __nv_fp8_e4m3 v;
-    v.__x = (__nv_fp8_storage_t)code;
-    return (float)v;
-}
+struct Sync {
+    uint64_t full[kMaxSlots];    // first CTA: the bytes of both CTAs' loads
+    uint64_t empty[kMaxSlots];   // each CTA: one epilogue lane has seen the stage's MMAs complete
+    uint64_t t_full[kMaxBufs];   // each CTA: commit
+    uint64_t t_empty[kMaxBufs];  // first CTA: the 16 epilogue warps of the pair
+    uint64_t s_full[kScaleSlots], s_empty[kScaleSlots];
+    uint64_t x_full, x_free;     // gate/up exchange: the other CTA's 8 warps have written here; have read what was sent there
+    uint64_t wg[2];              // the four epilogue warps of a group among themselves
+    uint64_t drain[2];
+    uint32_t tmem_base;
+    int abort;
+    int n_units, parts, width;   // width: token rows of the widest tile, rounded up to 32
+    alignas(16) TileEntry ring[kTileRing];
+};
+static_assert(sizeof(Sync) <= kBarrierBytes, "barrier block");
 
-constexpr int kRows = 16;
-template <bool GATE_UP>
-__global__ void __launch_bounds__(GATE_UP ? 256 : 128) simple_kernel(const Args a) {
-    __shared__ int row_start[kMaxExperts + 1];
-    __shared__ float xs[kRows][128];
-    __shared__ alignas(16) float h[kRows][128];
-    load_row_starts(a.group_list, a.G, a.M, a.gl_type, row_start, a.status);
-    int tile = blockIdx.y, g = 0, r0 = 0, rows = 0;
-    for (;; ++g) {
-        if (g == a.G) return;
-        const int n = row_start[g + 1] - row_start[g], tiles = (n + kRows - 1) / kRows;
-        if (tile < tiles) {
-            r0 = row_start[g] + tile * kRows;
-            rows = min(kRows, n - tile * kRows);
-            break;
-        }
-        tile -= tiles;
-    }
-    const int half = threadIdx.x >> 7, c = threadIdx.x & 127;
-    const int col = blockIdx.x * 128 + c + (GATE_UP ? half * (a.N >> 1) : 0);
-    float acc[kRows] = {};
-    for (int kb = 0; kb < a.KB; ++kb) {
-        const int k0 = kb * 128, kn = min(128, a.K - k0);
-        __syncthreads();
-        for (int i = threadIdx.x; i < kRows * 128; i += blockDim.x) {
-            const int r = i >> 7, k = i & 127;
-            xs[r][k] = r < rows && k < kn ? e4m3_to_float(a.x[(size_t)(r0 + r) * a.K + k0 + k]) : 0.f;
-        }
-        __syncthreads();
-        float part[kRows] = {};
-        if (col < a.N) {
-            for (int k = 0; k < kn; ++k) {
-                const float w = e4m3_to_float(a.weight[((size_t)g * a.K + k0 + k) * a.N + col]);
-#pragma unroll
-                for (int r = 0; r < kRows; ++r) part[r] = fmaf(xs[r][k], w, part[r]);
+struct Tile {
+    int g, row0, rows, n, nt, kb0, kb1, part;  // n: rows rounded up to 32; nt: 256 weight columns (gate/up: 128 of each)
+};
+
+__device__ __forceinline__ bool wait_slow(uint32_t bar, uint32_t parity, Sync* sy, int* status, int id) {
+    volatile int* abort = &sy->abort;
+    const uint64_t t0 = ptx::globaltimer_ns();
+    uint32_t spins = 0;
+    while (!ptx::mbar_try_wait_cluster(bar, parity)) {
+        if ((++spins & 0xFF) == 0) {
+            if (*abort) return false;
+            if (ptx::globaltimer_ns() - t0 > ptx::kWaitLimitNs) {
+                *abort = 1;
+                report_status(status, kDevWaitExpired, id);
+                return false;
             }
-            const float ws = a.w_scale[((size_t)g * a.KB + kb) * a.NB + (col >> 7)];
-#pragma unroll
-            for (int r = 0; r < kRows; ++r)
-                if (r < rows) acc[r] = fmaf(part[r], ws * a.x_scale[(size_t)(r0 + r) * a.KB + kb], acc[r]);
         }
     }
-    if constexpr (!GATE_UP) {
-        if (col < a.N)
-            for (int r = 0; r < rows; ++r) static_cast<__nv_bfloat16*>(a.out)[(size_t)(r0 + r) * a.N + col] = __float2bfloat16_rn(acc[r]);
-    } else {
-        __syncthreads();
-        if (half == 1)
-            for (int r = 0; r < kRows; ++r) xs[r][c] = acc[r];
-        __syncthreads();
-        if (half == 0)
-            for (int r = 0; r < kRows; ++r) h[r][c] = acc[r] / (1.f + expf(-acc[r])) * xs[r][c];
-        __syncthreads();
-        const int inter = a.N >> 1;
-        for (int r = threadIdx.x >> 5; r < rows; r += 8) {
-            const int lane = threadIdx.x & 31;
-            const float4 v = reinterpret_cast<const float4*>(h[r])[lane];
-            uint32_t top = 0;  // magnitudes order as their bits do, infinities and NaN last
-            top = max(max(__float_as_uint(v.x) & 0x7FFFFFFFu, __float_as_uint(v.y) & 0x7FFFFFFFu),
-                      max(__float_as_uint(v.z) & 0x7FFFFFFFu, __float_as_uint(v.w) & 0x7FFFFFFFu));
-            top = __reduce_max_sync(0xffffffffu, top);
-            const fp8_block::Quantizer q(__uint_as_float(top));
-            reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + (size_t)(r0 + r) * inter + blockIdx.x * 128)[lane] = q.four(v.x, v.y, v.z, v.w);
-            if (lane == 0) a.out_scale[(size_t)(r0 + r) * (inter >> 7) + blockIdx.x] = q.scale;
+    return true;
+}
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Sync* sy, int* status, int id) {
+    const uint32_t b = ptx::smem_u32(bar);
+    if (ptx::mbar_try_wait_cluster(b, parity)) return true;
+    return wait_slow(b, parity, sy, status, id);
+}
+
+// The seq-th tile of the pair (seq is advanced); false when the schedule has ended, a wait expired or another role aborted.
+__device__ __forceinline__ bool next_tile(Sync* sy, uint32_t& seq, Tile& t, const Args& a, int parts) {
+    const TileEntry* e = &sy->ring[seq % kTileRing];
+    const uint32_t want = seq + 1;
+    TileEntry v = ring_load(e);
+    if (!tile_entry_is(v, want)) {
+        volatile int* abort = &sy->abort;
+        const uint64_t t0 = ptx::globaltimer_ns();
+        uint32_t spins = 0;
+        while (!tile_entry_is(v = ring_load(e), want)) {
+            if ((++spins & 0xFF) == 0) {
+                if (*abort) return false;
+                if (ptx::globaltimer_ns() - t0 > ptx::kWaitLimitNs) {
+                    *abort = 1;
+                    report_status(a.status, kDevWaitExpired, 90);
+                    return false;
+                }
+            }
         }
+    }
+    ++seq;
+    t.rows = tile_entry_rows(v);
+    if (t.rows == 0) return false;
+    t.row0 = tile_entry_row0(v);
+    t.g = tile_entry_expert(v);
+    t.n = (t.rows + 31) & ~31;
+    const int c = tile_entry_column(v);
+    if (parts == 1) {
+        t.nt = c;
+        t.part = 0;
+        t.kb0 = 0;
+        t.kb1 = a.KB;
+    } else {
+        t.nt = c / parts;
+        t.part = c - t.nt * parts;
+        t.kb0 = (int)((long long)t.part * a.KB / parts);
+        t.kb1 = (int)((long long)(t.part + 1) * a.KB / parts);
+    }
+    return true;
+}
+
+// An expert's rows are cut into the fewest tiles, of equal size rounded up to 32.
+__device__ __forceinline__ int tiles_of(int rows) { return (rows + kMaxR - 1) / kMaxR; }
+__device__ __forceinline__ int tile_rows_of(int rows, int tiles) { return ((rows + tiles - 1) / tiles + 31) & ~31; }
+
+// unit -> ring entry; inside an expert the row tiles of a weight column run together, so that they share the weights in L2
+__device__ __forceinline__ TileEntry locate(uint32_t seq, int unit, int parts, const int* prefix, const int* row_start, int G, int n_nt) {
+    const int t = unit / parts, part = unit - t * parts;
+    int lo = 0, hi = G;  // largest g with prefix[g] <= t
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (prefix[mid] <= t) lo = mid;
+        else hi = mid;
+    }
+    const int j = t - prefix[lo], mt = (prefix[lo + 1] - prefix[lo]) / n_nt;
+    const int nt = j / mt, m = j - nt * mt;
+    const int rows = row_start[lo + 1] - row_start[lo], tr = tile_rows_of(rows, mt);
+    return tile_entry(seq, (uint32_t)(row_start[lo] + m * tr), (uint32_t)min(tr, rows - m * tr), (uint32_t)lo, (uint32_t)(nt * parts + part));
+}
+
+__device__ __forceinline__ float silu(float g) {
+    const float e = __expf(-fabsf(g));  // (at most 1: nothing overflows)
+    return g * __fdividef(g < 0.f ? e : 1.f, 1.f + e);
+}
+
+// Where the sums of a chunk's 16-lane half lie in the gate/up exchange: [group of warps][chunk][half][thread] pieces of 16 bytes.
+__device__ __forceinline__ uint32_t exchange_at(int wg, int n_ch, int c, int h, int thread) {
+    return (uint32_t)((((wg * n_ch + c) * 2 + h) * 128 + thread) * 16);
+}
+
+template <bool GATE_UP>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x64,
+                   const __grid_constant__ CUtensorMap map_x16, const Args a) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* base = smem_raw + ((1024u - (ptx::smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* ring = base;
+    Sync* sy = reinterpret_cast<Sync*>(base + kRingBytes);
+    float* scales = reinterpret_cast<float*>(base + kRingBytes + kBarrierBytes);
+    uint8_t* strips = reinterpret_cast<uint8_t*>(scales) + kScaleRingBytes;
+    float* tops = reinterpret_cast<float*>(strips + kEpiWarps * kStripBytes);
+    int* row_start = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(tops) + kTopBytes);
+    int* prefix = row_start + kMaxExperts + 4;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = ptx::cluster_rank();
+    const int n_nt = GATE_UP ? a.N / 256 : (a.NB + 1) / 2;
+
+    load_row_starts(a.group_list, a.G, a.M, a.gl_type, row_start, a.status);
+    if (warp == 0) {
+        int lo, hi, mine = 0, total, wide = 0;
+        lane_experts(a.G, lo, hi);
+        for (int g = lo; g < hi; ++g) {
+            const int rows = row_start[g + 1] - row_start[g], mt = tiles_of(rows);
+            mine += mt;
+            if (mt) wide = max(wide, tile_rows_of(rows, mt));
+        }
+        int at = warp_exclusive_sum(mine, total);
+        wide = __reduce_max_sync(0xffffffffu, wide);
+        for (int g = lo; g < hi; ++g) {
+            prefix[g] = at * n_nt;
+            at += tiles_of(row_start[g + 1] - row_start[g]);
+        }
+        if (lane == 0) {
+            const int tiles = total * n_nt, pairs = (int)gridDim.x / 2;
+            prefix[a.G] = tiles;
+            int parts = 1;
+            if (a.parts != nullptr && tiles > 0 && tiles < pairs) parts = min(a.max_parts, (pairs + tiles - 1) / tiles);
+            sy->parts = parts;
+            sy->n_units = tiles * parts;
+            sy->width = max(wide, 32);
+            if (blockIdx.x == 0) {
+                a.status[kWordParts] = parts;
+                a.status[kWordRows] = row_start[a.G];
+            }
+        }
+    }
+    if (threadIdx.x == 32) {
+        sy->abort = 0;
+        for (int i = 0; i < kTileRing; ++i) sy->ring[i] = tile_entry(0u, 0u, 0u, 0u, 0u);
+        const auto init = [](uint64_t* b, int n, uint32_t count) {
+            for (int i = 0; i < n; ++i) ptx::mbar_init(ptx::smem_u32(b + i), count);
+        };
+        init(sy->full, kMaxSlots, 1);
+        init(sy->empty, kMaxSlots, 1);
+        init(sy->t_full, kMaxBufs, 1);
+        init(sy->t_empty, kMaxBufs, 2 * kEpiWarps);
+        init(sy->s_full, kScaleSlots, 1);
+        init(sy->s_empty, kScaleSlots, kEpiWarps);
+        init(&sy->x_full, 1, kEpiWarps);
+        init(&sy->x_free, 1, kEpiWarps);
+        init(sy->wg, 2, 4);
+        init(sy->drain, 2, 1);
+        ptx::fence_mbar_init();
+        ptx::prefetch_tensormap(&map_w);
+        ptx::prefetch_tensormap(&map_x64);
+        ptx::prefetch_tensormap(&map_x16);
+    }
+    if (warp == kWarpMma0) {
+        ptx::tmem_alloc_pair(ptx::smem_u32(&sy->tmem_base), kTmemCols);
+        ptx::tmem_relinquish_pair();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::cluster_sync();
+    ptx::tc_fence_after();
+
+    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sy->tmem_base);
+    const int parts = sy->parts, n_units = sy->n_units, width = sy->width;
+    const int slot_bytes = kABytes + width * 64;
+    const int exchange_bytes = GATE_UP ? width * 256 : 0;
+    const int n_slots = min(kMaxSlots, (kRingBytes - exchange_bytes) / slot_bytes);
+    const int n_bufs = min(kMaxBufs, (int)kTmemCols / width);
+    uint8_t* exchange = ring + kRingBytes - exchange_bytes;
+
+    if (warp < kWarpEpi0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == kWarpLoad) {
+            // ------------------------------ loads ------------------------------
+            if (lane == 0) {
+                uint32_t seq = 0, published = 0, it = 0, slot = 0, ph = 0;
+                int held = 0;
+                bool live = true, ok = true;
+                const uint32_t ring_there = ptx::map_rank(ptx::smem_u32(sy->ring), 1);
+                const auto publish = [&]() {
+                    if (rank != 0 || !live) return;
+                    held = atomicAdd(a.status + kWordTicket, 1);
+                    live = held < n_units;
+                    const TileEntry e = live ? locate(published + 1, held, parts, prefix, row_start, a.G, n_nt)
+                                             : tile_entry(published + 1, 0u, 0u, 0u, 0u);  // rows 0: the schedule has ended
+                    const uint32_t at = (published % kTileRing) * (uint32_t)sizeof(TileEntry);
+                    ring_store(&sy->ring[published % kTileRing], e);
+                    ptx::st_cluster_u64(ring_there + at, e.a);
+                    ptx::st_cluster_u64(ring_there + at + 8, e.b);
+                    ++published;
+                };
+                publish();
+                Tile t;
+                while (ok) {
+                    publish();  // (a tile ahead: the other roles find it there)
+                    if (!next_tile(sy, seq, t, a, parts)) break;
+                    const int half = t.n >> 1, n_big = half / kBigBox, n_small = (half % kBigBox) / kSmallBox;
+                    const uint32_t bytes = 2u * (uint32_t)(kABytes + half * 128);
+                    const int col = GATE_UP ? (int)rank * (a.N >> 1) + t.nt * 128 : t.nt * 256 + (int)rank * 128;
+                    const int row = t.row0 + (int)rank * half;
+                    for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+                        if (it >= (uint32_t)n_slots && !wait(&sy->empty[slot], ph ^ 1, sy, a.status, 10)) { ok = false; break; }
+                        const uint32_t bar = ptx::smem_u32(&sy->full[slot]), bar0 = ptx::map_rank(bar, 0);
+                        const uint32_t dst = ptx::smem_u32(ring) + slot * (uint32_t)slot_bytes;
+                        if (rank == 0) ptx::mbar_arrive_expect_tx(bar, bytes);
+                        ptx::tma_load_3d_pair(dst, &map_w, bar0, col, kb * 128, t.g);
+                        uint32_t at = dst + kABytes;
+                        int r = row;
+                        for (int b = 0; b < n_big; ++b, at += kBigBox * 128, r += kBigBox)
+                            ptx::tma_load_2d_pair(at, &map_x64, bar0, kb * 128, r);
+                        for (int b = 0; b < n_small; ++b, at += kSmallBox * 128, r += kSmallBox)
+                            ptx::tma_load_2d_pair(at, &map_x16, bar0, kb * 128, r);
+                        if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
+                    }
+                }
+                if (*reinterpret_cast<volatile int*>(&sy->abort)) {
+                    // copies in flight land before the shared memory goes (those of both CTAs are counted in the first one)
+                    if (rank == 0) {
+                        const uint32_t from = it > (uint32_t)n_slots ? it - n_slots : 0;
+                        for (uint32_t j = from; j < it; ++j)
+                            (void)ptx::mbar_wait(ptx::smem_u32(&sy->full[j % n_slots]), (j / n_slots) & 1);
+                    }
+                    const uint64_t t0 = ptx::globaltimer_ns();
+                    while (ptx::globaltimer_ns() - t0 < 10000000ull) {}
+                }
+            }
+            __syncwarp();
+        } else if (warp == kWarpScale) {
+            // ------------------------------ scales ------------------------------
+            // Row scale times the tile's weight scale, in the order in which the epilogue's lanes take them: 16 tokens are four
+            // pieces of 16 bytes, piece q the tokens 2q, 2q + 1, 8 + 2q, 9 + 2q.
+            uint32_t seq = 0, it = 0;
+            const int home = (lane & 16) + ((lane & 7) >> 1) * 4 + ((lane >> 3) & 1) * 2 + (lane & 1);
+            bool ok = true;
+            Tile t;
+            while (ok && next_tile(sy, seq, t, a, parts)) {
+                const int nb = min(a.NB - 1, GATE_UP ? (int)rank * (a.N >> 8) + t.nt : t.nt * 2 + (int)rank);
+                const float* ws = a.w_scale + (size_t)t.g * a.KB * a.NB + nb;
+                const float* xs = a.x_scale + (size_t)(t.row0 + lane) * a.KB;
+                for (int kb = t.kb0; kb < t.kb1 && ok; kb += 4) {
+                    float w[4], v[8][4];
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) w[b] = kb + b < t.kb1 ? __ldg(ws + (size_t)(kb + b) * a.NB) : 0.f;
+#pragma unroll
+                    for (int g = 0; g < 8; ++g)
+#pragma unroll
+                        for (int b = 0; b < 4; ++b)
+                            v[g][b] = g * 32 + lane < t.rows && kb + b < t.kb1 ? __ldg(xs + (size_t)(g * 32) * a.KB + kb + b) : 0.f;
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        if (kb + b >= t.kb1 || !ok) break;
+                        const uint32_t s = it % kScaleSlots;
+                        if (it >= kScaleSlots) ok = __all_sync(0xffffffffu, wait(&sy->s_empty[s], ((it / kScaleSlots) & 1) ^ 1, sy, a.status, 20));
+                        if (!ok) break;
+#pragma unroll
+                        for (int g = 0; g < 8; ++g)
+                            if (g * 32 < t.n) scales[s * kMaxR + g * 32 + home] = v[g][b] * w[b];
+                        __syncwarp();
+                        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->s_full[s]));
+                        ++it;
+                    }
+                }
+            }
+        } else if (rank == 0) {
+            // ------------------------------ MMA issue ------------------------------
+            // The warp walks together, one lane issues; this warp takes every other block.
+            const uint32_t turn = (uint32_t)(warp - kWarpMma0);
+            const bool leader = ptx::elect_one();
+            uint32_t seq = 0, it = 0, slot = 0, ph = 0, buf = 0, tph = 0;
+            bool ok = true;
+            const uint64_t da0 = ptx::umma_desc_sw128(ptx::smem_u32(ring), kABytes, 1024);
+            const uint64_t db0 = ptx::umma_desc_sw128(ptx::smem_u32(ring) + kABytes, 0, 1024);
+            Tile t;
+            while (ok && next_tile(sy, seq, t, a, parts)) {
+                const uint32_t idesc = ptx::umma_idesc_e4m3_mn_k(256, t.n);
+                for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+                    if ((it & 1) == turn) {
+                        // the epilogue of both CTAs has taken what the buffer held
+                        if (it >= (uint32_t)n_bufs && !wait(&sy->t_empty[buf], tph ^ 1, sy, a.status, 30)) { ok = false; break; }
+                        if (!wait(&sy->full[slot], ph, sy, a.status, 40)) { ok = false; break; }
+                        ptx::tc_fence_after();
+                        if (leader) {
+                            const uint64_t at = (uint64_t)(slot * (uint32_t)slot_bytes >> 4);
+#pragma unroll
+                            for (int k32 = 0; k32 < 4; ++k32)
+                                ptx::umma_f8_pair(tmem_base + buf * (uint32_t)width, da0 + at + (uint64_t)(k32 * 256),
+                                                  db0 + at + (uint64_t)(k32 * 2), idesc, (uint32_t)(k32 != 0));
+                            ptx::umma_commit_pair(ptx::smem_u32(&sy->t_full[buf]));
+                        }
+                        __syncwarp();
+                    }
+                    if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
+                    if (++buf == (uint32_t)n_bufs) { buf = 0; tph ^= 1; }
+                }
+            }
+            // every MMA issued here must have completed before tensor and shared memory go
+            if (leader) {
+                ptx::umma_commit_pair(ptx::smem_u32(&sy->drain[turn]));
+                (void)ptx::mbar_wait(ptx::smem_u32(&sy->drain[turn]), 0);
+            }
+            __syncwarp();
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        // ------------------------------ epilogue ------------------------------
+        // A warp holds 32 weight columns (tensor-memory lanes) x half of the tile's tokens: acc[chunk of 16 tokens][16 lanes][8 tokens]
+        // [8 lanes], two tokens to a register pair.
+        const int ew = warp - kWarpEpi0, wg = ew >> 2, quarter = warp & 3, g8 = lane >> 2, q = lane & 3;
+        uint8_t* strip = strips + ew * kStripBytes;
+        const uint32_t strip_u32 = ptx::smem_u32(strip);
+        const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+        uint32_t seq = 0, slot = 0, buf = 0, tph = 0, sc = 0, sph = 0, tiles = 0;
+        bool ok = true;
+        Tile t;
+        while (ok && next_tile(sy, seq, t, a, parts)) {
+            const int half = t.n >> 1, n_ch = half >> 4, first = wg * half;
+            f32x2 acc[8][2][2][2];
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[c][i >> 2][(i >> 1) & 1][i & 1] = 0ull;
+            for (int kb = t.kb0; kb < t.kb1; ++kb) {
+                ok = wait(&sy->s_full[sc], sph, sy, a.status, 50) && wait(&sy->t_full[buf], tph, sy, a.status, 51);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                ptx::tc_fence_after();
+                // the block's MMAs have completed: its stage may be loaded again
+                if (ew == 0 && lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->empty[slot]));
+                const float4* sv = reinterpret_cast<const float4*>(scales + sc * kMaxR + first) + q;
+                const uint32_t td = tmem_base + lane_base + buf * (uint32_t)width + (uint32_t)first;
+#pragma unroll
+                for (int c0 = 0; c0 < 8; c0 += 2) {
+                    if (c0 < n_ch) {
+                        uint32_t v[2][2][8];
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+                            if (c0 + c < n_ch) {
+                                ptx::tmem_ld_16x16(td + (uint32_t)((c0 + c) * 16), v[c][0]);
+                                ptx::tmem_ld_16x16(td + (uint32_t)((c0 + c) * 16) + (16u << 16), v[c][1]);
+                            }
+                        ptx::tmem_ld_wait();
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+                            if (c0 + c < n_ch) {
+                                const float4 s4 = sv[(c0 + c) * 4];
+                                const f32x2 s2[2] = {pack_f32x2(s4.x, s4.y), pack_f32x2(s4.z, s4.w)};
+#pragma unroll
+                                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                                        for (int i = 0; i < 2; ++i)
+                                            acc[c0 + c][h][j][i] = fma_f32x2(pack_u32x2(v[c][h][4 * j + 2 * i], v[c][h][4 * j + 2 * i + 1]),
+                                                                             s2[j], acc[c0 + c][h][j][i]);
+                            }
+                    }
+                }
+                ptx::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    ptx::mbar_arrive_cluster(ptx::map_rank(ptx::smem_u32(&sy->t_empty[buf]), 0));
+                    ptx::mbar_arrive(ptx::smem_u32(&sy->s_empty[sc]));
+                }
+                if (++slot == (uint32_t)n_slots) slot = 0;
+                if (++buf == (uint32_t)n_bufs) { buf = 0; tph ^= 1; }
+                if (++sc == kScaleSlots) { sc = 0; sph ^= 1; }
+            }
+            if (!ok) break;
+
+            if (parts > 1) {
+                // a part's sums as they are, [part][row][column]
+                const int col0 = (GATE_UP ? (int)rank * (a.N >> 1) + t.nt * 128 : t.nt * 256 + (int)rank * 128) + quarter * 32 + g8;
+                float* dst = a.parts + ((size_t)t.part * a.M + t.row0) * a.N;
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const int token = first + c * 16 + j * 8 + 2 * q, col = col0 + h * 16 + i * 8;
+                                if (c < n_ch && col < a.N) {
+                                    if (token < t.rows) dst[(size_t)token * a.N + col] = f32x2_lo(acc[c][h][j][i]);
+                                    if (token + 1 < t.rows) dst[(size_t)(token + 1) * a.N + col] = f32x2_hi(acc[c][h][j][i]);
+                                }
+                            }
+            } else if constexpr (!GATE_UP) {
+                // 16 tokens x 32 columns at a time through the warp's strip: the transposing store gives 16-byte pieces of
+                // eight columns, 64 contiguous bytes of a row
+                const int col = t.nt * 256 + (int)rank * 128 + quarter * 32 + q * 8;
+                __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (size_t)t.row0 * a.N + col;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    if (c < n_ch) {
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            uint32_t o[4];
+#pragma unroll
+                            for (int m = 0; m < 4; ++m) o[m] = pack_bf16x2(f32x2_lo(acc[c][m >> 1][j][m & 1]), f32x2_hi(acc[c][m >> 1][j][m & 1]));
+                            // row lane % 8 (a token), piece lane / 8
+                            const int token = j * 8 + (lane & 7);
+                            ptx::stmatrix_x4_trans(strip_u32 + (uint32_t)(token * 64 + (((lane >> 3) ^ (token >> 1)) & 3) * 16), o[0], o[1], o[2], o[3]);
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const int token = j * 8 + g8, row = first + c * 16 + token;
+                            const uint4 o = *reinterpret_cast<const uint4*>(strip + token * 64 + ((q ^ (token >> 1)) & 3) * 16);
+                            if (row < t.rows && col < a.N) *reinterpret_cast<uint4*>(dst + (size_t)row * a.N) = o;
+                        }
+                        __syncwarp();
+                    }
+                }
+            } else {
+                // this CTA finishes the tokens of group j = rank of every chunk; the other group's sums go to the other CTA
+                const int thread = quarter * 32 + lane;
+                const uint32_t there = ptx::map_rank(ptx::smem_u32(exchange), rank ^ 1);
+                if (tiles > 0) ok = __all_sync(0xffffffffu, wait(&sy->x_free, (tiles - 1) & 1, sy, a.status, 60));
+                if (!ok) break;
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    if (c < n_ch) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const f32x2 s0 = rank == 0 ? acc[c][h][1][0] : acc[c][h][0][0], s1 = rank == 0 ? acc[c][h][1][1] : acc[c][h][0][1];
+                            ptx::st_cluster_v4(there + exchange_at(wg, n_ch, c, h, thread), (uint32_t)s0, (uint32_t)(s0 >> 32), (uint32_t)s1, (uint32_t)(s1 >> 32));
+                        }
+                    }
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_rank(ptx::smem_u32(&sy->x_full), rank ^ 1));
+                ok = __all_sync(0xffffffffu, wait(&sy->x_full, tiles & 1, sy, a.status, 61));
+                if (!ok) break;
+                float* top = tops + (tiles & 1) * kTopWords;
+                float h8[8][8];  // [chunk][2 * m + b]: column 8 m + g8, token 2 q + b
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    if (c < n_ch) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint4 o = *reinterpret_cast<const uint4*>(exchange + exchange_at(wg, n_ch, c, h, thread));
+                            const f32x2 k0 = rank == 0 ? acc[c][h][0][0] : acc[c][h][1][0], k1 = rank == 0 ? acc[c][h][0][1] : acc[c][h][1][1];
+                            const float own[4] = {f32x2_lo(k0), f32x2_hi(k0), f32x2_lo(k1), f32x2_hi(k1)};
+                            const float other[4] = {__uint_as_float(o.x), __uint_as_float(o.y), __uint_as_float(o.z), __uint_as_float(o.w)};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                h8[c][h * 4 + i] = silu(rank == 0 ? own[i] : other[i]) * (rank == 0 ? other[i] : own[i]);
+                        }
+                        // the largest magnitude over the warp's 32 columns (magnitudes order as their bits do, infinities and NaN last)
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            uint32_t m = 0;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(h8[c][2 * i + b]) & 0x7FFFFFFFu);
+#pragma unroll
+                            for (int o = 4; o < 32; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                            if (g8 == 0) top[(wg * 64 + c * 8 + 2 * q + b) * 4 + quarter] = __uint_as_float(m);
+                        }
+                    }
+                __syncwarp();
+                if (lane == 0) {
+                    ptx::mbar_arrive_cluster(ptx::map_rank(ptx::smem_u32(&sy->x_free), rank ^ 1));  // what was sent here has been read
+                    ptx::mbar_arrive(ptx::smem_u32(&sy->wg[wg]));
+                }
+                ok = __all_sync(0xffffffffu, wait(&sy->wg[wg], tiles & 1, sy, a.status, 62));
+                if (!ok) break;
+                const int inter = a.N >> 1;
+                uint8_t* dst = static_cast<uint8_t*>(a.out) + (size_t)t.row0 * inter + t.nt * 128 + quarter * 32 + (lane & 1) * 16;
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    if (c < n_ch) {
+                        const int token0 = first + c * 16 + (int)rank * 8;
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            const uint4 m4 = *reinterpret_cast<const uint4*>(top + (wg * 64 + c * 8 + 2 * q + b) * 4);
+                            const fp8_block::Quantizer qz(__uint_as_float(max(max(m4.x, m4.y), max(m4.z, m4.w))));
+                            const uint32_t o = qz.four(h8[c][b], h8[c][2 + b], h8[c][4 + b], h8[c][6 + b]);
+                            uint8_t* at = strip + (2 * q + b) * 32 + g8;
+                            at[0] = (uint8_t)o;
+                            at[8] = (uint8_t)(o >> 8);
+                            at[16] = (uint8_t)(o >> 16);
+                            at[24] = (uint8_t)(o >> 24);
+                            const int token = token0 + 2 * q + b;
+                            if (quarter == 0 && g8 == 0 && token < t.rows) a.out_scale[(size_t)(t.row0 + token) * (inter >> 7) + t.nt] = qz.scale;
+                        }
+                        __syncwarp();
+                        const int token = token0 + (lane >> 1);
+                        if (lane < 16 && token < t.rows)
+                            *reinterpret_cast<uint4*>(dst + (size_t)token * inter) = *reinterpret_cast<const uint4*>(strip + lane * 16);
+                        __syncwarp();
+                    }
+            }
+            ++tiles;
+        }
+    }
+
+    __syncwarp();
+    if (threadIdx.x == 0 && a.findings != nullptr) {
+        const volatile int* st = a.status;
+        if (st[0] != 0 && atomicCAS(a.findings, 0, st[0]) == 0) a.findings[1] = st[1];
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::cluster_sync();  // (what one CTA sends the other, loads and MMAs of the pair among it, has arrived)
+    if (warp == kWarpMma0) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc_pair(tmem_base, kTmemCols);
+    }
+    grid_dep_launch();
+}
+
+// The parts of a split k range, added in their order.  A warp takes 128 columns of a row.
+template <bool GATE_UP>
+__global__ void __launch_bounds__(256) join_kernel(const Args a) {
+    grid_dep_wait();
+    const int parts = __ldcg(a.status + kWordParts), rows = __ldcg(a.status + kWordRows);
+    if (parts == 1) return;
+    const int lane = threadIdx.x & 31, out_n = GATE_UP ? a.N >> 1 : a.N, blocks = (out_n + 127) / 128;
+    const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int row = (int)(unit / blocks), nb = (int)(unit % blocks), col = nb * 128 + lane * 4;
+    if (row >= rows) return;
+    float4 s[2] = {};
+    for (int p = 0; p < parts; ++p)
+#pragma unroll
+        for (int u = 0; u < (GATE_UP ? 2 : 1); ++u)
+            if (col < out_n) {
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(a.parts + ((size_t)p * a.M + row) * a.N + u * out_n + col));
+                s[u].x += v.x; s[u].y += v.y; s[u].z += v.z; s[u].w += v.w;
+            }
+    if constexpr (!GATE_UP) {
+        if (col < out_n)
+            *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)row * a.N + col) =
+                make_uint2(pack_bf16x2(s[0].x, s[0].y), pack_bf16x2(s[0].z, s[0].w));
+    } else {
+        const float h[4] = {silu(s[0].x) * s[1].x, silu(s[0].y) * s[1].y, silu(s[0].z) * s[1].z, silu(s[0].w) * s[1].w};
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(h[i]) & 0x7FFFFFFFu);
+        const fp8_block::Quantizer q(__uint_as_float(__reduce_max_sync(0xffffffffu, m)));
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + (size_t)row * out_n + col) = q.four(h[0], h[1], h[2], h[3]);
+        if (lane == 0) a.out_scale[(size_t)row * blocks + nb] = q.scale;
     }
 }
 
-__global__ void keep_finding_kernel(const int* status, int* findings) {
-    if (status[0] != 0 && atomicCAS(findings, 0, status[0]) == 0) findings[1] = status[1];
+// Whether a call can have fewer tiles than there are pairs of multiprocessors, and in how many parts its k range is cut at most: parts of
+// four blocks or more, sums of 32 MB or less.
+static int max_parts(int64_t M, int64_t K, int64_t N, int64_t G, int gate_up) {
+    const int64_t n_nt = (N + 255) / 256, experts = std::min(G, M);
+    if (experts * n_nt >= 74) return 1;
+    const int64_t kb = (K + 127) / 128, room = (32ll << 20) / (M * N * 4);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({16, kb / 4, room}));
 }
 
 }  // namespace fb
@@ -108,7 +651,9 @@ __global__ void keep_finding_kernel(const int* status, int* findings) {
 using namespace b200moe;
 
 extern "C" size_t b200moe_grouped_gemm_fp8_block_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, int gate_up_silu) {
-    return B200MOE_STATUS_BYTES;
+    if (M <= 0 || K <= 0 || N <= 0 || G <= 0) return B200MOE_STATUS_BYTES;
+    const int parts = fb::max_parts(M, K, N, G, gate_up_silu);
+    return B200MOE_STATUS_BYTES + (parts > 1 ? (size_t)parts * (size_t)M * (size_t)N * 4 : 0);
 }
 
 extern "C" int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scale, const void* weight, const float* weight_scale,
@@ -121,16 +666,17 @@ extern "C" int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scal
     if (group_list_type != B200MOE_GROUP_LIST_CUMSUM && group_list_type != B200MOE_GROUP_LIST_COUNTS) return B200MOE_ERR_ARGUMENT;
     if (gate_up_silu != 0 && gate_up_silu != 1) return B200MOE_ERR_ARGUMENT;
     if (M == 0) return B200MOE_OK;
+    // (unit numbers and ring entries)
+    if ((M / fb::kMaxR + G) * ((N + 255) / 256) > 0x3FFFFFFLL) return B200MOE_ERR_SHAPE;
     if (!x || !x_scale || !weight || !weight_scale || !group_list || !out || (gate_up_silu && !out_scale))
         return B200MOE_ERR_NULL_POINTER;
     if (!aligned16(x) || !aligned16(weight) || !aligned16(out)) return B200MOE_ERR_ALIGNMENT;
     if (!workspace || workspace_bytes < b200moe_grouped_gemm_fp8_block_workspace_bytes(M, K, N, G, gate_up_silu))
         return B200MOE_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return B200MOE_ERR_ALIGNMENT;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    fb::Args a;
-    a.x = static_cast<const uint8_t*>(x);
+    fb::Args a = {};
     a.x_scale = x_scale;
-    a.weight = static_cast<const uint8_t*>(weight);
     a.w_scale = weight_scale;
     a.group_list = group_list;
     a.out = out;
@@ -141,16 +687,23 @@ extern "C" int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scal
     a.NB = (int)((N + 127) / 128);
     a.status = static_cast<int*>(workspace);
     a.findings = findings;
+    a.max_parts = fb::max_parts(M, K, N, G, gate_up_silu);
+    if (a.max_parts > 1) a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + B200MOE_STATUS_BYTES);
+    CUtensorMap map_w, map_x64, map_x16;
+    int rc = make_tensor_map_3d_u8(&map_w, weight, (uint64_t)G, (uint64_t)K, (uint64_t)N, 128, 128);
+    if (rc == B200MOE_OK) rc = make_tensor_map_2d(&map_x64, x, 1, (uint64_t)M, (uint64_t)K, fb::kBigBox, 128, true);
+    if (rc == B200MOE_OK) rc = make_tensor_map_2d(&map_x16, x, 1, (uint64_t)M, (uint64_t)K, fb::kSmallBox, 128, true);
+    if (rc != B200MOE_OK) return rc;
+    const unsigned grid = (unsigned)(sm_count() / 2 * 2);
+    const auto kernel = gate_up_silu ? fb::grouped_kernel<true> : fb::grouped_kernel<false>;
+    B200MOE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, fb::kSmemBytes));
     B200MOE_CUDA_TRY(cudaMemsetAsync(workspace, 0, B200MOE_STATUS_BYTES, st));
-    const long long tiles = (M + fb::kRows - 1) / fb::kRows + G;
-    if (tiles > 65535) return B200MOE_ERR_SHAPE;
-    const dim3 grid((unsigned)(gate_up_silu ? N / 256 : a.NB), (unsigned)tiles);
-    if (gate_up_silu) fb::simple_kernel<true><<<grid, 256, 0, st>>>(a);
-    else fb::simple_kernel<false><<<grid, 128, 0, st>>>(a);
+    kernel<<<grid, fb::kThreads, fb::kSmemBytes, st>>>(map_w, map_x64, map_x16, a);
     B200MOE_CUDA_TRY(cudaGetLastError());
-    if (findings) {
-        fb::keep_finding_kernel<<<1, 1, 0, st>>>(a.status, findings);
-        B200MOE_CUDA_TRY(cudaGetLastError());
+    if (a.max_parts > 1) {
+        const int64_t out_n = gate_up_silu ? N / 2 : N;
+        const unsigned blocks = (unsigned)((M * ((out_n + 127) / 128) + 7) / 8);
+        B200MOE_CUDA_TRY(launch_dependent(gate_up_silu ? fb::join_kernel<true> : fb::join_kernel<false>, blocks, 256, 0, st, a));
     }
     return B200MOE_OK;
 }

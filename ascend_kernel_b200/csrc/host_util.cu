@@ -52,6 +52,20 @@ int make_tensor_map_2d(CUtensorMap* out, const void* base, int elem_bytes, uint6
     return r == CUDA_SUCCESS ? B200MOE_OK : B200MOE_ERR_CUDA;
 }
 
+int make_tensor_map_3d_u8(CUtensorMap* out, const void* base, uint64_t outer, uint64_t rows, uint64_t cols, uint32_t box_rows,
+                          uint32_t box_cols) {
+    auto fn = encode_fn();
+    if (fn == nullptr) return B200MOE_ERR_CUDA;
+    cuuint64_t dims[3] = {cols, rows, outer};
+    cuuint64_t strides[2] = {cols, cols * rows};
+    cuuint32_t box[3] = {box_cols, box_rows, 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? B200MOE_OK : B200MOE_ERR_CUDA;
+}
+
 }  // namespace b200moe
 
 extern "C" {
