@@ -37,11 +37,11 @@ constexpr int kThreads = 384;
 constexpr int kWarpLoad = 0, kWarpMma0 = 1, kWarpScale = 3, kWarpEpi0 = 4, kEpiWarps = 8;
 constexpr int kMaxR = 256;             // token rows of a tile
 constexpr int kABytes = 128 * 128;     // a CTA's weights of a stage
-constexpr int kMaxSlots = 12, kMaxBufs = 4, kScaleSlots = 8;
+constexpr int kMaxSlots = 12, kMaxBufs = 8;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kStripBytes = 1024;      // of an epilogue warp
 constexpr int kBigBox = 64, kSmallBox = 16;
-constexpr int kScaleRingBytes = kScaleSlots * kMaxR * 4;
+constexpr int kScaleRingBytes = (int)kTmemCols * 4;  // a row of scales for every accumulator column
 constexpr int kTopWords = kMaxR / 2 * 4;   // gate/up: magnitudes of a tile, [the CTA's tokens][4 warps]
 constexpr int kTopBytes = 2 * kTopWords * 4;  // of two tiles in turn
 constexpr int kBarrierBytes = 2048;
@@ -67,10 +67,10 @@ constexpr int kWordTicket = 2, kWordParts = 8, kWordRows = 9;
 
 struct Sync {
     uint64_t full[kMaxSlots];    // first CTA: the bytes of both CTAs' loads
-    uint64_t empty[kMaxSlots];   // each CTA: one epilogue lane has seen the stage's MMAs complete
-    uint64_t t_full[kMaxBufs];   // each CTA: commit
+    uint64_t empty[kMaxSlots];   // each CTA: commit
+    uint64_t t_full[kMaxBufs];   // each CTA: commit, and the buffer's scales are written
     uint64_t t_empty[kMaxBufs];  // first CTA: the 16 epilogue warps of the pair
-    uint64_t s_full[kScaleSlots], s_empty[kScaleSlots];
+    uint64_t s_empty[kMaxBufs];  // each CTA: its 8 epilogue warps
     uint64_t x_full, x_free;     // gate/up exchange: the other CTA's 8 warps have written here; have read what was sent there
     uint64_t wg[2];              // the four epilogue warps of a group among themselves
     uint64_t drain[2];
@@ -85,48 +85,48 @@ struct Tile {
     int g, row0, rows, n, nt, kb0, kb1, part;  // n: rows rounded up to 32; nt: 256 weight columns (gate/up: 128 of each)
 };
 
-__device__ __forceinline__ bool wait_slow(uint32_t bar, uint32_t parity, Sync* sy, int* status, int id) {
-    volatile int* abort = &sy->abort;
-    const uint64_t t0 = ptx::globaltimer_ns();
-    uint32_t spins = 0;
-    while (!ptx::mbar_try_wait_cluster(bar, parity)) {
-        if ((++spins & 0xFF) == 0) {
-            if (*abort) return false;
-            if (ptx::globaltimer_ns() - t0 > ptx::kWaitLimitNs) {
-                *abort = 1;
-                report_status(status, kDevWaitExpired, id);
-                return false;
-            }
-        }
-    }
-    return true;
+// Waits and tile look-ups of whole warps vote at every poll, so that a warp leaves them together (instructions for the whole warp
+// follow); kWarp false: a single lane.
+template <bool kWarp>
+__device__ __forceinline__ bool all(bool v) {
+    if constexpr (kWarp) return __all_sync(0xffffffffu, v);
+    else return v;
 }
+// Whether a poll that has failed `spins` times gives up: the other roles have, or the time is over.
+template <bool kWarp>
+__device__ __forceinline__ bool give_up(uint32_t spins, uint64_t& t0, Sync* sy, int* status, int id) {
+    if ((spins & 0xFF) != 0) return false;
+    if (spins == 0) {
+        t0 = ptx::globaltimer_ns();
+        return false;
+    }
+    bool out = *reinterpret_cast<volatile int*>(&sy->abort) != 0;
+    if (!out && ptx::globaltimer_ns() - t0 > ptx::kWaitLimitNs) {
+        *reinterpret_cast<volatile int*>(&sy->abort) = 1;
+        report_status(status, kDevWaitExpired, id);
+        out = true;
+    }
+    return !all<kWarp>(!out);
+}
+// kCluster: for what the other CTA of the pair wrote into this one's shared memory
+template <bool kWarp, bool kCluster = false>
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Sync* sy, int* status, int id) {
     const uint32_t b = ptx::smem_u32(bar);
-    if (ptx::mbar_try_wait_cluster(b, parity)) return true;
-    return wait_slow(b, parity, sy, status, id);
+    uint64_t t0 = 0;
+    for (uint32_t spins = 0; !all<kWarp>(kCluster ? ptx::mbar_try_wait_cluster(b, parity) : ptx::mbar_try_wait(b, parity)); ++spins)
+        if (give_up<kWarp>(spins, t0, sy, status, id)) return false;
+    return true;
 }
 
 // The seq-th tile of the pair (seq is advanced); false when the schedule has ended, a wait expired or another role aborted.
+template <bool kWarp>
 __device__ __forceinline__ bool next_tile(Sync* sy, uint32_t& seq, Tile& t, const Args& a, int parts) {
     const TileEntry* e = &sy->ring[seq % kTileRing];
     const uint32_t want = seq + 1;
-    TileEntry v = ring_load(e);
-    if (!tile_entry_is(v, want)) {
-        volatile int* abort = &sy->abort;
-        const uint64_t t0 = ptx::globaltimer_ns();
-        uint32_t spins = 0;
-        while (!tile_entry_is(v = ring_load(e), want)) {
-            if ((++spins & 0xFF) == 0) {
-                if (*abort) return false;
-                if (ptx::globaltimer_ns() - t0 > ptx::kWaitLimitNs) {
-                    *abort = 1;
-                    report_status(a.status, kDevWaitExpired, 90);
-                    return false;
-                }
-            }
-        }
-    }
+    TileEntry v;
+    uint64_t t0 = 0;
+    for (uint32_t spins = 0; !all<kWarp>(tile_entry_is(v = ring_load(e), want)); ++spins)
+        if (give_up<kWarp>(spins, t0, sy, a.status, 90)) return false;
     ++seq;
     t.rows = tile_entry_rows(v);
     if (t.rows == 0) return false;
@@ -175,6 +175,201 @@ __device__ __forceinline__ float silu(float g) {
 // Where the sums of a chunk's 16-lane half lie in the gate/up exchange: [group of warps][chunk][half][thread] pieces of 16 bytes.
 __device__ __forceinline__ uint32_t exchange_at(int wg, int n_ch, int c, int h, int thread) {
     return (uint32_t)((((wg * n_ch + c) * 2 + h) * 128 + thread) * 16);
+}
+
+struct EpilogueState {
+    int warp, parts;
+    uint32_t rank, buf, ph, tiles, n_bufs, width, tmem, t_empty;
+    float* scales;
+    uint8_t *strip, *exchange;
+    float* tops;
+};
+
+// A tile's sums and what becomes of them.  A warp holds 32 weight columns (tensor-memory lanes) x half of the tile's tokens, NCH chunks
+// of 16: acc[chunk][16 lanes][8 tokens][8 lanes], two tokens to a register pair.  The number of chunks is a constant: a warp passes
+// here once a block of 128 k, and its instructions are what a block costs (with a test at every chunk, 130 for one chunk: 1000 cycles).
+template <bool GATE_UP, int NCH>
+__device__ __forceinline__ bool finish_tile(const Tile& t, EpilogueState& e, Sync* sy, const Args& a) {
+    const uint32_t rank = e.rank;
+    const int lane = threadIdx.x & 31, wg = e.warp >> 2, quarter = e.warp & 3, g8 = lane >> 2, q = lane & 3, first = wg * (NCH * 16);
+    bool ok = true;
+    f32x2 acc[NCH][2][2][2];
+#pragma unroll
+    for (int c = 0; c < NCH; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[c][i >> 2][(i >> 1) & 1][i & 1] = 0ull;
+    for (int kb = t.kb0; kb < t.kb1; ++kb) {
+        if (!wait<true>(&sy->t_full[e.buf], e.ph, sy, a.status, 50)) return false;
+        ptx::tc_fence_after();
+        const float4* sv = reinterpret_cast<const float4*>(e.scales + e.buf * e.width + first) + q;
+        const uint32_t td = e.tmem + e.buf * e.width + (uint32_t)first;
+        constexpr int kSet = NCH <= 4 ? 2 : 1;  // chunks that are fetched together while the set before is added
+        uint32_t v[2][kSet][2][8];
+        const auto fetch = [&](int c0, uint32_t(&d)[kSet][2][8]) {
+#pragma unroll
+            for (int c = 0; c < kSet; ++c)
+                if (c0 + c < NCH) {
+                    ptx::tmem_ld_16x16(td + (uint32_t)((c0 + c) * 16), d[c][0]);
+                    ptx::tmem_ld_16x16(td + (uint32_t)((c0 + c) * 16) + (16u << 16), d[c][1]);
+                }
+        };
+        fetch(0, v[0]);
+#pragma unroll
+        for (int c0 = 0; c0 < NCH; c0 += kSet) {
+            ptx::tmem_ld_wait();
+            if (c0 + kSet < NCH) {
+                fetch(c0 + kSet, v[(c0 / kSet + 1) & 1]);
+            } else {
+                // all is in registers: the buffer goes back
+                ptx::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive_remote(e.t_empty + e.buf * 8);
+            }
+#pragma unroll
+            for (int c = 0; c < kSet; ++c)
+                if (c0 + c < NCH) {
+                    const float4 s4 = sv[(c0 + c) * 4];
+                    const f32x2 s2[2] = {pack_f32x2(s4.x, s4.y), pack_f32x2(s4.z, s4.w)};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const uint32_t(&d)[8] = v[(c0 / kSet) & 1][c][h];
+                                acc[c0 + c][h][j][i] = fma_f32x2(pack_u32x2(d[4 * j + 2 * i], d[4 * j + 2 * i + 1]), s2[j], acc[c0 + c][h][j][i]);
+                            }
+                }
+        }
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->s_empty[e.buf]));
+        if (++e.buf == e.n_bufs) { e.buf = 0; e.ph ^= 1; }
+    }
+
+    if (e.parts > 1) {
+        // a part's sums as they are, [part][row][column]
+        const int col0 = (GATE_UP ? (int)rank * (a.N >> 1) + t.nt * 128 : t.nt * 256 + (int)rank * 128) + quarter * 32 + g8;
+        float* dst = a.parts + ((size_t)t.part * a.M + t.row0) * a.N;
+#pragma unroll
+        for (int c = 0; c < NCH; ++c)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int token = first + c * 16 + j * 8 + 2 * q, col = col0 + h * 16 + i * 8;
+                        if (col < a.N) {
+                            if (token < t.rows) dst[(size_t)token * a.N + col] = f32x2_lo(acc[c][h][j][i]);
+                            if (token + 1 < t.rows) dst[(size_t)(token + 1) * a.N + col] = f32x2_hi(acc[c][h][j][i]);
+                        }
+                    }
+    } else if constexpr (!GATE_UP) {
+        // 16 tokens x 32 columns at a time through the warp's strip: the transposing store gives 16-byte pieces of
+        // eight columns, 64 contiguous bytes of a row
+        const int col = t.nt * 256 + (int)rank * 128 + quarter * 32 + q * 8;
+        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (size_t)t.row0 * a.N + col;
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    uint32_t o[4];
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) o[m] = pack_bf16x2(f32x2_lo(acc[c][m >> 1][j][m & 1]), f32x2_hi(acc[c][m >> 1][j][m & 1]));
+                    // row lane % 8 (a token), piece lane / 8
+                    const int token = j * 8 + (lane & 7);
+                    ptx::stmatrix_x4_trans(ptx::smem_u32(e.strip) + (uint32_t)(token * 64 + (((lane >> 3) ^ (token >> 1)) & 3) * 16), o[0], o[1], o[2], o[3]);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int token = j * 8 + g8, row = first + c * 16 + token;
+                    const uint4 o = *reinterpret_cast<const uint4*>(e.strip + token * 64 + ((q ^ (token >> 1)) & 3) * 16);
+                    if (row < t.rows && col < a.N) *reinterpret_cast<uint4*>(dst + (size_t)row * a.N) = o;
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        // this CTA finishes the tokens of group j = rank of every chunk; the other group's sums go to the other CTA
+        const int thread = quarter * 32 + lane;
+        const uint32_t there = ptx::map_rank(ptx::smem_u32(e.exchange), rank ^ 1);
+        if (e.tiles > 0) ok = wait<true, true>(&sy->x_free, (e.tiles - 1) & 1, sy, a.status, 60);
+        if (!ok) return false;
+#pragma unroll
+        for (int c = 0; c < NCH; ++c)
+            {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const f32x2 s0 = rank == 0 ? acc[c][h][1][0] : acc[c][h][0][0], s1 = rank == 0 ? acc[c][h][1][1] : acc[c][h][0][1];
+                    ptx::st_cluster_v4(there + exchange_at(wg, NCH, c, h, thread), (uint32_t)s0, (uint32_t)(s0 >> 32), (uint32_t)s1, (uint32_t)(s1 >> 32));
+                }
+            }
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_rank(ptx::smem_u32(&sy->x_full), rank ^ 1));
+        ok = wait<true, true>(&sy->x_full, e.tiles & 1, sy, a.status, 61);
+        if (!ok) return false;
+        float* top = e.tops + (e.tiles & 1) * kTopWords;
+        float h8[NCH][8];  // [chunk][2 * m + b]: column 8 m + g8, token 2 q + b
+#pragma unroll
+        for (int c = 0; c < NCH; ++c)
+            {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint4 o = *reinterpret_cast<const uint4*>(e.exchange + exchange_at(wg, NCH, c, h, thread));
+                    const f32x2 k0 = rank == 0 ? acc[c][h][0][0] : acc[c][h][1][0], k1 = rank == 0 ? acc[c][h][0][1] : acc[c][h][1][1];
+                    const float own[4] = {f32x2_lo(k0), f32x2_hi(k0), f32x2_lo(k1), f32x2_hi(k1)};
+                    const float other[4] = {__uint_as_float(o.x), __uint_as_float(o.y), __uint_as_float(o.z), __uint_as_float(o.w)};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        h8[c][h * 4 + i] = silu(rank == 0 ? own[i] : other[i]) * (rank == 0 ? other[i] : own[i]);
+                }
+                // the largest magnitude over the warp's 32 columns (magnitudes order as their bits do, infinities and NaN last)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    uint32_t m = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(h8[c][2 * i + b]) & 0x7FFFFFFFu);
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                    if (g8 == 0) top[(wg * 64 + c * 8 + 2 * q + b) * 4 + quarter] = __uint_as_float(m);
+                }
+            }
+        __syncwarp();
+        if (lane == 0) {
+            ptx::mbar_arrive_cluster(ptx::map_rank(ptx::smem_u32(&sy->x_free), rank ^ 1));  // what was sent here has been read
+            ptx::mbar_arrive(ptx::smem_u32(&sy->wg[wg]));
+        }
+        ok = wait<true>(&sy->wg[wg], e.tiles & 1, sy, a.status, 62);
+        if (!ok) return false;
+        const int inter = a.N >> 1;
+        uint8_t* dst = static_cast<uint8_t*>(a.out) + (size_t)t.row0 * inter + t.nt * 128 + quarter * 32 + (lane & 1) * 16;
+#pragma unroll
+        for (int c = 0; c < NCH; ++c)
+            {
+                const int token0 = first + c * 16 + (int)rank * 8;
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const uint4 m4 = *reinterpret_cast<const uint4*>(top + (wg * 64 + c * 8 + 2 * q + b) * 4);
+                    const fp8_block::Quantizer qz(__uint_as_float(max(max(m4.x, m4.y), max(m4.z, m4.w))));
+                    const uint32_t o = qz.four(h8[c][b], h8[c][2 + b], h8[c][4 + b], h8[c][6 + b]);
+                    uint8_t* at = e.strip + (2 * q + b) * 32 + g8;
+                    at[0] = (uint8_t)o;
+                    at[8] = (uint8_t)(o >> 8);
+                    at[16] = (uint8_t)(o >> 16);
+                    at[24] = (uint8_t)(o >> 24);
+                    const int token = token0 + 2 * q + b;
+                    if (quarter == 0 && g8 == 0 && token < t.rows) a.out_scale[(size_t)(t.row0 + token) * (inter >> 7) + t.nt] = qz.scale;
+                }
+                __syncwarp();
+                const int token = token0 + (lane >> 1);
+                if (lane < 16 && token < t.rows)
+                    *reinterpret_cast<uint4*>(dst + (size_t)token * inter) = *reinterpret_cast<const uint4*>(e.strip + lane * 16);
+                __syncwarp();
+            }
+    }
+    return true;
 }
 
 template <bool GATE_UP>
@@ -232,10 +427,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         };
         init(sy->full, kMaxSlots, 1);
         init(sy->empty, kMaxSlots, 1);
-        init(sy->t_full, kMaxBufs, 1);
+        init(sy->t_full, kMaxBufs, 2);
         init(sy->t_empty, kMaxBufs, 2 * kEpiWarps);
-        init(sy->s_full, kScaleSlots, 1);
-        init(sy->s_empty, kScaleSlots, kEpiWarps);
+        init(sy->s_empty, kMaxBufs, kEpiWarps);
         init(&sy->x_full, 1, kEpiWarps);
         init(&sy->x_free, 1, kEpiWarps);
         init(sy->wg, 2, 4);
@@ -287,13 +481,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 Tile t;
                 while (ok) {
                     publish();  // (a tile ahead: the other roles find it there)
-                    if (!next_tile(sy, seq, t, a, parts)) break;
+                    if (!next_tile<false>(sy, seq, t, a, parts)) break;
                     const int half = t.n >> 1, n_big = half / kBigBox, n_small = (half % kBigBox) / kSmallBox;
                     const uint32_t bytes = 2u * (uint32_t)(kABytes + half * 128);
                     const int col = GATE_UP ? (int)rank * (a.N >> 1) + t.nt * 128 : t.nt * 256 + (int)rank * 128;
                     const int row = t.row0 + (int)rank * half;
                     for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
-                        if (it >= (uint32_t)n_slots && !wait(&sy->empty[slot], ph ^ 1, sy, a.status, 10)) { ok = false; break; }
+                        if (it >= (uint32_t)n_slots && !wait<false>(&sy->empty[slot], ph ^ 1, sy, a.status, 10)) { ok = false; break; }
                         const uint32_t bar = ptx::smem_u32(&sy->full[slot]), bar0 = ptx::map_rank(bar, 0);
                         const uint32_t dst = ptx::smem_u32(ring) + slot * (uint32_t)slot_bytes;
                         if (rank == 0) ptx::mbar_arrive_expect_tx(bar, bytes);
@@ -323,35 +517,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             // ------------------------------ scales ------------------------------
             // Row scale times the tile's weight scale, in the order in which the epilogue's lanes take them: 16 tokens are four
             // pieces of 16 bytes, piece q the tokens 2q, 2q + 1, 8 + 2q, 9 + 2q.
-            uint32_t seq = 0, it = 0;
-            const int home = (lane & 16) + ((lane & 7) >> 1) * 4 + ((lane >> 3) & 1) * 2 + (lane & 1);
+            uint32_t seq = 0, it = 0, buf = 0, ph = 0;
+            float* home = scales + (lane & 16) + ((lane & 7) >> 1) * 4 + ((lane >> 3) & 1) * 2 + (lane & 1);
             bool ok = true;
             Tile t;
-            while (ok && next_tile(sy, seq, t, a, parts)) {
+            while (ok && next_tile<true>(sy, seq, t, a, parts)) {
                 const int nb = min(a.NB - 1, GATE_UP ? (int)rank * (a.N >> 8) + t.nt : t.nt * 2 + (int)rank);
                 const float* ws = a.w_scale + (size_t)t.g * a.KB * a.NB + nb;
                 const float* xs = a.x_scale + (size_t)(t.row0 + lane) * a.KB;
-                for (int kb = t.kb0; kb < t.kb1 && ok; kb += 4) {
+                const size_t group = (size_t)a.KB * 32;
+                for (int kb = t.kb0; kb < t.kb1 && ok; kb += 4) {  // (four blocks' loads in flight)
                     float w[4], v[8][4];
+                    const int last = t.kb1 - 1 - kb;
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) w[b] = kb + b < t.kb1 ? __ldg(ws + (size_t)(kb + b) * a.NB) : 0.f;
+                    for (int b = 0; b < 4; ++b) w[b] = __ldg(ws + (size_t)(kb + min(b, last)) * a.NB);
 #pragma unroll
                     for (int g = 0; g < 8; ++g)
+                        if (g * 32 < t.n) {
+                            const bool row = g * 32 + lane < t.rows;
 #pragma unroll
-                        for (int b = 0; b < 4; ++b)
-                            v[g][b] = g * 32 + lane < t.rows && kb + b < t.kb1 ? __ldg(xs + (size_t)(g * 32) * a.KB + kb + b) : 0.f;
+                            for (int b = 0; b < 4; ++b) v[g][b] = row ? __ldg(xs + g * group + kb + min(b, last)) : 0.f;
+                        }
 #pragma unroll
                     for (int b = 0; b < 4; ++b) {
-                        if (kb + b >= t.kb1 || !ok) break;
-                        const uint32_t s = it % kScaleSlots;
-                        if (it >= kScaleSlots) ok = __all_sync(0xffffffffu, wait(&sy->s_empty[s], ((it / kScaleSlots) & 1) ^ 1, sy, a.status, 20));
+                        if (b > last || !ok) break;
+                        if (it >= (uint32_t)n_bufs) ok = wait<true>(&sy->s_empty[buf], ph ^ 1, sy, a.status, 20);
                         if (!ok) break;
+                        float* dst = home + buf * (uint32_t)width;
 #pragma unroll
                         for (int g = 0; g < 8; ++g)
-                            if (g * 32 < t.n) scales[s * kMaxR + g * 32 + home] = v[g][b] * w[b];
+                            if (g * 32 < t.n) dst[g * 32] = v[g][b] * w[b];
                         __syncwarp();
-                        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->s_full[s]));
+                        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->t_full[buf]));
                         ++it;
+                        if (++buf == (uint32_t)n_bufs) { buf = 0; ph ^= 1; }
                     }
                 }
             }
@@ -365,13 +564,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const uint64_t da0 = ptx::umma_desc_sw128(ptx::smem_u32(ring), kABytes, 1024);
             const uint64_t db0 = ptx::umma_desc_sw128(ptx::smem_u32(ring) + kABytes, 0, 1024);
             Tile t;
-            while (ok && next_tile(sy, seq, t, a, parts)) {
+            while (ok && next_tile<true>(sy, seq, t, a, parts)) {
                 const uint32_t idesc = ptx::umma_idesc_e4m3_mn_k(256, t.n);
                 for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
                     if ((it & 1) == turn) {
                         // the epilogue of both CTAs has taken what the buffer held
-                        if (it >= (uint32_t)n_bufs && !wait(&sy->t_empty[buf], tph ^ 1, sy, a.status, 30)) { ok = false; break; }
-                        if (!wait(&sy->full[slot], ph, sy, a.status, 40)) { ok = false; break; }
+                        if (it >= (uint32_t)n_bufs && !wait<true>(&sy->t_empty[buf], tph ^ 1, sy, a.status, 30)) { ok = false; break; }
+                        if (!wait<true>(&sy->full[slot], ph, sy, a.status, 40)) { ok = false; break; }
                         ptx::tc_fence_after();
                         if (leader) {
                             const uint64_t at = (uint64_t)(slot * (uint32_t)slot_bytes >> 4);
@@ -380,6 +579,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                 ptx::umma_f8_pair(tmem_base + buf * (uint32_t)width, da0 + at + (uint64_t)(k32 * 256),
                                                   db0 + at + (uint64_t)(k32 * 2), idesc, (uint32_t)(k32 != 0));
                             ptx::umma_commit_pair(ptx::smem_u32(&sy->t_full[buf]));
+                            ptx::umma_commit_pair(ptx::smem_u32(&sy->empty[slot]));
                         }
                         __syncwarp();
                     }
@@ -397,194 +597,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         // ------------------------------ epilogue ------------------------------
-        // A warp holds 32 weight columns (tensor-memory lanes) x half of the tile's tokens: acc[chunk of 16 tokens][16 lanes][8 tokens]
-        // [8 lanes], two tokens to a register pair.
-        const int ew = warp - kWarpEpi0, wg = ew >> 2, quarter = warp & 3, g8 = lane >> 2, q = lane & 3;
-        uint8_t* strip = strips + ew * kStripBytes;
-        const uint32_t strip_u32 = ptx::smem_u32(strip);
-        const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-        uint32_t seq = 0, slot = 0, buf = 0, tph = 0, sc = 0, sph = 0, tiles = 0;
+        EpilogueState e;
+        e.warp = warp - kWarpEpi0;
+        e.rank = rank;
+        e.buf = e.ph = e.tiles = 0;
+        e.n_bufs = (uint32_t)n_bufs;
+        e.width = (uint32_t)width;
+        e.parts = parts;
+        e.tmem = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+        e.t_empty = ptx::map_rank(ptx::smem_u32(sy->t_empty), 0);
+        e.scales = scales;
+        e.strip = strips + e.warp * kStripBytes;
+        e.exchange = exchange;
+        e.tops = tops;
+        uint32_t seq = 0;
         bool ok = true;
         Tile t;
-        while (ok && next_tile(sy, seq, t, a, parts)) {
-            const int half = t.n >> 1, n_ch = half >> 4, first = wg * half;
-            f32x2 acc[8][2][2][2];
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) acc[c][i >> 2][(i >> 1) & 1][i & 1] = 0ull;
-            for (int kb = t.kb0; kb < t.kb1; ++kb) {
-                ok = wait(&sy->s_full[sc], sph, sy, a.status, 50) && wait(&sy->t_full[buf], tph, sy, a.status, 51);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                ptx::tc_fence_after();
-                // the block's MMAs have completed: its stage may be loaded again
-                if (ew == 0 && lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->empty[slot]));
-                const float4* sv = reinterpret_cast<const float4*>(scales + sc * kMaxR + first) + q;
-                const uint32_t td = tmem_base + lane_base + buf * (uint32_t)width + (uint32_t)first;
-#pragma unroll
-                for (int c0 = 0; c0 < 8; c0 += 2) {
-                    if (c0 < n_ch) {
-                        uint32_t v[2][2][8];
-#pragma unroll
-                        for (int c = 0; c < 2; ++c)
-                            if (c0 + c < n_ch) {
-                                ptx::tmem_ld_16x16(td + (uint32_t)((c0 + c) * 16), v[c][0]);
-                                ptx::tmem_ld_16x16(td + (uint32_t)((c0 + c) * 16) + (16u << 16), v[c][1]);
-                            }
-                        ptx::tmem_ld_wait();
-#pragma unroll
-                        for (int c = 0; c < 2; ++c)
-                            if (c0 + c < n_ch) {
-                                const float4 s4 = sv[(c0 + c) * 4];
-                                const f32x2 s2[2] = {pack_f32x2(s4.x, s4.y), pack_f32x2(s4.z, s4.w)};
-#pragma unroll
-                                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                                    for (int j = 0; j < 2; ++j)
-#pragma unroll
-                                        for (int i = 0; i < 2; ++i)
-                                            acc[c0 + c][h][j][i] = fma_f32x2(pack_u32x2(v[c][h][4 * j + 2 * i], v[c][h][4 * j + 2 * i + 1]),
-                                                                             s2[j], acc[c0 + c][h][j][i]);
-                            }
-                    }
-                }
-                ptx::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    ptx::mbar_arrive_cluster(ptx::map_rank(ptx::smem_u32(&sy->t_empty[buf]), 0));
-                    ptx::mbar_arrive(ptx::smem_u32(&sy->s_empty[sc]));
-                }
-                if (++slot == (uint32_t)n_slots) slot = 0;
-                if (++buf == (uint32_t)n_bufs) { buf = 0; tph ^= 1; }
-                if (++sc == kScaleSlots) { sc = 0; sph ^= 1; }
+        while (ok && next_tile<true>(sy, seq, t, a, parts)) {
+            switch (t.n >> 5) {  // chunks of 16 tokens a warp has
+                case 1: ok = finish_tile<GATE_UP, 1>(t, e, sy, a); break;
+                case 2: ok = finish_tile<GATE_UP, 2>(t, e, sy, a); break;
+                case 3: ok = finish_tile<GATE_UP, 3>(t, e, sy, a); break;
+                case 4: ok = finish_tile<GATE_UP, 4>(t, e, sy, a); break;
+                case 5: ok = finish_tile<GATE_UP, 5>(t, e, sy, a); break;
+                case 6: ok = finish_tile<GATE_UP, 6>(t, e, sy, a); break;
+                case 7: ok = finish_tile<GATE_UP, 7>(t, e, sy, a); break;
+                default: ok = finish_tile<GATE_UP, 8>(t, e, sy, a); break;
             }
-            if (!ok) break;
-
-            if (parts > 1) {
-                // a part's sums as they are, [part][row][column]
-                const int col0 = (GATE_UP ? (int)rank * (a.N >> 1) + t.nt * 128 : t.nt * 256 + (int)rank * 128) + quarter * 32 + g8;
-                float* dst = a.parts + ((size_t)t.part * a.M + t.row0) * a.N;
-#pragma unroll
-                for (int c = 0; c < 8; ++c)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j)
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const int token = first + c * 16 + j * 8 + 2 * q, col = col0 + h * 16 + i * 8;
-                                if (c < n_ch && col < a.N) {
-                                    if (token < t.rows) dst[(size_t)token * a.N + col] = f32x2_lo(acc[c][h][j][i]);
-                                    if (token + 1 < t.rows) dst[(size_t)(token + 1) * a.N + col] = f32x2_hi(acc[c][h][j][i]);
-                                }
-                            }
-            } else if constexpr (!GATE_UP) {
-                // 16 tokens x 32 columns at a time through the warp's strip: the transposing store gives 16-byte pieces of
-                // eight columns, 64 contiguous bytes of a row
-                const int col = t.nt * 256 + (int)rank * 128 + quarter * 32 + q * 8;
-                __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (size_t)t.row0 * a.N + col;
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    if (c < n_ch) {
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            uint32_t o[4];
-#pragma unroll
-                            for (int m = 0; m < 4; ++m) o[m] = pack_bf16x2(f32x2_lo(acc[c][m >> 1][j][m & 1]), f32x2_hi(acc[c][m >> 1][j][m & 1]));
-                            // row lane % 8 (a token), piece lane / 8
-                            const int token = j * 8 + (lane & 7);
-                            ptx::stmatrix_x4_trans(strip_u32 + (uint32_t)(token * 64 + (((lane >> 3) ^ (token >> 1)) & 3) * 16), o[0], o[1], o[2], o[3]);
-                        }
-                        __syncwarp();
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const int token = j * 8 + g8, row = first + c * 16 + token;
-                            const uint4 o = *reinterpret_cast<const uint4*>(strip + token * 64 + ((q ^ (token >> 1)) & 3) * 16);
-                            if (row < t.rows && col < a.N) *reinterpret_cast<uint4*>(dst + (size_t)row * a.N) = o;
-                        }
-                        __syncwarp();
-                    }
-                }
-            } else {
-                // this CTA finishes the tokens of group j = rank of every chunk; the other group's sums go to the other CTA
-                const int thread = quarter * 32 + lane;
-                const uint32_t there = ptx::map_rank(ptx::smem_u32(exchange), rank ^ 1);
-                if (tiles > 0) ok = __all_sync(0xffffffffu, wait(&sy->x_free, (tiles - 1) & 1, sy, a.status, 60));
-                if (!ok) break;
-#pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    if (c < n_ch) {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const f32x2 s0 = rank == 0 ? acc[c][h][1][0] : acc[c][h][0][0], s1 = rank == 0 ? acc[c][h][1][1] : acc[c][h][0][1];
-                            ptx::st_cluster_v4(there + exchange_at(wg, n_ch, c, h, thread), (uint32_t)s0, (uint32_t)(s0 >> 32), (uint32_t)s1, (uint32_t)(s1 >> 32));
-                        }
-                    }
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_rank(ptx::smem_u32(&sy->x_full), rank ^ 1));
-                ok = __all_sync(0xffffffffu, wait(&sy->x_full, tiles & 1, sy, a.status, 61));
-                if (!ok) break;
-                float* top = tops + (tiles & 1) * kTopWords;
-                float h8[8][8];  // [chunk][2 * m + b]: column 8 m + g8, token 2 q + b
-#pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    if (c < n_ch) {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const uint4 o = *reinterpret_cast<const uint4*>(exchange + exchange_at(wg, n_ch, c, h, thread));
-                            const f32x2 k0 = rank == 0 ? acc[c][h][0][0] : acc[c][h][1][0], k1 = rank == 0 ? acc[c][h][0][1] : acc[c][h][1][1];
-                            const float own[4] = {f32x2_lo(k0), f32x2_hi(k0), f32x2_lo(k1), f32x2_hi(k1)};
-                            const float other[4] = {__uint_as_float(o.x), __uint_as_float(o.y), __uint_as_float(o.z), __uint_as_float(o.w)};
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                h8[c][h * 4 + i] = silu(rank == 0 ? own[i] : other[i]) * (rank == 0 ? other[i] : own[i]);
-                        }
-                        // the largest magnitude over the warp's 32 columns (magnitudes order as their bits do, infinities and NaN last)
-#pragma unroll
-                        for (int b = 0; b < 2; ++b) {
-                            uint32_t m = 0;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(h8[c][2 * i + b]) & 0x7FFFFFFFu);
-#pragma unroll
-                            for (int o = 4; o < 32; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-                            if (g8 == 0) top[(wg * 64 + c * 8 + 2 * q + b) * 4 + quarter] = __uint_as_float(m);
-                        }
-                    }
-                __syncwarp();
-                if (lane == 0) {
-                    ptx::mbar_arrive_cluster(ptx::map_rank(ptx::smem_u32(&sy->x_free), rank ^ 1));  // what was sent here has been read
-                    ptx::mbar_arrive(ptx::smem_u32(&sy->wg[wg]));
-                }
-                ok = __all_sync(0xffffffffu, wait(&sy->wg[wg], tiles & 1, sy, a.status, 62));
-                if (!ok) break;
-                const int inter = a.N >> 1;
-                uint8_t* dst = static_cast<uint8_t*>(a.out) + (size_t)t.row0 * inter + t.nt * 128 + quarter * 32 + (lane & 1) * 16;
-#pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    if (c < n_ch) {
-                        const int token0 = first + c * 16 + (int)rank * 8;
-#pragma unroll
-                        for (int b = 0; b < 2; ++b) {
-                            const uint4 m4 = *reinterpret_cast<const uint4*>(top + (wg * 64 + c * 8 + 2 * q + b) * 4);
-                            const fp8_block::Quantizer qz(__uint_as_float(max(max(m4.x, m4.y), max(m4.z, m4.w))));
-                            const uint32_t o = qz.four(h8[c][b], h8[c][2 + b], h8[c][4 + b], h8[c][6 + b]);
-                            uint8_t* at = strip + (2 * q + b) * 32 + g8;
-                            at[0] = (uint8_t)o;
-                            at[8] = (uint8_t)(o >> 8);
-                            at[16] = (uint8_t)(o >> 16);
-                            at[24] = (uint8_t)(o >> 24);
-                            const int token = token0 + 2 * q + b;
-                            if (quarter == 0 && g8 == 0 && token < t.rows) a.out_scale[(size_t)(t.row0 + token) * (inter >> 7) + t.nt] = qz.scale;
-                        }
-                        __syncwarp();
-                        const int token = token0 + (lane >> 1);
-                        if (lane < 16 && token < t.rows)
-                            *reinterpret_cast<uint4*>(dst + (size_t)token * inter) = *reinterpret_cast<const uint4*>(strip + lane * 16);
-                        __syncwarp();
-                    }
-            }
-            ++tiles;
+            ++e.tiles;
         }
     }
 
