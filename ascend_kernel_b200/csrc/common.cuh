@@ -29,6 +29,11 @@ __device__ __forceinline__ void report_status(int* status, int code, int detail)
     if (atomicCAS(status + 4, 0, code) == 0) status[5] = detail;
 }
 
+// The same in a pair of words of its own (code, detail) that keep the first finding until the caller zeroes them; may be NULL.
+__device__ __forceinline__ void keep_finding(int* findings, int code, int detail) {
+    if (findings != nullptr && atomicCAS(findings, 0, code) == 0) findings[1] = detail;
+}
+
 // Largest expert count the kernels keep in shared memory.
 constexpr int kMaxExperts = 1024;
 
@@ -234,7 +239,7 @@ __device__ __forceinline__ void lane_experts(int G, int& lo, int& hi) {
 // experts: with one thread walking the 256 entries, the GEMV of one token (8 rows, 7168 x 4096, fp8) took
 // 152 us instead of 110 and that of 37 tokens (2048 x 7168, fp4) 475 instead of 429.
 __device__ __forceinline__ void load_row_starts(const int64_t* __restrict__ gl, int G, int M, int gl_type,
-                                                int* row_start, int* status) {
+                                                int* row_start, int* status, int* findings = nullptr) {
     for (int g = threadIdx.x; g < G; g += blockDim.x) {
         const long long v = gl[g];
         row_start[g + 1] = (int)(v < -1 ? -1 : (v > (long long)M + 1 ? (long long)M + 1 : v));
@@ -276,6 +281,7 @@ __device__ __forceinline__ void load_row_starts(const int64_t* __restrict__ gl, 
         if (lane == 0 && bad_at < G) {
             grid_dep_wait();  // the kernel before this one may still have to zero the status words
             report_status(status, kDevBadGroupList, bad_at);
+            keep_finding(findings, kDevBadGroupList, bad_at);
         }
     }
     __syncthreads();

@@ -5,12 +5,12 @@
 // x e4m3 [M, K] with fp32 scales per row and 128 k, weights e4m3 [G, K, N] with fp32 scales per 128 x 128.
 //
 // Persistent kernel on pairs of CTAs.  The operands are swapped: the 256 lanes of a pair's MMA (tcgen05 kind::f8f6f4, M = 256) are
-// weight columns, 128 to a CTA, and its N extent is the tile's token rows rounded up to 32 (32 .. 256), so an expert with 130 rows costs
+// weight columns, 128 to a CTA, and its N extent is the tile's token rows rounded up to 32 (32 .. 160), so an expert with 130 rows costs
 // 160 columns, and a decode step's few rows cost 32.  The weights enter as they are stored: a TMA box of 128 k x 128 columns is
 // the MN-major A operand.  The rows of x are split between the two CTAs' shared memory and read by both.
 //
 // An arbitrary fp32 scale cannot ride in the MMA, so a block of 128 k is a sum of its own: the MMA warps write it to one
-// of 2 .. 4 tensor-memory buffers, and the epilogue warps add it, times scale, to the tile's sums in their registers (one fused
+// of the 2 .. 8 tensor-memory buffers that fit, and the epilogue warps add it, times scale, to the tile's sums in their registers (one fused
 // multiply-add per two elements; a lane's 4 weight columns x 2 tokens of each 8 x 8 patch need one 16-byte read of scales per 16 tokens).
 // Blocks being independent, two warps issue them in turn: a block's MMAs last about as many cycles as it has token rows, fewer
 // than the waits, four issues and the commit cost one warp.
@@ -35,7 +35,7 @@ namespace fb {
 
 constexpr int kThreads = 384;
 constexpr int kWarpLoad = 0, kWarpMma0 = 1, kWarpScale = 3, kWarpEpi0 = 4, kEpiWarps = 8;
-constexpr int kMaxR = 256;             // token rows of a tile
+constexpr int kMaxR = 160;             // token rows of a tile
 constexpr int kABytes = 128 * 128;     // a CTA's weights of a stage
 constexpr int kMaxSlots = 12, kMaxBufs = 8;
 constexpr uint32_t kTmemCols = 512;
@@ -59,18 +59,18 @@ struct Args {
     float* parts;      // [max_parts][M][N], or NULL
     int max_parts;
     int M, K, N, G, gl_type, KB, NB;
-    int* status;
+    int dynamic;       // whether the pairs draw their units (from the ticket) or take every n-th
+    int* words;        // the workspace's first: kWord*
     int* findings;
 };
-// words of the workspace's first 256 bytes behind the status words
-constexpr int kWordTicket = 2, kWordParts = 8, kWordRows = 9;
+constexpr int kWordTicket = 0, kWordParts = 1, kWordRows = 2, kWordBytes = 256;
 
 struct Sync {
     uint64_t full[kMaxSlots];    // first CTA: the bytes of both CTAs' loads
     uint64_t empty[kMaxSlots];   // each CTA: commit
     uint64_t t_full[kMaxBufs];   // each CTA: commit, and the buffer's scales are written
-    uint64_t t_empty[kMaxBufs];  // first CTA: the 16 epilogue warps of the pair
-    uint64_t s_empty[kMaxBufs];  // each CTA: its 8 epilogue warps
+    uint64_t t_empty[kMaxBufs];  // first CTA: the 16 epilogue warps of the pair have the buffer's sums
+    uint64_t s_empty[kMaxBufs];  // each CTA: its 8 epilogue warps have done with the buffer's scales
     uint64_t x_full, x_free;     // gate/up exchange: the other CTA's 8 warps have written here; have read what was sent there
     uint64_t wg[2];              // the four epilogue warps of a group among themselves
     uint64_t drain[2];
@@ -94,7 +94,7 @@ __device__ __forceinline__ bool all(bool v) {
 }
 // Whether a poll that has failed `spins` times gives up: the other roles have, or the time is over.
 template <bool kWarp>
-__device__ __forceinline__ bool give_up(uint32_t spins, uint64_t& t0, Sync* sy, int* status, int id) {
+__device__ __forceinline__ bool give_up(uint32_t spins, uint64_t& t0, Sync* sy, int* findings, int id) {
     if ((spins & 0xFF) != 0) return false;
     if (spins == 0) {
         t0 = ptx::globaltimer_ns();
@@ -103,18 +103,18 @@ __device__ __forceinline__ bool give_up(uint32_t spins, uint64_t& t0, Sync* sy, 
     bool out = *reinterpret_cast<volatile int*>(&sy->abort) != 0;
     if (!out && ptx::globaltimer_ns() - t0 > ptx::kWaitLimitNs) {
         *reinterpret_cast<volatile int*>(&sy->abort) = 1;
-        report_status(status, kDevWaitExpired, id);
+        keep_finding(findings, kDevWaitExpired, id);
         out = true;
     }
     return !all<kWarp>(!out);
 }
 // kCluster: for what the other CTA of the pair wrote into this one's shared memory
 template <bool kWarp, bool kCluster = false>
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Sync* sy, int* status, int id) {
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Sync* sy, int* findings, int id) {
     const uint32_t b = ptx::smem_u32(bar);
     uint64_t t0 = 0;
     for (uint32_t spins = 0; !all<kWarp>(kCluster ? ptx::mbar_try_wait_cluster(b, parity) : ptx::mbar_try_wait(b, parity)); ++spins)
-        if (give_up<kWarp>(spins, t0, sy, status, id)) return false;
+        if (give_up<kWarp>(spins, t0, sy, findings, id)) return false;
     return true;
 }
 
@@ -126,7 +126,7 @@ __device__ __forceinline__ bool next_tile(Sync* sy, uint32_t& seq, Tile& t, cons
     TileEntry v;
     uint64_t t0 = 0;
     for (uint32_t spins = 0; !all<kWarp>(tile_entry_is(v = ring_load(e), want)); ++spins)
-        if (give_up<kWarp>(spins, t0, sy, a.status, 90)) return false;
+        if (give_up<kWarp>(spins, t0, sy, a.findings, 90)) return false;
     ++seq;
     t.rows = tile_entry_rows(v);
     if (t.rows == 0) return false;
@@ -199,10 +199,11 @@ __device__ __forceinline__ bool finish_tile(const Tile& t, EpilogueState& e, Syn
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[c][i >> 2][(i >> 1) & 1][i & 1] = 0ull;
     for (int kb = t.kb0; kb < t.kb1; ++kb) {
-        if (!wait<true>(&sy->t_full[e.buf], e.ph, sy, a.status, 50)) return false;
+        const uint32_t column = e.buf * e.width + (uint32_t)first;
+        const float4* sv = reinterpret_cast<const float4*>(e.scales + column) + q;
+        const uint32_t td = e.tmem + column;
+        if (!wait<true>(&sy->t_full[e.buf], e.ph, sy, a.findings, 50)) return false;
         ptx::tc_fence_after();
-        const float4* sv = reinterpret_cast<const float4*>(e.scales + e.buf * e.width + first) + q;
-        const uint32_t td = e.tmem + e.buf * e.width + (uint32_t)first;
         constexpr int kSet = NCH <= 4 ? 2 : 1;  // chunks that are fetched together while the set before is added
         uint32_t v[2][kSet][2][8];
         const auto fetch = [&](int c0, uint32_t(&d)[kSet][2][8]) {
@@ -295,7 +296,7 @@ __device__ __forceinline__ bool finish_tile(const Tile& t, EpilogueState& e, Syn
         // this CTA finishes the tokens of group j = rank of every chunk; the other group's sums go to the other CTA
         const int thread = quarter * 32 + lane;
         const uint32_t there = ptx::map_rank(ptx::smem_u32(e.exchange), rank ^ 1);
-        if (e.tiles > 0) ok = wait<true, true>(&sy->x_free, (e.tiles - 1) & 1, sy, a.status, 60);
+        if (e.tiles > 0) ok = wait<true, true>(&sy->x_free, (e.tiles - 1) & 1, sy, a.findings, 60);
         if (!ok) return false;
 #pragma unroll
         for (int c = 0; c < NCH; ++c)
@@ -308,7 +309,7 @@ __device__ __forceinline__ bool finish_tile(const Tile& t, EpilogueState& e, Syn
             }
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_rank(ptx::smem_u32(&sy->x_full), rank ^ 1));
-        ok = wait<true, true>(&sy->x_full, e.tiles & 1, sy, a.status, 61);
+        ok = wait<true, true>(&sy->x_full, e.tiles & 1, sy, a.findings, 61);
         if (!ok) return false;
         float* top = e.tops + (e.tiles & 1) * kTopWords;
         float h8[NCH][8];  // [chunk][2 * m + b]: column 8 m + g8, token 2 q + b
@@ -333,7 +334,7 @@ __device__ __forceinline__ bool finish_tile(const Tile& t, EpilogueState& e, Syn
                     for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(h8[c][2 * i + b]) & 0x7FFFFFFFu);
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-                    if (g8 == 0) top[(wg * 64 + c * 8 + 2 * q + b) * 4 + quarter] = __uint_as_float(m);
+                    if (g8 == 0) top[(wg * (kMaxR / 4) + c * 8 + 2 * q + b) * 4 + quarter] = __uint_as_float(m);
                 }
             }
         __syncwarp();
@@ -341,7 +342,7 @@ __device__ __forceinline__ bool finish_tile(const Tile& t, EpilogueState& e, Syn
             ptx::mbar_arrive_cluster(ptx::map_rank(ptx::smem_u32(&sy->x_free), rank ^ 1));  // what was sent here has been read
             ptx::mbar_arrive(ptx::smem_u32(&sy->wg[wg]));
         }
-        ok = wait<true>(&sy->wg[wg], e.tiles & 1, sy, a.status, 62);
+        ok = wait<true>(&sy->wg[wg], e.tiles & 1, sy, a.findings, 62);
         if (!ok) return false;
         const int inter = a.N >> 1;
         uint8_t* dst = static_cast<uint8_t*>(a.out) + (size_t)t.row0 * inter + t.nt * 128 + quarter * 32 + (lane & 1) * 16;
@@ -351,7 +352,7 @@ __device__ __forceinline__ bool finish_tile(const Tile& t, EpilogueState& e, Syn
                 const int token0 = first + c * 16 + (int)rank * 8;
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
-                    const uint4 m4 = *reinterpret_cast<const uint4*>(top + (wg * 64 + c * 8 + 2 * q + b) * 4);
+                    const uint4 m4 = *reinterpret_cast<const uint4*>(top + (wg * (kMaxR / 4) + c * 8 + 2 * q + b) * 4);
                     const fp8_block::Quantizer qz(__uint_as_float(max(max(m4.x, m4.y), max(m4.z, m4.w))));
                     const uint32_t o = qz.four(h8[c][b], h8[c][2 + b], h8[c][4 + b], h8[c][6 + b]);
                     uint8_t* at = e.strip + (2 * q + b) * 32 + g8;
@@ -390,7 +391,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t rank = ptx::cluster_rank();
     const int n_nt = GATE_UP ? a.N / 256 : (a.NB + 1) / 2;
 
-    load_row_starts(a.group_list, a.G, a.M, a.gl_type, row_start, a.status);
+    load_row_starts(a.group_list, a.G, a.M, a.gl_type, row_start, nullptr, blockIdx.x == 0 ? a.findings : nullptr);
     if (warp == 0) {
         int lo, hi, mine = 0, total, wide = 0;
         lane_experts(a.G, lo, hi);
@@ -414,8 +415,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             sy->n_units = tiles * parts;
             sy->width = max(wide, 32);
             if (blockIdx.x == 0) {
-                a.status[kWordParts] = parts;
-                a.status[kWordRows] = row_start[a.G];
+                a.words[kWordParts] = parts;
+                a.words[kWordRows] = row_start[a.G];
             }
         }
     }
@@ -462,15 +463,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             // ------------------------------ loads ------------------------------
             if (lane == 0) {
                 uint32_t seq = 0, published = 0, it = 0, slot = 0, ph = 0;
-                int held = 0;
+                const int pairs = (int)gridDim.x / 2;
+                int unit = (int)blockIdx.x / 2;
                 bool live = true, ok = true;
                 const uint32_t ring_there = ptx::map_rank(ptx::smem_u32(sy->ring), 1);
                 const auto publish = [&]() {
                     if (rank != 0 || !live) return;
-                    held = atomicAdd(a.status + kWordTicket, 1);
-                    live = held < n_units;
-                    const TileEntry e = live ? locate(published + 1, held, parts, prefix, row_start, a.G, n_nt)
+                    live = unit < n_units;
+                    const TileEntry e = live ? locate(published + 1, unit, parts, prefix, row_start, a.G, n_nt)
                                              : tile_entry(published + 1, 0u, 0u, 0u, 0u);  // rows 0: the schedule has ended
+                    if (live) unit = a.dynamic ? pairs + atomicAdd(a.words + kWordTicket, 1) : unit + pairs;  // (needed a tile later)
                     const uint32_t at = (published % kTileRing) * (uint32_t)sizeof(TileEntry);
                     ring_store(&sy->ring[published % kTileRing], e);
                     ptx::st_cluster_u64(ring_there + at, e.a);
@@ -487,7 +489,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     const int col = GATE_UP ? (int)rank * (a.N >> 1) + t.nt * 128 : t.nt * 256 + (int)rank * 128;
                     const int row = t.row0 + (int)rank * half;
                     for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
-                        if (it >= (uint32_t)n_slots && !wait<false>(&sy->empty[slot], ph ^ 1, sy, a.status, 10)) { ok = false; break; }
+                        if (it >= (uint32_t)n_slots && !wait<false>(&sy->empty[slot], ph ^ 1, sy, a.findings, 10)) { ok = false; break; }
                         const uint32_t bar = ptx::smem_u32(&sy->full[slot]), bar0 = ptx::map_rank(bar, 0);
                         const uint32_t dst = ptx::smem_u32(ring) + slot * (uint32_t)slot_bytes;
                         if (rank == 0) ptx::mbar_arrive_expect_tx(bar, bytes);
@@ -527,12 +529,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const float* xs = a.x_scale + (size_t)(t.row0 + lane) * a.KB;
                 const size_t group = (size_t)a.KB * 32;
                 for (int kb = t.kb0; kb < t.kb1 && ok; kb += 4) {  // (four blocks' loads in flight)
-                    float w[4], v[8][4];
+                    float w[4], v[kMaxR / 32][4];
                     const int last = t.kb1 - 1 - kb;
 #pragma unroll
                     for (int b = 0; b < 4; ++b) w[b] = __ldg(ws + (size_t)(kb + min(b, last)) * a.NB);
 #pragma unroll
-                    for (int g = 0; g < 8; ++g)
+                    for (int g = 0; g < kMaxR / 32; ++g)
                         if (g * 32 < t.n) {
                             const bool row = g * 32 + lane < t.rows;
 #pragma unroll
@@ -541,11 +543,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int b = 0; b < 4; ++b) {
                         if (b > last || !ok) break;
-                        if (it >= (uint32_t)n_bufs) ok = wait<true>(&sy->s_empty[buf], ph ^ 1, sy, a.status, 20);
+                        if (it >= (uint32_t)n_bufs) ok = wait<true>(&sy->s_empty[buf], ph ^ 1, sy, a.findings, 20);
                         if (!ok) break;
                         float* dst = home + buf * (uint32_t)width;
 #pragma unroll
-                        for (int g = 0; g < 8; ++g)
+                        for (int g = 0; g < kMaxR / 32; ++g)
                             if (g * 32 < t.n) dst[g * 32] = v[g][b] * w[b];
                         __syncwarp();
                         if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->t_full[buf]));
@@ -569,8 +571,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
                     if ((it & 1) == turn) {
                         // the epilogue of both CTAs has taken what the buffer held
-                        if (it >= (uint32_t)n_bufs && !wait<true>(&sy->t_empty[buf], tph ^ 1, sy, a.status, 30)) { ok = false; break; }
-                        if (!wait<true>(&sy->full[slot], ph, sy, a.status, 40)) { ok = false; break; }
+                        if (it >= (uint32_t)n_bufs && !wait<true>(&sy->t_empty[buf], tph ^ 1, sy, a.findings, 30)) { ok = false; break; }
+                        if (!wait<true>(&sy->full[slot], ph, sy, a.findings, 40)) { ok = false; break; }
                         ptx::tc_fence_after();
                         if (leader) {
                             const uint64_t at = (uint64_t)(slot * (uint32_t)slot_bytes >> 4);
@@ -619,20 +621,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 case 2: ok = finish_tile<GATE_UP, 2>(t, e, sy, a); break;
                 case 3: ok = finish_tile<GATE_UP, 3>(t, e, sy, a); break;
                 case 4: ok = finish_tile<GATE_UP, 4>(t, e, sy, a); break;
-                case 5: ok = finish_tile<GATE_UP, 5>(t, e, sy, a); break;
-                case 6: ok = finish_tile<GATE_UP, 6>(t, e, sy, a); break;
-                case 7: ok = finish_tile<GATE_UP, 7>(t, e, sy, a); break;
-                default: ok = finish_tile<GATE_UP, 8>(t, e, sy, a); break;
+                default: ok = finish_tile<GATE_UP, 5>(t, e, sy, a); break;
             }
             ++e.tiles;
         }
     }
 
     __syncwarp();
-    if (threadIdx.x == 0 && a.findings != nullptr) {
-        const volatile int* st = a.status;
-        if (st[0] != 0 && atomicCAS(a.findings, 0, st[0]) == 0) a.findings[1] = st[1];
-    }
     ptx::tc_fence_before();
     __syncthreads();
     ptx::cluster_sync();  // (what one CTA sends the other, loads and MMAs of the pair among it, has arrived)
@@ -647,7 +642,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 template <bool GATE_UP>
 __global__ void __launch_bounds__(256) join_kernel(const Args a) {
     grid_dep_wait();
-    const int parts = __ldcg(a.status + kWordParts), rows = __ldcg(a.status + kWordRows);
+    const int parts = __ldcg(a.words + kWordParts), rows = __ldcg(a.words + kWordRows);
     if (parts == 1) return;
     const int lane = threadIdx.x & 31, out_n = GATE_UP ? a.N >> 1 : a.N, blocks = (out_n + 127) / 128;
     const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -691,9 +686,9 @@ static int max_parts(int64_t M, int64_t K, int64_t N, int64_t G, int gate_up) {
 using namespace b200moe;
 
 extern "C" size_t b200moe_grouped_gemm_fp8_block_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, int gate_up_silu) {
-    if (M <= 0 || K <= 0 || N <= 0 || G <= 0) return B200MOE_STATUS_BYTES;
+    if (M <= 0 || K <= 0 || N <= 0 || G <= 0) return fb::kWordBytes;
     const int parts = fb::max_parts(M, K, N, G, gate_up_silu);
-    return B200MOE_STATUS_BYTES + (parts > 1 ? (size_t)parts * (size_t)M * (size_t)N * 4 : 0);
+    return fb::kWordBytes + (parts > 1 ? (size_t)parts * (size_t)M * (size_t)N * 4 : 0);
 }
 
 extern "C" int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scale, const void* weight, const float* weight_scale,
@@ -725,10 +720,10 @@ extern "C" int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scal
     a.gl_type = group_list_type;
     a.KB = (int)((K + 127) / 128);
     a.NB = (int)((N + 127) / 128);
-    a.status = static_cast<int*>(workspace);
+    a.words = static_cast<int*>(workspace);
     a.findings = findings;
     a.max_parts = fb::max_parts(M, K, N, G, gate_up_silu);
-    if (a.max_parts > 1) a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + B200MOE_STATUS_BYTES);
+    if (a.max_parts > 1) a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + fb::kWordBytes);
     CUtensorMap map_w, map_x64, map_x16;
     int rc = make_tensor_map_3d_u8(&map_w, weight, (uint64_t)G, (uint64_t)K, (uint64_t)N, 128, 128);
     if (rc == B200MOE_OK) rc = make_tensor_map_2d(&map_x64, x, 1, (uint64_t)M, (uint64_t)K, fb::kBigBox, 128, true);
@@ -737,7 +732,8 @@ extern "C" int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scal
     const unsigned grid = (unsigned)(sm_count() / 2 * 2);
     const auto kernel = gate_up_silu ? fb::grouped_kernel<true> : fb::grouped_kernel<false>;
     B200MOE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, fb::kSmemBytes));
-    B200MOE_CUDA_TRY(cudaMemsetAsync(workspace, 0, B200MOE_STATUS_BYTES, st));
+    a.dynamic = ((N + 255) / 256) * std::min(G, M) >= 8 * (int64_t)grid;
+    if (a.dynamic) B200MOE_CUDA_TRY(cudaMemsetAsync(workspace, 0, fb::kWordBytes, st));
     kernel<<<grid, fb::kThreads, fb::kSmemBytes, st>>>(map_w, map_x64, map_x16, a);
     B200MOE_CUDA_TRY(cudaGetLastError());
     if (a.max_parts > 1) {

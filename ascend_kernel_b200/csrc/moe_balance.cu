@@ -218,9 +218,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a, float*
     if (threadIdx.x == 0) {
         s_n = 0;
         const long long given = a.seq_list ? a.seq_list[s] : a.T;
-        if (findings != nullptr && (given != end || end < start)) {  // (kept until the caller clears them)
-            if (atomicCAS(findings, 0, kDevBadGroupList) == 0) findings[1] = s;
-        }
+        if (given != end || end < start) keep_finding(findings, kDevBadGroupList, s);
     }
     __syncthreads();
     const int groups = (a.pitch + 127) / 128, rows_at_once = 32 / groups;  // pitch <= 1024

@@ -314,8 +314,8 @@ int b200moe_fp8_quantize_rows(const void* x, const int32_t* index, void* codes, 
  * silu(gate) * up in fp32, quantised as b200moe_fp8_quantize_rows does: out e4m3 [M, I], out_scale fp32 [M, I / 128].
  * K % 16 == 0 and N % 16 == 0; x, weight and out aligned to 16 bytes.  Rows of no expert are left as they were.
  * The workspace belongs to the call until it has completed on the stream, and the next call may have another (calls that overlap must).
- * findings: NULL, or two int32 in device memory that keep the first (code, detail) of the status words of any call until the
- * caller zeroes them. */
+ * findings: NULL, or two int32 in device memory that keep the first (code, detail) found by any call that got them until the caller
+ * zeroes them; codes and details are those of status words 0 and 1. */
 size_t b200moe_grouped_gemm_fp8_block_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, int gate_up_silu);
 int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scale, const void* weight, const float* weight_scale,
                                    const int64_t* group_list, void* out, float* out_scale, int64_t M, int64_t K, int64_t N, int64_t G,
