@@ -461,38 +461,45 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == kWarpLoad) {
             // ------------------------------ loads ------------------------------
-            if (lane == 0) {
-                uint32_t seq = 0, published = 0, it = 0, slot = 0, ph = 0;
-                const int pairs = (int)gridDim.x / 2;
-                int unit = (int)blockIdx.x / 2;
-                bool live = true, ok = true;
-                const uint32_t ring_there = ptx::map_rank(ptx::smem_u32(sy->ring), 1);
-                const auto publish = [&]() {
-                    if (rank != 0 || !live) return;
-                    live = unit < n_units;
-                    const TileEntry e = live ? locate(published + 1, unit, parts, prefix, row_start, a.G, n_nt)
-                                             : tile_entry(published + 1, 0u, 0u, 0u, 0u);  // rows 0: the schedule has ended
-                    if (live) unit = a.dynamic ? pairs + atomicAdd(a.words + kWordTicket, 1) : unit + pairs;  // (needed a tile later)
+            // The warp walks together and one lane issues (a lane on its own took 550 cycles a stage).
+            const bool leader = ptx::elect_one();
+            uint32_t seq = 0, published = 0, it = 0, slot = 0, ph = 0;
+            const int pairs = (int)gridDim.x / 2;
+            int unit = (int)blockIdx.x / 2;
+            bool live = true, ok = true;
+            const uint32_t ring_there = ptx::map_rank(ptx::smem_u32(sy->ring), 1);
+            const uint32_t full0 = ptx::map_rank(ptx::smem_u32(sy->full), 0), full_here = ptx::smem_u32(sy->full);
+            const auto publish = [&]() {
+                if (rank != 0 || !live) return;
+                live = unit < n_units;
+                const TileEntry e = live ? locate(published + 1, unit, parts, prefix, row_start, a.G, n_nt)
+                                         : tile_entry(published + 1, 0u, 0u, 0u, 0u);  // rows 0: the schedule has ended
+                int drawn = 0;
+                if (leader) {
                     const uint32_t at = (published % kTileRing) * (uint32_t)sizeof(TileEntry);
                     ring_store(&sy->ring[published % kTileRing], e);
                     ptx::st_cluster_u64(ring_there + at, e.a);
                     ptx::st_cluster_u64(ring_there + at + 8, e.b);
-                    ++published;
-                };
-                publish();
-                Tile t;
-                while (ok) {
-                    publish();  // (a tile ahead: the other roles find it there)
-                    if (!next_tile<false>(sy, seq, t, a, parts)) break;
-                    const int half = t.n >> 1, n_big = half / kBigBox, n_small = (half % kBigBox) / kSmallBox;
-                    const uint32_t bytes = 2u * (uint32_t)(kABytes + half * 128);
-                    const int col = GATE_UP ? (int)rank * (a.N >> 1) + t.nt * 128 : t.nt * 256 + (int)rank * 128;
-                    const int row = t.row0 + (int)rank * half;
-                    for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
-                        if (it >= (uint32_t)n_slots && !wait<false>(&sy->empty[slot], ph ^ 1, sy, a.findings, 10)) { ok = false; break; }
-                        const uint32_t bar = ptx::smem_u32(&sy->full[slot]), bar0 = ptx::map_rank(bar, 0);
-                        const uint32_t dst = ptx::smem_u32(ring) + slot * (uint32_t)slot_bytes;
-                        if (rank == 0) ptx::mbar_arrive_expect_tx(bar, bytes);
+                    if (live && a.dynamic) drawn = atomicAdd(a.words + kWordTicket, 1);
+                }
+                if (a.dynamic) unit = pairs + __reduce_add_sync(0xffffffffu, drawn);
+                else unit += pairs;
+                ++published;
+            };
+            publish();
+            Tile t;
+            while (ok) {
+                publish();  // (a tile ahead: the other roles find it there)
+                if (!next_tile<true>(sy, seq, t, a, parts)) break;
+                const int half = t.n >> 1, n_big = half / kBigBox, n_small = (half % kBigBox) / kSmallBox;
+                const uint32_t bytes = 2u * (uint32_t)(kABytes + half * 128);
+                const int col = GATE_UP ? (int)rank * (a.N >> 1) + t.nt * 128 : t.nt * 256 + (int)rank * 128;
+                const int row = t.row0 + (int)rank * half;
+                for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+                    if (it >= (uint32_t)n_slots && !wait<true>(&sy->empty[slot], ph ^ 1, sy, a.findings, 10)) { ok = false; break; }
+                    if (leader) {
+                        const uint32_t bar0 = full0 + slot * 8, dst = ptx::smem_u32(ring) + slot * (uint32_t)slot_bytes;
+                        if (rank == 0) ptx::mbar_arrive_expect_tx(full_here + slot * 8, bytes);
                         ptx::tma_load_3d_pair(dst, &map_w, bar0, col, kb * 128, t.g);
                         uint32_t at = dst + kABytes;
                         int r = row;
@@ -500,19 +507,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             ptx::tma_load_2d_pair(at, &map_x64, bar0, kb * 128, r);
                         for (int b = 0; b < n_small; ++b, at += kSmallBox * 128, r += kSmallBox)
                             ptx::tma_load_2d_pair(at, &map_x16, bar0, kb * 128, r);
-                        if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
                     }
+                    __syncwarp();
+                    if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
                 }
-                if (*reinterpret_cast<volatile int*>(&sy->abort)) {
-                    // copies in flight land before the shared memory goes (those of both CTAs are counted in the first one)
-                    if (rank == 0) {
-                        const uint32_t from = it > (uint32_t)n_slots ? it - n_slots : 0;
-                        for (uint32_t j = from; j < it; ++j)
-                            (void)ptx::mbar_wait(ptx::smem_u32(&sy->full[j % n_slots]), (j / n_slots) & 1);
-                    }
-                    const uint64_t t0 = ptx::globaltimer_ns();
-                    while (ptx::globaltimer_ns() - t0 < 10000000ull) {}
+            }
+            if (leader && *reinterpret_cast<volatile int*>(&sy->abort)) {
+                // copies in flight land before the shared memory goes (those of both CTAs are counted in the first one)
+                if (rank == 0) {
+                    const uint32_t from = it > (uint32_t)n_slots ? it - n_slots : 0;
+                    for (uint32_t j = from; j < it; ++j)
+                        (void)ptx::mbar_wait(ptx::smem_u32(&sy->full[j % n_slots]), (j / n_slots) & 1);
                 }
+                const uint64_t t0 = ptx::globaltimer_ns();
+                while (ptx::globaltimer_ns() - t0 < 10000000ull) {}
             }
             __syncwarp();
         } else if (warp == kWarpScale) {
