@@ -29,6 +29,9 @@ struct Quantizer {
         a_ = a * 0x1p-10f;
         step_ = inv_ * (1024.f / kMax);
     }
+    // what four() needs, for a thread that did not see the block's magnitude
+    __device__ __forceinline__ float4 packed() const { return make_float4(inv_, a_, step_, finite_ ? 1.f : 0.f); }
+    __device__ __forceinline__ explicit Quantizer(const float4& p) : scale(0.f), inv_(p.x), a_(p.y), step_(p.z), finite_(p.w != 0.f) {}
     __device__ __forceinline__ float ratio(float x) const {
         // x * 448 / a = (x * 7 * 2^-4) / (a * 2^-10): neither product overflows, and neither is rounded where it matters
         const float q = x * inv_;

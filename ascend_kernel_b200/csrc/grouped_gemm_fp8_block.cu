@@ -10,17 +10,14 @@
 // the MN-major A operand.  The rows of x are split between the two CTAs' shared memory and read by both.
 //
 // An arbitrary fp32 scale cannot ride in the MMA, so a block of 128 k is a sum of its own: the MMA warps write it to one
-// of the 2 .. 8 tensor-memory buffers that fit, and the epilogue warps add it, times scale, to the tile's sums in their registers (one fused
-// multiply-add per two elements; a lane's 4 weight columns x 2 tokens of each 8 x 8 patch need one 16-byte read of scales per 16 tokens).
-// Blocks being independent, two warps issue them in turn: a block's MMAs last about as many cycles as it has token rows, fewer
-// than the waits, four issues and the commit cost one warp.
+// of the 3 .. 8 tensor-memory buffers that fit, and the epilogue warps add it, times scale, to the tile's sums in their registers (one
+// fused multiply-add per two elements).  Blocks being independent, two warps issue them in turn.
 //
-// Gate/up: CTA 0 of the pair holds 128 gate columns and CTA 1 the up columns of the same indices.  At the end of a tile each
-// sends the other half of its sums through distributed shared memory, and both finish half of the tokens: silu(gate) * up in fp32,
-// the largest magnitude over the 128 columns, e4m3.
+// Gate/up: a stage holds 128 gate columns and the 128 up columns of the same indices for the same rows of x, two blocks, and a thread
+// has both sums of its columns and tokens: silu(gate) * up in fp32, the largest magnitude over the 128 columns, e4m3.
 //
-// Warp roles (12 warps): 0 loads (and, in the pair's first CTA, tile tickets); 1 and 2 MMA issue (first CTA); 3 scales;
-// 4 - 11 epilogue.  The shared-memory ring holds as many stages as the call's widest tile leaves room for.  Every wait is bounded.
+// Warp roles: 0 loads (and, in the pair's first CTA, deals out the tiles); 1 and 2 MMA issue (first CTA); 3 scales; from 4 on epilogue.
+// The shared-memory ring holds as many stages as the call's widest tile leaves room for.  Every wait is bounded.
 //
 // Few tiles: the k range is split into parts whose fp32 sums go to the workspace, and a second kernel adds them in their order.
 #include <algorithm>
@@ -33,22 +30,29 @@
 namespace b200moe {
 namespace fb {
 
-constexpr int kThreads = 384;
-constexpr int kWarpLoad = 0, kWarpMma0 = 1, kWarpScale = 3, kWarpEpi0 = 4, kEpiWarps = 8;
+constexpr int kWarpLoad = 0, kWarpMma0 = 1, kWarpScale = 3, kWarpEpi0 = 4;
 constexpr int kMaxR = 160;             // token rows of a tile
-constexpr int kABytes = 128 * 128;     // a CTA's weights of a stage
+constexpr int kABytes = 128 * 128;     // 128 weight columns of a stage
 constexpr int kMaxSlots = 12, kMaxBufs = 8;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kStripBytes = 1024;      // of an epilogue warp
 constexpr int kBigBox = 64, kSmallBox = 16;
-constexpr int kScaleRingBytes = (int)kTmemCols * 4;  // a row of scales for every accumulator column
-constexpr int kTopWords = kMaxR / 2 * 4;   // gate/up: magnitudes of a tile, [the CTA's tokens][4 warps]
-constexpr int kTopBytes = 2 * kTopWords * 4;  // of two tiles in turn
+constexpr int kScaleRingBytes = (int)kTmemCols * 4;  // a scale for every accumulator column
 constexpr int kBarrierBytes = 2048;
-constexpr int kFixedBytes = 1024 + kBarrierBytes + kScaleRingBytes + kEpiWarps * kStripBytes + kTopBytes + 2 * (kMaxExperts + 4) * 4;
 constexpr int kSmemBytes = 227 * 1024;
-constexpr int kRingBytes = kSmemBytes - kFixedBytes;  // stages, and the gate/up exchange
-static_assert(kRingBytes - kMaxR * 256 >= 4 * (kABytes + kMaxR / 2 * 128), "stages");
+
+// The epilogue's warps come in groups of four (128 weight columns), which share the tile's tokens.  A thread's sums and what it
+// fetches ahead have to fit its registers: 16 warps where it sums one block, 8 with twice the registers where it sums two.
+template <bool GATE_UP>
+struct Shape {
+    static constexpr int kHalves = GATE_UP ? 2 : 1;  // blocks of a stage
+    static constexpr int kGroups = 2, kEpiWarps = 4 * kGroups, kThreads = (kWarpEpi0 + kEpiWarps) * 32;
+    static constexpr int kUnit = 32 / (8 * kGroups);  // 8-token patches of a warp per 32 token rows: 1 or 2
+    static constexpr int kTopBytes = GATE_UP ? kMaxR * 16 : 0;  // [tokens][4 warps] magnitudes, and as much for what they give
+    static constexpr int kFixedBytes = 1024 + kBarrierBytes + kScaleRingBytes + kEpiWarps * kStripBytes + 2 * kTopBytes + 2 * (kMaxExperts + 4) * 4;
+    static constexpr int kRingBytes = kSmemBytes - kFixedBytes;
+    static_assert(kRingBytes % 16 == 0 && kRingBytes >= 4 * (kHalves * kABytes + kMaxR * 64), "stages");
+};
 
 struct Args {
     const float* x_scale;
@@ -67,12 +71,11 @@ constexpr int kWordTicket = 0, kWordParts = 1, kWordRows = 2, kWordBytes = 256;
 
 struct Sync {
     uint64_t full[kMaxSlots];    // first CTA: the bytes of both CTAs' loads
-    uint64_t empty[kMaxSlots];   // each CTA: commit
+    uint64_t empty[kMaxSlots];   // each CTA: commit of the stage's blocks
     uint64_t t_full[kMaxBufs];   // each CTA: commit, and the buffer's scales are written
-    uint64_t t_empty[kMaxBufs];  // first CTA: the 16 epilogue warps of the pair have the buffer's sums
-    uint64_t s_empty[kMaxBufs];  // each CTA: its 8 epilogue warps have done with the buffer's scales
-    uint64_t x_full, x_free;     // gate/up exchange: the other CTA's 8 warps have written here; have read what was sent there
-    uint64_t wg[2];              // the four epilogue warps of a group among themselves
+    uint64_t t_empty[kMaxBufs];  // first CTA: the epilogue warps of the pair have the buffer's sums
+    uint64_t s_empty[kMaxBufs];  // each CTA: its epilogue warps have done with the buffer's scales
+    uint64_t wg[4];              // the four epilogue warps of a group among themselves
     uint64_t drain[2];
     uint32_t tmem_base;
     int abort;
@@ -82,7 +85,7 @@ struct Sync {
 static_assert(sizeof(Sync) <= kBarrierBytes, "barrier block");
 
 struct Tile {
-    int g, row0, rows, n, nt, kb0, kb1, part;  // n: rows rounded up to 32; nt: 256 weight columns (gate/up: 128 of each)
+    int g, row0, rows, n, nt, kb0, kb1, part;  // n: rows rounded up to 32; nt: 256 columns (gate/up: 256 of each)
 };
 
 // Waits and tile look-ups of whole warps vote at every poll, so that a warp leaves them together (instructions for the whole warp
@@ -172,224 +175,234 @@ __device__ __forceinline__ float silu(float g) {
     return g * __fdividef(g < 0.f ? e : 1.f, 1.f + e);
 }
 
-// Where the sums of a chunk's 16-lane half lie in the gate/up exchange: [group of warps][chunk][half][thread] pieces of 16 bytes.
-__device__ __forceinline__ uint32_t exchange_at(int wg, int n_ch, int c, int h, int thread) {
-    return (uint32_t)((((wg * n_ch + c) * 2 + h) * 128 + thread) * 16);
-}
-
-struct EpilogueState {
+// What an epilogue warp carries from tile to tile.
+struct Epilogue {
     int warp, parts;
-    uint32_t rank, buf, ph, tiles, n_bufs, width, tmem, t_empty;
+    uint32_t rank, buf, ph, wg_ph, n_bufs, width, tmem, t_empty;
     float* scales;
-    uint8_t *strip, *exchange;
-    float* tops;
+    uint8_t* strip;
+    float *tops, *quantizers;
 };
 
-// A tile's sums and what becomes of them.  A warp holds 32 weight columns (tensor-memory lanes) x half of the tile's tokens, NCH chunks
-// of 16: acc[chunk][16 lanes][8 tokens][8 lanes], two tokens to a register pair.  The number of chunks is a constant: a warp passes
-// here once a block of 128 k, and its instructions are what a block costs (with a test at every chunk, 130 for one chunk: 1000 cycles).
-template <bool GATE_UP, int NCH>
-__device__ __forceinline__ bool finish_tile(const Tile& t, EpilogueState& e, Sync* sy, const Args& a) {
-    const uint32_t rank = e.rank;
-    const int lane = threadIdx.x & 31, wg = e.warp >> 2, quarter = e.warp & 3, g8 = lane >> 2, q = lane & 3, first = wg * (NCH * 16);
-    bool ok = true;
-    f32x2 acc[NCH][2][2][2];
+// One block into the warp's sums.  The warp holds 32 weight columns (tensor-memory lanes) x NP patches of 8 tokens:
+// acc[patch][16 lanes][8 lanes], two tokens to a register pair: lane (g8, q) has columns g8, g8 + 8, .. and tokens 2q, 2q + 1.  The number
+// of patches is a constant: a warp passes here once a block of 128 k, and its instructions are what a block costs (with a
+// test at every patch, 1000 cycles a block instead of 600).
+template <int NP>
+__device__ __forceinline__ bool add_block(f32x2 (&acc)[NP][2][2], Epilogue& e, uint32_t first, Sync* sy, const Args& a) {
+    const int lane = threadIdx.x & 31, q = lane & 3;
+    const uint32_t column = e.buf * e.width + first, td = e.tmem + column;
+    const float2* sv = reinterpret_cast<const float2*>(e.scales + column) + q;
+    if (!wait<true>(&sy->t_full[e.buf], e.ph, sy, a.findings, 50)) return false;
+    ptx::tc_fence_after();
+    uint32_t v[2][2][8];  // two patches are fetched while the two before them are added
+    const auto fetch = [&](int p, uint32_t(&d)[2][8]) {
 #pragma unroll
-    for (int c = 0; c < NCH; ++c)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) acc[c][i >> 2][(i >> 1) & 1][i & 1] = 0ull;
-    for (int kb = t.kb0; kb < t.kb1; ++kb) {
-        const uint32_t column = e.buf * e.width + (uint32_t)first;
-        const float4* sv = reinterpret_cast<const float4*>(e.scales + column) + q;
-        const uint32_t td = e.tmem + column;
-        if (!wait<true>(&sy->t_full[e.buf], e.ph, sy, a.findings, 50)) return false;
-        ptx::tc_fence_after();
-        constexpr int kSet = NCH <= 4 ? 2 : 1;  // chunks that are fetched together while the set before is added
-        uint32_t v[2][kSet][2][8];
-        const auto fetch = [&](int c0, uint32_t(&d)[kSet][2][8]) {
-#pragma unroll
-            for (int c = 0; c < kSet; ++c)
-                if (c0 + c < NCH) {
-                    ptx::tmem_ld_16x16(td + (uint32_t)((c0 + c) * 16), d[c][0]);
-                    ptx::tmem_ld_16x16(td + (uint32_t)((c0 + c) * 16) + (16u << 16), d[c][1]);
-                }
-        };
-        fetch(0, v[0]);
-#pragma unroll
-        for (int c0 = 0; c0 < NCH; c0 += kSet) {
-            ptx::tmem_ld_wait();
-            if (c0 + kSet < NCH) {
-                fetch(c0 + kSet, v[(c0 / kSet + 1) & 1]);
-            } else {
-                // all is in registers: the buffer goes back
-                ptx::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive_remote(e.t_empty + e.buf * 8);
-            }
-#pragma unroll
-            for (int c = 0; c < kSet; ++c)
-                if (c0 + c < NCH) {
-                    const float4 s4 = sv[(c0 + c) * 4];
-                    const f32x2 s2[2] = {pack_f32x2(s4.x, s4.y), pack_f32x2(s4.z, s4.w)};
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j)
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const uint32_t(&d)[8] = v[(c0 / kSet) & 1][c][h];
-                                acc[c0 + c][h][j][i] = fma_f32x2(pack_u32x2(d[4 * j + 2 * i], d[4 * j + 2 * i + 1]), s2[j], acc[c0 + c][h][j][i]);
-                            }
-                }
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t at = td + (uint32_t)(p * 8) + ((uint32_t)(h * 16) << 16);
+            if (p + 1 < NP) ptx::tmem_ld_16x16(at, d[h]);
+            else ptx::tmem_ld_16x8(at, d[h]);
         }
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->s_empty[e.buf]));
-        if (++e.buf == e.n_bufs) { e.buf = 0; e.ph ^= 1; }
-    }
-
-    if (e.parts > 1) {
-        // a part's sums as they are, [part][row][column]
-        const int col0 = (GATE_UP ? (int)rank * (a.N >> 1) + t.nt * 128 : t.nt * 256 + (int)rank * 128) + quarter * 32 + g8;
-        float* dst = a.parts + ((size_t)t.part * a.M + t.row0) * a.N;
+    };
+    fetch(0, v[0]);
 #pragma unroll
-        for (int c = 0; c < NCH; ++c)
+    for (int p = 0; p < NP; p += 2) {
+        ptx::tmem_ld_wait();
+        if (p + 2 < NP) {
+            fetch(p + 2, v[(p / 2 + 1) & 1]);
+        } else {
+            // all is in registers: the buffer goes back
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive_remote(e.t_empty + e.buf * 8);
+        }
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+        for (int j = 0; j < 2; ++j)
+            if (p + j < NP) {
+                const float2 s = sv[(p + j) * 4];
+                const f32x2 s2 = pack_f32x2(s.x, s.y);
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const int token = first + c * 16 + j * 8 + 2 * q, col = col0 + h * 16 + i * 8;
-                        if (col < a.N) {
-                            if (token < t.rows) dst[(size_t)token * a.N + col] = f32x2_lo(acc[c][h][j][i]);
-                            if (token + 1 < t.rows) dst[(size_t)(token + 1) * a.N + col] = f32x2_hi(acc[c][h][j][i]);
-                        }
+                        const uint32_t(&d)[8] = v[(p / 2) & 1][h];
+                        acc[p + j][h][i] = fma_f32x2(pack_u32x2(d[4 * j + 2 * i], d[4 * j + 2 * i + 1]), s2, acc[p + j][h][i]);
                     }
-    } else if constexpr (!GATE_UP) {
-        // 16 tokens x 32 columns at a time through the warp's strip: the transposing store gives 16-byte pieces of
-        // eight columns, 64 contiguous bytes of a row
-        const int col = t.nt * 256 + (int)rank * 128 + quarter * 32 + q * 8;
-        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (size_t)t.row0 * a.N + col;
-#pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    uint32_t o[4];
-#pragma unroll
-                    for (int m = 0; m < 4; ++m) o[m] = pack_bf16x2(f32x2_lo(acc[c][m >> 1][j][m & 1]), f32x2_hi(acc[c][m >> 1][j][m & 1]));
-                    // row lane % 8 (a token), piece lane / 8
-                    const int token = j * 8 + (lane & 7);
-                    ptx::stmatrix_x4_trans(ptx::smem_u32(e.strip) + (uint32_t)(token * 64 + (((lane >> 3) ^ (token >> 1)) & 3) * 16), o[0], o[1], o[2], o[3]);
-                }
-                __syncwarp();
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int token = j * 8 + g8, row = first + c * 16 + token;
-                    const uint4 o = *reinterpret_cast<const uint4*>(e.strip + token * 64 + ((q ^ (token >> 1)) & 3) * 16);
-                    if (row < t.rows && col < a.N) *reinterpret_cast<uint4*>(dst + (size_t)row * a.N) = o;
-                }
-                __syncwarp();
             }
-        }
-    } else {
-        // this CTA finishes the tokens of group j = rank of every chunk; the other group's sums go to the other CTA
-        const int thread = quarter * 32 + lane;
-        const uint32_t there = ptx::map_rank(ptx::smem_u32(e.exchange), rank ^ 1);
-        if (e.tiles > 0) ok = wait<true, true>(&sy->x_free, (e.tiles - 1) & 1, sy, a.findings, 60);
-        if (!ok) return false;
+    }
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->s_empty[e.buf]));
+    if (++e.buf == e.n_bufs) { e.buf = 0; e.ph ^= 1; }
+    return true;
+}
+
+// A part's sums as they are, [part][row][column]; `columns`: how many from `col` on the tile has.
+template <int NP>
+__device__ __forceinline__ void store_part(const f32x2 (&acc)[NP][2][2], const Tile& t, int first, int col, int columns, const Args& a) {
+    const int lane = threadIdx.x & 31, g8 = lane >> 2, q = lane & 3;
+    float* dst = a.parts + ((size_t)t.part * a.M + t.row0) * a.N + col;
 #pragma unroll
-        for (int c = 0; c < NCH; ++c)
-            {
+    for (int p = 0; p < NP; ++p)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const f32x2 s0 = rank == 0 ? acc[c][h][1][0] : acc[c][h][0][0], s1 = rank == 0 ? acc[c][h][1][1] : acc[c][h][0][1];
-                    ptx::st_cluster_v4(there + exchange_at(wg, NCH, c, h, thread), (uint32_t)s0, (uint32_t)(s0 >> 32), (uint32_t)s1, (uint32_t)(s1 >> 32));
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int token = first + p * 8 + 2 * q, c = h * 16 + i * 8 + g8;
+                if (c < columns) {
+                    if (token < t.rows) dst[(size_t)token * a.N + c] = f32x2_lo(acc[p][h][i]);
+                    if (token + 1 < t.rows) dst[(size_t)(token + 1) * a.N + c] = f32x2_hi(acc[p][h][i]);
                 }
             }
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_rank(ptx::smem_u32(&sy->x_full), rank ^ 1));
-        ok = wait<true, true>(&sy->x_full, e.tiles & 1, sy, a.findings, 61);
-        if (!ok) return false;
-        float* top = e.tops + (e.tiles & 1) * kTopWords;
-        float h8[NCH][8];  // [chunk][2 * m + b]: column 8 m + g8, token 2 q + b
+}
+
+// bf16 rows, up to 16 tokens x 32 columns at a time through the warp's strip: the transposing store gives 16-byte pieces of eight
+// columns, 64 contiguous bytes of a row.
+template <int NP>
+__device__ __forceinline__ void store_rows(const f32x2 (&acc)[NP][2][2], const Tile& t, const Epilogue& e, int first, int col, const Args& a) {
+    const int lane = threadIdx.x & 31, g8 = lane >> 2, q = lane & 3;
+    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (size_t)t.row0 * a.N + col + q * 8;
+    const bool inside = col + q * 8 < a.N;
 #pragma unroll
-        for (int c = 0; c < NCH; ++c)
-            {
+    for (int p = 0; p < NP; p += 2) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint4 o = *reinterpret_cast<const uint4*>(e.exchange + exchange_at(wg, NCH, c, h, thread));
-                    const f32x2 k0 = rank == 0 ? acc[c][h][0][0] : acc[c][h][1][0], k1 = rank == 0 ? acc[c][h][0][1] : acc[c][h][1][1];
-                    const float own[4] = {f32x2_lo(k0), f32x2_hi(k0), f32x2_lo(k1), f32x2_hi(k1)};
-                    const float other[4] = {__uint_as_float(o.x), __uint_as_float(o.y), __uint_as_float(o.z), __uint_as_float(o.w)};
+        for (int j = 0; j < 2; ++j)
+            if (p + j < NP) {
+                uint32_t o[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        h8[c][h * 4 + i] = silu(rank == 0 ? own[i] : other[i]) * (rank == 0 ? other[i] : own[i]);
-                }
-                // the largest magnitude over the warp's 32 columns (magnitudes order as their bits do, infinities and NaN last)
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    uint32_t m = 0;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(h8[c][2 * i + b]) & 0x7FFFFFFFu);
-#pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-                    if (g8 == 0) top[(wg * (kMaxR / 4) + c * 8 + 2 * q + b) * 4 + quarter] = __uint_as_float(m);
-                }
+                for (int m = 0; m < 4; ++m) o[m] = pack_bf16x2(f32x2_lo(acc[p + j][m >> 1][m & 1]), f32x2_hi(acc[p + j][m >> 1][m & 1]));
+                const int token = j * 8 + (lane & 7);  // row lane % 8 of piece lane / 8
+                ptx::stmatrix_x4_trans(ptx::smem_u32(e.strip) + (uint32_t)(token * 64 + (((lane >> 3) ^ (token >> 1)) & 3) * 16), o[0], o[1], o[2], o[3]);
             }
         __syncwarp();
-        if (lane == 0) {
-            ptx::mbar_arrive_cluster(ptx::map_rank(ptx::smem_u32(&sy->x_free), rank ^ 1));  // what was sent here has been read
-            ptx::mbar_arrive(ptx::smem_u32(&sy->wg[wg]));
-        }
-        ok = wait<true>(&sy->wg[wg], e.tiles & 1, sy, a.findings, 62);
-        if (!ok) return false;
-        const int inter = a.N >> 1;
-        uint8_t* dst = static_cast<uint8_t*>(a.out) + (size_t)t.row0 * inter + t.nt * 128 + quarter * 32 + (lane & 1) * 16;
 #pragma unroll
-        for (int c = 0; c < NCH; ++c)
-            {
-                const int token0 = first + c * 16 + (int)rank * 8;
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const uint4 m4 = *reinterpret_cast<const uint4*>(top + (wg * (kMaxR / 4) + c * 8 + 2 * q + b) * 4);
-                    const fp8_block::Quantizer qz(__uint_as_float(max(max(m4.x, m4.y), max(m4.z, m4.w))));
-                    const uint32_t o = qz.four(h8[c][b], h8[c][2 + b], h8[c][4 + b], h8[c][6 + b]);
-                    uint8_t* at = e.strip + (2 * q + b) * 32 + g8;
-                    at[0] = (uint8_t)o;
-                    at[8] = (uint8_t)(o >> 8);
-                    at[16] = (uint8_t)(o >> 16);
-                    at[24] = (uint8_t)(o >> 24);
-                    const int token = token0 + 2 * q + b;
-                    if (quarter == 0 && g8 == 0 && token < t.rows) a.out_scale[(size_t)(t.row0 + token) * (inter >> 7) + t.nt] = qz.scale;
-                }
-                __syncwarp();
-                const int token = token0 + (lane >> 1);
-                if (lane < 16 && token < t.rows)
-                    *reinterpret_cast<uint4*>(dst + (size_t)token * inter) = *reinterpret_cast<const uint4*>(e.strip + lane * 16);
-                __syncwarp();
+        for (int j = 0; j < 2; ++j)
+            if (p + j < NP) {
+                const int token = j * 8 + g8, row = first + p * 8 + token;
+                const uint4 o = *reinterpret_cast<const uint4*>(e.strip + token * 64 + ((q ^ (token >> 1)) & 3) * 16);
+                if (row < t.rows && inside) *reinterpret_cast<uint4*>(dst + (size_t)row * a.N) = o;
             }
+        __syncwarp();
+    }
+}
+
+// silu(gate) * up of the thread's columns and tokens, quantised by the rows' 128 columns: the warps of a group put what their 32
+// columns have as largest magnitudes together, a thread per token makes the scale, and the codes leave through the strip.
+template <int NP>
+__device__ __forceinline__ bool store_quantized(f32x2 (&gate)[NP][2][2], const f32x2 (&up)[NP][2][2], const Tile& t, Epilogue& e, int first,
+                                                int block, Sync* sy, const Args& a) {
+    const int lane = threadIdx.x & 31, g8 = lane >> 2, q = lane & 3, quarter = e.warp & 3, wg = e.warp >> 2;
+    const int inter = a.N >> 1, blocks = inter >> 7;
+    const bool inside = block < blocks;  // (an odd number of blocks leaves the pair's last CTA without one)
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+        uint32_t m0 = 0, m1 = 0;  // magnitudes order as their bits do, infinities and NaN last
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float lo = silu(f32x2_lo(gate[p][h][i])) * f32x2_lo(up[p][h][i]);
+                const float hi = silu(f32x2_hi(gate[p][h][i])) * f32x2_hi(up[p][h][i]);
+                m0 = max(m0, __float_as_uint(lo) & 0x7FFFFFFFu);
+                m1 = max(m1, __float_as_uint(hi) & 0x7FFFFFFFu);
+                gate[p][h][i] = pack_f32x2(lo, hi);
+            }
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+            m0 = max(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+            m1 = max(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+        }
+        if (g8 < 2) e.tops[(first + p * 8 + 2 * q + g8) * 4 + quarter] = __uint_as_float(g8 ? m1 : m0);
+    }
+    const auto meet = [&]() {
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->wg[wg]));
+        const bool ok = wait<true>(&sy->wg[wg], e.wg_ph, sy, a.findings, 62);
+        e.wg_ph ^= 1;
+        return ok;
+    };
+    if (!meet()) return false;
+    const int mine = quarter * 32 + lane;
+    if (mine < NP * 8) {
+        const int token = first + mine;
+        const uint4 m = reinterpret_cast<const uint4*>(e.tops)[token];
+        const fp8_block::Quantizer qz(__uint_as_float(max(max(m.x, m.y), max(m.z, m.w))));
+        reinterpret_cast<float4*>(e.quantizers)[token] = qz.packed();
+        if (inside && token < t.rows) a.out_scale[(size_t)(t.row0 + token) * blocks + block] = qz.scale;
+    }
+    if (!meet()) return false;
+    uint8_t* dst = static_cast<uint8_t*>(a.out) + (size_t)t.row0 * inter + block * 128 + quarter * 32 + (lane & 1) * 16;
+#pragma unroll
+    for (int p = 0; p < NP; p += 2) {  // (NP is even)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const fp8_block::Quantizer qz(reinterpret_cast<const float4*>(e.quantizers)[first + (p + j) * 8 + 2 * q + b]);
+                float h[4];
+#pragma unroll
+                for (int m = 0; m < 4; ++m) h[m] = b ? f32x2_hi(gate[p + j][m >> 1][m & 1]) : f32x2_lo(gate[p + j][m >> 1][m & 1]);
+                const uint32_t o = qz.four(h[0], h[1], h[2], h[3]);
+                uint8_t* at = e.strip + (j * 8 + 2 * q + b) * 32 + g8;
+                at[0] = (uint8_t)o;
+                at[8] = (uint8_t)(o >> 8);
+                at[16] = (uint8_t)(o >> 16);
+                at[24] = (uint8_t)(o >> 24);
+            }
+        __syncwarp();
+        const int token = first + p * 8 + (lane >> 1);
+        if (inside && token < t.rows) *reinterpret_cast<uint4*>(dst + (size_t)token * inter) = *reinterpret_cast<const uint4*>(e.strip + lane * 16);
+        __syncwarp();
     }
     return true;
 }
 
+// A tile's sums and what becomes of them; NP: patches of 8 tokens a warp has.
+template <bool GATE_UP, int NP>
+__device__ __forceinline__ bool finish_tile(const Tile& t, Epilogue& e, Sync* sy, const Args& a) {
+    constexpr int kHalves = Shape<GATE_UP>::kHalves;
+    const int first = (e.warp >> 2) * (NP * 8), quarter = e.warp & 3;
+    f32x2 acc[kHalves][NP][2][2];
+#pragma unroll
+    for (int u = 0; u < kHalves; ++u)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) acc[u][p][0][0] = acc[u][p][0][1] = acc[u][p][1][0] = acc[u][p][1][1] = 0ull;
+    for (int kb = t.kb0; kb < t.kb1; ++kb)
+#pragma unroll
+        for (int u = 0; u < kHalves; ++u)
+            if (!add_block<NP>(acc[u], e, (uint32_t)first, sy, a)) return false;
+    const int block = t.nt * 2 + (int)e.rank, col = block * 128 + quarter * 32;
+    if (e.parts > 1) {
+        const int out_n = GATE_UP ? a.N >> 1 : a.N;
+#pragma unroll
+        for (int u = 0; u < kHalves; ++u) store_part<NP>(acc[u], t, first, u * out_n + col, out_n - col, a);
+        return true;
+    }
+    if constexpr (GATE_UP) {
+        return store_quantized<NP>(acc[0], acc[1], t, e, first, block, sy, a);
+    } else {
+        store_rows<NP>(acc[0], t, e, first, col, a);
+        return true;
+    }
+}
+
 template <bool GATE_UP>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<GATE_UP>::kThreads, 1)
     grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x64,
                    const __grid_constant__ CUtensorMap map_x16, const Args a) {
+    using S = Shape<GATE_UP>;
+    constexpr int kHalves = S::kHalves;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t* base = smem_raw + ((1024u - (ptx::smem_u32(smem_raw) & 1023u)) & 1023u);
-    uint8_t* ring = base;
-    Sync* sy = reinterpret_cast<Sync*>(base + kRingBytes);
-    float* scales = reinterpret_cast<float*>(base + kRingBytes + kBarrierBytes);
+    uint8_t* ring = smem_raw + ((1024u - (ptx::smem_u32(smem_raw) & 1023u)) & 1023u);
+    Sync* sy = reinterpret_cast<Sync*>(ring + S::kRingBytes);
+    float* scales = reinterpret_cast<float*>(ring + S::kRingBytes + kBarrierBytes);
     uint8_t* strips = reinterpret_cast<uint8_t*>(scales) + kScaleRingBytes;
-    float* tops = reinterpret_cast<float*>(strips + kEpiWarps * kStripBytes);
-    int* row_start = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(tops) + kTopBytes);
+    float* tops = reinterpret_cast<float*>(strips + S::kEpiWarps * kStripBytes);
+    int* row_start = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(tops) + 2 * S::kTopBytes);
     int* prefix = row_start + kMaxExperts + 4;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = ptx::cluster_rank();
-    const int n_nt = GATE_UP ? a.N / 256 : (a.NB + 1) / 2;
+    const int n_nt = GATE_UP ? (a.N + 511) / 512 : (a.N + 255) / 256;
 
     load_row_starts(a.group_list, a.G, a.M, a.gl_type, row_start, nullptr, blockIdx.x == 0 ? a.findings : nullptr);
     if (warp == 0) {
@@ -427,13 +440,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             for (int i = 0; i < n; ++i) ptx::mbar_init(ptx::smem_u32(b + i), count);
         };
         init(sy->full, kMaxSlots, 1);
-        init(sy->empty, kMaxSlots, 1);
+        init(sy->empty, kMaxSlots, kHalves);
         init(sy->t_full, kMaxBufs, 2);
-        init(sy->t_empty, kMaxBufs, 2 * kEpiWarps);
-        init(sy->s_empty, kMaxBufs, kEpiWarps);
-        init(&sy->x_full, 1, kEpiWarps);
-        init(&sy->x_free, 1, kEpiWarps);
-        init(sy->wg, 2, 4);
+        init(sy->t_empty, kMaxBufs, 2 * S::kEpiWarps);
+        init(sy->s_empty, kMaxBufs, S::kEpiWarps);
+        init(sy->wg, S::kGroups, 4);
         init(sy->drain, 2, 1);
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&map_w);
@@ -451,11 +462,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sy->tmem_base);
     const int parts = sy->parts, n_units = sy->n_units, width = sy->width;
-    const int slot_bytes = kABytes + width * 64;
-    const int exchange_bytes = GATE_UP ? width * 256 : 0;
-    const int n_slots = min(kMaxSlots, (kRingBytes - exchange_bytes) / slot_bytes);
+    const int slot_bytes = kHalves * kABytes + width * 64;
+    const int n_slots = min(kMaxSlots, S::kRingBytes / slot_bytes);
     const int n_bufs = min(kMaxBufs, (int)kTmemCols / width);
-    uint8_t* exchange = ring + kRingBytes - exchange_bytes;
 
     if (warp < kWarpEpi0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
@@ -492,16 +501,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 publish();  // (a tile ahead: the other roles find it there)
                 if (!next_tile<true>(sy, seq, t, a, parts)) break;
                 const int half = t.n >> 1, n_big = half / kBigBox, n_small = (half % kBigBox) / kSmallBox;
-                const uint32_t bytes = 2u * (uint32_t)(kABytes + half * 128);
-                const int col = GATE_UP ? (int)rank * (a.N >> 1) + t.nt * 128 : t.nt * 256 + (int)rank * 128;
+                const uint32_t bytes = 2u * (uint32_t)(kHalves * kABytes + half * 128);
+                const int col = t.nt * 256 + (int)rank * 128;
                 const int row = t.row0 + (int)rank * half;
                 for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
                     if (it >= (uint32_t)n_slots && !wait<true>(&sy->empty[slot], ph ^ 1, sy, a.findings, 10)) { ok = false; break; }
                     if (leader) {
                         const uint32_t bar0 = full0 + slot * 8, dst = ptx::smem_u32(ring) + slot * (uint32_t)slot_bytes;
                         if (rank == 0) ptx::mbar_arrive_expect_tx(full_here + slot * 8, bytes);
-                        ptx::tma_load_3d_pair(dst, &map_w, bar0, col, kb * 128, t.g);
-                        uint32_t at = dst + kABytes;
+#pragma unroll
+                        for (int u = 0; u < kHalves; ++u)
+                            ptx::tma_load_3d_pair(dst + u * kABytes, &map_w, bar0, col + u * (a.N >> 1), kb * 128, t.g);
+                        uint32_t at = dst + kHalves * kABytes;
                         int r = row;
                         for (int b = 0; b < n_big; ++b, at += kBigBox * 128, r += kBigBox)
                             ptx::tma_load_2d_pair(at, &map_x64, bar0, kb * 128, r);
@@ -525,22 +536,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             __syncwarp();
         } else if (warp == kWarpScale) {
             // ------------------------------ scales ------------------------------
-            // Row scale times the tile's weight scale, in the order in which the epilogue's lanes take them: 16 tokens are four
-            // pieces of 16 bytes, piece q the tokens 2q, 2q + 1, 8 + 2q, 9 + 2q.
+            // Row scale times the block's weight scale.
             uint32_t seq = 0, it = 0, buf = 0, ph = 0;
-            float* home = scales + (lane & 16) + ((lane & 7) >> 1) * 4 + ((lane >> 3) & 1) * 2 + (lane & 1);
             bool ok = true;
             Tile t;
             while (ok && next_tile<true>(sy, seq, t, a, parts)) {
-                const int nb = min(a.NB - 1, GATE_UP ? (int)rank * (a.N >> 8) + t.nt : t.nt * 2 + (int)rank);
-                const float* ws = a.w_scale + (size_t)t.g * a.KB * a.NB + nb;
+                const float* ws = a.w_scale + (size_t)t.g * a.KB * a.NB;
+                int nb[kHalves];
+#pragma unroll
+                for (int u = 0; u < kHalves; ++u) nb[u] = min(a.NB - 1, t.nt * 2 + (int)rank + u * (a.NB >> 1));
                 const float* xs = a.x_scale + (size_t)(t.row0 + lane) * a.KB;
                 const size_t group = (size_t)a.KB * 32;
-                for (int kb = t.kb0; kb < t.kb1 && ok; kb += 4) {  // (four blocks' loads in flight)
-                    float w[4], v[kMaxR / 32][4];
+                for (int kb = t.kb0; kb < t.kb1 && ok; kb += 4) {  // (four stages' loads in flight)
+                    float w[4][kHalves], v[kMaxR / 32][4];
                     const int last = t.kb1 - 1 - kb;
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) w[b] = __ldg(ws + (size_t)(kb + min(b, last)) * a.NB);
+                    for (int b = 0; b < 4; ++b)
+#pragma unroll
+                        for (int u = 0; u < kHalves; ++u) w[b][u] = __ldg(ws + (size_t)(kb + min(b, last)) * a.NB + nb[u]);
 #pragma unroll
                     for (int g = 0; g < kMaxR / 32; ++g)
                         if (g * 32 < t.n) {
@@ -551,16 +564,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int b = 0; b < 4; ++b) {
                         if (b > last || !ok) break;
-                        if (it >= (uint32_t)n_bufs) ok = wait<true>(&sy->s_empty[buf], ph ^ 1, sy, a.findings, 20);
-                        if (!ok) break;
-                        float* dst = home + buf * (uint32_t)width;
 #pragma unroll
-                        for (int g = 0; g < kMaxR / 32; ++g)
-                            if (g * 32 < t.n) dst[g * 32] = v[g][b] * w[b];
-                        __syncwarp();
-                        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->t_full[buf]));
-                        ++it;
-                        if (++buf == (uint32_t)n_bufs) { buf = 0; ph ^= 1; }
+                        for (int u = 0; u < kHalves; ++u) {
+                            if (ok && it >= (uint32_t)n_bufs) ok = wait<true>(&sy->s_empty[buf], ph ^ 1, sy, a.findings, 20);
+                            if (!ok) break;
+                            float* dst = scales + buf * (uint32_t)width + lane;
+#pragma unroll
+                            for (int g = 0; g < kMaxR / 32; ++g)
+                                if (g * 32 < t.n) dst[g * 32] = v[g][b] * w[b][u];
+                            __syncwarp();
+                            if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->t_full[buf]));
+                            ++it;
+                            if (++buf == (uint32_t)n_bufs) { buf = 0; ph ^= 1; }
+                        }
                     }
                 }
             }
@@ -572,29 +588,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             uint32_t seq = 0, it = 0, slot = 0, ph = 0, buf = 0, tph = 0;
             bool ok = true;
             const uint64_t da0 = ptx::umma_desc_sw128(ptx::smem_u32(ring), kABytes, 1024);
-            const uint64_t db0 = ptx::umma_desc_sw128(ptx::smem_u32(ring) + kABytes, 0, 1024);
+            const uint64_t db0 = ptx::umma_desc_sw128(ptx::smem_u32(ring) + kHalves * kABytes, 0, 1024);
             Tile t;
             while (ok && next_tile<true>(sy, seq, t, a, parts)) {
                 const uint32_t idesc = ptx::umma_idesc_e4m3_mn_k(256, t.n);
-                for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
-                    if ((it & 1) == turn) {
-                        // the epilogue of both CTAs has taken what the buffer held
-                        if (it >= (uint32_t)n_bufs && !wait<true>(&sy->t_empty[buf], tph ^ 1, sy, a.findings, 30)) { ok = false; break; }
-                        if (!wait<true>(&sy->full[slot], ph, sy, a.findings, 40)) { ok = false; break; }
-                        ptx::tc_fence_after();
-                        if (leader) {
-                            const uint64_t at = (uint64_t)(slot * (uint32_t)slot_bytes >> 4);
+                for (int kb = t.kb0; kb < t.kb1 && ok; ++kb) {
 #pragma unroll
-                            for (int k32 = 0; k32 < 4; ++k32)
-                                ptx::umma_f8_pair(tmem_base + buf * (uint32_t)width, da0 + at + (uint64_t)(k32 * 256),
-                                                  db0 + at + (uint64_t)(k32 * 2), idesc, (uint32_t)(k32 != 0));
-                            ptx::umma_commit_pair(ptx::smem_u32(&sy->t_full[buf]));
-                            ptx::umma_commit_pair(ptx::smem_u32(&sy->empty[slot]));
+                    for (int u = 0; u < kHalves; ++u, ++it) {
+                        if ((it & 1) == turn) {
+                            // the epilogue of both CTAs has taken what the buffer held
+                            if (it >= (uint32_t)n_bufs && !wait<true>(&sy->t_empty[buf], tph ^ 1, sy, a.findings, 30)) { ok = false; break; }
+                            if (!wait<true>(&sy->full[slot], ph, sy, a.findings, 40)) { ok = false; break; }
+                            ptx::tc_fence_after();
+                            if (leader) {
+                                const uint64_t at = (uint64_t)(slot * (uint32_t)slot_bytes >> 4);
+#pragma unroll
+                                for (int k32 = 0; k32 < 4; ++k32)
+                                    ptx::umma_f8_pair(tmem_base + buf * (uint32_t)width, da0 + at + (uint64_t)(u * (kABytes >> 4) + k32 * 256),
+                                                      db0 + at + (uint64_t)(k32 * 2), idesc, (uint32_t)(k32 != 0));
+                                ptx::umma_commit_pair(ptx::smem_u32(&sy->t_full[buf]));
+                                ptx::umma_commit_pair(ptx::smem_u32(&sy->empty[slot]));
+                            }
+                            __syncwarp();
                         }
-                        __syncwarp();
+                        if (++buf == (uint32_t)n_bufs) { buf = 0; tph ^= 1; }
                     }
                     if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
-                    if (++buf == (uint32_t)n_bufs) { buf = 0; tph ^= 1; }
                 }
             }
             // every MMA issued here must have completed before tensor and shared memory go
@@ -607,31 +626,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         // ------------------------------ epilogue ------------------------------
-        EpilogueState e;
+        Epilogue e;
         e.warp = warp - kWarpEpi0;
+        e.parts = parts;
         e.rank = rank;
-        e.buf = e.ph = e.tiles = 0;
+        e.buf = e.ph = e.wg_ph = 0;
         e.n_bufs = (uint32_t)n_bufs;
         e.width = (uint32_t)width;
-        e.parts = parts;
         e.tmem = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
         e.t_empty = ptx::map_rank(ptx::smem_u32(sy->t_empty), 0);
         e.scales = scales;
         e.strip = strips + e.warp * kStripBytes;
-        e.exchange = exchange;
         e.tops = tops;
+        e.quantizers = tops + S::kTopBytes / 4;
         uint32_t seq = 0;
         bool ok = true;
         Tile t;
         while (ok && next_tile<true>(sy, seq, t, a, parts)) {
-            switch (t.n >> 5) {  // chunks of 16 tokens a warp has
-                case 1: ok = finish_tile<GATE_UP, 1>(t, e, sy, a); break;
-                case 2: ok = finish_tile<GATE_UP, 2>(t, e, sy, a); break;
-                case 3: ok = finish_tile<GATE_UP, 3>(t, e, sy, a); break;
-                case 4: ok = finish_tile<GATE_UP, 4>(t, e, sy, a); break;
-                default: ok = finish_tile<GATE_UP, 5>(t, e, sy, a); break;
+            switch (t.n >> 5) {
+                case 1: ok = finish_tile<GATE_UP, 1 * S::kUnit>(t, e, sy, a); break;
+                case 2: ok = finish_tile<GATE_UP, 2 * S::kUnit>(t, e, sy, a); break;
+                case 3: ok = finish_tile<GATE_UP, 3 * S::kUnit>(t, e, sy, a); break;
+                case 4: ok = finish_tile<GATE_UP, 4 * S::kUnit>(t, e, sy, a); break;
+                default: ok = finish_tile<GATE_UP, 5 * S::kUnit>(t, e, sy, a); break;
             }
-            ++e.tiles;
         }
     }
 
@@ -682,7 +700,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a) {
 // Whether a call can have fewer tiles than there are pairs of multiprocessors, and in how many parts its k range is cut at most: parts of
 // four blocks or more, sums of 32 MB or less.
 static int max_parts(int64_t M, int64_t K, int64_t N, int64_t G, int gate_up) {
-    const int64_t n_nt = (N + 255) / 256, experts = std::min(G, M);
+    const int64_t width = gate_up ? 512 : 256, n_nt = (N + width - 1) / width, experts = std::min(G, M);
     if (experts * n_nt >= 74) return 1;
     const int64_t kb = (K + 127) / 128, room = (32ll << 20) / (M * N * 4);
     return (int)std::max<int64_t>(1, std::min<int64_t>({16, kb / 4, room}));
@@ -742,7 +760,7 @@ extern "C" int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scal
     B200MOE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, fb::kSmemBytes));
     a.dynamic = ((N + 255) / 256) * std::min(G, M) >= 8 * (int64_t)grid;
     if (a.dynamic) B200MOE_CUDA_TRY(cudaMemsetAsync(workspace, 0, fb::kWordBytes, st));
-    kernel<<<grid, fb::kThreads, fb::kSmemBytes, st>>>(map_w, map_x64, map_x16, a);
+    kernel<<<grid, gate_up_silu ? fb::Shape<true>::kThreads : fb::Shape<false>::kThreads, fb::kSmemBytes, st>>>(map_w, map_x64, map_x16, a);
     B200MOE_CUDA_TRY(cudaGetLastError());
     if (a.max_parts > 1) {
         const int64_t out_n = gate_up_silu ? N / 2 : N;
