@@ -29,7 +29,7 @@ EXPORTS = [
     "b200moe_fp4_dequant_bf16_scale", "b200moe_fp8_dequant", "b200moe_fp4_scale_fold",
     "b200moe_silu_mul_dyn", "b200moe_grouped_gemm_int8_silu", "b200moe_grouped_gemm_fp4_e8m0", "b200moe_pack_weight_int8", "b200moe_grouped_gemm_int8_packed", "b200moe_grouped_gemm_int8_packed_scatter",
     "b200moe_fp8_quantize_rows", "b200moe_grouped_gemm_fp8_block", "b200moe_grouped_gemm_fp8_block_workspace_bytes",
-    "b200moe_moe_balance_scratch_bytes", "b200moe_moe_balance_loss", "b200moe_moe_balance_loss_grad",
+    "b200moe_moe_balance_scratch_bytes", "b200moe_moe_balance_loss", "b200moe_moe_balance_loss_grad", "b200moe_read_findings",
     "b200moe_set_gemm_reserved_sms", "b200moe_ipc_alloc", "b200moe_ipc_open", "b200moe_ipc_close", "b200moe_ipc_free",
 ]
 
@@ -122,14 +122,16 @@ def _load() -> ctypes.CDLL:
     lib.b200moe_fp8_quantize_rows.restype = i32
     lib.b200moe_grouped_gemm_fp8_block_workspace_bytes.argtypes = [i64, i64, i64, i64, i32]
     lib.b200moe_grouped_gemm_fp8_block_workspace_bytes.restype = sz
-    lib.b200moe_grouped_gemm_fp8_block.argtypes = [vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i32, i32, vp, sz, vp, vp]
+    lib.b200moe_grouped_gemm_fp8_block.argtypes = [vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i32, i32, vp, sz, vp]
     lib.b200moe_grouped_gemm_fp8_block.restype = i32
     lib.b200moe_moe_balance_scratch_bytes.argtypes = [i64, i64, i64]
     lib.b200moe_moe_balance_scratch_bytes.restype = sz
-    lib.b200moe_moe_balance_loss.argtypes = [vp, i32, vp, vp, vp, i64, i64, i64, i64, vp, vp, vp, vp, vp, sz, vp, vp]
+    lib.b200moe_moe_balance_loss.argtypes = [vp, i32, vp, vp, vp, i64, i64, i64, i64, vp, vp, vp, vp, vp, sz, vp]
     lib.b200moe_moe_balance_loss.restype = i32
     lib.b200moe_moe_balance_loss_grad.argtypes = [vp, i32, vp, vp, vp, vp, vp, i64, i64, i64, vp, vp]
     lib.b200moe_moe_balance_loss_grad.restype = i32
+    lib.b200moe_read_findings.argtypes = [ctypes.POINTER(ctypes.c_int32), i32, vp]
+    lib.b200moe_read_findings.restype = i32
     u64, comm = ctypes.c_uint64, ctypes.POINTER(EpComm)
     lib.b200moe_ep_post_counts.argtypes = [comm, vp, u64, vp]
     lib.b200moe_ep_dispatch.argtypes = [comm, vp, vp, i64, u64, vp, vp, vp, vp, vp]

@@ -9,7 +9,7 @@ were never published (``ascend-closed/README.md``).
 """
 REFERENCE_OPS = ["grouped_soft_gemv", "grouped_gemm"]                     # pybind.cpp:14-19 of the reference
 ADDED_OPS = ["fp4_dequant", "fp4_dequant_bf16_scale", "fp8_dequant", "fp4_scale_fold", "pack_weight_int8",
-             "grouped_gemm_packed", "last_status", "check_status"]
+             "grouped_gemm_packed", "fp8_quantize_rows", "grouped_gemm_fp8_block", "moe_balance_loss", "last_status", "check_status"]
 
 
 def check(verbose: bool = True) -> None:

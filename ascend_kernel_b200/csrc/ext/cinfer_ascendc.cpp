@@ -13,6 +13,7 @@
 #include <mutex>
 #include <stdexcept>
 #include <string>
+#include <tuple>
 #include <utility>
 #include <vector>
 
@@ -103,6 +104,12 @@ std::pair<int, int> LastStatus(bool clear) {
     };
     for (auto& kv : g_workspaces) read(kv.first, kv.second);
     for (auto& kv : g_kept_workspaces) read(kv.first, kv.second);
+    // what the operators without a workspace of status words found (their streams: all of the device's)
+    int32_t kept[2] = {0, 0};
+    TORCH_CHECK(cudaDeviceSynchronize() == cudaSuccess, "cudaDeviceSynchronize failed");
+    const int rc = b200moe_read_findings(kept, clear ? 1 : 0, c10::cuda::getCurrentCUDAStream().stream());
+    TORCH_CHECK(rc == B200MOE_OK, "read_findings: ", b200moe_strerror(rc));
+    if (found.first == 0 && kept[0] != 0) found = {kept[0], kept[1]};
     return found;
 }
 
@@ -314,6 +321,148 @@ at::Tensor Fp4ScaleFold(at::Tensor block_scale, at::Tensor global_scale) {
     return out;
 }
 
+// ---- rows and experts in 8-bit floats with a scale per block of 128, and the router's balance loss -----------------------
+
+using OptionalTensor = c10::optional<at::Tensor>;
+
+const at::Tensor* given(const OptionalTensor& t, const char* name, const at::Tensor& like) {
+    if (!t.has_value() || !t->defined()) return nullptr;
+    check_tensor(*t, name);
+    TORCH_CHECK(t->device() == like.device(), name, " is on another device");
+    return &*t;
+}
+void check_beside(const at::Tensor& t, const char* name, const at::Tensor& like) {
+    check_tensor(t, name);
+    TORCH_CHECK(t.device() == like.device(), name, " is on another device");
+}
+void check_e4m3(const at::Tensor& t, const char* name, int64_t dim) {
+    TORCH_CHECK((t.scalar_type() == at::kByte || t.scalar_type() == at::kFloat8_e4m3fn) && t.dim() == dim, name, " must be ", dim,
+                "-dimensional e4m3 codes (uint8 or float8_e4m3fn)");
+}
+void check_f32(const at::Tensor& t, const char* name, at::IntArrayRef shape) {
+    TORCH_CHECK(t.scalar_type() == at::kFloat && t.sizes() == shape, name, " must be float32 of shape ", shape, ", got ",
+                t.scalar_type(), " ", t.sizes());
+}
+int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
+
+std::tuple<at::Tensor, at::Tensor> Fp8QuantizeRows(const at::Tensor& x, const OptionalTensor& index_opt, const OptionalTensor& codes_opt,
+                                                   const OptionalTensor& scale_opt) {
+    check_tensor(x, "x");
+    TORCH_CHECK(x.dim() == 2 && x.scalar_type() == at::kBFloat16, "x must be bfloat16 [T, K]");
+    const at::Tensor* index = given(index_opt, "index", x);
+    TORCH_CHECK(!index || (index->scalar_type() == at::kInt && index->dim() == 1), "index must be int32 [R]");
+    const int64_t T = x.size(0), K = x.size(1), R = index ? index->numel() : T, KB = blocks_of(K);
+    c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor* codes_in = given(codes_opt, "codes", x);
+    const at::Tensor* scale_in = given(scale_opt, "scale", x);
+    at::Tensor codes = codes_in ? *codes_in : at::empty({R, K}, x.options().dtype(at::kByte));
+    at::Tensor scale = scale_in ? *scale_in : at::empty({R, KB}, x.options().dtype(at::kFloat));
+    check_e4m3(codes, "codes", 2);
+    TORCH_CHECK(codes.size(0) == R && codes.size(1) == K, "codes must be [", R, ", ", K, "]");
+    check_f32(scale, "scale", {R, KB});
+    raise_on(b200moe_fp8_quantize_rows(x.data_ptr(), index ? index->data_ptr<int32_t>() : nullptr, codes.data_ptr(),
+                                       scale.data_ptr<float>(), T, R, K, c10::cuda::getCurrentCUDAStream().stream()),
+             "fp8_quantize_rows");
+    return {codes, scale};
+}
+
+void GroupedGemmFp8Block(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& weight, const at::Tensor& weight_scale,
+                         const at::Tensor& group_list, const at::Tensor& output, const OptionalTensor& output_scale_opt,
+                         int64_t group_list_type, bool gate_up_silu) {
+    check_tensor(x, "x");
+    check_beside(x_scale, "x_scale", x); check_beside(weight, "weight", x); check_beside(weight_scale, "weight_scale", x);
+    check_beside(group_list, "group_list", x); check_beside(output, "output", x);
+    const at::Tensor* output_scale = given(output_scale_opt, "output_scale", x);
+    check_e4m3(x, "x", 2);
+    check_e4m3(weight, "weight", 3);
+    TORCH_CHECK(group_list.scalar_type() == at::kLong, "group_list must be int64");
+    const int64_t M = x.size(0), K = x.size(1), G = weight.size(0), N = weight.size(2);
+    TORCH_CHECK(weight.size(1) == K && group_list.numel() == G, "shape mismatch: x ", x.sizes(), ", weight ", weight.sizes(),
+                ", group_list ", group_list.numel());
+    check_f32(x_scale, "x_scale", {M, blocks_of(K)});
+    check_f32(weight_scale, "weight_scale", {G, blocks_of(K), blocks_of(N)});
+    if (gate_up_silu) {
+        TORCH_CHECK(N % 256 == 0, "gate_up_silu needs N to be a multiple of 256");
+        check_e4m3(output, "output", 2);
+        TORCH_CHECK(output.size(0) == M && output.size(1) == N / 2 && output_scale, "output must be [", M, ", ", N / 2,
+                    "], with an output_scale");
+        check_f32(*output_scale, "output_scale", {M, N / 256});
+    } else {
+        TORCH_CHECK(output.scalar_type() == at::kBFloat16 && output.dim() == 2 && output.size(0) == M && output.size(1) == N &&
+                    !output_scale, "output must be bfloat16 [", M, ", ", N, "], without output_scale");
+    }
+    TORCH_CHECK(group_list_type == 0 || group_list_type == 1, "group_list_type must be 0 or 1");
+    c10::cuda::CUDAGuard guard(x.device());
+    // a workspace for this call alone: two graphs captured on one stream may be replayed side by side
+    const size_t bytes = b200moe_grouped_gemm_fp8_block_workspace_bytes(M, K, N, G, gate_up_silu ? 1 : 0);
+    at::Tensor workspace = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+    raise_on(b200moe_grouped_gemm_fp8_block(x.data_ptr(), x_scale.data_ptr<float>(), weight.data_ptr(), weight_scale.data_ptr<float>(),
+                                            group_list.data_ptr<int64_t>(), output.data_ptr(),
+                                            output_scale ? output_scale->data_ptr<float>() : nullptr, M, K, N, G, (int)group_list_type,
+                                            gate_up_silu ? 1 : 0, workspace.data_ptr(), bytes,
+                                            c10::cuda::getCurrentCUDAStream().stream()),
+             "grouped_gemm_fp8_block");
+}
+
+struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& idx,
+                                                  const OptionalTensor& seq_opt, const OptionalTensor& mask_opt) {
+        const at::Tensor* seq = given(seq_opt, "seq_list", logits);
+        const at::Tensor* mask = given(mask_opt, "token_mask", logits);
+        const int64_t T = logits.size(0), E = logits.size(1), S = seq ? seq->numel() : 1;
+        c10::cuda::CUDAGuard guard(logits.device());
+        const auto f32 = logits.options().dtype(at::kFloat);
+        at::Tensor loss = at::empty({S}, f32), counts = at::empty({S, E}, f32.dtype(at::kLong));
+        at::Tensor kept = at::empty({S * (E + 1)}, f32);  // the load per sequence and expert, and the reciprocals of the token numbers
+        const size_t bytes = b200moe_moe_balance_scratch_bytes(T, E, S);
+        at::Tensor scratch = at::empty({(int64_t)bytes}, f32.dtype(at::kByte));
+        float* load = kept.data_ptr<float>();
+        raise_on(b200moe_moe_balance_loss(logits.data_ptr(), logits.scalar_type() == at::kFloat ? 1 : 0, idx.data_ptr<int32_t>(),
+                                          seq ? seq->data_ptr<int64_t>() : nullptr,
+                                          mask ? static_cast<const uint8_t*>(mask->data_ptr()) : nullptr, T, E, idx.size(1), S,
+                                          loss.data_ptr<float>(), counts.data_ptr<int64_t>(), load, load + S * E, scratch.data_ptr(),
+                                          bytes, c10::cuda::getCurrentCUDAStream().stream()),
+                 "moe_balance_loss");
+        ctx->save_for_backward({logits, seq ? *seq : at::Tensor(), mask ? *mask : at::Tensor(), kept});
+        ctx->mark_non_differentiable({counts});
+        return {loss, counts};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "moe_balance_loss is differentiable once");
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &logits = saved[0], &seq = saved[1], &mask = saved[2], &kept = saved[3];
+        if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+        const int64_t T = logits.size(0), E = logits.size(1), S = kept.numel() / (E + 1);
+        c10::cuda::CUDAGuard guard(logits.device());
+        const at::Tensor g = grads[0].to(at::kFloat).contiguous();
+        at::Tensor out = at::empty_like(logits);
+        const float* load = kept.data_ptr<float>();
+        raise_on(b200moe_moe_balance_loss_grad(logits.data_ptr(), logits.scalar_type() == at::kFloat ? 1 : 0,
+                                               seq.defined() ? seq.data_ptr<int64_t>() : nullptr,
+                                               mask.defined() ? static_cast<const uint8_t*>(mask.data_ptr()) : nullptr, load,
+                                               load + S * E, g.data_ptr<float>(), T, E, S, out.data_ptr(),
+                                               c10::cuda::getCurrentCUDAStream().stream()),
+                 "moe_balance_loss (gradient)");
+        return {out, at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
+std::tuple<at::Tensor, at::Tensor> MoeBalanceLoss(const at::Tensor& logits, const at::Tensor& idx, const OptionalTensor& seq_opt,
+                                                  const OptionalTensor& mask_opt) {
+    check_tensor(logits, "logits");
+    check_beside(idx, "idx", logits);
+    TORCH_CHECK(logits.dim() == 2 && (logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat),
+                "logits must be bfloat16 or float32 [T, E]");
+    const int64_t T = logits.size(0);
+    TORCH_CHECK(idx.scalar_type() == at::kInt && idx.dim() == 2 && idx.size(0) == T, "idx must be int32 [", T, ", k]");
+    const at::Tensor* seq = given(seq_opt, "seq_list", logits);
+    TORCH_CHECK(!seq || (seq->scalar_type() == at::kLong && seq->dim() == 1), "seq_list must be int64 [S]");
+    const at::Tensor* mask = given(mask_opt, "token_mask", logits);
+    TORCH_CHECK(!mask || (mask->scalar_type() == at::kBool && mask->dim() == 1 && mask->size(0) == T), "token_mask must be bool [", T, "]");
+    auto out = BalanceLoss::apply(logits, idx, seq_opt, mask_opt);
+    return {out[0], out[1]};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -334,6 +483,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "antiquantOffsetOptional"_a, "groupListOptional"_a, "output"_a, "group_list_type"_a = 0, "gate_up_silu"_a = false,
           "GROUP GEMM on int8 weights repacked once.");
     m.def("fp4_scale_fold", &Fp4ScaleFold, "block_scale"_a, "global_scale"_a, "Two-level FP4 scale fold.");
+    m.def("fp8_quantize_rows", &Fp8QuantizeRows, "x"_a, "index"_a = pybind11::none(), "codes"_a = pybind11::none(),
+          "scale"_a = pybind11::none(), "bf16 rows -> (e4m3 codes, fp32 scale per 128), optionally gathered by an index.");
+    m.def("grouped_gemm_fp8_block", &GroupedGemmFp8Block, "x"_a, "x_scale"_a, "weight"_a, "weight_scale"_a, "group_list"_a, "output"_a,
+          "output_scale"_a = pybind11::none(), "group_list_type"_a = 0, "gate_up_silu"_a = false,
+          "GROUP GEMM on e4m3 rows and e4m3 weights with scales per block of 128.");
+    m.def("moe_balance_loss", &MoeBalanceLoss, "logits"_a, "idx"_a, "seq_list"_a = pybind11::none(), "token_mask"_a = pybind11::none(),
+          "(balance loss per sequence, pairs per sequence and expert), differentiable in the logits.");
     m.def("last_status", [](bool clear) { return LastStatus(clear); }, "clear"_a = false,
           "(code, detail) of the first device-side finding since the status was last cleared.");
     m.def("check_status", &CheckStatus, "Raises if an operator call left a device-side finding (and clears it).");

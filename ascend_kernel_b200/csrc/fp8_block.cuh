@@ -14,36 +14,37 @@ constexpr float kFloor = 0x1p-100f;      // a block's largest magnitude counts a
 
 // code = e4m3_rne(x * 448 / a), and where x and a are bf16 values the codes are those of the exact quotient: x * 448 and a are then
 // integers of at most 11 and 8 bits times powers of two, so a quotient that is no tie of e4m3 is at least 2^-13 (relative) away
-// from one, and one that is a tie has at most five bits and comes out of the correction step as it is (r, the remainder, is
-// exact, and what the step leaves is of the second order in a first guess good to 2^-22).
+// from one, and one that is a tie has at most five bits and comes out of the correction step as it is: the first guess
+// is good to about 2^-21, its remainder is exact (11 bits), and what the step leaves is of the second order.
+// x * 448 / a = x' / a' with x' = x * 7 * 2^-4 and a' = a * 2^-10: neither product overflows, and neither is rounded where it matters.
 struct Quantizer {
     float scale;
-    float inv_, a_, step_;  // 448 / a, a * 2^-10, 2^10 / a
-    bool finite_;
+    float a, inv;  // a', 1 / a' (0 for a block that is not finite: its codes are 0)
     // `top`: the largest magnitude of the block, or infinity / NaN where the block holds one
     __device__ __forceinline__ explicit Quantizer(float top) {
-        finite_ = top < INFINITY;
-        const float a = fmaxf(top, kFloor);
-        scale = finite_ ? a / kMax : __uint_as_float(0x7FC00000u);
-        inv_ = finite_ ? kMax / a : 0.f;
-        a_ = a * 0x1p-10f;
-        step_ = inv_ * (1024.f / kMax);
+        const bool finite = top < INFINITY;
+        const float m = fmaxf(top, kFloor);
+        a = m * 0x1p-10f;
+        inv = finite ? __fdividef(1.f, a) : 0.f;
+        // m / 448 by the same correction step (for bf16 m the quotient rounded to nearest, which the tests check for all of them)
+        constexpr float kInv = 1.f / kMax;
+        const float q = m * kInv;
+        scale = finite ? fmaf(fmaf(-q, kMax, m), kInv, q) : __uint_as_float(0x7FC00000u);
     }
-    // what four() needs, for a thread that did not see the block's magnitude
-    __device__ __forceinline__ float4 packed() const { return make_float4(inv_, a_, step_, finite_ ? 1.f : 0.f); }
-    __device__ __forceinline__ explicit Quantizer(const float4& p) : scale(0.f), inv_(p.x), a_(p.y), step_(p.z), finite_(p.w != 0.f) {}
-    __device__ __forceinline__ float ratio(float x) const {
-        // x * 448 / a = (x * 7 * 2^-4) / (a * 2^-10): neither product overflows, and neither is rounded where it matters
-        const float q = x * inv_;
-        const float r = fmaf(-q, a_, x * 0.4375f);
-        return fmaf(r, step_, q);
+    // what codes2() needs, for a thread that did not see the block's magnitude
+    __device__ __forceinline__ float2 packed() const { return make_float2(a, inv); }
+    __device__ __forceinline__ explicit Quantizer(const float2& p) : scale(0.f), a(p.x), inv(p.y) {}
+    // two codes, the first value's in the low byte
+    __device__ __forceinline__ uint32_t codes2(f32x2 x) const {
+        const f32x2 inv2 = pack_f32x2(inv, inv), a2 = pack_f32x2(-a, -a);
+        x = mul_f32x2(x, pack_f32x2(0.4375f, 0.4375f));
+        const f32x2 q = mul_f32x2(x, inv2);
+        const f32x2 y = fma_f32x2(fma_f32x2(q, a2, x), inv2, q);
+        uint16_t o;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(o) : "f"(f32x2_hi(y)), "f"(f32x2_lo(y)));
+        return o;
     }
-    __device__ __forceinline__ uint32_t four(float x0, float x1, float x2, float x3) const {
-        if (!finite_) return 0u;
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(ratio(x0), ratio(x1)), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(ratio(x2), ratio(x3)), __NV_SATFINITE, __NV_E4M3);
-        return lo | (hi << 16);
-    }
+    __device__ __forceinline__ bool finite() const { return inv != 0.f; }
 };
 
 }  // namespace fp8_block

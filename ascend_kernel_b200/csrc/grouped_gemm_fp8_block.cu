@@ -48,7 +48,7 @@ struct Shape {
     static constexpr int kHalves = GATE_UP ? 2 : 1;  // blocks of a stage
     static constexpr int kGroups = 2, kEpiWarps = 4 * kGroups, kThreads = (kWarpEpi0 + kEpiWarps) * 32;
     static constexpr int kUnit = 32 / (8 * kGroups);  // 8-token patches of a warp per 32 token rows: 1 or 2
-    static constexpr int kTopBytes = GATE_UP ? kMaxR * 16 : 0;  // [tokens][4 warps] magnitudes, and as much for what they give
+    static constexpr int kTopBytes = GATE_UP ? kMaxR * 16 : 0;  // [tokens][4 warps] magnitudes, and less for what they give
     static constexpr int kFixedBytes = 1024 + kBarrierBytes + kScaleRingBytes + kEpiWarps * kStripBytes + 2 * kTopBytes + 2 * (kMaxExperts + 4) * 4;
     static constexpr int kRingBytes = kSmemBytes - kFixedBytes;
     static_assert(kRingBytes % 16 == 0 && kRingBytes >= 4 * (kHalves * kABytes + kMaxR * 64), "stages");
@@ -326,7 +326,7 @@ __device__ __forceinline__ bool store_quantized(f32x2 (&gate)[NP][2][2], const f
         const int token = first + mine;
         const uint4 m = reinterpret_cast<const uint4*>(e.tops)[token];
         const fp8_block::Quantizer qz(__uint_as_float(max(max(m.x, m.y), max(m.z, m.w))));
-        reinterpret_cast<float4*>(e.quantizers)[token] = qz.packed();
+        reinterpret_cast<float2*>(e.quantizers)[token] = qz.packed();
         if (inside && token < t.rows) a.out_scale[(size_t)(t.row0 + token) * blocks + block] = qz.scale;
     }
     if (!meet()) return false;
@@ -337,11 +337,11 @@ __device__ __forceinline__ bool store_quantized(f32x2 (&gate)[NP][2][2], const f
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                const fp8_block::Quantizer qz(reinterpret_cast<const float4*>(e.quantizers)[first + (p + j) * 8 + 2 * q + b]);
+                const fp8_block::Quantizer qz(reinterpret_cast<const float2*>(e.quantizers)[first + (p + j) * 8 + 2 * q + b]);
                 float h[4];
 #pragma unroll
                 for (int m = 0; m < 4; ++m) h[m] = b ? f32x2_hi(gate[p + j][m >> 1][m & 1]) : f32x2_lo(gate[p + j][m >> 1][m & 1]);
-                const uint32_t o = qz.four(h[0], h[1], h[2], h[3]);
+                const uint32_t o = qz.finite() ? qz.codes2(pack_f32x2(h[0], h[1])) | (qz.codes2(pack_f32x2(h[2], h[3])) << 16) : 0u;
                 uint8_t* at = e.strip + (j * 8 + 2 * q + b) * 32 + g8;
                 at[0] = (uint8_t)o;
                 at[8] = (uint8_t)(o >> 8);
@@ -692,7 +692,8 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(h[i]) & 0x7FFFFFFFu);
         const fp8_block::Quantizer q(__uint_as_float(__reduce_max_sync(0xffffffffu, m)));
-        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + (size_t)row * out_n + col) = q.four(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + (size_t)row * out_n + col) =
+            q.finite() ? q.codes2(pack_f32x2(h[0], h[1])) | (q.codes2(pack_f32x2(h[2], h[3])) << 16) : 0u;
         if (lane == 0) a.out_scale[(size_t)row * blocks + nb] = q.scale;
     }
 }
@@ -720,7 +721,7 @@ extern "C" size_t b200moe_grouped_gemm_fp8_block_workspace_bytes(int64_t M, int6
 extern "C" int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scale, const void* weight, const float* weight_scale,
                                               const int64_t* group_list, void* out, float* out_scale, int64_t M, int64_t K, int64_t N,
                                               int64_t G, int group_list_type, int gate_up_silu, void* workspace,
-                                              size_t workspace_bytes, int32_t* findings, void* stream) {
+                                              size_t workspace_bytes, void* stream) {
     if (M < 0 || K <= 0 || N <= 0 || G <= 0 || G > kMaxExperts || (K % 16) != 0 || (N % 16) != 0 || M > 0x3FFFFFFFLL ||
         K > 0x3FFFFFFFLL || N > 0x3FFFFFFFLL || (gate_up_silu && (N % 256) != 0))
         return B200MOE_ERR_SHAPE;
@@ -747,7 +748,7 @@ extern "C" int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scal
     a.KB = (int)((K + 127) / 128);
     a.NB = (int)((N + 127) / 128);
     a.words = static_cast<int*>(workspace);
-    a.findings = findings;
+    a.findings = findings_words();
     a.max_parts = fb::max_parts(M, K, N, G, gate_up_silu);
     if (a.max_parts > 1) a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + fb::kWordBytes);
     CUtensorMap map_w, map_x64, map_x16;

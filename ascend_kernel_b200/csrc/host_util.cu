@@ -21,6 +21,22 @@ int sm_count() {
     return cached[dev];
 }
 
+__device__ int g_findings[2];
+
+int* findings_words() {
+    static int* cached[64];
+    static std::mutex mu;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    std::lock_guard<std::mutex> lock(mu);
+    if (cached[dev] == nullptr) {
+        void* p = nullptr;
+        if (cudaGetSymbolAddress(&p, g_findings) == cudaSuccess) cached[dev] = static_cast<int*>(p);
+        else (void)cudaGetLastError();
+    }
+    return cached[dev];
+}
+
 static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
     static std::once_flag once;
@@ -68,6 +84,8 @@ int make_tensor_map_3d_u8(CUtensorMap* out, const void* base, uint64_t outer, ui
 
 }  // namespace b200moe
 
+using namespace b200moe;
+
 extern "C" {
 
 const char* b200moe_strerror(int code) {
@@ -102,6 +120,17 @@ int b200moe_read_sticky_status(void* workspace, int32_t out[2], int clear, void*
     B200MOE_CUDA_TRY(cudaMemcpyAsync(out, static_cast<const uint8_t*>(workspace) + 16, 2 * sizeof(int32_t),
                                      cudaMemcpyDeviceToHost, s));
     if (clear) B200MOE_CUDA_TRY(cudaMemsetAsync(static_cast<uint8_t*>(workspace) + 16, 0, 8, s));
+    B200MOE_CUDA_TRY(cudaStreamSynchronize(s));
+    return B200MOE_OK;
+}
+
+int b200moe_read_findings(int32_t out[2], int clear, void* stream) {
+    if (out == nullptr) return B200MOE_ERR_NULL_POINTER;
+    int* words = findings_words();
+    if (words == nullptr) return B200MOE_ERR_CUDA;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    B200MOE_CUDA_TRY(cudaMemcpyAsync(out, words, 2 * sizeof(int32_t), cudaMemcpyDeviceToHost, s));
+    if (clear) B200MOE_CUDA_TRY(cudaMemsetAsync(words, 0, 2 * sizeof(int32_t), s));
     B200MOE_CUDA_TRY(cudaStreamSynchronize(s));
     return B200MOE_OK;
 }

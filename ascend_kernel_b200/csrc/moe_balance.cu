@@ -359,7 +359,7 @@ extern "C" size_t b200moe_moe_balance_scratch_bytes(int64_t n_tokens, int64_t n_
 extern "C" int b200moe_moe_balance_loss(const void* logits, int logits_fp32, const int32_t* idx, const int64_t* seq_list,
                                         const uint8_t* token_mask, int64_t n_tokens, int64_t n_experts, int64_t top_k, int64_t n_seqs,
                                         float* loss, int64_t* counts, float* load, float* inv_tokens, void* scratch,
-                                        size_t scratch_bytes, int32_t* findings, void* stream) {
+                                        size_t scratch_bytes, void* stream) {
     if (!mb::sizes_ok(n_tokens, n_experts, top_k, n_seqs) || (!seq_list && n_seqs != 1)) return B200MOE_ERR_SHAPE;
     if (logits_fp32 != 0 && logits_fp32 != 1) return B200MOE_ERR_ARGUMENT;
     if ((n_tokens > 0 && (!logits || !idx)) || !loss || !counts || !load || !inv_tokens) return B200MOE_ERR_NULL_POINTER;
@@ -395,7 +395,7 @@ extern "C" int b200moe_moe_balance_loss(const void* logits, int logits_fp32, con
         B200MOE_CUDA_TRY(err);
     }
     B200MOE_CUDA_TRY(launch_dependent(mb::join_kernel, (unsigned)a.S, mb::kJoinThreads, 0, st, a, loss,
-                                      reinterpret_cast<long long*>(counts), load, inv_tokens, findings));
+                                      reinterpret_cast<long long*>(counts), load, inv_tokens, findings_words()));
     return B200MOE_OK;
 }
 

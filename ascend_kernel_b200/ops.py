@@ -127,7 +127,12 @@ def last_status(device=None, clear: bool = False):
             _abi.check(_lib.b200moe_read_sticky_status(_ptr(ws), out, int(bool(clear)), stream), "read_sticky_status")
         if found == (0, 0) and out[0] != 0:
             found = (int(out[0]), int(out[1]))
-    return found
+    # what the operators without a workspace of status words found (their streams: all of the device's)
+    out = (ctypes.c_int32 * 2)()
+    with torch.cuda.device(idx):
+        torch.cuda.synchronize()
+        _abi.check(_lib.b200moe_read_findings(out, int(bool(clear)), _stream()), "read_findings")
+    return (int(out[0]), int(out[1])) if found == (0, 0) else found
 
 
 def check_status(device=None):
@@ -506,46 +511,27 @@ def moe_route(logits, top_k: int, out=None):
     return idx, w, counts, token_of, slot
 
 
-def _findings(device):
-    """Words 4 / 5 of the persistent workspace, where operators with a workspace of their own for every call leave what they found."""
-    return _ptr(_workspace(_abi.STATUS_BYTES, device)) + 16
+_EXT = None
 
 
-def _need_one_device(**tensors):
-    devices = {t.device for t in tensors.values() if t is not None}
-    if len(devices) > 1:
-        raise RuntimeError(f"tensors on different devices: {', '.join(sorted(map(str, devices)))}")
+def _ext():
+    """The compiled module.  The operators below are bound there alone: a call costs it a few microseconds on the host, about what
+    the smallest of them takes on the device, and the same call through ctypes twenty to a hundred."""
+    global _EXT
+    if _EXT is None:
+        from . import cinfer_ascendc
 
-
-def _e4m3(name, t, dim):
-    if t.dtype not in (torch.uint8, torch.float8_e4m3fn) or t.dim() != dim:
-        raise RuntimeError(f"{name} must be {dim}-dimensional e4m3 codes (uint8 or float8_e4m3fn)")
+        _EXT = cinfer_ascendc
+    return _EXT
 
 
 def fp8_quantize_rows(x, index=None, codes=None, scale=None):
     """x bf16 [T, K] -> (codes uint8 [R, K], scale fp32 [R, ceil(K / 128)]): e4m3 with one scale per 128 elements, a / 448 for
     the block's largest magnitude a (at least 2^-100).  ``index`` int32 [R]: row i of the result is row index[i] of x (R = T and row i
     without it); an index outside x gives zeros.  A block with an infinity or a NaN gets scale NaN.  K % 16 == 0."""
-    _need_cuda(x=x, index=index, codes=codes, scale=scale)
-    _need_one_device(x=x, index=index, codes=codes, scale=scale)
-    if x.dim() != 2 or x.dtype != torch.bfloat16:
-        raise RuntimeError("x must be bfloat16 [T, K]")
-    if index is not None and (index.dtype != torch.int32 or index.dim() != 1):
-        raise RuntimeError("index must be int32 [R]")
-    T, K = x.shape
-    R, KB = (T if index is None else index.numel()), -(-K // 128)
-    if codes is None:
-        codes = torch.empty(R, K, dtype=torch.uint8, device=x.device)
-    if scale is None:
-        scale = torch.empty(R, KB, dtype=torch.float32, device=x.device)
-    _e4m3("codes", codes, 2)
-    if tuple(codes.shape) != (R, K) or scale.dtype != torch.float32 or tuple(scale.shape) != (R, KB):
-        raise RuntimeError(f"codes must be [{R}, {K}] and scale float32 [{R}, {KB}]")
-    with torch.cuda.device(x.device):
-        rc = _lib.b200moe_fp8_quantize_rows(_ptr(x), _ptr(index), _ptr(codes), _ptr(scale), T, R, K, _stream())
-    _abi.check(rc, "fp8_quantize_rows")
-    _count(int(R > 0))
-    return codes, scale
+    out = _ext().fp8_quantize_rows(x, index, codes, scale)
+    _count(1)
+    return out
 
 
 def grouped_gemm_fp8_block(x, x_scale, weight, weight_scale, group_list, output, output_scale=None, group_list_type: int = 0,
@@ -554,101 +540,22 @@ def grouped_gemm_fp8_block(x, x_scale, weight, weight_scale, group_list, output,
     (:func:`fp8_quantize_rows` makes them), weight [G, K, N] with weight_scale [G, ceil(K / 128), ceil(N / 128)] (the ``"fp8"``
     format of :func:`grouped_gemm`).  output bf16 [M, N].  ``gate_up_silu``: N = 2I with the gate columns first, output e4m3
     [M, I] and output_scale [M, I / 128] = silu(gate) * up quantised like :func:`fp8_quantize_rows`, which the down projection takes
-    as they are.  K and N multiples of 16, with ``gate_up_silu`` N of 256."""
-    _need_cuda(x=x, x_scale=x_scale, weight=weight, weight_scale=weight_scale, group_list=group_list, output=output,
-               output_scale=output_scale)
-    _need_one_device(x=x, x_scale=x_scale, weight=weight, weight_scale=weight_scale, group_list=group_list, output=output,
-                     output_scale=output_scale)
-    _e4m3("x", x, 2)
-    _e4m3("weight", weight, 3)
-    if group_list.dtype != torch.int64:
-        raise RuntimeError("group_list must be int64")
-    M, K = x.shape
-    G, Kw, N = weight.shape
-    KB, NB = -(-K // 128), -(-N // 128)
-    if Kw != K or group_list.numel() != G:
-        raise RuntimeError(f"shape mismatch: x {tuple(x.shape)}, weight {tuple(weight.shape)}, group_list {group_list.numel()}")
-    for name, t, shape in (("x_scale", x_scale, (M, KB)), ("weight_scale", weight_scale, (G, KB, NB))):
-        if t.dtype != torch.float32 or tuple(t.shape) != shape:
-            raise RuntimeError(f"{name} must be float32 of shape {shape}, got {t.dtype} {tuple(t.shape)}")
-    if gate_up_silu:
-        _e4m3("output", output, 2)
-        if N % 256 != 0:
-            raise RuntimeError("gate_up_silu needs N to be a multiple of 256")
-        if tuple(output.shape) != (M, N // 2) or output_scale is None or output_scale.dtype != torch.float32 \
-                or tuple(output_scale.shape) != (M, N // 256):
-            raise RuntimeError(f"output must be [{M}, {N // 2}] and output_scale float32 [{M}, {N // 256}]")
-    elif output.dtype != torch.bfloat16 or tuple(output.shape) != (M, N) or output_scale is not None:
-        raise RuntimeError(f"output must be bfloat16 [{M}, {N}], without output_scale")
-    need = _lib.b200moe_grouped_gemm_fp8_block_workspace_bytes(M, K, N, G, int(bool(gate_up_silu)))
-    # (a workspace for this call: two graphs captured on one stream may be replayed side by side)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
-        rc = _lib.b200moe_grouped_gemm_fp8_block(_ptr(x), _ptr(x_scale), _ptr(weight), _ptr(weight_scale), _ptr(group_list),
-                                                 _ptr(output), _ptr(output_scale), M, K, N, G, group_list_type,
-                                                 int(bool(gate_up_silu)), _ptr(ws), need, _findings(x.device), _stream())
-    _abi.check(rc, "grouped_gemm_fp8_block")
-    _count(int(M > 0))
-
-
-class _BalanceLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, idx, seq_list, token_mask):
-        T, E = logits.shape
-        S = 1 if seq_list is None else seq_list.numel()
-        dev = logits.device
-        f32 = int(logits.dtype == torch.float32)
-        loss = torch.empty(S, dtype=torch.float32, device=dev)
-        counts = torch.empty(S, E, dtype=torch.int64, device=dev)
-        load = torch.empty(S, E, dtype=torch.float32, device=dev)
-        inv_tokens = torch.empty(S, dtype=torch.float32, device=dev)
-        need = _lib.b200moe_moe_balance_scratch_bytes(T, E, S)
-        scratch = torch.empty(need, dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
-            rc = _lib.b200moe_moe_balance_loss(_ptr(logits), f32, _ptr(idx), _ptr(seq_list), _ptr(token_mask), T, E, idx.shape[1], S,
-                                               _ptr(loss), _ptr(counts), _ptr(load), _ptr(inv_tokens), _ptr(scratch), need,
-                                               _findings(dev), _stream())
-        _abi.check(rc, "moe_balance_loss")
-        _count(1 + (T > 0))
-        ctx.save_for_backward(logits, seq_list, token_mask, load, inv_tokens)
-        ctx.mark_non_differentiable(counts)
-        return loss, counts
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_loss, _):
-        logits, seq_list, token_mask, load, inv_tokens = ctx.saved_tensors
-        grad = torch.empty_like(logits)
-        T, E = logits.shape
-        g = grad_loss.to(torch.float32).contiguous()
-        with torch.cuda.device(logits.device):
-            rc = _lib.b200moe_moe_balance_loss_grad(_ptr(logits), int(logits.dtype == torch.float32), _ptr(seq_list), _ptr(token_mask),
-                                                    _ptr(load), _ptr(inv_tokens), _ptr(g), T, E, load.shape[0], _ptr(grad), _stream())
-        _abi.check(rc, "moe_balance_loss (gradient)")
-        _count(int(T > 0))
-        return grad, None, None, None
+    as they are.  K and N multiples of 16, with ``gate_up_silu`` N of 256.  Codes are uint8 or float8_e4m3fn tensors."""
+    _ext().grouped_gemm_fp8_block(x, x_scale, weight, weight_scale, group_list, output, output_scale, group_list_type, gate_up_silu)
+    _count(1)
 
 
 def moe_balance_loss(logits, idx, seq_list=None, token_mask=None):
-    """Balance loss of the router and the pairs per expert: (loss fp32 [S], counts int64 [S, E]), differentiable in ``logits``
+    """Balance loss of the router and the pairs per expert: (loss fp32 [S], counts int64 [S, E]), differentiable (once) in ``logits``
     (bf16 or fp32 [T, E]).  ``idx`` int32 [T, k]: the experts of each token, as :func:`moe_route` returns them (an entry outside
     0 .. E - 1 is a dropped pair and counts on no expert).  ``seq_list`` int64 [S]: cumulative token ends of the sequences, each of
     which gets a loss of its own; tokens behind the last belong to none.  ``token_mask`` bool [T]: False takes a token out.
 
     For T_s tokens with probabilities p = softmax(logits) and c_e pairs on expert e, loss = E / (k T_s) * sum_e c_e * mean_t p_te: 1
     where the load is even; 0 for a sequence without tokens.  The counts carry no gradient."""
-    _need_cuda(logits=logits, idx=idx, seq_list=seq_list, token_mask=token_mask)
-    _need_one_device(logits=logits, idx=idx, seq_list=seq_list, token_mask=token_mask)
-    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32):
-        raise RuntimeError("logits must be bfloat16 or float32 [T, E]")
-    T, E = logits.shape
-    if idx.dtype != torch.int32 or idx.dim() != 2 or idx.shape[0] != T:
-        raise RuntimeError(f"idx must be int32 [{T}, k]")
-    if seq_list is not None and (seq_list.dtype != torch.int64 or seq_list.dim() != 1):
-        raise RuntimeError("seq_list must be int64 [S]")
-    if token_mask is not None and (token_mask.dtype != torch.bool or tuple(token_mask.shape) != (T,)):
-        raise RuntimeError(f"token_mask must be bool [{T}]")
-    return _BalanceLoss.apply(logits, idx, seq_list, token_mask)
+    out = _ext().moe_balance_loss(logits, idx, seq_list, token_mask)
+    _count(2)
+    return out
 
 
 def silu_mul_dyn(h, n_rows, out=None):

@@ -313,14 +313,12 @@ int b200moe_fp8_quantize_rows(const void* x, const int32_t* index, void* codes, 
  * gate_up_silu == 0: out bf16 [M, N], out_scale unused.  gate_up_silu == 1: N = 2 I with the gate columns first, N % 256 == 0;
  * silu(gate) * up in fp32, quantised as b200moe_fp8_quantize_rows does: out e4m3 [M, I], out_scale fp32 [M, I / 128].
  * K % 16 == 0 and N % 16 == 0; x, weight and out aligned to 16 bytes.  Rows of no expert are left as they were.
- * The workspace belongs to the call until it has completed on the stream, and the next call may have another (calls that overlap must).
- * findings: NULL, or two int32 in device memory that keep the first (code, detail) found by any call that got them until the caller
- * zeroes them; codes and details are those of status words 0 and 1. */
+ * The workspace belongs to the call until it has completed on the stream, and calls that overlap have one each; it holds no status
+ * words: an invalid group_list (rows were clamped) or an expired wait is kept for b200moe_read_findings. */
 size_t b200moe_grouped_gemm_fp8_block_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, int gate_up_silu);
 int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scale, const void* weight, const float* weight_scale,
                                    const int64_t* group_list, void* out, float* out_scale, int64_t M, int64_t K, int64_t N, int64_t G,
-                                   int group_list_type, int gate_up_silu, void* workspace, size_t workspace_bytes, int32_t* findings,
-                                   void* stream);
+                                   int group_list_type, int gate_up_silu, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Balance loss of the router (for training it; no reference counterpart).  logits [T, E] bf16 or fp32 (logits_fp32), idx int32 [T, top_k]
  * the experts of each token as b200moe_moe_route returns them (an entry outside 0 .. E - 1 is a pair that was dropped: it counts on no
@@ -332,15 +330,19 @@ int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scale, const vo
  * are what b200moe_moe_balance_loss_grad takes with the gradient of the losses grad_loss fp32 [n_seqs]:
  *   grad_logits [T, E] (of the logits' type) = grad_loss[s] inv_tokens[s] p_te (load[s, e] - sum_j load[s, j] p_tj), 0 for a token of no sequence.
  * Sums have a fixed order.  A seq_list that falls or leaves 0 .. T is cut to that range and leaves code 1 with the sequence's number
- * in findings (as above; may be NULL).  E <= 1024, top_k <= 32, n_seqs <= 65535, T * top_k < 2^30. */
+ * for b200moe_read_findings.  E <= 1024, top_k <= 32, n_seqs <= 65535, T * top_k < 2^30. */
 size_t b200moe_moe_balance_scratch_bytes(int64_t n_tokens, int64_t n_experts, int64_t n_seqs);
 int b200moe_moe_balance_loss(const void* logits, int logits_fp32, const int32_t* idx, const int64_t* seq_list,
                              const uint8_t* token_mask, int64_t n_tokens, int64_t n_experts, int64_t top_k, int64_t n_seqs, float* loss,
-                             int64_t* counts, float* load, float* inv_tokens, void* scratch, size_t scratch_bytes, int32_t* findings,
-                             void* stream);
+                             int64_t* counts, float* load, float* inv_tokens, void* scratch, size_t scratch_bytes, void* stream);
 int b200moe_moe_balance_loss_grad(const void* logits, int logits_fp32, const int64_t* seq_list, const uint8_t* token_mask,
                                   const float* load, const float* inv_tokens, const float* grad_loss, int64_t n_tokens,
                                   int64_t n_experts, int64_t n_seqs, void* grad_logits, void* stream);
+
+/* The first finding (code, detail; those of status words 0 and 1) of any b200moe_grouped_gemm_fp8_block or b200moe_moe_balance_loss call
+ * on the current device since it was last cleared, kept in a fixed array of the library; (0, 0) if none.  Synchronises the
+ * stream (calls on other streams may still be running). */
+int b200moe_read_findings(int32_t out[2], int clear, void* stream);
 
 /* ---- expert-parallel token exchange over NVLink peer memory ----------------------------------
  * (No reference counterpart: the reference ships the two operators only; chitu exchanges tokens
