@@ -28,7 +28,7 @@ EXPORTS = [
     "b200moe_ep_post_counts", "b200moe_ep_dispatch", "b200moe_ep_wait", "b200moe_ep_post", "b200moe_ep_combine",
     "b200moe_fp4_dequant_bf16_scale", "b200moe_fp8_dequant", "b200moe_fp4_scale_fold",
     "b200moe_silu_mul_dyn", "b200moe_grouped_gemm_int8_silu", "b200moe_grouped_gemm_fp4_e8m0", "b200moe_pack_weight_int8", "b200moe_grouped_gemm_int8_packed", "b200moe_grouped_gemm_int8_packed_scatter",
-    "b200moe_fp8_quantize_rows", "b200moe_grouped_gemm_fp8_block", "b200moe_grouped_gemm_fp8_block_workspace_bytes",
+    "b200moe_fp8_quantize_rows", "b200moe_fp8_quantize_rows_scratch_bytes", "b200moe_grouped_gemm_fp8_block", "b200moe_grouped_gemm_fp8_block_workspace_bytes",
     "b200moe_moe_balance_scratch_bytes", "b200moe_moe_balance_loss", "b200moe_moe_balance_loss_grad", "b200moe_read_findings",
     "b200moe_set_gemm_reserved_sms", "b200moe_ipc_alloc", "b200moe_ipc_open", "b200moe_ipc_close", "b200moe_ipc_free",
 ]
@@ -118,7 +118,9 @@ def _load() -> ctypes.CDLL:
     lib.b200moe_moe_route.restype = i32
     lib.b200moe_moe_regroup_index.argtypes = [vp, i64, i64, vp, vp, vp, vp]
     lib.b200moe_moe_regroup_index.restype = i32
-    lib.b200moe_fp8_quantize_rows.argtypes = [vp, vp, vp, vp, i64, i64, i64, vp]
+    lib.b200moe_fp8_quantize_rows_scratch_bytes.argtypes = [i64, i64, i64, i32]
+    lib.b200moe_fp8_quantize_rows_scratch_bytes.restype = sz
+    lib.b200moe_fp8_quantize_rows.argtypes = [vp, vp, vp, vp, i64, i64, i64, vp, sz, vp]
     lib.b200moe_fp8_quantize_rows.restype = i32
     lib.b200moe_grouped_gemm_fp8_block_workspace_bytes.argtypes = [i64, i64, i64, i64, i32]
     lib.b200moe_grouped_gemm_fp8_block_workspace_bytes.restype = sz

@@ -17,15 +17,31 @@ constexpr float kFloor = 0x1p-100f;      // a block's largest magnitude counts a
 // from one, and one that is a tie has at most five bits and comes out of the correction step as it is: the first guess
 // is good to about 2^-21, its remainder is exact (11 bits), and what the step leaves is of the second order.
 // x * 448 / a = x' / a' with x' = x * 7 * 2^-4 and a' = a * 2^-10: neither product overflows, and neither is rounded where it matters.
+__device__ __forceinline__ float reciprocal(float a) {  // good to 2^-23, a normal
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));
+    return r;
+}
+// The largest magnitude of three; a NaN stays one.
+__device__ __forceinline__ float max_magnitude(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 struct Quantizer {
     float scale;
-    float a, inv;  // a', 1 / a' (0 for a block that is not finite: its codes are 0)
+    float a, inv;  // a', 1 / a' (0 for a block that is not finite: zeros have code 0 there)
     // `top`: the largest magnitude of the block, or infinity / NaN where the block holds one
     __device__ __forceinline__ explicit Quantizer(float top) {
-        const bool finite = top < INFINITY;
+        const bool finite = top < INFINITY;  // (not NaN either)
         const float m = fmaxf(top, kFloor);
-        a = m * 0x1p-10f;
-        inv = finite ? __fdividef(1.f, a) : 0.f;
+        a = finite ? m * 0x1p-10f : 0.f;
+        inv = finite ? reciprocal(a) : 0.f;
         // m / 448 by the same correction step (for bf16 m the quotient rounded to nearest, which the tests check for all of them)
         constexpr float kInv = 1.f / kMax;
         const float q = m * kInv;

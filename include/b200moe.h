@@ -302,9 +302,11 @@ int b200moe_moe_regroup_index(const int64_t* recv_counts, int64_t world, int64_t
  * index[i] of x [n_src, K], or row i where index is NULL (then n_rows <= n_src); an index outside x gives a row of zeros.
  *   a = max(2^-100, largest magnitude of the block), scale = a / 448, code = e4m3(x * 448 / a), round to nearest even;
  * a block that holds an infinity or a NaN gets scale NaN and codes 0.  codes [n_rows, K] bytes, scale fp32 [n_rows, ceil(K / 128)].
- * K % 16 == 0; x and codes aligned to 16 bytes. */
+ * K % 16 == 0; x and codes aligned to 16 bytes.  scratch (16-byte aligned, or NULL): with scratch_bytes of it, where that is not 0, a
+ * long call quantises every row of x once and gathers the bytes; without it every row of the result is quantised.  Same bits. */
+size_t b200moe_fp8_quantize_rows_scratch_bytes(int64_t n_src, int64_t n_rows, int64_t K, int has_index);
 int b200moe_fp8_quantize_rows(const void* x, const int32_t* index, void* codes, float* scale, int64_t n_src, int64_t n_rows,
-                              int64_t K, void* stream);
+                              int64_t K, void* scratch, size_t scratch_bytes, void* stream);
 
 /* Grouped GEMM on such rows and weights:
  *   y[m, n] = sum over blocks kb of 128 k:  x_scale[m, kb] * weight_scale[g, kb, n / 128] * sum_{k in kb} x[m, k] * w[g, k, n]

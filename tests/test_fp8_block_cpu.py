@@ -31,7 +31,7 @@ def test_grouped_gemm_refusals(change, code):
     ((A, None, A + 8, A, 4, 4, 128), ALIGN), ((None, None, None, None, 0, 0, 128), OK),
 ])
 def test_quantize_refusals(args, code):
-    assert lib.b200moe_fp8_quantize_rows(*args, None) == code
+    assert lib.b200moe_fp8_quantize_rows(*args, None, 0, None) == code
 
 
 def _loss(logits=A, f32=0, idx=A, seqs=A, mask=None, T=8, E=16, k=2, S=2, loss=A, counts=A, load=A, inv=A, scratch=A, nbytes=1 << 40):

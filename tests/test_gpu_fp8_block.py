@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import ascend_kernel_b200 as ak
+from ascend_kernel_b200 import _abi
 from tests import fp8_ref as R
 
 pytestmark = pytest.mark.gpu
@@ -120,6 +121,23 @@ def test_gathered_rows_and_indexes_outside():
     rows = torch.where(((index >= 0) & (index < 17)).unsqueeze(1), x[index.clamp(0, 16).long()].float(), 0.0)
     want, want_scale = R.quantize(rows.double())
     assert torch.equal(codes, want) and torch.equal(scale, want_scale.float())
+
+
+def test_rows_quantised_once_and_gathered_have_the_same_bits():
+    """A long call whose index names rows again and again takes two passes: indexes outside x, blocks that are not finite, a short last block."""
+    gen = _gen(4)
+    T, n_rows, K = 64, 40000, 1360
+    assert _abi.lib.b200moe_fp8_quantize_rows_scratch_bytes(T, n_rows, K, 1) > 0
+    x = torch.randn(T, K, generator=gen, device=DEV).to(torch.bfloat16)
+    x[3, 200], x[5, K - 1] = float("nan"), float("inf")
+    index = torch.randint(-1, T + 1, (n_rows,), generator=gen, device=DEV).to(torch.int32)
+    codes, scale = ak.fp8_quantize_rows(x, index)
+    once, once_scale = ak.fp8_quantize_rows(x)
+    at = index.clamp(0, T - 1).long()
+    inside = ((index >= 0) & (index < T)).unsqueeze(1)
+    want_scale = torch.where(inside, once_scale[at], torch.tensor(2.0 ** -100 / 448, device=DEV))
+    assert torch.equal(codes, torch.where(inside, once[at], torch.zeros_like(codes)))
+    assert torch.equal(torch.nan_to_num(scale), torch.nan_to_num(want_scale)) and torch.equal(torch.isnan(scale), torch.isnan(want_scale))
 
 
 def test_quantise_into_given_tensors_and_no_rows():
