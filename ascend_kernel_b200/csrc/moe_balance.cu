@@ -12,16 +12,16 @@
 // Forward: a CTA takes a range of tokens, a warp a token at a time, its lanes adding the probabilities of their experts up in
 // registers; what a CTA has of a sequence goes to row (range + sequence) of the scratch (going on by a range or by a sequence
 // raises that sum by one, so no two pieces share a row), and a second kernel adds a sequence's rows in their order: no
-// floating-point atomics, the same bits each time.  Backward: a warp per token, the softmax again from the logits.  Both read the
+// floating-point atomics, the same bits each time.  Backward: the softmax again from the logits, a warp four tokens at a time.  Both read the
 // logits once and are bound by that.
 #include <type_traits>
 
 #include "common.cuh"
+#include "ptx.cuh"
 
 namespace b200moe {
 namespace mb {
 
-constexpr int kWarps = 16, kThreads = kWarps * 32;
 constexpr int kMaxTopK = 32;
 
 template <class T>
@@ -64,6 +64,19 @@ struct Logit<float> {
             v[0] = __ldg(p);
         }
     }
+    // VEC values of a table whose rows are as wide as the logits': 16 bytes at a time where VEC says that these are aligned
+    template <int VEC>
+    static __device__ __forceinline__ void load_row(const float* p, float (&v)[VEC]) {
+        if constexpr (VEC == 8) {
+            float a[4], b[4];
+            load<4>(p, a);
+            load<4>(p + 4, b);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
+        } else {
+            load<VEC>(p, v);
+        }
+    }
     template <int VEC>
     static __device__ __forceinline__ void store(float* p, const float (&v)[VEC]) {
         if constexpr (VEC == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
@@ -102,56 +115,79 @@ __device__ __forceinline__ int seq_of(const Args& a, int t) {
     return lo;
 }
 
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 
-// A token's probabilities: lane l holds experts (c * 32 + l) * VEC + j.  A row of nothing but -infinity has none (all 0), a NaN or
-// +infinity makes the row NaN.
-template <class T, int VEC, int CHUNKS>
-__device__ __forceinline__ void softmax_row(const T* row, int E, float (&p)[CHUNKS][VEC]) {
+// The probabilities of U tokens, their chains of loads and reductions side by side: lane l holds experts (c * 32 + l) * VEC + j.  A row
+// of nothing but -infinity has none (all 0), a NaN or +infinity makes the row NaN.  A row that is not `on` is not read.
+template <class T, int VEC, int CHUNKS, int U>
+__device__ __forceinline__ void softmax_rows(const T* const (&row)[U], const bool (&on)[U], int E, float (&p)[U][CHUNKS][VEC]) {
     const int lane = threadIdx.x & 31;
-    float m = -INFINITY;
+    float m[U], sum[U];
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-        const int e = (c * 32 + lane) * VEC;
-        if (e < E) {
-            Logit<T>::template load<VEC>(row + e, p[c]);
-        } else {
+    for (int u = 0; u < U; ++u) {
+        m[u] = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) p[c][j] = -INFINITY;
+        for (int c = 0; c < CHUNKS; ++c) {
+            const int e = (c * 32 + lane) * VEC;
+            if (on[u] && e < E) {
+                Logit<T>::template load<VEC>(row[u] + e, p[u][c]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) p[u][c][j] = -INFINITY;
+            }
         }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) m = fmaxf(m, p[c][j]);
     }
-    m = warp_max(m);
-    float sum = 0.f;
-    // (a difference first: logits of the type's lowest value times log2(e) would overflow)
-    const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            p[c][j] = exp2f((p[c][j] - base) * 1.44269504f);
-            sum += p[c][j];
-        }
-    sum = warp_sum(sum);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c)
+            for (int j = 0; j < VEC; ++j) m[u] = fmaxf(m[u], p[u][c][j]);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) p[c][j] *= inv;
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int u = 0; u < U; ++u) m[u] = fmaxf(m[u], __shfl_xor_sync(0xffffffffu, m[u], o));
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        // (a difference first: logits of the type's lowest value times log2(e) would overflow)
+        const float base = m[u] == -INFINITY ? 0.f : m[u];
+        sum[u] = 0.f;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                p[u][c][j] = exp2f((p[u][c][j] - base) * 1.44269504f);
+                sum[u] += p[u][c][j];
+            }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int u = 0; u < U; ++u) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const float inv = sum[u] == 0.f ? 0.f : 1.f / sum[u];
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) p[u][c][j] *= inv;
+    }
 }
+// Tokens a warp has side by side: what 16 values a lane hold.
+template <int VEC, int CHUNKS>
+constexpr int kTokens = VEC * CHUNKS <= 8 ? 2 : 1;
+
+// Warps of a CTA of the forward pass: half as many where a lane's experts fill its registers.
+template <int VEC, int CHUNKS>
+constexpr int kForwardWarps = VEC * CHUNKS <= 16 ? 32 : 16;
 
 template <class T, int VEC, int CHUNKS>
-__global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
+__global__ void __launch_bounds__(32 * kForwardWarps<VEC, CHUNKS>) forward_kernel(const Args a) {
+    constexpr int U = kTokens<VEC, CHUNKS>, kWarps = kForwardWarps<VEC, CHUNKS>, kThreads = 32 * kWarps;
     extern __shared__ float smem[];  // [kWarps][pitch] probabilities, [pitch] counts, 1 number of tokens
     int* hist = reinterpret_cast<int*>(smem + kWarps * a.pitch);
     int* n_tokens = hist + a.pitch;
@@ -167,19 +203,28 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
         __syncthreads();
         float acc[CHUNKS][VEC] = {};
         int n = 0;
-        for (int t = lo + warp; t < hi; t += kWarps) {
-            if (a.mask != nullptr && __ldg(a.mask + t) == 0) continue;
-            ++n;
-            if (lane < a.k) {
-                const int e = __ldg(a.idx + (size_t)t * a.k + lane);
-                if ((unsigned)e < (unsigned)a.E) atomicAdd(&hist[e], 1);
+        for (int t = lo + warp; t < hi; t += kWarps * U) {
+            const T* row[U];
+            bool on[U];
+            float p[U][CHUNKS][VEC];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int tu = t + u * kWarps;
+                on[u] = tu < hi && (a.mask == nullptr || __ldg(a.mask + tu) != 0);
+                row[u] = logits + (size_t)(on[u] ? tu : t) * a.E;
+                if (on[u] && lane < a.k) {
+                    const int e = __ldg(a.idx + (size_t)tu * a.k + lane);
+                    if ((unsigned)e < (unsigned)a.E) atomicAdd(&hist[e], 1);
+                }
+                n += on[u];
             }
-            float p[CHUNKS][VEC];
-            softmax_row<T, VEC, CHUNKS>(logits + (size_t)t * a.E, a.E, p);
+            softmax_rows<T, VEC, CHUNKS, U>(row, on, a.E, p);
 #pragma unroll
-            for (int c = 0; c < CHUNKS; ++c)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) acc[c][j] += p[c][j];
+                for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) acc[c][j] += p[u][c][j];
         }
         if (lane == 0 && n) atomicAdd(n_tokens, n);
 #pragma unroll
@@ -204,33 +249,32 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
     grid_dep_launch();
 }
 
-// A CTA per sequence: its rows of the scratch in their order.  A warp takes 128 experts of every n-th row; what the warps have is
-// added in their order.
+// A CTA per sequence and 128 experts, the CTAs of a sequence as a cluster: a warp takes every 32nd of the sequence's rows, what the
+// warps have is added in their order, and the first CTA adds up the parts of the loss.  (One CTA of a sequence for all experts, in 64
+// bits: 21 us for 296 rows of 256.)
 constexpr int kJoinThreads = 1024;
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a, float* __restrict__ loss, long long* __restrict__ counts,
                                                             float* __restrict__ load, float* __restrict__ inv_n, int* findings) {
-    __shared__ alignas(16) float s_p[32 * 128];
-    __shared__ alignas(16) int s_c[32 * 128];
-    __shared__ float s_loss[32];
-    __shared__ int s_n;
-    const int s = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    __shared__ alignas(16) float s_p[32][128];
+    __shared__ alignas(16) int s_c[32][128];
+    __shared__ int s_n[32];
+    __shared__ int s_tokens;
+    __shared__ float s_part[4], s_loss;
+    const int s = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int start = seq_start(a, s), end = seq_end(a, s);
-    if (threadIdx.x == 0) {
-        s_n = 0;
+    if (threadIdx.x == 0 && blockIdx.x == 0) {
         const long long given = a.seq_list ? a.seq_list[s] : a.T;
         if (given != end || end < start) keep_finding(findings, kDevBadGroupList, s);
     }
-    __syncthreads();
-    const int groups = (a.pitch + 127) / 128, rows_at_once = 32 / groups;  // pitch <= 1024
-    const int e = (warp % groups) * 128 + lane * 4, r0 = warp / groups;
+    const int e = blockIdx.x * 128 + lane * 4;
     float4 p = make_float4(0.f, 0.f, 0.f, 0.f);
     int4 c = make_int4(0, 0, 0, 0);
     int n = 0;
     grid_dep_wait();
-    if (end > start && r0 < rows_at_once) {
+    if (end > start) {
         const int last = (end - 1) / a.chunk;
-#pragma unroll 4
-        for (int r = start / a.chunk + r0; r <= last; r += rows_at_once) {
+#pragma unroll 8
+        for (int r = start / a.chunk + warp; r <= last; r += 32) {
             const size_t row = (size_t)r + s;
             if (e < a.pitch) {
                 const float4 q = __ldcg(reinterpret_cast<const float4*>(a.psum + row * a.pitch + e));
@@ -238,88 +282,108 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a, float*
                 p.x += q.x; p.y += q.y; p.z += q.z; p.w += q.w;
                 c.x += d.x; c.y += d.y; c.z += d.z; c.w += d.w;
             }
-            if (e == 0) n += __ldcg(a.nsum + row);
+            n += __ldcg(a.nsum + row);
         }
     }
-    if (e == 0 && n) atomicAdd(&s_n, n);
-    reinterpret_cast<float4*>(s_p)[warp * 32 + lane] = p;
-    reinterpret_cast<int4*>(s_c)[warp * 32 + lane] = c;
+    reinterpret_cast<float4*>(s_p[warp])[lane] = p;
+    reinterpret_cast<int4*>(s_c[warp])[lane] = c;
+    if (lane == 0) s_n[warp] = n;
     __syncthreads();
-    const double tokens = s_n, pairs = tokens * a.k;
-    double part = 0.;
-    if ((int)threadIdx.x < a.E) {
-        const int at = (threadIdx.x >> 7) * 128 + (threadIdx.x & 127);
-        double sum = 0.;
-        long long count = 0;
-        for (int r = 0; r < rows_at_once; ++r) {
-            sum += s_p[r * groups * 128 + at];
-            count += s_c[r * groups * 128 + at];
+    if (warp < 4) {
+        const int tokens = __reduce_add_sync(0xffffffffu, s_n[lane]), x = (int)threadIdx.x, expert = blockIdx.x * 128 + x;
+        const long long pairs = (long long)tokens * a.k;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        int count = 0;
+#pragma unroll
+        for (int r = 0; r < 32; ++r) {
+            sum[r & 3] += s_p[r][x];
+            count += s_c[r][x];
         }
-        const size_t o = (size_t)s * a.E + threadIdx.x;
-        counts[o] = count;
-        load[o] = s_n ? (float)((count * (double)a.E - pairs) / pairs) : 0.f;
-        if (s_n) part = (double)count * sum;
+        float part = 0.f;
+        if (expert < a.E) {
+            const size_t o = (size_t)s * a.E + expert;
+            counts[o] = count;
+            // (the difference is of whole numbers)
+            load[o] = tokens ? (float)((long long)count * a.E - pairs) / (float)pairs : 0.f;
+            if (tokens) part = (float)count * ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        }
+        part = warp_sum(part);
+        if (lane == 0) s_part[warp] = part;
+        if (threadIdx.x == 0) s_tokens = tokens;
+        if (threadIdx.x == 0 && blockIdx.x == 0) inv_n[s] = tokens ? 1.f / (float)tokens : 0.f;
     }
-    // (sums of positive terms: fp32 from here on)
-    float v = warp_sum(s_n ? (float)(part / (pairs * tokens) * a.E) : 0.f);
-    if (lane == 0) s_loss[warp] = v;
     __syncthreads();
-    if (warp == 0) {
-        v = warp_sum(s_loss[lane]);
-        if (lane == 0) {
-            loss[s] = v;
-            inv_n[s] = s_n ? 1.f / (float)s_n : 0.f;
-        }
+    if (threadIdx.x == 0) s_loss = (s_part[0] + s_part[1]) + (s_part[2] + s_part[3]);
+    ptx::cluster_sync();
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        float sum = 0.f;
+        for (unsigned r = 0; r < gridDim.x; ++r) sum += ptx::ld_cluster_f32(ptx::map_rank(ptx::smem_u32(&s_loss), r));
+        const float tokens = (float)s_tokens;
+        loss[s] = s_tokens ? sum / (tokens * (float)a.k) * ((float)a.E / tokens) : 0.f;
     }
+    ptx::cluster_sync();  // (the other CTAs' shared memory has been read)
 }
 
 template <class T, int VEC, int CHUNKS>
 __global__ void __launch_bounds__(256) backward_kernel(const Args a, const float* __restrict__ load, const float* __restrict__ inv_n,
                                                        const float* __restrict__ grad, T* __restrict__ out) {
-    const int lane = threadIdx.x & 31, t = blockIdx.x * 8 + (threadIdx.x >> 5);
+    constexpr int U = kTokens<VEC, CHUNKS>;
+    const int lane = threadIdx.x & 31, t = (blockIdx.x * 8 + (threadIdx.x >> 5)) * U;
     if (t >= a.T) return;
-    const int s = seq_of(a, t);
-    T* dst = out + (size_t)t * a.E;
-    float p[CHUNKS][VEC];
-    // a token of no sequence, or one that the mask takes out, has no part in any loss (what its logits hold is not read)
-    if (s >= a.S || t < seq_start(a, s) || (a.mask != nullptr && __ldg(a.mask + t) == 0)) {
+    const T* row[U];
+    const float* f[U];
+    bool on[U];
+    float g[U], mean[U], p[U][CHUNKS][VEC];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        // a token of no sequence, or one that the mask takes out, has no part in any loss (what its logits hold is not read)
+        const int tu = t + u, s = tu < a.T ? seq_of(a, tu) : a.S;
+        on[u] = s < a.S && tu >= seq_start(a, s) && (a.mask == nullptr || __ldg(a.mask + tu) != 0);
+        row[u] = static_cast<const T*>(a.logits) + (size_t)(on[u] ? tu : t) * a.E;
+        f[u] = load + (size_t)(on[u] ? s : 0) * a.E;
+        g[u] = on[u] ? __ldg(grad + s) * __ldg(inv_n + s) : 0.f;
+        mean[u] = 0.f;
+    }
+    softmax_rows<T, VEC, CHUNKS, U>(row, on, a.E, p);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             const int e = (c * 32 + lane) * VEC;
+            if (e < a.E) {
+                float fv[VEC];
+                Logit<float>::template load_row<VEC>(f[u] + e, fv);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) p[c][j] = 0.f;
-            if (e < a.E) Logit<T>::template store<VEC>(dst + e, p[c]);
+                for (int j = 0; j < VEC; ++j) mean[u] = fmaf(fv[j], p[u][c][j], mean[u]);
+            }
         }
-        return;
-    }
-    const float g = __ldg(grad + s) * __ldg(inv_n + s);
-    softmax_row<T, VEC, CHUNKS>(static_cast<const T*>(a.logits) + (size_t)t * a.E, a.E, p);
-    const float* f = load + (size_t)s * a.E;
-    float fv[CHUNKS][VEC], mean = 0.f;
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-        const int e = (c * 32 + lane) * VEC;
+    for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            fv[c][j] = e < a.E ? __ldg(f + e + j) : 0.f;  // (VEC divides E)
-            mean = fmaf(fv[c][j], p[c][j], mean);
+        for (int u = 0; u < U; ++u) mean[u] += __shfl_xor_sync(0xffffffffu, mean[u], o);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (t + u >= a.T) break;
+        T* dst = out + (size_t)(t + u) * a.E;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            const int e = (c * 32 + lane) * VEC;
+            if (e < a.E) {
+                float fv[VEC];
+                Logit<float>::template load_row<VEC>(f[u] + e, fv);  // (again, from L1)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) fv[j] = on[u] ? p[u][c][j] * (g[u] * (fv[j] - mean[u])) : 0.f;
+                Logit<T>::template store<VEC>(dst + e, fv);
+            }
         }
-    }
-    mean = warp_sum(mean);
-#pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-        const int e = (c * 32 + lane) * VEC;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) p[c][j] *= g * (fv[c][j] - mean);
-        if (e < a.E) Logit<T>::template store<VEC>(dst + e, p[c]);
     }
 }
 
-// Tokens a CTA of the forward pass takes: about two CTAs a multiprocessor, a token a warp at least.
+// Tokens a CTA of the forward pass takes: about a CTA a multiprocessor, a token a warp at least.
 static int chunk_of(int64_t T) {
-    const int64_t ctas = 2LL * 148;  // (not the device's own number: the scratch size is a function of the sizes alone)
+    const int64_t ctas = 148;  // (not the device's own number: the scratch size is a function of the sizes alone)
     int64_t c = (T + ctas - 1) / ctas;
-    return (int)(c < kWarps ? kWarps : c);
+    return (int)(c < 32 ? 32 : c);
 }
 static int64_t scratch_rows(int64_t T, int64_t S) { return (T + chunk_of(T) - 1) / chunk_of(T) + S; }
 static int pitch_of(int64_t E) { return (int)((E + 3) & ~3LL); }
@@ -380,13 +444,14 @@ extern "C" int b200moe_moe_balance_loss(const void* logits, int logits_fp32, con
     a.nsum = a.csum + cells;
     if (a.T > 0) {
         const unsigned grid = (unsigned)((a.T + a.chunk - 1) / a.chunk);
-        const size_t smem = (size_t)(mb::kWarps + 1) * a.pitch * 4 + 4;
         cudaError_t err = cudaSuccess;
         const auto run = [&](auto vec, auto chunks, auto zero) {
             auto* k = mb::forward_kernel<decltype(zero), decltype(vec)::value, decltype(chunks)::value>;
-            if (smem > 48 * 1024) err = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
+            constexpr int warps = mb::kForwardWarps<decltype(vec)::value, decltype(chunks)::value>;
+            const size_t smem = (size_t)(warps + 1) * a.pitch * 4 + 4;
+            if (smem > 48 * 1024) err = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 140 * 1024);
             if (err == cudaSuccess) {
-                k<<<grid, mb::kThreads, smem, st>>>(a);
+                k<<<grid, 32 * warps, smem, st>>>(a);
                 err = cudaGetLastError();
             }
         };
@@ -394,8 +459,20 @@ extern "C" int b200moe_moe_balance_loss(const void* logits, int logits_fp32, con
         else mb::pick<__nv_bfloat16>(a.E, aligned16(logits), [&](auto v, auto c) { run(v, c, __nv_bfloat16()); });
         B200MOE_CUDA_TRY(err);
     }
-    B200MOE_CUDA_TRY(launch_dependent(mb::join_kernel, (unsigned)a.S, mb::kJoinThreads, 0, st, a, loss,
-                                      reinterpret_cast<long long*>(counts), load, inv_tokens, findings_words()));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((a.pitch + 127) / 128), (unsigned)a.S);
+    cfg.blockDim = dim3(mb::kJoinThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cfg.gridDim.x;  // 8 at most
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    B200MOE_CUDA_TRY(cudaLaunchKernelEx(&cfg, mb::join_kernel, a, loss, reinterpret_cast<long long*>(counts), load, inv_tokens,
+                                        findings_words()));
     return B200MOE_OK;
 }
 
@@ -412,10 +489,11 @@ extern "C" int b200moe_moe_balance_loss_grad(const void* logits, int logits_fp32
     a.seq_list = seq_list;
     a.mask = token_mask;
     a.T = (int)n_tokens; a.E = (int)n_experts; a.S = (int)n_seqs;
-    const unsigned grid = (unsigned)((n_tokens + 7) / 8);
-    const bool aligned = aligned16(logits) && aligned16(grad_logits);
+    const bool aligned = aligned16(logits) && aligned16(grad_logits) && aligned16(load);
     const auto run = [&](auto vec, auto chunks, auto zero) {
         using T = decltype(zero);
+        const int64_t per_cta = 8 * mb::kTokens<decltype(vec)::value, decltype(chunks)::value>;
+        const unsigned grid = (unsigned)((n_tokens + per_cta - 1) / per_cta);
         mb::backward_kernel<T, decltype(vec)::value, decltype(chunks)::value>
             <<<grid, 256, 0, st>>>(a, load, inv_tokens, grad_loss, static_cast<T*>(grad_logits));
     };

@@ -71,6 +71,10 @@ class MoELayer:
         bits and the product of the two phases of the reference's own kernel (dequantise to a bf16
         workspace, then multiply: grouped_matmul_antiquant.h:632-654, grouped_matmul.h:409-463), and
         SiLU(gate) * up runs in the first GEMM's epilogue.  ``bf13`` / ``bf2`` dequantise them on request.
+        ``weight_format="fp8"``: the experts are e4m3 with one fp32 scale per 128 x 128 block -- w13 uint8 [E_local, H, 2I], s13
+        [E_local, H/128, 2I/128], w2 uint8 [E_local, I, H], s2 [E_local, I/128, H/128], o13 / o2 None, H and I multiples of 128 -- and a
+        pass multiplies in 8 bits: the rows are quantised to e4m3 per 128 elements on their way to the experts, the gate/up
+        GEMM's epilogue quantises silu(gate) * up, and the down projection takes that as it is.
         ``exchange_buffers=2`` (p2p exchange only) doubles the exchange buffers, which ``OverlappedSteps``
         needs to run one step's token exchange beside the expert GEMMs of the step before."""
         self.ops = row_ops
@@ -87,14 +91,21 @@ class MoELayer:
         assert self.e_local * self.world == n_experts
         self.hidden, self.inter = w13.shape[1], w2.shape[1]
         self.device = w13.device
-        if weight_format not in ("int8", "fp4"):
-            raise ValueError("weight_format must be 'int8' or 'fp4'")
+        if weight_format not in ("int8", "fp4", "fp8"):
+            raise ValueError("weight_format must be 'int8', 'fp4' or 'fp8'")
         self.weight_format = weight_format
         if weight_format == "fp4":
             if o13 is not None or o2 is not None or row_ops is not CudaRowOps:
                 raise ValueError("FP4-stored experts take no offsets and run on the CUDA row operations only")
             if w13.shape[2] != self.inter or w2.shape[2] * 2 != self.hidden:
                 raise ValueError("expected w13 [E, H, 2I/2] and w2 [E, I, H/2] packed codes")
+            fuse_silu, gemm = False, "generic"
+        elif weight_format == "fp8":
+            if o13 is not None or o2 is not None or row_ops is not CudaRowOps:
+                raise ValueError("8-bit floating-point experts take no offsets and run on the CUDA row operations only")
+            if (self.hidden % 128 or self.inter % 128 or w13.shape[2] != 2 * self.inter or w2.shape[2] != self.hidden
+                    or w13.element_size() != 1 or w2.element_size() != 1):
+                raise ValueError("expected w13 [E, H, 2I] and w2 [E, I, H] e4m3 codes, H and I multiples of 128")
             fuse_silu, gemm = False, "generic"
         self.fuse_silu = (row_ops is CudaRowOps) if fuse_silu is None else bool(fuse_silu)
         if gemm is None:
@@ -162,14 +173,14 @@ class MoELayer:
         if self.mid_hook is not None:
             self.mid_hook()
 
-    def _experts(self, rows, counts, record, y=None, n_rows=None, scatter=None, rows_sum=None, max_rows=None):
+    def _experts(self, rows, counts, record, y=None, n_rows=None, scatter=None, rows_sum=None, max_rows=None, row_scale=None):
         """rows [R, H] expert-major with per-local-expert counts -> [R, H] (into ``y`` when given).
         ``n_rows``: int64 device tensor with the number of rows in use when R is only a capacity.
         ``scatter`` = (row_code, destination pointers, destination rows): the down projection stores
         each result row where its code says (the return buffer of the rank the token came from) instead
         of into ``y``; packed GEMMs only.  ``rows_sum``: fp32 sums of the rows when the caller has them (the
         packed gate/up GEMM then skips its own pass over the rows).  ``max_rows``: rows an expert has at most,
-        where that is known."""
+        where that is known.  ``row_scale``: the rows are e4m3 already, with these scales."""
         R = rows.shape[0]
         if y is None:
             y = torch.empty(R, self.hidden, dtype=torch.bfloat16, device=self.device)
@@ -186,6 +197,21 @@ class MoELayer:
                 ev[1].record()
                 ev[2].record()
             ops.grouped_gemm_fp4_e8m0(act, self.w2, self.s2, counts, y, group_list_type=1)
+            if ev:
+                ev[3].record()
+                self.timing = ev
+            return y
+        if self.weight_format == "fp8":
+            if row_scale is None:
+                rows, row_scale = ops.fp8_quantize_rows(rows)
+            act = torch.empty(R, self.inter, dtype=torch.uint8, device=self.device)
+            act_scale = torch.empty(R, self.inter // 128, dtype=torch.float32, device=self.device)
+            ops.grouped_gemm_fp8_block(rows, row_scale, self.w13, self.s13, counts, act, output_scale=act_scale, group_list_type=1,
+                                       gate_up_silu=True)
+            if ev:
+                ev[1].record()
+                ev[2].record()
+            ops.grouped_gemm_fp8_block(act, act_scale, self.w2, self.s2, counts, y, group_list_type=1)
             if ev:
                 ev[3].record()
                 self.timing = ev
@@ -278,8 +304,10 @@ class MoELayer:
             return out
         # one rank on the packed GEMMs: the gather also adds up each row (the gate/up GEMM's offset term needs
         # the sums and would otherwise read all rows once more)
-        sums = None
-        if (self.gather_sums and self.world == 1 and self.gemm == "packed" and self.o13 is not None
+        sums = row_scale = None
+        if self.world == 1 and self.weight_format == "fp8":
+            send, row_scale = ops.fp8_quantize_rows(x, token_of)  # gathered and quantised in one operator
+        elif (self.gather_sums and self.world == 1 and self.gemm == "packed" and self.o13 is not None
                 and self.ops is CudaRowOps):
             send, sums = ops.gather_rows(x, token_of, with_sums=True)
         else:
@@ -289,7 +317,7 @@ class MoELayer:
         if self.world == 1:
             self._mid()
             # (a token's experts differ, so none has more rows than there are tokens)
-            y = self._experts(send, counts, record, rows_sum=sums, max_rows=x.shape[0])
+            y = self._experts(send, counts, record, rows_sum=sums, max_rows=x.shape[0], row_scale=row_scale)
             mark("experts")
             out = finish(y, slot, wts)
             mark("combine")

@@ -62,7 +62,7 @@ def test_scratch_holds_a_row_for_every_piece():
     """Pieces are numbered range + sequence, so there are at most ranges + sequences of them."""
     for T, S in ((0, 1), (1, 1), (17, 3), (4096, 7), (100000, 65535)):
         for E in (1, 7, 256, 1024):
-            chunk = max(16, -(-T // 296))
+            chunk = max(32, -(-T // 148))
             rows = -(-T // chunk) + S
             assert lib.b200moe_moe_balance_scratch_bytes(T, E, S) >= rows * (8 * E + 4)
 

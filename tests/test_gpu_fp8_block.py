@@ -197,6 +197,17 @@ def test_gate_up(counts, K, N, spare):
     _check_gate_up(codes, scale, x, xs, w, ws, R.bounds(counts, 1, x.shape[0]))
 
 
+def test_no_rows():
+    x, xs, w, ws, gl = _problem([0, 0], 256, 512)
+    out, codes = torch.empty(0, 512, dtype=torch.bfloat16, device=DEV), torch.empty(0, 256, dtype=torch.uint8, device=DEV)
+    ak.grouped_gemm_fp8_block(x, xs, w, ws, gl, out, group_list_type=1)
+    ak.grouped_gemm_fp8_block(x, xs, w, ws, gl, codes, output_scale=torch.empty(0, 2, device=DEV), group_list_type=1, gate_up_silu=True)
+    x, xs, w, ws, gl = _problem([0, 0], 256, 512, spare=5)  # rows, but none of an expert's
+    out = torch.full((5, 512), 7.0, dtype=torch.bfloat16, device=DEV)
+    ak.grouped_gemm_fp8_block(x, xs, w, ws, gl, out, group_list_type=1)
+    assert bool((out == 7).all())
+
+
 def test_many_uneven_experts():
     gen = _gen(11)
     counts = (torch.rand(96, generator=gen, device=DEV) ** 4 * 500).int().tolist()

@@ -32,12 +32,12 @@ def _check(logits, idx, seq_list=None, mask=None, seed=0):
     assert torch.equal(counts, want_counts)
     # A probability: the difference of two logits, its product with log2(e), the power of two (2 units), the sum over E experts
     # (a lane's 32 and five steps at most) and the reciprocal: the first two scale with the exponent's size, 2 * 126 at most where
-    # the result is not flushed.  The sum over a sequence's tokens: one rounding for each of the at most T / (2 * 148) + 16 tokens a
+    # the result is not flushed.  The sum over a sequence's tokens: one rounding for each of the at most T / (32 * 148) + 1 tokens a
     # warp adds up, and some more joining.  All terms are positive, so the relative errors carry over to the loss.
     z = logits.float().masked_fill(~torch.isfinite(logits.float()), 0)
     span = float((z.amax(dim=1) - z.amin(dim=1)).clamp(max=126).max()) if T else 0.0
     rel_p = (2 * span + 50) * 2.0 ** -24
-    rel = rel_p + (T / 296 + 64) * 2.0 ** -24
+    rel = rel_p + (T / 4736 + 64) * 2.0 ** -24
     assert bool(((loss.double() - want).abs() <= rel * want + 1e-38).all()), (loss.double() - want, rel * want)
     # The gradient p F' with F' = F - sum F p: p's error, and F's own sum's
     seq = torch.zeros(T, dtype=torch.long, device=DEV) if seq_list is None else torch.searchsorted(seq_list, torch.arange(T, device=DEV), right=True)
