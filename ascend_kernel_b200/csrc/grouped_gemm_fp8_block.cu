@@ -35,24 +35,31 @@ constexpr int kMaxR = 160;             // token rows of a tile
 constexpr int kABytes = 128 * 128;     // 128 weight columns of a stage
 constexpr int kMaxSlots = 12, kMaxBufs = 8;
 constexpr uint32_t kTmemCols = 512;
-constexpr int kStripBytes = 1024;      // of an epilogue warp
+constexpr int kStripBytes = 2048;      // of an epilogue warp
+// The epilogue's warps come in groups of four (128 weight columns), which share the tile's tokens.
+constexpr int kGroups = 2, kEpiWarps = 4 * kGroups, kThreads = (kWarpEpi0 + kEpiWarps) * 32;
 constexpr int kBigBox = 64, kSmallBox = 16;
 constexpr int kScaleRingBytes = (int)kTmemCols * 4;  // a scale for every accumulator column
 constexpr int kBarrierBytes = 2048;
 constexpr int kSmemBytes = 227 * 1024;
 
-// The epilogue's warps come in groups of four (128 weight columns), which share the tile's tokens.  A thread's sums and what it
-// fetches ahead have to fit its registers: 16 warps where it sums one block, 8 with twice the registers where it sums two.
-template <bool GATE_UP>
-struct Shape {
-    static constexpr int kHalves = GATE_UP ? 2 : 1;  // blocks of a stage
-    static constexpr int kGroups = 2, kEpiWarps = 4 * kGroups, kThreads = (kWarpEpi0 + kEpiWarps) * 32;
-    static constexpr int kUnit = 32 / (8 * kGroups);  // 8-token patches of a warp per 32 token rows: 1 or 2
-    static constexpr int kTopBytes = GATE_UP ? kMaxR * 16 : 0;  // [tokens][4 warps] magnitudes, and less for what they give
+// What a tile is: the number of blocks of a stage (128 weight columns of a CTA each) and whether they are gate and up columns.
+template <int HALVES, bool GATE>
+struct Mode {
+    static constexpr int kHalves = HALVES;
+    static constexpr bool kGate = GATE;
+    // columns of a tile: what a pair advances by (gate/up: 256 of each), the CTA's first and the distance of its second block
+    static constexpr int kTileColumns = GATE ? 256 : 256 * HALVES;
+    static __device__ __forceinline__ int first_column(int nt, uint32_t rank) { return nt * kTileColumns + (int)rank * (kTileColumns / 2); }
+    static __device__ __forceinline__ int block_step(int N) { return GATE ? N >> 1 : 128; }
+    static constexpr int kTopBytes = GATE ? kMaxR * 16 : 0;  // [tokens][4 warps] magnitudes, and less for what they give
     static constexpr int kFixedBytes = 1024 + kBarrierBytes + kScaleRingBytes + kEpiWarps * kStripBytes + 2 * kTopBytes + 2 * (kMaxExperts + 4) * 4;
     static constexpr int kRingBytes = kSmemBytes - kFixedBytes;
-    static_assert(kRingBytes % 16 == 0 && kRingBytes >= 4 * (kHalves * kABytes + kMaxR * 64), "stages");
+    static_assert(kRingBytes % 16 == 0 && kRingBytes >= 4 * (HALVES * kABytes + kMaxR * 64), "stages");
 };
+using One = Mode<1, false>;
+using Two = Mode<2, false>;
+using GateUp = Mode<2, true>;
 
 struct Args {
     const float* x_scale;
@@ -255,34 +262,42 @@ __device__ __forceinline__ void store_part(const f32x2 (&acc)[NP][2][2], const T
             }
 }
 
-// bf16 rows, up to 16 tokens x 32 columns at a time through the warp's strip: the transposing store gives 16-byte pieces of eight
-// columns, 64 contiguous bytes of a row.
+// bf16 rows, 16 tokens x 32 columns at a time through the warp's strip: the transposing store gives 16-byte pieces of eight columns,
+// 64 contiguous bytes of a row.  The strip's halves take turns, and a chunk is on its way out while the next one is transposed.
 template <int NP>
 __device__ __forceinline__ void store_rows(const f32x2 (&acc)[NP][2][2], const Tile& t, const Epilogue& e, int first, int col, const Args& a) {
     const int lane = threadIdx.x & 31, g8 = lane >> 2, q = lane & 3;
-    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (size_t)t.row0 * a.N + col + q * 8;
+    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (size_t)(t.row0 + first) * a.N + col + q * 8;
     const bool inside = col + q * 8 < a.N;
+    uint4 out[2];
+    const auto send = [&](int p) {
 #pragma unroll
-    for (int p = 0; p < NP; p += 2) {
+        for (int j = 0; j < 2; ++j) {
+            const int token = p * 8 + j * 8 + g8;
+            if (first + token < t.rows && inside) *reinterpret_cast<uint4*>(dst + (size_t)token * a.N) = out[j];
+        }
+    };
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-            if (p + j < NP) {
-                uint32_t o[4];
+    for (int p = 0; p < NP; p += 2) {  // (NP is even)
+        uint8_t* half = e.strip + (p & 2) * 512;
 #pragma unroll
-                for (int m = 0; m < 4; ++m) o[m] = pack_bf16x2(f32x2_lo(acc[p + j][m >> 1][m & 1]), f32x2_hi(acc[p + j][m >> 1][m & 1]));
-                const int token = j * 8 + (lane & 7);  // row lane % 8 of piece lane / 8
-                ptx::stmatrix_x4_trans(ptx::smem_u32(e.strip) + (uint32_t)(token * 64 + (((lane >> 3) ^ (token >> 1)) & 3) * 16), o[0], o[1], o[2], o[3]);
-            }
+        for (int j = 0; j < 2; ++j) {
+            uint32_t o[4];
+#pragma unroll
+            for (int m = 0; m < 4; ++m) o[m] = pack_bf16x2(f32x2_lo(acc[p + j][m >> 1][m & 1]), f32x2_hi(acc[p + j][m >> 1][m & 1]));
+            const int token = j * 8 + (lane & 7);  // row lane % 8 of piece lane / 8
+            ptx::stmatrix_x4_trans(ptx::smem_u32(half) + (uint32_t)(token * 64 + (((lane >> 3) ^ (token >> 1)) & 3) * 16), o[0], o[1], o[2], o[3]);
+        }
         __syncwarp();
+        if (p > 0) send(p - 2);
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-            if (p + j < NP) {
-                const int token = j * 8 + g8, row = first + p * 8 + token;
-                const uint4 o = *reinterpret_cast<const uint4*>(e.strip + token * 64 + ((q ^ (token >> 1)) & 3) * 16);
-                if (row < t.rows && inside) *reinterpret_cast<uint4*>(dst + (size_t)row * a.N) = o;
-            }
-        __syncwarp();
+        for (int j = 0; j < 2; ++j) {
+            const int token = j * 8 + g8;
+            out[j] = *reinterpret_cast<const uint4*>(half + token * 64 + ((q ^ (token >> 1)) & 3) * 16);
+        }
     }
+    send(NP - 2);
+    __syncwarp();
 }
 
 // silu(gate) * up of the thread's columns and tokens, quantised by the rows' 128 columns: the warps of a group put what their 32
@@ -357,53 +372,80 @@ __device__ __forceinline__ bool store_quantized(f32x2 (&gate)[NP][2][2], const f
 }
 
 // A tile's sums and what becomes of them; NP: patches of 8 tokens a warp has.
-template <bool GATE_UP, int NP>
+template <class M, int NP>
 __device__ __forceinline__ bool finish_tile(const Tile& t, Epilogue& e, Sync* sy, const Args& a) {
-    constexpr int kHalves = Shape<GATE_UP>::kHalves;
+    constexpr int kHalves = M::kHalves;
     const int first = (e.warp >> 2) * (NP * 8), quarter = e.warp & 3;
     f32x2 acc[kHalves][NP][2][2];
 #pragma unroll
     for (int u = 0; u < kHalves; ++u)
 #pragma unroll
         for (int p = 0; p < NP; ++p) acc[u][p][0][0] = acc[u][p][0][1] = acc[u][p][1][0] = acc[u][p][1][1] = 0ull;
+    const int col = M::first_column(t.nt, e.rank) + quarter * 32;
     for (int kb = t.kb0; kb < t.kb1; ++kb)
 #pragma unroll
-        for (int u = 0; u < kHalves; ++u)
+        for (int u = 0; u < kHalves; ++u) {
             if (!add_block<NP>(acc[u], e, (uint32_t)first, sy, a)) return false;
-    const int block = t.nt * 2 + (int)e.rank, col = block * 128 + quarter * 32;
+            // (the first block's rows go out while the second one's last sum is made)
+            if (!M::kGate && u + 1 < kHalves && kb + 1 == t.kb1 && e.parts == 1) store_rows<NP>(acc[u], t, e, first, col + u * 128, a);
+        }
     if (e.parts > 1) {
-        const int out_n = GATE_UP ? a.N >> 1 : a.N;
+        const int step = M::block_step(a.N), end = M::kGate ? step : a.N;  // (a block's columns end there)
 #pragma unroll
-        for (int u = 0; u < kHalves; ++u) store_part<NP>(acc[u], t, first, u * out_n + col, out_n - col, a);
+        for (int u = 0; u < kHalves; ++u) store_part<NP>(acc[u], t, first, u * step + col, end - col - (M::kGate ? 0 : u * step), a);
         return true;
     }
-    if constexpr (GATE_UP) {
-        return store_quantized<NP>(acc[0], acc[1], t, e, first, block, sy, a);
+    if constexpr (M::kGate) {
+        return store_quantized<NP>(acc[0], acc[1], t, e, first, col >> 7, sy, a);
     } else {
-        store_rows<NP>(acc[0], t, e, first, col, a);
+        store_rows<NP>(acc[kHalves - 1], t, e, first, col + (kHalves - 1) * 128, a);
         return true;
     }
 }
 
-template <bool GATE_UP>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<GATE_UP>::kThreads, 1)
+template <class M>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x64,
                    const __grid_constant__ CUtensorMap map_x16, const Args a) {
-    using S = Shape<GATE_UP>;
-    constexpr int kHalves = S::kHalves;
+    constexpr int kHalves = M::kHalves;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = smem_raw + ((1024u - (ptx::smem_u32(smem_raw) & 1023u)) & 1023u);
-    Sync* sy = reinterpret_cast<Sync*>(ring + S::kRingBytes);
-    float* scales = reinterpret_cast<float*>(ring + S::kRingBytes + kBarrierBytes);
+    Sync* sy = reinterpret_cast<Sync*>(ring + M::kRingBytes);
+    float* scales = reinterpret_cast<float*>(ring + M::kRingBytes + kBarrierBytes);
     uint8_t* strips = reinterpret_cast<uint8_t*>(scales) + kScaleRingBytes;
-    float* tops = reinterpret_cast<float*>(strips + S::kEpiWarps * kStripBytes);
-    int* row_start = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(tops) + 2 * S::kTopBytes);
+    float* tops = reinterpret_cast<float*>(strips + kEpiWarps * kStripBytes);
+    int* row_start = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(tops) + 2 * M::kTopBytes);
     int* prefix = row_start + kMaxExperts + 4;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = ptx::cluster_rank();
-    const int n_nt = GATE_UP ? (a.N + 511) / 512 : (a.N + 255) / 256;
+    const int n_nt = ((M::kGate ? a.N >> 1 : a.N) + M::kTileColumns - 1) / M::kTileColumns;
 
+    // what needs nothing from memory comes first: the kernel may have started beside the end of the one before it
+    if (threadIdx.x == kThreads - 32) {
+        sy->abort = 0;
+        for (int i = 0; i < kTileRing; ++i) sy->ring[i] = tile_entry(0u, 0u, 0u, 0u, 0u);
+        const auto init = [](uint64_t* b, int n, uint32_t count) {
+            for (int i = 0; i < n; ++i) ptx::mbar_init(ptx::smem_u32(b + i), count);
+        };
+        init(sy->full, kMaxSlots, 1);
+        init(sy->empty, kMaxSlots, kHalves);
+        init(sy->t_full, kMaxBufs, 2);
+        init(sy->t_empty, kMaxBufs, 2 * kEpiWarps);
+        init(sy->s_empty, kMaxBufs, kEpiWarps);
+        init(sy->wg, kGroups, 4);
+        init(sy->drain, 2, 1);
+        ptx::fence_mbar_init();
+        ptx::prefetch_tensormap(&map_w);
+        ptx::prefetch_tensormap(&map_x64);
+        ptx::prefetch_tensormap(&map_x16);
+    }
+    if (warp == kWarpMma0) {
+        ptx::tmem_alloc_pair(ptx::smem_u32(&sy->tmem_base), kTmemCols);
+        ptx::tmem_relinquish_pair();
+    }
+    grid_dep_wait();
+    grid_dep_launch();
     load_row_starts(a.group_list, a.G, a.M, a.gl_type, row_start, nullptr, blockIdx.x == 0 ? a.findings : nullptr);
     if (warp == 0) {
         int lo, hi, mine = 0, total, wide = 0;
@@ -433,28 +475,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<GATE_UP>::kThr
             }
         }
     }
-    if (threadIdx.x == 32) {
-        sy->abort = 0;
-        for (int i = 0; i < kTileRing; ++i) sy->ring[i] = tile_entry(0u, 0u, 0u, 0u, 0u);
-        const auto init = [](uint64_t* b, int n, uint32_t count) {
-            for (int i = 0; i < n; ++i) ptx::mbar_init(ptx::smem_u32(b + i), count);
-        };
-        init(sy->full, kMaxSlots, 1);
-        init(sy->empty, kMaxSlots, kHalves);
-        init(sy->t_full, kMaxBufs, 2);
-        init(sy->t_empty, kMaxBufs, 2 * S::kEpiWarps);
-        init(sy->s_empty, kMaxBufs, S::kEpiWarps);
-        init(sy->wg, S::kGroups, 4);
-        init(sy->drain, 2, 1);
-        ptx::fence_mbar_init();
-        ptx::prefetch_tensormap(&map_w);
-        ptx::prefetch_tensormap(&map_x64);
-        ptx::prefetch_tensormap(&map_x16);
-    }
-    if (warp == kWarpMma0) {
-        ptx::tmem_alloc_pair(ptx::smem_u32(&sy->tmem_base), kTmemCols);
-        ptx::tmem_relinquish_pair();
-    }
     ptx::tc_fence_before();
     __syncthreads();
     ptx::cluster_sync();
@@ -463,7 +483,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<GATE_UP>::kThr
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sy->tmem_base);
     const int parts = sy->parts, n_units = sy->n_units, width = sy->width;
     const int slot_bytes = kHalves * kABytes + width * 64;
-    const int n_slots = min(kMaxSlots, S::kRingBytes / slot_bytes);
+    const int n_slots = min(kMaxSlots, M::kRingBytes / slot_bytes);
     const int n_bufs = min(kMaxBufs, (int)kTmemCols / width);
 
     if (warp < kWarpEpi0) {
@@ -502,7 +522,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<GATE_UP>::kThr
                 if (!next_tile<true>(sy, seq, t, a, parts)) break;
                 const int half = t.n >> 1, n_big = half / kBigBox, n_small = (half % kBigBox) / kSmallBox;
                 const uint32_t bytes = 2u * (uint32_t)(kHalves * kABytes + half * 128);
-                const int col = t.nt * 256 + (int)rank * 128;
+                const int col = M::first_column(t.nt, rank);
                 const int row = t.row0 + (int)rank * half;
                 for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
                     if (it >= (uint32_t)n_slots && !wait<true>(&sy->empty[slot], ph ^ 1, sy, a.findings, 10)) { ok = false; break; }
@@ -511,7 +531,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<GATE_UP>::kThr
                         if (rank == 0) ptx::mbar_arrive_expect_tx(full_here + slot * 8, bytes);
 #pragma unroll
                         for (int u = 0; u < kHalves; ++u)
-                            ptx::tma_load_3d_pair(dst + u * kABytes, &map_w, bar0, col + u * (a.N >> 1), kb * 128, t.g);
+                            ptx::tma_load_3d_pair(dst + u * kABytes, &map_w, bar0, col + u * M::block_step(a.N), kb * 128, t.g);
                         uint32_t at = dst + kHalves * kABytes;
                         int r = row;
                         for (int b = 0; b < n_big; ++b, at += kBigBox * 128, r += kBigBox)
@@ -544,7 +564,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<GATE_UP>::kThr
                 const float* ws = a.w_scale + (size_t)t.g * a.KB * a.NB;
                 int nb[kHalves];
 #pragma unroll
-                for (int u = 0; u < kHalves; ++u) nb[u] = min(a.NB - 1, t.nt * 2 + (int)rank + u * (a.NB >> 1));
+                for (int u = 0; u < kHalves; ++u) nb[u] = min(a.NB - 1, (M::first_column(t.nt, rank) + u * M::block_step(a.N)) >> 7);
                 const float* xs = a.x_scale + (size_t)(t.row0 + lane) * a.KB;
                 const size_t group = (size_t)a.KB * 32;
                 for (int kb = t.kb0; kb < t.kb1 && ok; kb += 4) {  // (four stages' loads in flight)
@@ -638,17 +658,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<GATE_UP>::kThr
         e.scales = scales;
         e.strip = strips + e.warp * kStripBytes;
         e.tops = tops;
-        e.quantizers = tops + S::kTopBytes / 4;
+        e.quantizers = tops + M::kTopBytes / 4;
         uint32_t seq = 0;
         bool ok = true;
         Tile t;
         while (ok && next_tile<true>(sy, seq, t, a, parts)) {
             switch (t.n >> 5) {
-                case 1: ok = finish_tile<GATE_UP, 1 * S::kUnit>(t, e, sy, a); break;
-                case 2: ok = finish_tile<GATE_UP, 2 * S::kUnit>(t, e, sy, a); break;
-                case 3: ok = finish_tile<GATE_UP, 3 * S::kUnit>(t, e, sy, a); break;
-                case 4: ok = finish_tile<GATE_UP, 4 * S::kUnit>(t, e, sy, a); break;
-                default: ok = finish_tile<GATE_UP, 5 * S::kUnit>(t, e, sy, a); break;
+                case 1: ok = finish_tile<M, 1 * 2>(t, e, sy, a); break;
+                case 2: ok = finish_tile<M, 2 * 2>(t, e, sy, a); break;
+                case 3: ok = finish_tile<M, 3 * 2>(t, e, sy, a); break;
+                case 4: ok = finish_tile<M, 4 * 2>(t, e, sy, a); break;
+                default: ok = finish_tile<M, 5 * 2>(t, e, sy, a); break;
             }
         }
     }
@@ -661,7 +681,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<GATE_UP>::kThr
         ptx::tc_fence_after();
         ptx::tmem_dealloc_pair(tmem_base, kTmemCols);
     }
-    grid_dep_launch();
 }
 
 // The parts of a split k range, added in their order.  A warp takes 128 columns of a row.
@@ -698,11 +717,29 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a) {
     }
 }
 
+constexpr int64_t kPairs = 74;  // of a B200's multiprocessors (rules and sizes go by the sizes of a call alone)
+
+// Whether a tile's stage holds two blocks of 128 columns a CTA: a pair then reads 512 contiguous bytes of a weight row and the rows of x
+// half as often, but has three to five stages in flight instead of seven to eleven.  One | two blocks, us (experts, tokens x
+// top_k, K x N): 256, 37 x 8, 2048 x 7168: 445 | 376; 256, 1024 x 8, 7168 x 4096: 1325 | 1138; 256, 2048 x 8, 2048 x 7168: 851 | 662, of 80 rows
+// an expert 840 | 772, of 96 rows 810 | 924, of 128 rows 966 | 1148.  Where the tiles are a few waves of the pairs, the cut that
+// fills its last wave better: 8 experts of a row, 2048 x 7168: 29.8 | 27.2; 64 experts of 64 rows, 2048 x 2048: 58.6 | 65.5.
+static bool two_blocks(int64_t M, int64_t N, int64_t G) {
+    if (N < 1024 || M > 80 * G) return false;
+    const int64_t tiles = std::min(G, M) * ((N + Two::kTileColumns - 1) / Two::kTileColumns);
+    if (tiles < kPairs || tiles >= 7 * kPairs) return true;
+    return 2 * ((tiles + kPairs - 1) / kPairs) <= (2 * tiles + kPairs - 1) / kPairs;
+}
+static int64_t tiles_across(int64_t M, int64_t N, int64_t G, int gate_up) {
+    const int64_t columns = gate_up ? 2 * GateUp::kTileColumns : two_blocks(M, N, G) ? Two::kTileColumns : One::kTileColumns;
+    return (N + columns - 1) / columns;
+}
+
 // Whether a call can have fewer tiles than there are pairs of multiprocessors, and in how many parts its k range is cut at most: parts of
 // four blocks or more, sums of 32 MB or less.
 static int max_parts(int64_t M, int64_t K, int64_t N, int64_t G, int gate_up) {
-    const int64_t width = gate_up ? 512 : 256, n_nt = (N + width - 1) / width, experts = std::min(G, M);
-    if (experts * n_nt >= 74) return 1;
+    const int64_t n_nt = tiles_across(M, N, G, gate_up), experts = std::min(G, M);
+    if (experts * n_nt >= kPairs) return 1;
     const int64_t kb = (K + 127) / 128, room = (32ll << 20) / (M * N * 4);
     return (int)std::max<int64_t>(1, std::min<int64_t>({16, kb / 4, room}));
 }
@@ -757,12 +794,11 @@ extern "C" int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scal
     if (rc == B200MOE_OK) rc = make_tensor_map_2d(&map_x16, x, 1, (uint64_t)M, (uint64_t)K, fb::kSmallBox, 128, true);
     if (rc != B200MOE_OK) return rc;
     const unsigned grid = (unsigned)(sm_count() / 2 * 2);
-    const auto kernel = gate_up_silu ? fb::grouped_kernel<true> : fb::grouped_kernel<false>;
+    const auto kernel = gate_up_silu ? fb::grouped_kernel<fb::GateUp> : fb::two_blocks(M, N, G) ? fb::grouped_kernel<fb::Two> : fb::grouped_kernel<fb::One>;
     B200MOE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, fb::kSmemBytes));
-    a.dynamic = ((N + 255) / 256) * std::min(G, M) >= 8 * (int64_t)grid;
+    a.dynamic = fb::tiles_across(M, N, G, gate_up_silu) * std::min(G, M) >= 16 * fb::kPairs;
     if (a.dynamic) B200MOE_CUDA_TRY(cudaMemsetAsync(workspace, 0, fb::kWordBytes, st));
-    kernel<<<grid, gate_up_silu ? fb::Shape<true>::kThreads : fb::Shape<false>::kThreads, fb::kSmemBytes, st>>>(map_w, map_x64, map_x16, a);
-    B200MOE_CUDA_TRY(cudaGetLastError());
+    B200MOE_CUDA_TRY(launch_dependent(kernel, grid, fb::kThreads, fb::kSmemBytes, st, map_w, map_x64, map_x16, a));
     if (a.max_parts > 1) {
         const int64_t out_n = gate_up_silu ? N / 2 : N;
         const unsigned blocks = (unsigned)((M * ((out_n + 127) / 128) + 7) / 8);
