@@ -181,6 +181,12 @@ __device__ __forceinline__ float silu(float g) {
     const float e = __expf(-fabsf(g));  // (at most 1: nothing overflows)
     return g * __fdividef(g < 0.f ? e : 1.f, 1.f + e);
 }
+// Of two values, with one reciprocal for both denominators, which are at most 2.
+__device__ __forceinline__ void silu2(float& g0, float& g1) {
+    const float e0 = __expf(-fabsf(g0)), e1 = __expf(-fabsf(g1)), d0 = 1.f + e0, d1 = 1.f + e1, r = __fdividef(1.f, d0 * d1);
+    g0 *= (g0 < 0.f ? e0 : 1.f) * (r * d1);
+    g1 *= (g1 < 0.f ? e1 : 1.f) * (r * d0);
+}
 
 // What an epilogue warp carries from tile to tile.
 struct Epilogue {
@@ -315,8 +321,10 @@ __device__ __forceinline__ bool store_quantized(f32x2 (&gate)[NP][2][2], const f
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float lo = silu(f32x2_lo(gate[p][h][i])) * f32x2_lo(up[p][h][i]);
-                const float hi = silu(f32x2_hi(gate[p][h][i])) * f32x2_hi(up[p][h][i]);
+                float lo = f32x2_lo(gate[p][h][i]), hi = f32x2_hi(gate[p][h][i]);
+                silu2(lo, hi);
+                lo *= f32x2_lo(up[p][h][i]);
+                hi *= f32x2_hi(up[p][h][i]);
                 m0 = max(m0, __float_as_uint(lo) & 0x7FFFFFFFu);
                 m1 = max(m1, __float_as_uint(hi) & 0x7FFFFFFFu);
                 gate[p][h][i] = pack_f32x2(lo, hi);
