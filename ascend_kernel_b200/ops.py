@@ -530,7 +530,7 @@ def fp8_quantize_rows(x, index=None, codes=None, scale=None):
     the block's largest magnitude a (at least 2^-100).  ``index`` int32 [R]: row i of the result is row index[i] of x (R = T and row i
     without it); an index outside x gives zeros.  A block with an infinity or a NaN gets scale NaN.  K % 16 == 0."""
     out = _ext().fp8_quantize_rows(x, index, codes, scale)
-    _count(1)
+    _count(int(out[0].numel() > 0))
     return out
 
 
@@ -542,7 +542,7 @@ def grouped_gemm_fp8_block(x, x_scale, weight, weight_scale, group_list, output,
     [M, I] and output_scale [M, I / 128] = silu(gate) * up quantised like :func:`fp8_quantize_rows`, which the down projection takes
     as they are.  K and N multiples of 16, with ``gate_up_silu`` N of 256.  Codes are uint8 or float8_e4m3fn tensors."""
     _ext().grouped_gemm_fp8_block(x, x_scale, weight, weight_scale, group_list, output, output_scale, group_list_type, gate_up_silu)
-    _count(1)
+    _count(int(x.shape[0] > 0))
 
 
 def moe_balance_loss(logits, idx, seq_list=None, token_mask=None):
@@ -554,7 +554,7 @@ def moe_balance_loss(logits, idx, seq_list=None, token_mask=None):
     For T_s tokens with probabilities p = softmax(logits) and c_e pairs on expert e, loss = E / (k T_s) * sum_e c_e * mean_t p_te: 1
     where the load is even; 0 for a sequence without tokens.  The counts carry no gradient."""
     out = _ext().moe_balance_loss(logits, idx, seq_list, token_mask)
-    _count(2)
+    _count(1 + (logits.shape[0] > 0))
     return out
 
 

@@ -360,3 +360,50 @@ def test_refusals():
                  (xb, None, torch.empty(3, 256, dtype=torch.uint8, device=DEV)), (xb, None, None, torch.empty(4, 1, device=DEV)), (xb.cpu(),)]:
         with pytest.raises(RuntimeError):
             ak.fp8_quantize_rows(*args)
+
+
+def test_offsets_behind_31_bits():
+    """Results and codes of more than 2^31 elements: the rows at the end against the same rows of a short call."""
+    gen = _gen(20)
+    M, K, N, tail = 300_000, 128, 7168, 300
+    assert M * N > 2 ** 31
+    x, w = _codes((M, K), gen), _codes((1, K, N), gen)
+    xs, ws = torch.rand(M, 1, generator=gen, device=DEV) + 0.5, torch.rand(1, 1, N // 128, generator=gen, device=DEV) / 1000
+    out = torch.empty(M, N, dtype=torch.bfloat16, device=DEV)
+    ak.grouped_gemm_fp8_block(x, xs, w, ws, torch.tensor([M], dtype=torch.int64, device=DEV), out, group_list_type=1)
+    short = torch.empty(tail, N, dtype=torch.bfloat16, device=DEV)
+    ak.grouped_gemm_fp8_block(x[-tail:].contiguous(), xs[-tail:].contiguous(), w, ws, torch.tensor([tail], dtype=torch.int64, device=DEV),
+                              short, group_list_type=1)
+    assert torch.equal(out[-tail:], short)
+    codes, scale = ak.fp8_quantize_rows(out)
+    want, want_scale = ak.fp8_quantize_rows(out[-tail:].contiguous())
+    assert torch.equal(codes[-tail:], want) and torch.equal(scale[-tail:], want_scale)
+
+
+def test_on_another_stream():
+    x, xs, w, ws, gl = _problem([5, 40, 2], 512, 1024, 0, seed=21)
+    want = torch.empty(47, 1024, dtype=torch.bfloat16, device=DEV)
+    ak.grouped_gemm_fp8_block(x, xs, w, ws, gl, want, group_list_type=1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    outs = [torch.empty_like(want) for _ in range(8)]
+    for i, out in enumerate(outs):  # two streams side by side
+        with torch.cuda.stream(side if i & 1 else torch.cuda.current_stream()):
+            ak.grouped_gemm_fp8_block(x, xs, w, ws, gl, out, group_list_type=1)
+    torch.cuda.synchronize()
+    for out in outs:
+        assert torch.equal(out, want)
+
+
+def test_cuts_of_the_columns_give_the_same_products():
+    """Few rows go through stages of two blocks of columns, many through stages of one, few tiles through parts of the k range: a row's
+    result differs by the order of its fp32 sums at most."""
+    K, N = 1280, 1024
+    x, xs, w, ws, _ = _problem([200], K, N, 0, seed=22)
+    many = torch.empty(200, N, dtype=torch.bfloat16, device=DEV)
+    ak.grouped_gemm_fp8_block(x, xs, w, ws, torch.tensor([200], dtype=torch.int64, device=DEV), many, group_list_type=1)
+    few = torch.empty(40, N, dtype=torch.bfloat16, device=DEV)
+    ak.grouped_gemm_fp8_block(x[:40].contiguous(), xs[:40].contiguous(), w, ws, torch.tensor([40], dtype=torch.int64, device=DEV), few,
+                              group_list_type=1)
+    for out, rows in ((many, 200), (few, 40)):
+        _check_product(out, x[:rows], xs[:rows], w, ws, [(0, rows)])

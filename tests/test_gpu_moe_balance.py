@@ -214,6 +214,46 @@ def test_behind_the_router_in_a_captured_graph():
         assert torch.equal(x, y)
 
 
+def test_offsets_behind_31_bits():
+    """More than 2^31 logits: the last sequence against a call on its tokens alone."""
+    T, E, tail = 2 ** 21 + 77, 1024, 500
+    logits = torch.randn(T, E, device=DEV, dtype=torch.bfloat16, generator=_gen(15))
+    idx = torch.randint(0, E, (T, 2), generator=_gen(16), device=DEV).to(torch.int32)
+    g = torch.tensor([0.0, 1.0], device=DEV)
+    leaf = logits.requires_grad_()
+    loss, counts = ak.moe_balance_loss(leaf, idx, torch.tensor([T - tail, T], dtype=torch.int64, device=DEV))
+    (grad,) = torch.autograd.grad(loss, leaf, g)
+    end = logits.detach()[-tail:].clone().requires_grad_()
+    want, want_counts = ak.moe_balance_loss(end, idx[-tail:].contiguous())
+    (want_grad,) = torch.autograd.grad(want, end, g[1:])
+    assert torch.equal(counts[1], want_counts[0]) and torch.equal(grad[-tail:], want_grad) and not bool(grad[:1000].any())
+    # (the sums of the probabilities in another order: one rounding for each of 500 tokens at most)
+    assert abs(float(loss[1].detach()) - float(want.detach())) <= 500 * 2.0 ** -24 * float(want.detach())
+
+
+def test_second_derivative_is_refused():
+    logits, idx = _router(10, 8, 2, torch.float32)
+    leaf = logits.requires_grad_()
+    loss, _ = ak.moe_balance_loss(leaf, idx)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(loss.sum(), leaf, create_graph=True)
+
+
+def test_upstream_gradients_of_every_kind():
+    """An expanded gradient (of a sum), none at all, one of another loss beside it, logits that are no leaf."""
+    logits, idx = _router(40, 16, 2, torch.float32, seed=17)
+    seq_list = torch.tensor([10, 40], dtype=torch.int64, device=DEV)
+    leaf = logits.clone().requires_grad_()
+    loss, counts = ak.moe_balance_loss(leaf * 1.0, idx, seq_list)
+    (loss.sum() + (leaf * 2).sum()).backward()
+    _, _, want = R.balance(logits, idx, seq_list, None, torch.ones(2, device=DEV))
+    # (the gradients are at most 16 / 10, good to some 2^-18 of that, and 2 is added)
+    assert bool(((leaf.grad.double() - 2 - want).abs() <= 2.0 ** -16).all())
+    assert not counts.requires_grad
+    with torch.no_grad():
+        assert not ak.moe_balance_loss(leaf, idx, seq_list)[0].requires_grad
+
+
 def test_refusals():
     logits, idx = _router(20, 16, 2, torch.float32)
     mask, seqs = torch.ones(20, dtype=torch.bool, device=DEV), torch.tensor([20], dtype=torch.int64, device=DEV)
