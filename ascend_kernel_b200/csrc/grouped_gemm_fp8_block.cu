@@ -181,7 +181,8 @@ __device__ __forceinline__ float silu(float g) {
     const float e = __expf(-fabsf(g));  // (at most 1: nothing overflows)
     return g * __fdividef(g < 0.f ? e : 1.f, 1.f + e);
 }
-// Of two values, with one reciprocal for both denominators, which are at most 2.
+// Of two values, with one reciprocal for both denominators, which are at most 2.  A NaN in one makes the other NaN: for two columns of a row
+// in the same block of 128, which has no finite scale then anyway, never for two rows.
 __device__ __forceinline__ void silu2(float& g0, float& g1) {
     const float e0 = __expf(-fabsf(g0)), e1 = __expf(-fabsf(g1)), d0 = 1.f + e0, d1 = 1.f + e1, r = __fdividef(1.f, d0 * d1);
     g0 *= (g0 < 0.f ? e0 : 1.f) * (r * d1);
@@ -318,17 +319,19 @@ __device__ __forceinline__ bool store_quantized(f32x2 (&gate)[NP][2][2], const f
     for (int p = 0; p < NP; ++p) {
         uint32_t m0 = 0, m1 = 0;  // magnitudes order as their bits do, infinities and NaN last
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) {
+            float lo[2] = {f32x2_lo(gate[p][h][0]), f32x2_lo(gate[p][h][1])}, hi[2] = {f32x2_hi(gate[p][h][0]), f32x2_hi(gate[p][h][1])};
+            silu2(lo[0], lo[1]);
+            silu2(hi[0], hi[1]);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                float lo = f32x2_lo(gate[p][h][i]), hi = f32x2_hi(gate[p][h][i]);
-                silu2(lo, hi);
-                lo *= f32x2_lo(up[p][h][i]);
-                hi *= f32x2_hi(up[p][h][i]);
-                m0 = max(m0, __float_as_uint(lo) & 0x7FFFFFFFu);
-                m1 = max(m1, __float_as_uint(hi) & 0x7FFFFFFFu);
-                gate[p][h][i] = pack_f32x2(lo, hi);
+                lo[i] *= f32x2_lo(up[p][h][i]);
+                hi[i] *= f32x2_hi(up[p][h][i]);
+                m0 = max(m0, __float_as_uint(lo[i]) & 0x7FFFFFFFu);
+                m1 = max(m1, __float_as_uint(hi[i]) & 0x7FFFFFFFu);
+                gate[p][h][i] = pack_f32x2(lo[i], hi[i]);
             }
+        }
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
             m0 = max(m0, __shfl_xor_sync(0xffffffffu, m0, o));

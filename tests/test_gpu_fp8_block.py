@@ -245,6 +245,24 @@ def test_a_bad_row_stays_its_own_and_the_next_experts_rows_too():
         assert torch.equal(out[r], clean[r])
 
 
+def test_a_bad_row_leaves_its_neighbours_codes_alone():
+    """The same of the quantised product: a NaN row, and NaN rows behind the last one of a tile."""
+    counts, K, N = [5, 3], 400, 512
+    x, xs, w, ws, gl = _problem(counts, K, N, 5, seed=23)
+
+    def run():
+        codes, scale = torch.zeros(13, N // 2, dtype=torch.uint8, device=DEV), torch.zeros(13, N // 256, device=DEV)
+        ak.grouped_gemm_fp8_block(x, xs, w, ws, gl, codes, output_scale=scale, group_list_type=1, gate_up_silu=True)
+        return codes, scale
+
+    codes, scale = run()
+    x[2, 17], x[8:] = 0x7F, 0xFF
+    got, got_scale = run()
+    assert bool(torch.isnan(got_scale[2]).all()) and not bool(got[2].any())
+    for r in (0, 1, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12):
+        assert torch.equal(got[r], codes[r]) and torch.equal(got_scale[r], scale[r])
+
+
 def test_nan_weights_stay_in_their_column_and_expert():
     counts, K, N = [3, 3, 3], 144, 272  # (K ends inside a block: what follows belongs to the next expert)
     x, xs, w, ws, gl = _problem(counts, K, N, 0, seed=7)
