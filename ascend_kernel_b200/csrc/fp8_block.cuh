@@ -8,7 +8,6 @@
 namespace b200moe {
 namespace fp8_block {
 
-constexpr int kBlock = 128;
 constexpr float kMax = 448.f;            // largest finite e4m3
 constexpr float kFloor = 0x1p-100f;      // a block's largest magnitude counts as at least this much
 

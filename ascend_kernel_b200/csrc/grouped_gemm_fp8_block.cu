@@ -95,15 +95,10 @@ struct Tile {
     int g, row0, rows, n, nt, kb0, kb1, part;  // n: rows rounded up to 32; nt: 256 columns (gate/up: 256 of each)
 };
 
-// Waits and tile look-ups of whole warps vote at every poll, so that a warp leaves them together (instructions for the whole warp
-// follow); kWarp false: a single lane.
-template <bool kWarp>
-__device__ __forceinline__ bool all(bool v) {
-    if constexpr (kWarp) return __all_sync(0xffffffffu, v);
-    else return v;
-}
+// Waits and tile look-ups are a whole warp's: it votes at every poll and so leaves them together (instructions for the whole warp
+// follow; with lanes that left at different times these ran in halves).
+__device__ __forceinline__ bool all(bool v) { return __all_sync(0xffffffffu, v); }
 // Whether a poll that has failed `spins` times gives up: the other roles have, or the time is over.
-template <bool kWarp>
 __device__ __forceinline__ bool give_up(uint32_t spins, uint64_t& t0, Sync* sy, int* findings, int id) {
     if ((spins & 0xFF) != 0) return false;
     if (spins == 0) {
@@ -116,27 +111,24 @@ __device__ __forceinline__ bool give_up(uint32_t spins, uint64_t& t0, Sync* sy, 
         keep_finding(findings, kDevWaitExpired, id);
         out = true;
     }
-    return !all<kWarp>(!out);
+    return !all(!out);
 }
-// kCluster: for what the other CTA of the pair wrote into this one's shared memory
-template <bool kWarp, bool kCluster = false>
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Sync* sy, int* findings, int id) {
     const uint32_t b = ptx::smem_u32(bar);
     uint64_t t0 = 0;
-    for (uint32_t spins = 0; !all<kWarp>(kCluster ? ptx::mbar_try_wait_cluster(b, parity) : ptx::mbar_try_wait(b, parity)); ++spins)
-        if (give_up<kWarp>(spins, t0, sy, findings, id)) return false;
+    for (uint32_t spins = 0; !all(ptx::mbar_try_wait(b, parity)); ++spins)
+        if (give_up(spins, t0, sy, findings, id)) return false;
     return true;
 }
 
 // The seq-th tile of the pair (seq is advanced); false when the schedule has ended, a wait expired or another role aborted.
-template <bool kWarp>
 __device__ __forceinline__ bool next_tile(Sync* sy, uint32_t& seq, Tile& t, const Args& a, int parts) {
     const TileEntry* e = &sy->ring[seq % kTileRing];
     const uint32_t want = seq + 1;
     TileEntry v;
     uint64_t t0 = 0;
-    for (uint32_t spins = 0; !all<kWarp>(tile_entry_is(v = ring_load(e), want)); ++spins)
-        if (give_up<kWarp>(spins, t0, sy, a.findings, 90)) return false;
+    for (uint32_t spins = 0; !all(tile_entry_is(v = ring_load(e), want)); ++spins)
+        if (give_up(spins, t0, sy, a.findings, 90)) return false;
     ++seq;
     t.rows = tile_entry_rows(v);
     if (t.rows == 0) return false;
@@ -201,22 +193,19 @@ struct Epilogue {
 // One block into the warp's sums.  The warp holds 32 weight columns (tensor-memory lanes) x NP patches of 8 tokens:
 // acc[patch][16 lanes][8 lanes], two tokens to a register pair: lane (g8, q) has columns g8, g8 + 8, .. and tokens 2q, 2q + 1.  The number
 // of patches is a constant: a warp passes here once a block of 128 k, and its instructions are what a block costs (with a
-// test at every patch, 1000 cycles a block instead of 600).
+// test at every patch, 1000 cycles a block instead of 600).  It is even.
 template <int NP>
 __device__ __forceinline__ bool add_block(f32x2 (&acc)[NP][2][2], Epilogue& e, uint32_t first, Sync* sy, const Args& a) {
+    static_assert(NP % 2 == 0, "patches go in twos");
     const int lane = threadIdx.x & 31, q = lane & 3;
     const uint32_t column = e.buf * e.width + first, td = e.tmem + column;
     const float2* sv = reinterpret_cast<const float2*>(e.scales + column) + q;
-    if (!wait<true>(&sy->t_full[e.buf], e.ph, sy, a.findings, 50)) return false;
+    if (!wait(&sy->t_full[e.buf], e.ph, sy, a.findings, 50)) return false;
     ptx::tc_fence_after();
     uint32_t v[2][2][8];  // two patches are fetched while the two before them are added
     const auto fetch = [&](int p, uint32_t(&d)[2][8]) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t at = td + (uint32_t)(p * 8) + ((uint32_t)(h * 16) << 16);
-            if (p + 1 < NP) ptx::tmem_ld_16x16(at, d[h]);
-            else ptx::tmem_ld_16x8(at, d[h]);
-        }
+        for (int h = 0; h < 2; ++h) ptx::tmem_ld_16x16(td + (uint32_t)(p * 8) + ((uint32_t)(h * 16) << 16), d[h]);
     };
     fetch(0, v[0]);
 #pragma unroll
@@ -231,18 +220,17 @@ __device__ __forceinline__ bool add_block(f32x2 (&acc)[NP][2][2], Epilogue& e, u
             if (lane == 0) ptx::mbar_arrive_remote(e.t_empty + e.buf * 8);
         }
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-            if (p + j < NP) {
-                const float2 s = sv[(p + j) * 4];
-                const f32x2 s2 = pack_f32x2(s.x, s.y);
+        for (int j = 0; j < 2; ++j) {
+            const float2 s = sv[(p + j) * 4];
+            const f32x2 s2 = pack_f32x2(s.x, s.y);
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t(&d)[8] = v[(p / 2) & 1][h];
-                        acc[p + j][h][i] = fma_f32x2(pack_u32x2(d[4 * j + 2 * i], d[4 * j + 2 * i + 1]), s2, acc[p + j][h][i]);
-                    }
-            }
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t(&d)[8] = v[(p / 2) & 1][h];
+                    acc[p + j][h][i] = fma_f32x2(pack_u32x2(d[4 * j + 2 * i], d[4 * j + 2 * i + 1]), s2, acc[p + j][h][i]);
+                }
+        }
     }
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->s_empty[e.buf]));
@@ -285,7 +273,7 @@ __device__ __forceinline__ void store_rows(const f32x2 (&acc)[NP][2][2], const T
         }
     };
 #pragma unroll
-    for (int p = 0; p < NP; p += 2) {  // (NP is even)
+    for (int p = 0; p < NP; p += 2) {
         uint8_t* half = e.strip + (p & 2) * 512;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -342,7 +330,7 @@ __device__ __forceinline__ bool store_quantized(f32x2 (&gate)[NP][2][2], const f
     const auto meet = [&]() {
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->wg[wg]));
-        const bool ok = wait<true>(&sy->wg[wg], e.wg_ph, sy, a.findings, 62);
+        const bool ok = wait(&sy->wg[wg], e.wg_ph, sy, a.findings, 62);
         e.wg_ph ^= 1;
         return ok;
     };
@@ -358,7 +346,7 @@ __device__ __forceinline__ bool store_quantized(f32x2 (&gate)[NP][2][2], const f
     if (!meet()) return false;
     uint8_t* dst = static_cast<uint8_t*>(a.out) + (size_t)t.row0 * inter + block * 128 + quarter * 32 + (lane & 1) * 16;
 #pragma unroll
-    for (int p = 0; p < NP; p += 2) {  // (NP is even)
+    for (int p = 0; p < NP; p += 2) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -530,13 +518,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             Tile t;
             while (ok) {
                 publish();  // (a tile ahead: the other roles find it there)
-                if (!next_tile<true>(sy, seq, t, a, parts)) break;
+                if (!next_tile(sy, seq, t, a, parts)) break;
                 const int half = t.n >> 1, n_big = half / kBigBox, n_small = (half % kBigBox) / kSmallBox;
                 const uint32_t bytes = 2u * (uint32_t)(kHalves * kABytes + half * 128);
                 const int col = M::first_column(t.nt, rank);
                 const int row = t.row0 + (int)rank * half;
                 for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
-                    if (it >= (uint32_t)n_slots && !wait<true>(&sy->empty[slot], ph ^ 1, sy, a.findings, 10)) { ok = false; break; }
+                    if (it >= (uint32_t)n_slots && !wait(&sy->empty[slot], ph ^ 1, sy, a.findings, 10)) { ok = false; break; }
                     if (leader) {
                         const uint32_t bar0 = full0 + slot * 8, dst = ptx::smem_u32(ring) + slot * (uint32_t)slot_bytes;
                         if (rank == 0) ptx::mbar_arrive_expect_tx(full_here + slot * 8, bytes);
@@ -571,7 +559,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             uint32_t seq = 0, it = 0, buf = 0, ph = 0;
             bool ok = true;
             Tile t;
-            while (ok && next_tile<true>(sy, seq, t, a, parts)) {
+            while (ok && next_tile(sy, seq, t, a, parts)) {
                 const float* ws = a.w_scale + (size_t)t.g * a.KB * a.NB;
                 int nb[kHalves];
 #pragma unroll
@@ -597,7 +585,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         if (b > last || !ok) break;
 #pragma unroll
                         for (int u = 0; u < kHalves; ++u) {
-                            if (ok && it >= (uint32_t)n_bufs) ok = wait<true>(&sy->s_empty[buf], ph ^ 1, sy, a.findings, 20);
+                            if (ok && it >= (uint32_t)n_bufs) ok = wait(&sy->s_empty[buf], ph ^ 1, sy, a.findings, 20);
                             if (!ok) break;
                             float* dst = scales + buf * (uint32_t)width + lane;
 #pragma unroll
@@ -621,15 +609,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const uint64_t da0 = ptx::umma_desc_sw128(ptx::smem_u32(ring), kABytes, 1024);
             const uint64_t db0 = ptx::umma_desc_sw128(ptx::smem_u32(ring) + kHalves * kABytes, 0, 1024);
             Tile t;
-            while (ok && next_tile<true>(sy, seq, t, a, parts)) {
+            while (ok && next_tile(sy, seq, t, a, parts)) {
                 const uint32_t idesc = ptx::umma_idesc_e4m3_mn_k(256, t.n);
                 for (int kb = t.kb0; kb < t.kb1 && ok; ++kb) {
 #pragma unroll
                     for (int u = 0; u < kHalves; ++u, ++it) {
                         if ((it & 1) == turn) {
                             // the epilogue of both CTAs has taken what the buffer held
-                            if (it >= (uint32_t)n_bufs && !wait<true>(&sy->t_empty[buf], tph ^ 1, sy, a.findings, 30)) { ok = false; break; }
-                            if (!wait<true>(&sy->full[slot], ph, sy, a.findings, 40)) { ok = false; break; }
+                            if (it >= (uint32_t)n_bufs && !wait(&sy->t_empty[buf], tph ^ 1, sy, a.findings, 30)) { ok = false; break; }
+                            if (!wait(&sy->full[slot], ph, sy, a.findings, 40)) { ok = false; break; }
                             ptx::tc_fence_after();
                             if (leader) {
                                 const uint64_t at = (uint64_t)(slot * (uint32_t)slot_bytes >> 4);
@@ -673,7 +661,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         uint32_t seq = 0;
         bool ok = true;
         Tile t;
-        while (ok && next_tile<true>(sy, seq, t, a, parts)) {
+        while (ok && next_tile(sy, seq, t, a, parts)) {
             switch (t.n >> 5) {
                 case 1: ok = finish_tile<M, 1 * 2>(t, e, sy, a); break;
                 case 2: ok = finish_tile<M, 2 * 2>(t, e, sy, a); break;

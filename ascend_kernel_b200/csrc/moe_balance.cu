@@ -400,8 +400,8 @@ static void pick(int E, bool aligned, F&& fn) {
         const int c = (E + 32 * V - 1) / (32 * V);
         if (c <= 1) fn(std::integral_constant<int, V>(), std::integral_constant<int, 1>());
         else if (c <= 2) fn(std::integral_constant<int, V>(), std::integral_constant<int, 2>());
-        else if (c <= 4) fn(std::integral_constant<int, V>(), std::integral_constant<int, 4>());
-        else fn(std::integral_constant<int, V>(), std::integral_constant<int, 8>());
+        else if (V == 8 || c <= 4) fn(std::integral_constant<int, V>(), std::integral_constant<int, 4>());  // (E is 1024 at most)
+        else if constexpr (V == 4) fn(std::integral_constant<int, V>(), std::integral_constant<int, 8>());
     } else {
         const int c = (E + 31) / 32;
         if (c <= 4) fn(std::integral_constant<int, 1>(), std::integral_constant<int, 4>());
@@ -464,13 +464,14 @@ extern "C" int b200moe_moe_balance_loss(const void* logits, int logits_fp32, con
     cfg.blockDim = dim3(mb::kJoinThreads);
     cfg.stream = st;
     cudaLaunchAttribute attr[2] = {};
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = cfg.gridDim.x;  // 8 at most
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cfg.gridDim.x;  // 8 at most
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    // (the list is read before the wait for the kernel ahead, so that must be the forward kernel, which began when the list was there)
+    cfg.numAttrs = a.T > 0 ? 2 : 1;
     B200MOE_CUDA_TRY(cudaLaunchKernelEx(&cfg, mb::join_kernel, a, loss, reinterpret_cast<long long*>(counts), load, inv_tokens,
                                         findings_words()));
     return B200MOE_OK;

@@ -548,8 +548,9 @@ def grouped_gemm_fp8_block(x, x_scale, weight, weight_scale, group_list, output,
 def moe_balance_loss(logits, idx, seq_list=None, token_mask=None):
     """Balance loss of the router and the pairs per expert: (loss fp32 [S], counts int64 [S, E]), differentiable (once) in ``logits``
     (bf16 or fp32 [T, E]).  ``idx`` int32 [T, k]: the experts of each token, as :func:`moe_route` returns them (an entry outside
-    0 .. E - 1 is a dropped pair and counts on no expert).  ``seq_list`` int64 [S]: cumulative token ends of the sequences, each of
-    which gets a loss of its own; tokens behind the last belong to none.  ``token_mask`` bool [T]: False takes a token out.
+    0 .. E - 1 is a dropped pair and counts on no expert).  ``seq_list`` int64 [S]: cumulative token ends of the sequences, which must
+    not fall and each of which gets a loss of its own; tokens behind the last belong to none.  ``token_mask`` bool [T]: False takes a
+    token out.
 
     For T_s tokens with probabilities p = softmax(logits) and c_e pairs on expert e, loss = E / (k T_s) * sum_e c_e * mean_t p_te: 1
     where the load is even; 0 for a sequence without tokens.  The counts carry no gradient."""

@@ -331,8 +331,8 @@ int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scale, const vo
  * counts int64 [n_seqs, E] = c.  load fp32 [n_seqs, E] = E c / (top_k T_s) - 1 and inv_tokens fp32 [n_seqs] = 1 / T_s (0 where T_s is 0)
  * are what b200moe_moe_balance_loss_grad takes with the gradient of the losses grad_loss fp32 [n_seqs]:
  *   grad_logits [T, E] (of the logits' type) = grad_loss[s] inv_tokens[s] p_te (load[s, e] - sum_j load[s, j] p_tj), 0 for a token of no sequence.
- * Sums have a fixed order.  A seq_list that falls or leaves 0 .. T is cut to that range and leaves code 1 with the sequence's number
- * for b200moe_read_findings.  E <= 1024, top_k <= 32, n_seqs <= 65535, T * top_k < 2^30. */
+ * Sums have a fixed order.  A seq_list that leaves 0 .. T is cut to that range; of one that falls the losses, counts and gradients are
+ * unspecified (no access leaves its tensor).  Both leave code 1 with a sequence's number for b200moe_read_findings.  E <= 1024, top_k <= 32, n_seqs <= 65535, T * top_k < 2^30. */
 size_t b200moe_moe_balance_scratch_bytes(int64_t n_tokens, int64_t n_experts, int64_t n_seqs);
 int b200moe_moe_balance_loss(const void* logits, int logits_fp32, const int32_t* idx, const int64_t* seq_list,
                              const uint8_t* token_mask, int64_t n_tokens, int64_t n_experts, int64_t top_k, int64_t n_seqs, float* loss,

@@ -355,6 +355,60 @@ def test_a_captured_chain_replayed_beside_another():
     assert torch.equal(outs[0], want[2]) and torch.equal(outs[1], want[3])
 
 
+def test_a_captured_call_that_deals_out_its_tiles_is_replayed():
+    """Tiles of many waves are drawn from a counter, which every replay has to clear: 256 experts, 2560 and 2 x 1280 columns."""
+    G, K, N = 256, 144, 2560
+    x, xs, w, ws, gl = _problem([1, 3] * (G // 2), K, N, 4, seed=24)
+    M = x.shape[0]
+
+    def run():
+        out, codes = torch.zeros(M, N, dtype=torch.bfloat16, device=DEV), torch.zeros(M, N // 2, dtype=torch.uint8, device=DEV)
+        scale = torch.zeros(M, N // 256, device=DEV)
+        ak.grouped_gemm_fp8_block(x, xs, w, ws, gl, out, group_list_type=1)
+        ak.grouped_gemm_fp8_block(x, xs, w, ws, gl, codes, output_scale=scale, group_list_type=1, gate_up_silu=True)
+        return out, codes, scale
+
+    graph = torch.cuda.CUDAGraph()
+    run()
+    with torch.cuda.graph(graph):
+        got = run()
+    for counts in ([1, 3] * (G // 2), [0, 2] * (G // 2), [M] + [0] * (G - 1)):
+        gl.copy_(torch.tensor(counts))
+        want = run()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+        _check_product(got[0], x, xs, w, ws, R.bounds(counts, 1, M))
+
+
+@pytest.mark.parametrize("G", [1023, 1024])
+def test_as_many_experts_as_there_may_be(G):
+    """Most of them without rows; the last one has some."""
+    K, N = 160, 256
+    counts = [0] * G
+    for g, c in ((0, 2), (500, 33), (G - 1, 170)):
+        counts[g] = c
+    x, xs, w, ws, gl = _problem(counts, K, N, 1, seed=25)
+    out = torch.full((x.shape[0], N), 7.0, dtype=torch.bfloat16, device=DEV)
+    ak.grouped_gemm_fp8_block(x, xs, w, ws, gl, out, group_list_type=1)
+    assert bool((out[-1] == 7).all())
+    _check_product(out, x, xs, w, ws, R.bounds(counts, 1, x.shape[0]))
+
+
+def test_inputs_that_are_misaligned_are_refused():
+    x, xs, w, ws, gl = _problem([2, 2], 128, 128)
+    out = torch.empty(4, 128, dtype=torch.bfloat16, device=DEV)
+    off = torch.empty(4 * 128 + 8, dtype=torch.uint8, device=DEV)[8:].view(4, 128)
+    with pytest.raises(RuntimeError):
+        ak.grouped_gemm_fp8_block(off, xs, w, ws, gl, out)
+    half = torch.empty(4 * 128 + 4, dtype=torch.bfloat16, device=DEV)[4:].view(4, 128)
+    with pytest.raises(RuntimeError):
+        ak.grouped_gemm_fp8_block(x, xs, w, ws, gl, half)
+    with pytest.raises(RuntimeError):
+        ak.fp8_quantize_rows(half)
+
+
 def test_refusals():
     x, xs, w, ws, gl = _problem([2, 2], 256, 256)
     out = torch.empty(4, 256, dtype=torch.bfloat16, device=DEV)
