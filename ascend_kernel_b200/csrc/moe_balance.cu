@@ -9,11 +9,16 @@
 // (the 1 cancels in the difference; taking it out first keeps the digits that an almost even load leaves).  The counts are piecewise
 // constant and have no gradient.
 //
-// Forward: a CTA takes a range of tokens, a warp a token at a time, its lanes adding the probabilities of their experts up in
-// registers; what a CTA has of a sequence goes to row (range + sequence) of the scratch (going on by a range or by a sequence
-// raises that sum by one, so no two pieces share a row), and a second kernel adds a sequence's rows in their order: no
-// floating-point atomics, the same bits each time.  Backward: the softmax again from the logits, a warp four tokens at a time.  Both read the
-// logits once and are bound by that.
+// Forward: a CTA takes a range of tokens, a warp (or a group of 8 or 16 lanes, where a row needs no more) a row at a time, its lanes
+// adding the probabilities of their experts up in registers, and counts the range's pairs in shared memory; what a CTA has of a sequence goes
+// to row (range + sequence) of the scratch (going on by a range or by a sequence raises that sum by one, so no two pieces share a row), and
+// a second kernel adds a sequence's rows in their order: no floating-point atomics, the same bits each time.  Backward: the
+// softmax again from the logits.  Each reads the logits once.
+//
+// Measured, forward (both kernels) | backward, rows larger than L2 among them, us: 4096 fp32 rows of 256: 9.0 | 5.9 (launches);
+// 65536: 21 | 24; 262144: 55 | 90 (4.9 and 6.0 TB/s); 262144 bf16 rows of 256: 51 | 67; of 64: 25 | 19.  Memory bounds the fp32 backward, the
+// others their instructions: a probability at a time and a warp for every row, the five were 9.8 | 6.4, 27 | 25, 74 | 87, 75 | 80 and
+// 72 | 75.
 #include <type_traits>
 
 #include "common.cuh"
@@ -121,61 +126,80 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// The probabilities of U tokens, their chains of loads and reductions side by side: lane l holds experts (c * 32 + l) * VEC + j.  A row
-// of nothing but -infinity has none (all 0), a NaN or +infinity makes the row NaN.  A row that is not `on` is not read.
-template <class T, int VEC, int CHUNKS, int U>
-__device__ __forceinline__ void softmax_rows(const T* const (&row)[U], const bool (&on)[U], int E, float (&p)[U][CHUNKS][VEC]) {
-    const int lane = threadIdx.x & 31;
-    float m[U], sum[U];
+// The largest of the values of a group of LANES lanes (NaN where all are NaN).
+template <int LANES>
+__device__ __forceinline__ float group_max(float v) {
+    if constexpr (LANES == 32) {
+        float r;
+        asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+        return r;
+    } else {
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+        return v;
+    }
+}
+// 2^v, results below 2^-126 as 0: of a row's largest probability that is none.
+__device__ __forceinline__ float exp2_flushed(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// exp(logit - the row's largest) of U tokens and the reciprocals of the rows' sums, their chains of loads and reductions side by
+// side.  LANES lanes take a row, lane l of them experts (c * LANES + l) * VEC + j; where that is no whole warp, its groups have rows of their own.  A row of nothing but -infinity has no probability (all 0), a NaN or +infinity makes the
+// row NaN.  A row that is not `on` is not read.  Instructions are what these kernels cost, so the arithmetic is two-wide.
+template <class T, int VEC, int CHUNKS, int LANES, int U>
+__device__ __forceinline__ void softmax_rows(const T* const (&row)[U], const bool (&on)[U], int E, f32x2 (&p)[U][VEC * CHUNKS / 2],
+                                             float (&inv)[U]) {
+    constexpr int N = VEC * CHUNKS;
+    const int lane = threadIdx.x & (LANES - 1);
+    float m[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        float z[CHUNKS][VEC];
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            const int e = (c * LANES + lane) * VEC;
+            if (on[u] && e < E) {
+                Logit<T>::template load<VEC>(row[u] + e, z[c]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) z[c][j] = -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) p[u][i] = pack_f32x2(z[2 * i / VEC][2 * i % VEC], z[(2 * i + 1) / VEC][(2 * i + 1) % VEC]);
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         m[u] = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-            const int e = (c * 32 + lane) * VEC;
-            if (on[u] && e < E) {
-                Logit<T>::template load<VEC>(row[u] + e, p[u][c]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) p[u][c][j] = -INFINITY;
-            }
-        }
+        for (int i = 0; i < N / 2; ++i) m[u] = fmaxf(m[u], fmaxf(f32x2_lo(p[u][i]), f32x2_hi(p[u][i])));
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int c = 0; c < CHUNKS; ++c)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) m[u] = fmaxf(m[u], p[u][c][j]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-        for (int u = 0; u < U; ++u) m[u] = fmaxf(m[u], __shfl_xor_sync(0xffffffffu, m[u], o));
+    for (int u = 0; u < U; ++u) m[u] = group_max<LANES>(m[u]);
+    float sum[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         // (a difference first: logits of the type's lowest value times log2(e) would overflow)
         const float base = m[u] == -INFINITY ? 0.f : m[u];
-        sum[u] = 0.f;
+        const f32x2 base2 = pack_f32x2(base, base), log2e = pack_f32x2(1.44269504f, 1.44269504f);
+        f32x2 total = 0ull;
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                p[u][c][j] = exp2f((p[u][c][j] - base) * 1.44269504f);
-                sum[u] += p[u][c][j];
-            }
+        for (int i = 0; i < N / 2; ++i) {
+            const f32x2 x = mul_f32x2(sub_f32x2(p[u][i], base2), log2e);
+            p[u][i] = pack_f32x2(exp2_flushed(f32x2_lo(x)), exp2_flushed(f32x2_hi(x)));
+            total = add_f32x2(total, p[u][i]);
+        }
+        sum[u] = f32x2_lo(total) + f32x2_hi(total);
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
+    for (int o = LANES / 2; o > 0; o >>= 1)
 #pragma unroll
         for (int u = 0; u < U; ++u) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const float inv = sum[u] == 0.f ? 0.f : 1.f / sum[u];
-#pragma unroll
-        for (int c = 0; c < CHUNKS; ++c)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) p[u][c][j] *= inv;
-    }
+    for (int u = 0; u < U; ++u) inv[u] = sum[u] == 0.f ? 0.f : __fdividef(1.f, sum[u]);  // (the sum is 1 .. 1024)
 }
 // Tokens a warp has side by side: what 16 values a lane hold.
 template <int VEC, int CHUNKS>
@@ -185,15 +209,16 @@ constexpr int kTokens = VEC * CHUNKS <= 8 ? 2 : 1;
 template <int VEC, int CHUNKS>
 constexpr int kForwardWarps = VEC * CHUNKS <= 16 ? 32 : 16;
 
-template <class T, int VEC, int CHUNKS>
-__global__ void __launch_bounds__(32 * kForwardWarps<VEC, CHUNKS>) forward_kernel(const Args a) {
-    constexpr int U = kTokens<VEC, CHUNKS>, kWarps = kForwardWarps<VEC, CHUNKS>, kThreads = 32 * kWarps;
+template <class T, int VEC, int CHUNKS, int LANES>
+__global__ void __launch_bounds__(32 * kForwardWarps<VEC, CHUNKS>, 1) forward_kernel(const Args a) {
+    constexpr int U = kTokens<VEC, CHUNKS>, kWarps = kForwardWarps<VEC, CHUNKS>, kThreads = 32 * kWarps, kGroups = 32 / LANES;
     extern __shared__ float smem[];  // [kWarps][pitch] probabilities, [pitch] counts, 1 number of tokens
     int* hist = reinterpret_cast<int*>(smem + kWarps * a.pitch);
     int* n_tokens = hist + a.pitch;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & (LANES - 1), group = (threadIdx.x & 31) / LANES;
     const int t0 = blockIdx.x * a.chunk, t1 = min(t0 + a.chunk, a.T);
     const T* logits = static_cast<const T*>(a.logits);
+    const auto counts = [&](int t) { return a.mask == nullptr || __ldg(a.mask + t) != 0; };
     for (int s = seq_of(a, t0); s < a.S; ++s) {
         const int start = seq_start(a, s);
         if (start >= t1) break;
@@ -201,39 +226,45 @@ __global__ void __launch_bounds__(32 * kForwardWarps<VEC, CHUNKS>) forward_kerne
         if (lo >= hi) continue;
         for (int e = threadIdx.x; e <= a.pitch; e += kThreads) hist[e] = 0;  // (and the number of tokens behind them)
         __syncthreads();
-        float acc[CHUNKS][VEC] = {};
+        // the pairs, all threads side by side
+        const int32_t* idx = a.idx + (size_t)lo * a.k;
+        const int pairs = (hi - lo) * a.k;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < pairs; i += kThreads) {
+            const int e = __ldg(idx + i);
+            if ((unsigned)e < (unsigned)a.E && counts(lo + i / a.k)) atomicAdd(&hist[e], 1);
+        }
+        f32x2 acc[VEC * CHUNKS / 2] = {};
         int n = 0;
-        for (int t = lo + warp; t < hi; t += kWarps * U) {
+        for (int t = lo + warp * kGroups; t < hi; t += kWarps * U * kGroups) {
             const T* row[U];
             bool on[U];
-            float p[U][CHUNKS][VEC];
+            f32x2 p[U][VEC * CHUNKS / 2];
+            float inv[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int tu = t + u * kWarps;
-                on[u] = tu < hi && (a.mask == nullptr || __ldg(a.mask + tu) != 0);
+                const int tu = t + u * kWarps * kGroups + group;
+                on[u] = tu < hi && counts(tu);
                 row[u] = logits + (size_t)(on[u] ? tu : t) * a.E;
-                if (on[u] && lane < a.k) {
-                    const int e = __ldg(a.idx + (size_t)tu * a.k + lane);
-                    if ((unsigned)e < (unsigned)a.E) atomicAdd(&hist[e], 1);
-                }
                 n += on[u];
             }
-            softmax_rows<T, VEC, CHUNKS, U>(row, on, a.E, p);
+            softmax_rows<T, VEC, CHUNKS, LANES, U>(row, on, a.E, p, inv);
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int c = 0; c < CHUNKS; ++c)
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) acc[c][j] += p[u][c][j];
+                for (int i = 0; i < VEC * CHUNKS / 2; ++i) acc[i] = fma_f32x2(p[u][i], pack_f32x2(inv[u], inv[u]), acc[i]);
         }
         if (lane == 0 && n) atomicAdd(n_tokens, n);
+        // the groups of a warp, then the warps in their order
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c)
+        for (int o = LANES; o < 32; o <<= 1)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const int e = (c * 32 + lane) * VEC + j;
-                if (e < a.pitch) smem[warp * a.pitch + e] = acc[c][j];
-            }
+            for (int i = 0; i < VEC * CHUNKS / 2; ++i) acc[i] = add_f32x2(acc[i], __shfl_xor_sync(0xffffffffu, acc[i], o));
+#pragma unroll
+        for (int i = 0; i < VEC * CHUNKS; ++i) {
+            const int e = (i / VEC * LANES + lane) * VEC + i % VEC;
+            if (group == 0 && e < a.pitch) smem[warp * a.pitch + e] = i & 1 ? f32x2_hi(acc[i >> 1]) : f32x2_lo(acc[i >> 1]);
+        }
         __syncthreads();
         const size_t row = (size_t)blockIdx.x + s;
         for (int e = threadIdx.x; e < a.pitch; e += kThreads) {
@@ -324,55 +355,74 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a, float*
     ptx::cluster_sync();  // (the other CTAs' shared memory has been read)
 }
 
-template <class T, int VEC, int CHUNKS>
+template <class T, int VEC, int CHUNKS, int LANES>
 __global__ void __launch_bounds__(256) backward_kernel(const Args a, const float* __restrict__ load, const float* __restrict__ inv_n,
                                                        const float* __restrict__ grad, T* __restrict__ out) {
-    constexpr int U = kTokens<VEC, CHUNKS>;
-    const int lane = threadIdx.x & 31, t = (blockIdx.x * 8 + (threadIdx.x >> 5)) * U;
+    constexpr int U = kTokens<VEC, CHUNKS>, kGroups = 32 / LANES;
+    const int lane = threadIdx.x & (LANES - 1), t = (blockIdx.x * 8 + (threadIdx.x >> 5)) * (U * kGroups);
     if (t >= a.T) return;
+    const int first = t + (threadIdx.x & 31) / LANES;  // of the lane's tokens, every kGroups-th
     const T* row[U];
     const float* f[U];
     bool on[U];
-    float g[U], mean[U], p[U][CHUNKS][VEC];
+    float g[U], mean[U], inv[U];
+    f32x2 p[U][VEC * CHUNKS / 2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         // a token of no sequence, or one that the mask takes out, has no part in any loss (what its logits hold is not read)
-        const int tu = t + u, s = tu < a.T ? seq_of(a, tu) : a.S;
+        const int tu = first + u * kGroups, s = tu < a.T ? seq_of(a, tu) : a.S;
         on[u] = s < a.S && tu >= seq_start(a, s) && (a.mask == nullptr || __ldg(a.mask + tu) != 0);
         row[u] = static_cast<const T*>(a.logits) + (size_t)(on[u] ? tu : t) * a.E;
         f[u] = load + (size_t)(on[u] ? s : 0) * a.E;
         g[u] = on[u] ? __ldg(grad + s) * __ldg(inv_n + s) : 0.f;
         mean[u] = 0.f;
     }
-    softmax_rows<T, VEC, CHUNKS, U>(row, on, a.E, p);
+    softmax_rows<T, VEC, CHUNKS, LANES, U>(row, on, a.E, p, inv);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            const int e = (c * 32 + lane) * VEC;
+            const int e = (c * LANES + lane) * VEC;
             if (e < a.E) {
                 float fv[VEC];
                 Logit<float>::template load_row<VEC>(f[u] + e, fv);
+                if constexpr (VEC == 1) {
+                    mean[u] = fmaf(fv[0], c & 1 ? f32x2_hi(p[u][c / 2]) : f32x2_lo(p[u][c / 2]), mean[u]);
+                } else {
+                    f32x2 sum = 0ull;
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) mean[u] = fmaf(fv[j], p[u][c][j], mean[u]);
+                    for (int j = 0; j < VEC; j += 2) sum = fma_f32x2(pack_f32x2(fv[j], fv[j + 1]), p[u][(c * VEC + j) / 2], sum);
+                    mean[u] += f32x2_lo(sum) + f32x2_hi(sum);
+                }
             }
         }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
+    for (int o = LANES / 2; o > 0; o >>= 1)
 #pragma unroll
         for (int u = 0; u < U; ++u) mean[u] += __shfl_xor_sync(0xffffffffu, mean[u], o);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        if (t + u >= a.T) break;
-        T* dst = out + (size_t)(t + u) * a.E;
+        if (first + u * kGroups >= a.T) break;
+        const float of = -mean[u] * inv[u], by = g[u] * inv[u];
+        T* dst = out + (size_t)(first + u * kGroups) * a.E;
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            const int e = (c * 32 + lane) * VEC;
+            const int e = (c * LANES + lane) * VEC;
             if (e < a.E) {
                 float fv[VEC];
                 Logit<float>::template load_row<VEC>(f[u] + e, fv);  // (again, from L1)
+                // (a token that is not on has by = 0 and probabilities of 0)
+                if constexpr (VEC == 1) {
+                    fv[0] = ((c & 1 ? f32x2_hi(p[u][c / 2]) : f32x2_lo(p[u][c / 2])) * by) * (fv[0] + of);
+                } else {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) fv[j] = on[u] ? p[u][c][j] * (g[u] * (fv[j] - mean[u])) : 0.f;
+                    for (int j = 0; j < VEC; j += 2) {
+                        const f32x2 d = mul_f32x2(mul_f32x2(p[u][(c * VEC + j) / 2], pack_f32x2(by, by)),
+                                                  add_f32x2(pack_f32x2(fv[j], fv[j + 1]), pack_f32x2(of, of)));
+                        fv[j] = f32x2_lo(d);
+                        fv[j + 1] = f32x2_hi(d);
+                    }
+                }
                 Logit<T>::template store<VEC>(dst + e, fv);
             }
         }
@@ -392,21 +442,27 @@ static bool sizes_ok(int64_t T, int64_t E, int64_t k, int64_t S) {
     return T >= 0 && E > 0 && E <= 1024 && k > 0 && k <= kMaxTopK && k <= E && S > 0 && S <= 65535 && T * k <= 0x3FFFFFFFLL;
 }
 
-// Calls fn<VEC, CHUNKS> with the widest loads that E and the pointers allow and as many of them as E needs.
+// Calls fn(VEC, CHUNKS, LANES) with the widest loads that E and the pointers allow and as many of them as E needs; rows that need half
+// the lanes of a warp or fewer get a group of 16 or 8.
 template <class T, class F>
 static void pick(int E, bool aligned, F&& fn) {
     constexpr int V = Logit<T>::kVec;
+    constexpr std::integral_constant<int, V> wide;
+    constexpr std::integral_constant<int, 1> one;
+    constexpr std::integral_constant<int, 4> four;
+    constexpr std::integral_constant<int, 32> warp;
     if (aligned && E % V == 0) {
-        const int c = (E + 32 * V - 1) / (32 * V);
-        if (c <= 1) fn(std::integral_constant<int, V>(), std::integral_constant<int, 1>());
-        else if (c <= 2) fn(std::integral_constant<int, V>(), std::integral_constant<int, 2>());
-        else if (V == 8 || c <= 4) fn(std::integral_constant<int, V>(), std::integral_constant<int, 4>());  // (E is 1024 at most)
-        else if constexpr (V == 4) fn(std::integral_constant<int, V>(), std::integral_constant<int, 8>());
+        const int n = E / V;
+        if (n <= 8) fn(wide, one, std::integral_constant<int, 8>());
+        else if (n <= 16) fn(wide, one, std::integral_constant<int, 16>());
+        else if (n <= 32) fn(wide, one, warp);
+        else if (n <= 64) fn(wide, std::integral_constant<int, 2>(), warp);
+        else if (V == 8 || n <= 128) fn(wide, four, warp);  // (E is 1024 at most)
+        else if constexpr (V == 4) fn(wide, std::integral_constant<int, 8>(), warp);
     } else {
-        const int c = (E + 31) / 32;
-        if (c <= 4) fn(std::integral_constant<int, 1>(), std::integral_constant<int, 4>());
-        else if (c <= 16) fn(std::integral_constant<int, 1>(), std::integral_constant<int, 16>());
-        else fn(std::integral_constant<int, 1>(), std::integral_constant<int, 32>());
+        if (E <= 128) fn(one, four, warp);
+        else if (E <= 512) fn(one, std::integral_constant<int, 16>(), warp);
+        else fn(one, warp, warp);
     }
 }
 
@@ -445,8 +501,8 @@ extern "C" int b200moe_moe_balance_loss(const void* logits, int logits_fp32, con
     if (a.T > 0) {
         const unsigned grid = (unsigned)((a.T + a.chunk - 1) / a.chunk);
         cudaError_t err = cudaSuccess;
-        const auto run = [&](auto vec, auto chunks, auto zero) {
-            auto* k = mb::forward_kernel<decltype(zero), decltype(vec)::value, decltype(chunks)::value>;
+        const auto run = [&](auto vec, auto chunks, auto lanes, auto zero) {
+            auto* k = mb::forward_kernel<decltype(zero), decltype(vec)::value, decltype(chunks)::value, decltype(lanes)::value>;
             constexpr int warps = mb::kForwardWarps<decltype(vec)::value, decltype(chunks)::value>;
             const size_t smem = (size_t)(warps + 1) * a.pitch * 4 + 4;
             if (smem > 48 * 1024) err = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 140 * 1024);
@@ -455,8 +511,8 @@ extern "C" int b200moe_moe_balance_loss(const void* logits, int logits_fp32, con
                 err = cudaGetLastError();
             }
         };
-        if (logits_fp32) mb::pick<float>(a.E, aligned16(logits), [&](auto v, auto c) { run(v, c, float()); });
-        else mb::pick<__nv_bfloat16>(a.E, aligned16(logits), [&](auto v, auto c) { run(v, c, __nv_bfloat16()); });
+        if (logits_fp32) mb::pick<float>(a.E, aligned16(logits), [&](auto v, auto c, auto l) { run(v, c, l, float()); });
+        else mb::pick<__nv_bfloat16>(a.E, aligned16(logits), [&](auto v, auto c, auto l) { run(v, c, l, __nv_bfloat16()); });
         B200MOE_CUDA_TRY(err);
     }
     cudaLaunchConfig_t cfg = {};
@@ -491,15 +547,15 @@ extern "C" int b200moe_moe_balance_loss_grad(const void* logits, int logits_fp32
     a.mask = token_mask;
     a.T = (int)n_tokens; a.E = (int)n_experts; a.S = (int)n_seqs;
     const bool aligned = aligned16(logits) && aligned16(grad_logits) && aligned16(load);
-    const auto run = [&](auto vec, auto chunks, auto zero) {
+    const auto run = [&](auto vec, auto chunks, auto lanes, auto zero) {
         using T = decltype(zero);
-        const int64_t per_cta = 8 * mb::kTokens<decltype(vec)::value, decltype(chunks)::value>;
+        const int64_t per_cta = 8 * mb::kTokens<decltype(vec)::value, decltype(chunks)::value> * (32 / decltype(lanes)::value);
         const unsigned grid = (unsigned)((n_tokens + per_cta - 1) / per_cta);
-        mb::backward_kernel<T, decltype(vec)::value, decltype(chunks)::value>
+        mb::backward_kernel<T, decltype(vec)::value, decltype(chunks)::value, decltype(lanes)::value>
             <<<grid, 256, 0, st>>>(a, load, inv_tokens, grad_loss, static_cast<T*>(grad_logits));
     };
-    if (logits_fp32) mb::pick<float>(a.E, aligned, [&](auto v, auto c) { run(v, c, float()); });
-    else mb::pick<__nv_bfloat16>(a.E, aligned, [&](auto v, auto c) { run(v, c, __nv_bfloat16()); });
+    if (logits_fp32) mb::pick<float>(a.E, aligned, [&](auto v, auto c, auto l) { run(v, c, l, float()); });
+    else mb::pick<__nv_bfloat16>(a.E, aligned, [&](auto v, auto c, auto l) { run(v, c, l, __nv_bfloat16()); });
     B200MOE_CUDA_TRY(cudaGetLastError());
     return B200MOE_OK;
 }

@@ -97,6 +97,17 @@ def test_masked_tokens(kept):
     _check(logits, idx, seq_list, mask)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("E,k", [(4, 2), (16, 16), (32, 3), (40, 5), (64, 32), (68, 4), (72, 8), (128, 6), (136, 1), (512, 4), (520, 2)])
+def test_every_width_of_a_row(E, k, dtype):
+    """Rows of 8, 16 and 32 lanes and of several loads a lane, with sequences that end inside a warp's tokens and a mask."""
+    T = 403
+    logits, idx = _router(T, E, k, dtype, seed=E)
+    ends = torch.tensor([1, 34, 34, 291, 399], dtype=torch.int64, device=DEV)
+    mask = torch.rand(T, generator=_gen(E + 1), device=DEV) < 0.7
+    _check(logits, idx, ends, mask, seed=3)
+
+
 def test_experts_that_are_masked_out_and_rows_without_any():
     for lowest in (-float("inf"), torch.finfo(torch.bfloat16).min):
         logits, idx = _router(50, 24, 2, torch.bfloat16, seed=6)
