@@ -12,8 +12,9 @@ namespace b200moe {
 namespace fq {
 
 // Eight lanes take a block, 16 elements (32 bytes in, 16 out) each, a warp kSteps times four blocks; a CTA takes a row or up to eight
-// warps' blocks of it.  Bound by memory where the rows are read once (32768 rows of 2048: 32 us, 6.4 TB/s).  Tried and not kept: one
-// step (104 us where two take 84), four (88), warps that walk over rows with the next one's loads under way (88 - 92).
+// warps' blocks of it.  Bound by memory where the rows are read once (32768 rows of 7168: 104 us, 6.8 TB/s; of 2048:
+// 37 us; 4096 of 7168: 15.6 us, 5.7 TB/s), by its launch where they are few (8 rows: 1.8 us).  Tried and not kept: one step (104 us where two take
+// 84: 4096 rows of 7168, each named eight times), four (88), warps that walk over rows with the next one's loads under way (88 - 92).
 constexpr int kSteps = 2;
 constexpr int kWarpBlocks = 4 * kSteps;
 

@@ -17,8 +17,8 @@
 //
 // Measured, forward (both kernels) | backward, rows larger than L2 among them, us: 4096 fp32 rows of 256: 9.0 | 5.9 (launches);
 // 65536: 21 | 24; 262144: 55 | 90 (4.9 and 6.0 TB/s); 262144 bf16 rows of 256: 51 | 67; of 64: 25 | 19.  Memory bounds the fp32 backward, the
-// others their instructions: a probability at a time and a warp for every row, the five were 9.8 | 6.4, 27 | 25, 74 | 87, 75 | 80 and
-// 72 | 75.
+// latency of the loads the fp32 forward (two rows of each of 32 warps under way), instructions the others: a probability at a time and
+// a warp for every row, the five were 9.8 | 6.4, 27 | 25, 74 | 87, 75 | 80 and 72 | 75.
 #include <type_traits>
 
 #include "common.cuh"
