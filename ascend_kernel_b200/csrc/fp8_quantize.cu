@@ -91,6 +91,10 @@ __global__ void __launch_bounds__(256) gather_kernel(const uint4* __restrict__ s
     }
 }
 
+static bool sizes_ok(int64_t n_src, int64_t n_rows, int64_t K) {
+    return n_src >= 0 && n_src <= 0x3FFFFFFFLL && n_rows >= 0 && n_rows <= 0x3FFFFFFFLL && K > 0 && K <= 0x3FFFFFFLL;
+}
+
 // Whether the rows of x are quantised once, into scratch, and their bytes gathered: where an index names every row of x four times or
 // more and the second launch does not matter.  Every row of the result quantised | two passes, us (rows of x, times each is named,
 // K): 4096 x 8, 7168: 84.0 | 69.6 (cudaMemset takes 62 for as many bytes); 1024 x 8, 7168: 22.6 | 18.5; 512 x 8, 7168: 12.3 | 12.2;
@@ -114,15 +118,13 @@ static int launch_quantize(const void* x, const int32_t* index, void* codes, flo
 using namespace b200moe;
 
 extern "C" size_t b200moe_fp8_quantize_rows_scratch_bytes(int64_t n_src, int64_t n_rows, int64_t K, int has_index) {
-    if (n_src <= 0 || K <= 0 || !has_index || !fq::two_passes(n_src, n_rows, K)) return 0;
+    if (!fq::sizes_ok(n_src, n_rows, K) || n_src == 0 || !has_index || !fq::two_passes(n_src, n_rows, K)) return 0;
     return (size_t)n_src * ((size_t)K + 4u * (size_t)((K + 127) / 128));
 }
 
 extern "C" int b200moe_fp8_quantize_rows(const void* x, const int32_t* index, void* codes, float* scale, int64_t n_src,
                                          int64_t n_rows, int64_t K, void* scratch, size_t scratch_bytes, void* stream) {
-    if (n_src < 0 || n_rows < 0 || K <= 0 || (K % 16) != 0 || n_src > 0x3FFFFFFFLL || n_rows > 0x3FFFFFFFLL || K > 0x3FFFFFFLL ||
-        (!index && n_rows > n_src))
-        return B200MOE_ERR_SHAPE;
+    if (!fq::sizes_ok(n_src, n_rows, K) || (K % 16) != 0 || (!index && n_rows > n_src)) return B200MOE_ERR_SHAPE;
     if (n_rows == 0) return B200MOE_OK;
     if ((!x && n_src > 0) || !codes || !scale) return B200MOE_ERR_NULL_POINTER;
     if (!aligned16(x) || !aligned16(codes) || !aligned16(scratch)) return B200MOE_ERR_ALIGNMENT;

@@ -725,6 +725,11 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a) {
     }
 }
 
+static bool sizes_ok(int64_t M, int64_t K, int64_t N, int64_t G) {
+    constexpr int64_t kMost = 0x3FFFFFFF;  // (products of two sizes stay in 64 bits)
+    return M >= 0 && M <= kMost && K > 0 && K <= kMost && N > 0 && N <= kMost && G > 0 && G <= kMaxExperts;
+}
+
 constexpr int64_t kPairs = 74;  // of a B200's multiprocessors (rules and sizes go by the sizes of a call alone)
 
 // Whether a tile's stage holds two blocks of 128 columns a CTA: a pair then reads 512 contiguous bytes of a weight row and the rows of x
@@ -758,7 +763,7 @@ static int max_parts(int64_t M, int64_t K, int64_t N, int64_t G, int gate_up) {
 using namespace b200moe;
 
 extern "C" size_t b200moe_grouped_gemm_fp8_block_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, int gate_up_silu) {
-    if (M <= 0 || K <= 0 || N <= 0 || G <= 0) return fb::kWordBytes;
+    if (!fb::sizes_ok(M, K, N, G) || M == 0) return fb::kWordBytes;
     const int parts = fb::max_parts(M, K, N, G, gate_up_silu);
     return fb::kWordBytes + (parts > 1 ? (size_t)parts * (size_t)M * (size_t)N * 4 : 0);
 }
@@ -767,8 +772,7 @@ extern "C" int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scal
                                               const int64_t* group_list, void* out, float* out_scale, int64_t M, int64_t K, int64_t N,
                                               int64_t G, int group_list_type, int gate_up_silu, void* workspace,
                                               size_t workspace_bytes, void* stream) {
-    if (M < 0 || K <= 0 || N <= 0 || G <= 0 || G > kMaxExperts || (K % 16) != 0 || (N % 16) != 0 || M > 0x3FFFFFFFLL ||
-        K > 0x3FFFFFFFLL || N > 0x3FFFFFFFLL || (gate_up_silu && (N % 256) != 0))
+    if (!fb::sizes_ok(M, K, N, G) || (K % 16) != 0 || (N % 16) != 0 || (gate_up_silu && (N % 256) != 0))
         return B200MOE_ERR_SHAPE;
     if (group_list_type != B200MOE_GROUP_LIST_CUMSUM && group_list_type != B200MOE_GROUP_LIST_COUNTS) return B200MOE_ERR_ARGUMENT;
     if (gate_up_silu != 0 && gate_up_silu != 1) return B200MOE_ERR_ARGUMENT;

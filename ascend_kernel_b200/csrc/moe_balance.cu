@@ -439,7 +439,7 @@ static int64_t scratch_rows(int64_t T, int64_t S) { return (T + chunk_of(T) - 1)
 static int pitch_of(int64_t E) { return (int)((E + 3) & ~3LL); }
 
 static bool sizes_ok(int64_t T, int64_t E, int64_t k, int64_t S) {
-    return T >= 0 && E > 0 && E <= 1024 && k > 0 && k <= kMaxTopK && k <= E && S > 0 && S <= 65535 && T * k <= 0x3FFFFFFFLL;
+    return T >= 0 && T <= 0x3FFFFFFFLL && E > 0 && E <= 1024 && k > 0 && k <= kMaxTopK && k <= E && S > 0 && S <= 65535 && T * k <= 0x3FFFFFFFLL;
 }
 
 // Calls fn(VEC, CHUNKS, LANES) with the widest loads that E and the pointers allow and as many of them as E needs; rows that need half

@@ -67,6 +67,26 @@ def test_scratch_holds_a_row_for_every_piece():
             assert lib.b200moe_moe_balance_scratch_bytes(T, E, S) >= rows * (8 * E + 4)
 
 
+@pytest.mark.parametrize("big", [1 << 30, 1 << 46, 1 << 58, 1 << 59, 1 << 62, (1 << 63) - 1, -(1 << 63)])
+def test_sizes_whose_products_leave_64_bits(big):
+    """(2^58 rows of 16 columns of four bytes are 2^64, which is 0: such a product must not be divided by.)"""
+    for gu in (0, 1):
+        assert lib.b200moe_grouped_gemm_fp8_block_workspace_bytes(big, 256, 16, 2, gu) == 256
+        assert lib.b200moe_grouped_gemm_fp8_block_workspace_bytes(4, big, 256, 2, gu) == 256
+        assert lib.b200moe_grouped_gemm_fp8_block_workspace_bytes(4, 256, big, 2, gu) == 256
+    for change in (dict(M=big), dict(K=big), dict(N=big), dict(G=big)):
+        assert _gemm(**change) == SHAPE
+    for sizes in ((big, 64, 128), (4, big, 128), (4, 64, big), (big, big, big)):
+        assert lib.b200moe_fp8_quantize_rows_scratch_bytes(*sizes, 1) == 0
+        assert lib.b200moe_fp8_quantize_rows(A, A, A, A, *sizes, None, 0, None) == SHAPE
+    assert lib.b200moe_moe_balance_scratch_bytes(big, 16, 1) == 0
+    assert _loss(T=big) == SHAPE and _loss(T=big, k=16) == SHAPE and _loss(S=big) == SHAPE and _loss(E=big) == SHAPE
+
+
+def test_scratch_of_the_quantisation_is_aligned():
+    assert lib.b200moe_fp8_quantize_rows(A, A, A, A, 64, 1 << 20, 128, A + 8, 1 << 40, None) == ALIGN
+
+
 def test_python_refuses_host_tensors():
     x = torch.zeros(4, 128, dtype=torch.bfloat16)
     with pytest.raises(RuntimeError):
