@@ -91,6 +91,24 @@ def test_router_trained_beside_the_pass():
     assert bool(((router.grad.double() - dense).abs() <= (2.0 ** -8 + 2.0 ** -12) * mag + 2.0 ** -8 * dense.abs() + 1e-9).all())
 
 
+def test_rows_that_come_through_the_exchange():
+    """exchange="p2p" with one rank: the rows are quantised where they arrive, in a buffer with room for more."""
+    E, H, I, k = 8, 256, 128, 2
+    layer, gen = _layer(E, H, I, k, seed=4)
+    p2p = MoELayer(layer.w13, layer.s13, None, layer.w2, layer.s2, None, E, k, weight_format="fp8", exchange="p2p", max_tokens=64)
+    try:
+        for T in (64, 7, 50):
+            x = torch.randn(T, H, generator=gen, device=DEV).to(torch.bfloat16)
+            logits = torch.randn(T, E, generator=gen, device=DEV).to(torch.bfloat16)
+            a, b = layer.forward(x, logits).double(), p2p.forward(x, logits).double()
+            # Another number of rows may cut the k range otherwise: sums that differ by some 2^-20 at most. Where one lies at a border it
+            # moves a result to the next bf16 value (2^-8), or one of a row's I codes by a step (2^-3, of a row 2^-3 / sqrt(I) < 2^-6.4).
+            assert float((a - b).norm() / a.norm()) <= 2.0 ** -6
+        p2p.read_status()
+    finally:
+        p2p.px.close()
+
+
 def test_refusals():
     layer, _ = _layer(4, 128, 128, 2)
     for change in (dict(o13=layer.s13), dict(w13=layer.w13[:, :, :128]), dict(w2=layer.w2.to(torch.int16))):
