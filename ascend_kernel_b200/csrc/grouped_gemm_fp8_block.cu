@@ -35,18 +35,20 @@
 #include "fp8_block.cuh"
 #include "ptx.cuh"
 #include "tile_ring.h"
+#include "token_slots.h"
 
 namespace b200moe {
 namespace fb {
 
 constexpr int kWarpLoad = 0, kWarpMma0 = 1, kWarpScale = 3, kWarpEpi0 = 4;
-constexpr int kMaxR = 160;             // token rows of a tile
+constexpr int kMaxR = kTileTokens;     // token rows of a tile
 constexpr int kABytes = 128 * 128;     // 128 weight columns of a stage
 constexpr int kMaxSlots = 12, kMaxBufs = 8;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kStripBytes = 2048;      // of an epilogue warp
 // The epilogue's warps come in groups of four (128 weight columns), which share the tile's tokens.
 constexpr int kGroups = 2, kEpiWarps = 4 * kGroups, kThreads = (kWarpEpi0 + kEpiWarps) * 32;
+static_assert(kGroups * kGroupTokens == kMaxR, "token slots");
 constexpr int kBigBox = 64, kSmallBox = 16;
 constexpr int kScaleRingBytes = (int)kTmemCols * 4;  // a scale for every accumulator column
 constexpr int kBarrierBytes = 2048;
@@ -309,7 +311,9 @@ __device__ __forceinline__ void store_rows(const f32x2 (&acc)[NP][2][2], const T
 template <int NP>
 __device__ __forceinline__ bool store_quantized(f32x2 (&gate)[NP][2][2], const f32x2 (&up)[NP][2][2], const Tile& t, Epilogue& e, int first,
                                                 int block, Sync* sy, const Args& a) {
+    static_assert(NP * 8 <= kGroupTokens, "token slots");
     const int lane = threadIdx.x & 31, g8 = lane >> 2, q = lane & 3, quarter = e.warp & 3, wg = e.warp >> 2;
+    const int slots = token_slot(wg, 0);  // of the group's tokens in `tops` and `quantizers`
     const int inter = a.N >> 1, blocks = inter >> 7;
     const bool inside = block < blocks;  // (an odd number of blocks leaves the pair's last CTA without one)
 #pragma unroll
@@ -334,7 +338,7 @@ __device__ __forceinline__ bool store_quantized(f32x2 (&gate)[NP][2][2], const f
             m0 = max(m0, __shfl_xor_sync(0xffffffffu, m0, o));
             m1 = max(m1, __shfl_xor_sync(0xffffffffu, m1, o));
         }
-        if (g8 < 2) e.tops[(first + p * 8 + 2 * q + g8) * 4 + quarter] = __uint_as_float(g8 ? m1 : m0);
+        if (g8 < 2) e.tops[(slots + p * 8 + 2 * q + g8) * 4 + quarter] = __uint_as_float(g8 ? m1 : m0);
     }
     const auto meet = [&]() {
         __syncwarp();
@@ -347,9 +351,9 @@ __device__ __forceinline__ bool store_quantized(f32x2 (&gate)[NP][2][2], const f
     const int mine = quarter * 32 + lane;
     if (mine < NP * 8) {
         const int token = first + mine;
-        const uint4 m = reinterpret_cast<const uint4*>(e.tops)[token];
+        const uint4 m = reinterpret_cast<const uint4*>(e.tops)[slots + mine];
         const fp8_block::Quantizer qz(__uint_as_float(max(max(m.x, m.y), max(m.z, m.w))));
-        reinterpret_cast<float2*>(e.quantizers)[token] = qz.packed();
+        reinterpret_cast<float2*>(e.quantizers)[slots + mine] = qz.packed();
         if (inside && token < t.rows) a.out_scale[(size_t)(t.row0 + token) * blocks + block] = qz.scale;
     }
     if (!meet()) return false;
@@ -360,7 +364,7 @@ __device__ __forceinline__ bool store_quantized(f32x2 (&gate)[NP][2][2], const f
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                const fp8_block::Quantizer qz(reinterpret_cast<const float2*>(e.quantizers)[first + (p + j) * 8 + 2 * q + b]);
+                const fp8_block::Quantizer qz(reinterpret_cast<const float2*>(e.quantizers)[slots + (p + j) * 8 + 2 * q + b]);
                 float h[4];
 #pragma unroll
                 for (int m = 0; m < 4; ++m) h[m] = b ? f32x2_hi(gate[p + j][m >> 1][m & 1]) : f32x2_lo(gate[p + j][m >> 1][m & 1]);
