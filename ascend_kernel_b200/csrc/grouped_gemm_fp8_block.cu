@@ -555,6 +555,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
                 }
             }
+            // The commits that give the last stages back have arrived before the CTA ends: those for the second CTA's barriers come from the
+            // first one, and nothing else there waits for them.
+            for (uint32_t i = it; ok && i < it + (uint32_t)n_slots; ++i) {
+                if (i >= (uint32_t)n_slots) ok = wait(&sy->empty[slot], ph ^ 1, sy, a.findings, 11);
+                if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
+            }
             if (leader && *reinterpret_cast<volatile int*>(&sy->abort)) {
                 // copies in flight land before the shared memory goes (those of both CTAs are counted in the first one)
                 if (rank == 0) {
@@ -688,6 +694,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     __syncwarp();
     ptx::tc_fence_before();
     __syncthreads();
+    // (so have the last commits of both MMA warps, which arrive here too; the first CTA's warps waited for theirs)
+    if (rank != 0 && (warp == kWarpMma0 || warp == kWarpMma0 + 1)) (void)ptx::mbar_wait(ptx::smem_u32(&sy->drain[warp - kWarpMma0]), 0);
+    __syncwarp();
     ptx::cluster_sync();  // (what one CTA sends the other, loads and MMAs of the pair among it, has arrived)
     if (warp == kWarpMma0) {
         ptx::tc_fence_after();
