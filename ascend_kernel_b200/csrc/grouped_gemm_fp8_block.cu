@@ -574,7 +574,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             __syncwarp();
         } else if (warp == kWarpScale) {
             // ------------------------------ scales ------------------------------
-            // Row scale times the block's weight scale.
+            // Row scale times the block's weight scale, with ordinary loads: the kernel ahead may have written either.
             uint32_t seq = 0, it = 0, buf = 0, ph = 0;
             bool ok = true;
             Tile t;
@@ -591,13 +591,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int b = 0; b < 4; ++b)
 #pragma unroll
-                        for (int u = 0; u < kHalves; ++u) w[b][u] = __ldg(ws + (size_t)(kb + min(b, last)) * a.NB + nb[u]);
+                        for (int u = 0; u < kHalves; ++u) w[b][u] = __ldca(ws + (size_t)(kb + min(b, last)) * a.NB + nb[u]);
 #pragma unroll
                     for (int g = 0; g < kMaxR / 32; ++g)
                         if (g * 32 < t.n) {
                             const bool row = g * 32 + lane < t.rows;
 #pragma unroll
-                            for (int b = 0; b < 4; ++b) v[g][b] = row ? __ldg(xs + g * group + kb + min(b, last)) : 0.f;
+                            for (int b = 0; b < 4; ++b) v[g][b] = row ? __ldca(xs + g * group + kb + min(b, last)) : 0.f;
                         }
 #pragma unroll
                     for (int b = 0; b < 4; ++b) {
