@@ -117,7 +117,11 @@ def last_status(device=None, clear: bool = False):
     is incomplete.  Synchronises the streams the operators ran on."""
     import ctypes
 
-    idx = torch.cuda.current_device() if device is None else torch.device(device).index
+    if device is not None and torch.device(device).type != "cuda":
+        return (0, 0)  # (no operator runs there)
+    idx = None if device is None else torch.device(device).index
+    if idx is None:
+        idx = torch.cuda.current_device()
     found = (0, 0)
     for (d, stream), ws in list(_WS.items()) + _WS_KEPT:
         if d != idx:
