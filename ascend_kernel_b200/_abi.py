@@ -30,6 +30,7 @@ EXPORTS = [
     "b200moe_silu_mul_dyn", "b200moe_grouped_gemm_int8_silu", "b200moe_grouped_gemm_fp4_e8m0", "b200moe_pack_weight_int8", "b200moe_grouped_gemm_int8_packed", "b200moe_grouped_gemm_int8_packed_scatter",
     "b200moe_fp8_quantize_rows", "b200moe_fp8_quantize_rows_scratch_bytes", "b200moe_grouped_gemm_fp8_block", "b200moe_grouped_gemm_fp8_block_workspace_bytes",
     "b200moe_moe_balance_scratch_bytes", "b200moe_moe_balance_loss", "b200moe_moe_balance_loss_grad", "b200moe_read_findings",
+    "b200moe_grouped_gemm_fp8_block_findings", "b200moe_moe_balance_loss_findings", "b200moe_findings_pair", "b200moe_read_findings_at",
     "b200moe_set_gemm_reserved_sms", "b200moe_ipc_alloc", "b200moe_ipc_open", "b200moe_ipc_close", "b200moe_ipc_free",
 ]
 
@@ -132,6 +133,14 @@ def _load() -> ctypes.CDLL:
     lib.b200moe_moe_balance_loss.restype = i32
     lib.b200moe_moe_balance_loss_grad.argtypes = [vp, i32, vp, vp, vp, vp, vp, i64, i64, i64, vp, vp]
     lib.b200moe_moe_balance_loss_grad.restype = i32
+    lib.b200moe_grouped_gemm_fp8_block_findings.argtypes = lib.b200moe_grouped_gemm_fp8_block.argtypes[:-1] + [vp, vp]
+    lib.b200moe_grouped_gemm_fp8_block_findings.restype = i32
+    lib.b200moe_moe_balance_loss_findings.argtypes = lib.b200moe_moe_balance_loss.argtypes[:-1] + [vp, vp]
+    lib.b200moe_moe_balance_loss_findings.restype = i32
+    lib.b200moe_findings_pair.argtypes = [i32, ctypes.POINTER(vp)]
+    lib.b200moe_findings_pair.restype = i32
+    lib.b200moe_read_findings_at.argtypes = [vp, ctypes.POINTER(ctypes.c_int32), i32, vp]
+    lib.b200moe_read_findings_at.restype = i32
     lib.b200moe_read_findings.argtypes = [ctypes.POINTER(ctypes.c_int32), i32, vp]
     lib.b200moe_read_findings.restype = i32
     u64, comm = ctypes.c_uint64, ctypes.POINTER(EpComm)

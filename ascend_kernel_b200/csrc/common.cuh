@@ -29,7 +29,7 @@ __device__ __forceinline__ void report_status(int* status, int code, int detail)
     if (atomicCAS(status + 4, 0, code) == 0) status[5] = detail;
 }
 
-// The same in the library's pair of words (code, detail), which keep the first finding on the device until they are cleared; may be NULL.
+// The same in a pair of words (code, detail) that keep the first finding until they are cleared; may be NULL.
 __device__ __forceinline__ void keep_finding(int* findings, int code, int detail) {
     if (findings != nullptr && atomicCAS(findings, 0, code) == 0) findings[1] = detail;
 }
@@ -89,8 +89,8 @@ __device__ __forceinline__ uint32_t ldg_stream4(const uint8_t* p) {
 
 // Multiprocessor count of the current device (cached per device).
 int sm_count();
-// The words of keep_finding on the current device; NULL if their address cannot be had.
-int* findings_words();
+// The `pair`-th of the library's pairs of words for keep_finding on the current device; NULL if their address cannot be had.
+int* findings_words(int pair = 0);
 
 // ---- tensor maps (driver entry point fetched through the runtime, no libcuda link) ---------
 // 2-D row-major tensor [rows, cols] of `elem_bytes`-byte elements, box [box_rows, box_cols].

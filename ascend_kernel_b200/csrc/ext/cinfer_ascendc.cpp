@@ -8,6 +8,7 @@
 #include <cuda_runtime_api.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cstdio>
 #include <map>
 #include <mutex>
@@ -90,6 +91,69 @@ at::Tensor workspace_for(const at::Tensor& like, size_t bytes, void* stream) {
     return it->second;
 }
 
+// The operators without a workspace of status words keep their findings in pairs of words of the library's, one for each of the two
+// bindings and every stream that they were called on: like the workspaces, so that a status call waits for those streams
+// alone and clears what its own binding found.  (Should a device run out of pairs, the streams that come last share one.)
+enum Binding { kDropIn, kMirror };  // this module, and the package's functions of the same names
+struct FindingWords {
+    Binding binding;
+    int device;
+    void* stream;
+    int32_t* words;
+};
+std::vector<FindingWords> g_findings;  // (guarded by g_ws_mutex)
+
+// for the current device
+int32_t* findings_for(Binding binding, int device, void* stream) {
+    std::lock_guard<std::mutex> lock(g_ws_mutex);
+    int used = 0;
+    for (const auto& f : g_findings) {
+        if (f.binding == binding && f.device == device && f.stream == stream) return f.words;
+        used += f.device == device;
+    }
+    int32_t* words = nullptr;
+    const int rc = b200moe_findings_pair(std::min(used + 1, B200MOE_FINDINGS_PAIRS - 1), &words);
+    TORCH_CHECK(rc == B200MOE_OK, "findings_pair: ", b200moe_strerror(rc));
+    g_findings.push_back({binding, device, stream, words});
+    return words;
+}
+
+// Whether work may be queued on the stream now (not while it is captured: what is recorded there has not run).
+bool may_wait_for(void* stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &status) == cudaSuccess) return status == cudaStreamCaptureStatusNone;
+    (void)cudaGetLastError();
+    return false;
+}
+
+// The first finding of a binding's calls on the current device.  Waits for the streams that they ran on and, since replays of
+// captured calls run where the caller says, for the caller's own; only where there were such calls.  g_ws_mutex is held.
+std::pair<int, int> read_findings(Binding binding, int device, bool clear) {
+    std::pair<int, int> found{0, 0};
+    bool waited = false;
+    for (const auto& f : g_findings) {
+        if (f.binding != binding || f.device != device) continue;
+        if (!waited) {
+            waited = true;
+            const auto own = c10::cuda::getCurrentCUDAStream().stream();
+            if (may_wait_for(own)) TORCH_CHECK(cudaStreamSynchronize(own) == cudaSuccess, "cudaStreamSynchronize failed");
+        }
+        if (!may_wait_for(f.stream)) continue;
+        int32_t out[2] = {0, 0};
+        const int rc = b200moe_read_findings_at(f.words, out, clear ? 1 : 0, f.stream);
+        TORCH_CHECK(rc == B200MOE_OK, "read_findings: ", b200moe_strerror(rc));
+        if (found.first == 0 && out[0] != 0) found = {out[0], out[1]};
+    }
+    return found;
+}
+
+// What the package's own functions found on a device, for its status calls (which know its workspaces).
+std::pair<int, int> MirrorFindings(int64_t device, bool clear) {
+    c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+    std::lock_guard<std::mutex> lock(g_ws_mutex);
+    return read_findings(kMirror, (int)device, clear);
+}
+
 std::pair<int, int> LastStatus(bool clear) {
     std::lock_guard<std::mutex> lock(g_ws_mutex);
     int dev = 0;
@@ -104,13 +168,9 @@ std::pair<int, int> LastStatus(bool clear) {
     };
     for (auto& kv : g_workspaces) read(kv.first, kv.second);
     for (auto& kv : g_kept_workspaces) read(kv.first, kv.second);
-    // what the operators without a workspace of status words found (their streams: all of the device's)
-    int32_t kept[2] = {0, 0};
-    TORCH_CHECK(cudaDeviceSynchronize() == cudaSuccess, "cudaDeviceSynchronize failed");
-    const int rc = b200moe_read_findings(kept, clear ? 1 : 0, c10::cuda::getCurrentCUDAStream().stream());
-    TORCH_CHECK(rc == B200MOE_OK, "read_findings: ", b200moe_strerror(rc));
-    if (found.first == 0 && kept[0] != 0) found = {kept[0], kept[1]};
-    return found;
+    // and what the operators without a workspace of status words found
+    const auto kept = read_findings(kDropIn, dev, clear);
+    return found.first != 0 ? found : kept;
 }
 
 void CheckStatus() {
@@ -370,6 +430,7 @@ std::tuple<at::Tensor, at::Tensor> Fp8QuantizeRows(const at::Tensor& x, const Op
     return {codes, scale};
 }
 
+template <Binding BINDING>
 void GroupedGemmFp8Block(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& weight, const at::Tensor& weight_scale,
                          const at::Tensor& group_list, const at::Tensor& output, const OptionalTensor& output_scale_opt,
                          int64_t group_list_type, bool gate_up_silu) {
@@ -400,17 +461,18 @@ void GroupedGemmFp8Block(const at::Tensor& x, const at::Tensor& x_scale, const a
     // a workspace for this call alone: two graphs captured on one stream may be replayed side by side
     const size_t bytes = b200moe_grouped_gemm_fp8_block_workspace_bytes(M, K, N, G, gate_up_silu ? 1 : 0);
     at::Tensor workspace = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
-    raise_on(b200moe_grouped_gemm_fp8_block(x.data_ptr(), x_scale.data_ptr<float>(), weight.data_ptr(), weight_scale.data_ptr<float>(),
-                                            group_list.data_ptr<int64_t>(), output.data_ptr(),
-                                            output_scale ? output_scale->data_ptr<float>() : nullptr, M, K, N, G, (int)group_list_type,
-                                            gate_up_silu ? 1 : 0, workspace.data_ptr(), bytes,
-                                            c10::cuda::getCurrentCUDAStream().stream()),
+    const auto stream = c10::cuda::getCurrentCUDAStream().stream();
+    raise_on(b200moe_grouped_gemm_fp8_block_findings(x.data_ptr(), x_scale.data_ptr<float>(), weight.data_ptr(),
+                                                     weight_scale.data_ptr<float>(), group_list.data_ptr<int64_t>(), output.data_ptr(),
+                                                     output_scale ? output_scale->data_ptr<float>() : nullptr, M, K, N, G,
+                                                     (int)group_list_type, gate_up_silu ? 1 : 0, workspace.data_ptr(), bytes,
+                                                     findings_for(BINDING, x.get_device(), stream), stream),
              "grouped_gemm_fp8_block");
 }
 
 struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& idx,
-                                                  const OptionalTensor& seq_opt, const OptionalTensor& mask_opt) {
+                                                  const OptionalTensor& seq_opt, const OptionalTensor& mask_opt, int64_t binding) {
         const at::Tensor* seq = given(seq_opt, "seq_list", logits);
         const at::Tensor* mask = given(mask_opt, "token_mask", logits);
         const int64_t T = logits.size(0), E = logits.size(1), S = seq ? seq->numel() : 1;
@@ -421,11 +483,13 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
         const size_t bytes = b200moe_moe_balance_scratch_bytes(T, E, S);
         at::Tensor scratch = at::empty({(int64_t)bytes}, f32.dtype(at::kByte));
         float* load = kept.data_ptr<float>();
-        raise_on(b200moe_moe_balance_loss(logits.data_ptr(), logits.scalar_type() == at::kFloat ? 1 : 0, idx.data_ptr<int32_t>(),
-                                          seq ? seq->data_ptr<int64_t>() : nullptr,
-                                          mask ? static_cast<const uint8_t*>(mask->data_ptr()) : nullptr, T, E, idx.size(1), S,
-                                          loss.data_ptr<float>(), counts.data_ptr<int64_t>(), load, load + S * E, scratch.data_ptr(),
-                                          bytes, c10::cuda::getCurrentCUDAStream().stream()),
+        const auto stream = c10::cuda::getCurrentCUDAStream().stream();
+        raise_on(b200moe_moe_balance_loss_findings(logits.data_ptr(), logits.scalar_type() == at::kFloat ? 1 : 0, idx.data_ptr<int32_t>(),
+                                                   seq ? seq->data_ptr<int64_t>() : nullptr,
+                                                   mask ? static_cast<const uint8_t*>(mask->data_ptr()) : nullptr, T, E, idx.size(1), S,
+                                                   loss.data_ptr<float>(), counts.data_ptr<int64_t>(), load, load + S * E,
+                                                   scratch.data_ptr(), bytes, findings_for((Binding)binding, logits.get_device(), stream),
+                                                   stream),
                  "moe_balance_loss");
         ctx->save_for_backward({logits, seq ? *seq : at::Tensor(), mask ? *mask : at::Tensor(), kept});
         ctx->mark_non_differentiable({counts});
@@ -435,7 +499,7 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
         TORCH_CHECK(!at::GradMode::is_enabled(), "moe_balance_loss is differentiable once");
         const auto saved = ctx->get_saved_variables();
         const at::Tensor &logits = saved[0], &seq = saved[1], &mask = saved[2], &kept = saved[3];
-        if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+        if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
         const int64_t T = logits.size(0), E = logits.size(1), S = kept.numel() / (E + 1);
         c10::cuda::CUDAGuard guard(logits.device());
         const at::Tensor g = grads[0].to(at::kFloat).contiguous();
@@ -447,10 +511,11 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
                                                load + S * E, g.data_ptr<float>(), T, E, S, out.data_ptr(),
                                                c10::cuda::getCurrentCUDAStream().stream()),
                  "moe_balance_loss (gradient)");
-        return {out, at::Tensor(), at::Tensor(), at::Tensor()};
+        return {out, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
     }
 };
 
+template <Binding BINDING>
 std::tuple<at::Tensor, at::Tensor> MoeBalanceLoss(const at::Tensor& logits, const at::Tensor& idx, const OptionalTensor& seq_opt,
                                                   const OptionalTensor& mask_opt) {
     check_tensor(logits, "logits");
@@ -463,7 +528,7 @@ std::tuple<at::Tensor, at::Tensor> MoeBalanceLoss(const at::Tensor& logits, cons
     TORCH_CHECK(!seq || (seq->scalar_type() == at::kLong && seq->dim() == 1), "seq_list must be int64 [S]");
     const at::Tensor* mask = given(mask_opt, "token_mask", logits);
     TORCH_CHECK(!mask || (mask->scalar_type() == at::kBool && mask->dim() == 1 && mask->size(0) == T), "token_mask must be bool [", T, "]");
-    auto out = BalanceLoss::apply(logits, idx, seq_opt, mask_opt);
+    auto out = BalanceLoss::apply(logits, idx, seq_opt, mask_opt, (int64_t)BINDING);
     return {out[0], out[1]};
 }
 
@@ -489,11 +554,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("fp4_scale_fold", &Fp4ScaleFold, "block_scale"_a, "global_scale"_a, "Two-level FP4 scale fold.");
     m.def("fp8_quantize_rows", &Fp8QuantizeRows, "x"_a, "index"_a = pybind11::none(), "codes"_a = pybind11::none(),
           "scale"_a = pybind11::none(), "bf16 rows -> (e4m3 codes, fp32 scale per 128), optionally gathered by an index.");
-    m.def("grouped_gemm_fp8_block", &GroupedGemmFp8Block, "x"_a, "x_scale"_a, "weight"_a, "weight_scale"_a, "group_list"_a, "output"_a,
+    m.def("grouped_gemm_fp8_block", &GroupedGemmFp8Block<kDropIn>, "x"_a, "x_scale"_a, "weight"_a, "weight_scale"_a, "group_list"_a, "output"_a,
           "output_scale"_a = pybind11::none(), "group_list_type"_a = 0, "gate_up_silu"_a = false,
           "GROUP GEMM on e4m3 rows and e4m3 weights with scales per block of 128.");
-    m.def("moe_balance_loss", &MoeBalanceLoss, "logits"_a, "idx"_a, "seq_list"_a = pybind11::none(), "token_mask"_a = pybind11::none(),
+    m.def("moe_balance_loss", &MoeBalanceLoss<kDropIn>, "logits"_a, "idx"_a, "seq_list"_a = pybind11::none(), "token_mask"_a = pybind11::none(),
           "(balance loss per sequence, pairs per sequence and expert), differentiable in the logits.");
+    // the package's functions of the same names: their findings are read by its status calls
+    m.def("_mirror_grouped_gemm_fp8_block", &GroupedGemmFp8Block<kMirror>);
+    m.def("_mirror_moe_balance_loss", &MoeBalanceLoss<kMirror>);
+    m.def("_mirror_findings", &MirrorFindings);
     m.def("last_status", [](bool clear) { return LastStatus(clear); }, "clear"_a = false,
           "(code, detail) of the first device-side finding since the status was last cleared.");
     m.def("check_status", &CheckStatus, "Raises if an operator call left a device-side finding (and clears it).");

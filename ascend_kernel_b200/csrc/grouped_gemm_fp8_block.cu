@@ -781,10 +781,10 @@ extern "C" size_t b200moe_grouped_gemm_fp8_block_workspace_bytes(int64_t M, int6
     return fb::kWordBytes + (parts > 1 ? (size_t)parts * (size_t)M * (size_t)N * 4 : 0);
 }
 
-extern "C" int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scale, const void* weight, const float* weight_scale,
-                                              const int64_t* group_list, void* out, float* out_scale, int64_t M, int64_t K, int64_t N,
-                                              int64_t G, int group_list_type, int gate_up_silu, void* workspace,
-                                              size_t workspace_bytes, void* stream) {
+extern "C" int b200moe_grouped_gemm_fp8_block_findings(const void* x, const float* x_scale, const void* weight, const float* weight_scale,
+                                                       const int64_t* group_list, void* out, float* out_scale, int64_t M, int64_t K,
+                                                       int64_t N, int64_t G, int group_list_type, int gate_up_silu, void* workspace,
+                                                       size_t workspace_bytes, int32_t* findings, void* stream) {
     if (!fb::sizes_ok(M, K, N, G) || (K % 16) != 0 || (N % 16) != 0 || (gate_up_silu && (N % 256) != 0))
         return B200MOE_ERR_SHAPE;
     if (group_list_type != B200MOE_GROUP_LIST_CUMSUM && group_list_type != B200MOE_GROUP_LIST_COUNTS) return B200MOE_ERR_ARGUMENT;
@@ -810,7 +810,7 @@ extern "C" int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scal
     a.KB = (int)((K + 127) / 128);
     a.NB = (int)((N + 127) / 128);
     a.words = static_cast<int*>(workspace);
-    a.findings = findings_words();
+    a.findings = findings != nullptr ? findings : findings_words();
     a.max_parts = fb::max_parts(M, K, N, G, gate_up_silu);
     if (a.max_parts > 1) a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + fb::kWordBytes);
     CUtensorMap map_w, map_x64, map_x16;
@@ -830,4 +830,12 @@ extern "C" int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scal
         B200MOE_CUDA_TRY(launch_dependent(gate_up_silu ? fb::join_kernel<true> : fb::join_kernel<false>, blocks, 256, 0, st, a));
     }
     return B200MOE_OK;
+}
+
+extern "C" int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scale, const void* weight, const float* weight_scale,
+                                              const int64_t* group_list, void* out, float* out_scale, int64_t M, int64_t K, int64_t N,
+                                              int64_t G, int group_list_type, int gate_up_silu, void* workspace,
+                                              size_t workspace_bytes, void* stream) {
+    return b200moe_grouped_gemm_fp8_block_findings(x, x_scale, weight, weight_scale, group_list, out, out_scale, M, K, N, G, group_list_type,
+                                                   gate_up_silu, workspace, workspace_bytes, nullptr, stream);
 }

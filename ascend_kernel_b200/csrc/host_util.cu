@@ -21,20 +21,24 @@ int sm_count() {
     return cached[dev];
 }
 
-__device__ int g_findings[2];
+__device__ int g_findings[B200MOE_FINDINGS_PAIRS][2];
 
-int* findings_words() {
+int* findings_words(int pair) {
     static int* cached[64];
     static std::mutex mu;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
     std::lock_guard<std::mutex> lock(mu);
     if (cached[dev] == nullptr) {
+        // (the first call on a device may come while a stream is captured, and loads the module then)
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        const bool swapped = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
         void* p = nullptr;
         if (cudaGetSymbolAddress(&p, g_findings) == cudaSuccess) cached[dev] = static_cast<int*>(p);
         else (void)cudaGetLastError();
+        if (swapped) (void)cudaThreadExchangeStreamCaptureMode(&mode);
     }
-    return cached[dev];
+    return cached[dev] == nullptr ? nullptr : cached[dev] + 2 * pair;
 }
 
 static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -124,15 +128,27 @@ int b200moe_read_sticky_status(void* workspace, int32_t out[2], int clear, void*
     return B200MOE_OK;
 }
 
-int b200moe_read_findings(int32_t out[2], int clear, void* stream) {
-    if (out == nullptr) return B200MOE_ERR_NULL_POINTER;
-    int* words = findings_words();
-    if (words == nullptr) return B200MOE_ERR_CUDA;
+int b200moe_findings_pair(int pair, int32_t** findings) {
+    if (findings == nullptr) return B200MOE_ERR_NULL_POINTER;
+    if (pair < 0 || pair >= B200MOE_FINDINGS_PAIRS) return B200MOE_ERR_ARGUMENT;
+    *findings = findings_words(pair);
+    return *findings == nullptr ? B200MOE_ERR_CUDA : B200MOE_OK;
+}
+
+int b200moe_read_findings_at(int32_t* findings, int32_t out[2], int clear, void* stream) {
+    if (findings == nullptr || out == nullptr) return B200MOE_ERR_NULL_POINTER;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    B200MOE_CUDA_TRY(cudaMemcpyAsync(out, words, 2 * sizeof(int32_t), cudaMemcpyDeviceToHost, s));
-    if (clear) B200MOE_CUDA_TRY(cudaMemsetAsync(words, 0, 2 * sizeof(int32_t), s));
+    B200MOE_CUDA_TRY(cudaMemcpyAsync(out, findings, 2 * sizeof(int32_t), cudaMemcpyDeviceToHost, s));
+    if (clear) B200MOE_CUDA_TRY(cudaMemsetAsync(findings, 0, 2 * sizeof(int32_t), s));
     B200MOE_CUDA_TRY(cudaStreamSynchronize(s));
     return B200MOE_OK;
+}
+
+int b200moe_read_findings(int32_t out[2], int clear, void* stream) {
+    if (out == nullptr) return B200MOE_ERR_NULL_POINTER;
+    int32_t* words = nullptr;
+    const int rc = b200moe_findings_pair(0, &words);
+    return rc == B200MOE_OK ? b200moe_read_findings_at(words, out, clear, stream) : rc;
 }
 
 }  // extern "C"

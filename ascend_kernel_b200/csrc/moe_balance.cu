@@ -476,10 +476,10 @@ extern "C" size_t b200moe_moe_balance_scratch_bytes(int64_t n_tokens, int64_t n_
     return (size_t)mb::scratch_rows(n_tokens, n_seqs) * (8u * (size_t)mb::pitch_of(n_experts) + 4u);
 }
 
-extern "C" int b200moe_moe_balance_loss(const void* logits, int logits_fp32, const int32_t* idx, const int64_t* seq_list,
-                                        const uint8_t* token_mask, int64_t n_tokens, int64_t n_experts, int64_t top_k, int64_t n_seqs,
-                                        float* loss, int64_t* counts, float* load, float* inv_tokens, void* scratch,
-                                        size_t scratch_bytes, void* stream) {
+extern "C" int b200moe_moe_balance_loss_findings(const void* logits, int logits_fp32, const int32_t* idx, const int64_t* seq_list,
+                                                 const uint8_t* token_mask, int64_t n_tokens, int64_t n_experts, int64_t top_k,
+                                                 int64_t n_seqs, float* loss, int64_t* counts, float* load, float* inv_tokens,
+                                                 void* scratch, size_t scratch_bytes, int32_t* findings, void* stream) {
     if (!mb::sizes_ok(n_tokens, n_experts, top_k, n_seqs) || (!seq_list && n_seqs != 1)) return B200MOE_ERR_SHAPE;
     if (logits_fp32 != 0 && logits_fp32 != 1) return B200MOE_ERR_ARGUMENT;
     if ((n_tokens > 0 && (!logits || !idx)) || !loss || !counts || !load || !inv_tokens) return B200MOE_ERR_NULL_POINTER;
@@ -529,8 +529,16 @@ extern "C" int b200moe_moe_balance_loss(const void* logits, int logits_fp32, con
     // (the list is read before the wait for the kernel ahead, so that must be the forward kernel, which began when the list was there)
     cfg.numAttrs = a.T > 0 ? 2 : 1;
     B200MOE_CUDA_TRY(cudaLaunchKernelEx(&cfg, mb::join_kernel, a, loss, reinterpret_cast<long long*>(counts), load, inv_tokens,
-                                        findings_words()));
+                                        findings != nullptr ? findings : findings_words()));
     return B200MOE_OK;
+}
+
+extern "C" int b200moe_moe_balance_loss(const void* logits, int logits_fp32, const int32_t* idx, const int64_t* seq_list,
+                                        const uint8_t* token_mask, int64_t n_tokens, int64_t n_experts, int64_t top_k, int64_t n_seqs,
+                                        float* loss, int64_t* counts, float* load, float* inv_tokens, void* scratch,
+                                        size_t scratch_bytes, void* stream) {
+    return b200moe_moe_balance_loss_findings(logits, logits_fp32, idx, seq_list, token_mask, n_tokens, n_experts, top_k, n_seqs, loss, counts,
+                                             load, inv_tokens, scratch, scratch_bytes, nullptr, stream);
 }
 
 extern "C" int b200moe_moe_balance_loss_grad(const void* logits, int logits_fp32, const int64_t* seq_list, const uint8_t* token_mask,

@@ -158,7 +158,7 @@ class MoELayer:
 
     def read_status(self, clear: bool = True):
         """Device-side findings of the passes run so far, read at a synchronisation point of the caller's
-        choosing (it waits for the layer's stream): raises if a grouped GEMM saw an invalid group list or
+        choosing (it waits for the streams that operators ran on, not for the device): raises if a grouped GEMM saw an invalid group list or
         a bounded wait expired, in an operator or in the token exchange; returns (0, 0) otherwise."""
         code, detail = ops.last_status(self.device, clear=clear)
         if code == 0 and self.px is not None:

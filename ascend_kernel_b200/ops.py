@@ -114,7 +114,8 @@ def last_status(device=None, clear: bool = False):
     """(code, detail) of the first device-side finding of any operator call on ``device`` (default: the
     current one) since the status was last cleared; (0, 0) if none.  code 1: a group_list was invalid and
     rows were clamped (detail = expert index); 2: a bounded wait inside a kernel expired and the output
-    is incomplete.  Synchronises the streams the operators ran on."""
+    is incomplete.  Synchronises the streams the operators ran on (and the caller's, where 8-bit products or balance losses are
+    among them: replays of captured ones run there); a stream that is being captured is left alone."""
     import ctypes
 
     if device is not None and torch.device(device).type != "cuda":
@@ -131,12 +132,9 @@ def last_status(device=None, clear: bool = False):
             _abi.check(_lib.b200moe_read_sticky_status(_ptr(ws), out, int(bool(clear)), stream), "read_sticky_status")
         if found == (0, 0) and out[0] != 0:
             found = (int(out[0]), int(out[1]))
-    # what the operators without a workspace of status words found (their streams: all of the device's)
-    out = (ctypes.c_int32 * 2)()
-    with torch.cuda.device(idx):
-        torch.cuda.synchronize()
-        _abi.check(_lib.b200moe_read_findings(out, int(bool(clear)), _stream()), "read_findings")
-    return (int(out[0]), int(out[1])) if found == (0, 0) else found
+    # what the operators of the compiled module found
+    kept = (0, 0) if _EXT is None else tuple(_EXT._mirror_findings(idx, clear))
+    return kept if found == (0, 0) else found
 
 
 def check_status(device=None):
@@ -545,7 +543,7 @@ def grouped_gemm_fp8_block(x, x_scale, weight, weight_scale, group_list, output,
     format of :func:`grouped_gemm`).  output bf16 [M, N].  ``gate_up_silu``: N = 2I with the gate columns first, output e4m3
     [M, I] and output_scale [M, I / 128] = silu(gate) * up quantised like :func:`fp8_quantize_rows`, which the down projection takes
     as they are.  K and N multiples of 16, with ``gate_up_silu`` N of 256.  Codes are uint8 or float8_e4m3fn tensors."""
-    _ext().grouped_gemm_fp8_block(x, x_scale, weight, weight_scale, group_list, output, output_scale, group_list_type, gate_up_silu)
+    _ext()._mirror_grouped_gemm_fp8_block(x, x_scale, weight, weight_scale, group_list, output, output_scale, group_list_type, gate_up_silu)
     _count(int(x.shape[0] > 0))
 
 
@@ -558,7 +556,7 @@ def moe_balance_loss(logits, idx, seq_list=None, token_mask=None):
 
     For T_s tokens with probabilities p = softmax(logits) and c_e pairs on expert e, loss = E / (k T_s) * sum_e c_e * mean_t p_te: 1
     where the load is even; 0 for a sequence without tokens.  The counts carry no gradient."""
-    out = _ext().moe_balance_loss(logits, idx, seq_list, token_mask)
+    out = _ext()._mirror_moe_balance_loss(logits, idx, seq_list, token_mask)
     _count(1 + (logits.shape[0] > 0))
     return out
 

@@ -316,11 +316,15 @@ int b200moe_fp8_quantize_rows(const void* x, const int32_t* index, void* codes, 
  * silu(gate) * up in fp32, quantised as b200moe_fp8_quantize_rows does: out e4m3 [M, I], out_scale fp32 [M, I / 128].
  * K % 16 == 0 and N % 16 == 0; x, weight and out aligned to 16 bytes.  Rows of no expert are left as they were.
  * The workspace belongs to the call until it has completed on the stream, and calls that overlap have one each; it holds no status
- * words: an invalid group_list (rows were clamped) or an expired wait is kept for b200moe_read_findings. */
+ * words: an invalid group_list (rows were clamped) or an expired wait is kept for b200moe_read_findings, or where `findings` says. */
 size_t b200moe_grouped_gemm_fp8_block_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, int gate_up_silu);
 int b200moe_grouped_gemm_fp8_block(const void* x, const float* x_scale, const void* weight, const float* weight_scale,
                                    const int64_t* group_list, void* out, float* out_scale, int64_t M, int64_t K, int64_t N, int64_t G,
                                    int group_list_type, int gate_up_silu, void* workspace, size_t workspace_bytes, void* stream);
+int b200moe_grouped_gemm_fp8_block_findings(const void* x, const float* x_scale, const void* weight, const float* weight_scale,
+                                            const int64_t* group_list, void* out, float* out_scale, int64_t M, int64_t K, int64_t N,
+                                            int64_t G, int group_list_type, int gate_up_silu, void* workspace, size_t workspace_bytes,
+                                            int32_t* findings, void* stream);
 
 /* Balance loss of the router (for training it; no reference counterpart).  logits [T, E] bf16 or fp32 (logits_fp32), idx int32 [T, top_k]
  * the experts of each token as b200moe_moe_route returns them (an entry outside 0 .. E - 1 is a pair that was dropped: it counts on no
@@ -337,13 +341,23 @@ size_t b200moe_moe_balance_scratch_bytes(int64_t n_tokens, int64_t n_experts, in
 int b200moe_moe_balance_loss(const void* logits, int logits_fp32, const int32_t* idx, const int64_t* seq_list,
                              const uint8_t* token_mask, int64_t n_tokens, int64_t n_experts, int64_t top_k, int64_t n_seqs, float* loss,
                              int64_t* counts, float* load, float* inv_tokens, void* scratch, size_t scratch_bytes, void* stream);
+int b200moe_moe_balance_loss_findings(const void* logits, int logits_fp32, const int32_t* idx, const int64_t* seq_list,
+                                      const uint8_t* token_mask, int64_t n_tokens, int64_t n_experts, int64_t top_k, int64_t n_seqs,
+                                      float* loss, int64_t* counts, float* load, float* inv_tokens, void* scratch, size_t scratch_bytes,
+                                      int32_t* findings, void* stream);
 int b200moe_moe_balance_loss_grad(const void* logits, int logits_fp32, const int64_t* seq_list, const uint8_t* token_mask,
                                   const float* load, const float* inv_tokens, const float* grad_loss, int64_t n_tokens,
                                   int64_t n_experts, int64_t n_seqs, void* grad_logits, void* stream);
 
-/* The first finding (code, detail; those of status words 0 and 1) of any b200moe_grouped_gemm_fp8_block or b200moe_moe_balance_loss call
- * on the current device since it was last cleared, kept in a fixed array of the library; (0, 0) if none.  Synchronises the
- * stream (calls on other streams may still be running). */
+/* A finding (code, detail; those of status words 0 and 1) of b200moe_grouped_gemm_fp8_block or b200moe_moe_balance_loss is kept in two
+ * words on the device, which hold the first one until they are cleared.  The `_findings` entries take them (zeroed device memory that
+ * outlives the call and its replays); NULL, and the entries without, stand for one pair of a device that all such calls share.
+ * b200moe_findings_pair: the address, on the current device, of one of the B200MOE_FINDINGS_PAIRS pairs that the library has, zero at the
+ * start; pair 0 is the shared one.  b200moe_read_findings_at: what a pair holds, (0, 0) if nothing; b200moe_read_findings: the shared one.
+ * Both synchronise the stream (calls on other streams may still be running). */
+#define B200MOE_FINDINGS_PAIRS 1024
+int b200moe_findings_pair(int pair, int32_t** findings);
+int b200moe_read_findings_at(int32_t* findings, int32_t out[2], int clear, void* stream);
 int b200moe_read_findings(int32_t out[2], int clear, void* stream);
 
 /* ---- expert-parallel token exchange over NVLink peer memory ----------------------------------
