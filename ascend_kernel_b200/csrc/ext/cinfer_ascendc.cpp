@@ -127,7 +127,8 @@ bool may_wait_for(void* stream) {
 }
 
 // The first finding of a binding's calls on the current device.  Waits for the streams that they ran on and, since replays of
-// captured calls run where the caller says, for the caller's own; only where there were such calls.  g_ws_mutex is held.
+// captured calls run where the caller says, for the caller's own; only where there were such calls.  `clear` takes the finding
+// that is returned and leaves the others to the calls that follow.  g_ws_mutex is held.
 std::pair<int, int> read_findings(Binding binding, int device, bool clear) {
     std::pair<int, int> found{0, 0};
     bool waited = false;
@@ -140,9 +141,12 @@ std::pair<int, int> read_findings(Binding binding, int device, bool clear) {
         }
         if (!may_wait_for(f.stream)) continue;
         int32_t out[2] = {0, 0};
-        const int rc = b200moe_read_findings_at(f.words, out, clear ? 1 : 0, f.stream);
+        int rc = b200moe_read_findings_at(f.words, out, 0, f.stream);
+        if (rc == B200MOE_OK && found.first == 0 && out[0] != 0) {
+            found = {out[0], out[1]};
+            if (clear) rc = b200moe_read_findings_at(f.words, out, 1, f.stream);
+        }
         TORCH_CHECK(rc == B200MOE_OK, "read_findings: ", b200moe_strerror(rc));
-        if (found.first == 0 && out[0] != 0) found = {out[0], out[1]};
     }
     return found;
 }
@@ -169,7 +173,7 @@ std::pair<int, int> LastStatus(bool clear) {
     for (auto& kv : g_workspaces) read(kv.first, kv.second);
     for (auto& kv : g_kept_workspaces) read(kv.first, kv.second);
     // and what the operators without a workspace of status words found
-    const auto kept = read_findings(kDropIn, dev, clear);
+    const auto kept = read_findings(kDropIn, dev, clear && found.first == 0);
     return found.first != 0 ? found : kept;
 }
 

@@ -115,7 +115,8 @@ def last_status(device=None, clear: bool = False):
     current one) since the status was last cleared; (0, 0) if none.  code 1: a group_list was invalid and
     rows were clamped (detail = expert index); 2: a bounded wait inside a kernel expired and the output
     is incomplete.  Synchronises the streams the operators ran on (and the caller's, where 8-bit products or balance losses are
-    among them: replays of captured ones run there); a stream that is being captured is left alone."""
+    among them: replays of captured ones run there); a stream that is being captured is left alone.  ``clear`` leaves a finding of these
+    two that is not the one returned to the next call, on whichever stream it was made."""
     import ctypes
 
     if device is not None and torch.device(device).type != "cuda":
@@ -133,7 +134,7 @@ def last_status(device=None, clear: bool = False):
         if found == (0, 0) and out[0] != 0:
             found = (int(out[0]), int(out[1]))
     # what the operators of the compiled module found
-    kept = (0, 0) if _EXT is None else tuple(_EXT._mirror_findings(idx, clear))
+    kept = (0, 0) if _EXT is None else tuple(_EXT._mirror_findings(idx, bool(clear) and found == (0, 0)))
     return kept if found == (0, 0) else found
 
 

@@ -99,3 +99,33 @@ def test_findings_of_a_side_stream_and_of_replays():
     gl[1] = 4
     graph.replay()
     assert ak.last_status() == (0, 0)
+
+
+def _bad_gemm(m, at):
+    """The same of an operator that keeps its findings in its stream's workspace."""
+    x = torch.zeros(12, 64, dtype=torch.bfloat16, device=DEV)
+    w = torch.zeros(3, 64, 256, dtype=torch.int8, device=DEV)
+    s = torch.ones(3, 256, dtype=torch.bfloat16, device=DEV)
+    counts = [0, 0, 0]
+    counts[at] = 100
+    offset = torch.zeros(0, device=DEV) if m is cinfer_ascendc else None
+    m.grouped_gemm(x, w, s, offset, torch.tensor(counts, device=DEV), "int8", torch.zeros(12, 256, dtype=torch.bfloat16, device=DEV),
+                   group_list_type=1)
+
+
+@pytest.mark.parametrize("m", [ak, cinfer_ascendc], ids=["mirror", "drop-in"])
+def test_clearing_takes_what_is_returned(m):
+    """Two operators that keep their findings in different places, and the second one's on two streams: each is reported once."""
+    side = torch.cuda.Stream()
+    _bad_gemm(m, 0)
+    _bad_product(m, 1)
+    with torch.cuda.stream(side):
+        _bad_product(m, 2)
+    got = [tuple(m.last_status(clear=True)) for _ in range(4)]
+    assert got[0] == (1, 0) and sorted(got[1:3]) == [(1, 1), (1, 2)] and got[3] == (0, 0)
+    _bad_gemm(m, 0)
+    _bad_product(m, 1)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="status"):
+            m.check_status()
+    m.check_status()
