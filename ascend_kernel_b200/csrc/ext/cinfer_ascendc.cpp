@@ -9,6 +9,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdio>
 #include <map>
 #include <mutex>
@@ -409,8 +410,9 @@ void check_f32(const at::Tensor& t, const char* name, at::IntArrayRef shape) {
 }
 int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
 
-std::tuple<at::Tensor, at::Tensor> Fp8QuantizeRows(const at::Tensor& x, const OptionalTensor& index_opt, const OptionalTensor& codes_opt,
-                                                   const OptionalTensor& scale_opt) {
+// (codes, scale, number of kernels launched)
+std::tuple<at::Tensor, at::Tensor, int> QuantizeRows(const at::Tensor& x, const OptionalTensor& index_opt, const OptionalTensor& codes_opt,
+                                                     const OptionalTensor& scale_opt) {
     check_tensor(x, "x");
     TORCH_CHECK(x.dim() == 2 && x.scalar_type() == at::kBFloat16, "x must be bfloat16 [T, K]");
     const at::Tensor* index = given(index_opt, "index", x);
@@ -431,11 +433,18 @@ std::tuple<at::Tensor, at::Tensor> Fp8QuantizeRows(const at::Tensor& x, const Op
                                        scale.data_ptr<float>(), T, R, K, scratch_bytes > 0 ? scratch.data_ptr() : nullptr,
                                        scratch_bytes, c10::cuda::getCurrentCUDAStream().stream()),
              "fp8_quantize_rows");
-    return {codes, scale};
+    return {codes, scale, R == 0 ? 0 : scratch_bytes > 0 ? 2 : 1};
 }
 
+std::tuple<at::Tensor, at::Tensor> Fp8QuantizeRows(const at::Tensor& x, const OptionalTensor& index, const OptionalTensor& codes,
+                                                   const OptionalTensor& scale) {
+    const auto out = QuantizeRows(x, index, codes, scale);
+    return {std::get<0>(out), std::get<1>(out)};
+}
+
+// The number of kernels launched.
 template <Binding BINDING>
-void GroupedGemmFp8Block(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& weight, const at::Tensor& weight_scale,
+int ProductFp8Block(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& weight, const at::Tensor& weight_scale,
                          const at::Tensor& group_list, const at::Tensor& output, const OptionalTensor& output_scale_opt,
                          int64_t group_list_type, bool gate_up_silu) {
     check_tensor(x, "x");
@@ -472,11 +481,23 @@ void GroupedGemmFp8Block(const at::Tensor& x, const at::Tensor& x_scale, const a
                                                      (int)group_list_type, gate_up_silu ? 1 : 0, workspace.data_ptr(), bytes,
                                                      findings_for(BINDING, x.get_device(), stream), stream),
              "grouped_gemm_fp8_block");
+    // (a workspace with room for parts of the k range comes with the kernel that adds them)
+    return M == 0 ? 0 : bytes > b200moe_grouped_gemm_fp8_block_workspace_bytes(0, K, N, G, gate_up_silu ? 1 : 0) ? 2 : 1;
 }
 
-struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
+void GroupedGemmFp8Block(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& weight, const at::Tensor& weight_scale,
+                         const at::Tensor& group_list, const at::Tensor& output, const OptionalTensor& output_scale,
+                         int64_t group_list_type, bool gate_up_silu) {
+    ProductFp8Block<kDropIn>(x, x_scale, weight, weight_scale, group_list, output, output_scale, group_list_type, gate_up_silu);
+}
+
+// Kernels that backward passes of the package's own functions launched: no caller of theirs sees one.
+std::atomic<int64_t> g_mirror_backward_launches{0};
+
+template <Binding BINDING>
+struct BalanceLoss : torch::autograd::Function<BalanceLoss<BINDING>> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& idx,
-                                                  const OptionalTensor& seq_opt, const OptionalTensor& mask_opt, int64_t binding) {
+                                                  const OptionalTensor& seq_opt, const OptionalTensor& mask_opt) {
         const at::Tensor* seq = given(seq_opt, "seq_list", logits);
         const at::Tensor* mask = given(mask_opt, "token_mask", logits);
         const int64_t T = logits.size(0), E = logits.size(1), S = seq ? seq->numel() : 1;
@@ -492,7 +513,7 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
                                                    seq ? seq->data_ptr<int64_t>() : nullptr,
                                                    mask ? static_cast<const uint8_t*>(mask->data_ptr()) : nullptr, T, E, idx.size(1), S,
                                                    loss.data_ptr<float>(), counts.data_ptr<int64_t>(), load, load + S * E,
-                                                   scratch.data_ptr(), bytes, findings_for((Binding)binding, logits.get_device(), stream),
+                                                   scratch.data_ptr(), bytes, findings_for(BINDING, logits.get_device(), stream),
                                                    stream),
                  "moe_balance_loss");
         ctx->save_for_backward({logits, seq ? *seq : at::Tensor(), mask ? *mask : at::Tensor(), kept});
@@ -503,7 +524,7 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
         TORCH_CHECK(!at::GradMode::is_enabled(), "moe_balance_loss is differentiable once");
         const auto saved = ctx->get_saved_variables();
         const at::Tensor &logits = saved[0], &seq = saved[1], &mask = saved[2], &kept = saved[3];
-        if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+        if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
         const int64_t T = logits.size(0), E = logits.size(1), S = kept.numel() / (E + 1);
         c10::cuda::CUDAGuard guard(logits.device());
         const at::Tensor g = grads[0].to(at::kFloat).contiguous();
@@ -515,7 +536,8 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
                                                load + S * E, g.data_ptr<float>(), T, E, S, out.data_ptr(),
                                                c10::cuda::getCurrentCUDAStream().stream()),
                  "moe_balance_loss (gradient)");
-        return {out, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+        if (T > 0 && BINDING == kMirror) ++g_mirror_backward_launches;
+        return {out, at::Tensor(), at::Tensor(), at::Tensor()};
     }
 };
 
@@ -532,7 +554,7 @@ std::tuple<at::Tensor, at::Tensor> MoeBalanceLoss(const at::Tensor& logits, cons
     TORCH_CHECK(!seq || (seq->scalar_type() == at::kLong && seq->dim() == 1), "seq_list must be int64 [S]");
     const at::Tensor* mask = given(mask_opt, "token_mask", logits);
     TORCH_CHECK(!mask || (mask->scalar_type() == at::kBool && mask->dim() == 1 && mask->size(0) == T), "token_mask must be bool [", T, "]");
-    auto out = BalanceLoss::apply(logits, idx, seq_opt, mask_opt, (int64_t)BINDING);
+    auto out = BalanceLoss<BINDING>::apply(logits, idx, seq_opt, mask_opt);
     return {out[0], out[1]};
 }
 
@@ -558,15 +580,17 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("fp4_scale_fold", &Fp4ScaleFold, "block_scale"_a, "global_scale"_a, "Two-level FP4 scale fold.");
     m.def("fp8_quantize_rows", &Fp8QuantizeRows, "x"_a, "index"_a = pybind11::none(), "codes"_a = pybind11::none(),
           "scale"_a = pybind11::none(), "bf16 rows -> (e4m3 codes, fp32 scale per 128), optionally gathered by an index.");
-    m.def("grouped_gemm_fp8_block", &GroupedGemmFp8Block<kDropIn>, "x"_a, "x_scale"_a, "weight"_a, "weight_scale"_a, "group_list"_a, "output"_a,
+    m.def("grouped_gemm_fp8_block", &GroupedGemmFp8Block, "x"_a, "x_scale"_a, "weight"_a, "weight_scale"_a, "group_list"_a, "output"_a,
           "output_scale"_a = pybind11::none(), "group_list_type"_a = 0, "gate_up_silu"_a = false,
           "GROUP GEMM on e4m3 rows and e4m3 weights with scales per block of 128.");
     m.def("moe_balance_loss", &MoeBalanceLoss<kDropIn>, "logits"_a, "idx"_a, "seq_list"_a = pybind11::none(), "token_mask"_a = pybind11::none(),
           "(balance loss per sequence, pairs per sequence and expert), differentiable in the logits.");
-    // the package's functions of the same names: their findings are read by its status calls
-    m.def("_mirror_grouped_gemm_fp8_block", &GroupedGemmFp8Block<kMirror>);
+    // the package's functions of the same names: their findings are read by its status calls, their launches counted there
+    m.def("_mirror_fp8_quantize_rows", &QuantizeRows);
+    m.def("_mirror_grouped_gemm_fp8_block", &ProductFp8Block<kMirror>);
     m.def("_mirror_moe_balance_loss", &MoeBalanceLoss<kMirror>);
     m.def("_mirror_findings", &MirrorFindings);
+    m.def("_mirror_backward_launches", []() { return g_mirror_backward_launches.load(); });
     m.def("last_status", [](bool clear) { return LastStatus(clear); }, "clear"_a = false,
           "(code, detail) of the first device-side finding since the status was last cleared.");
     m.def("check_status", &CheckStatus, "Raises if an operator call left a device-side finding (and clears it).");

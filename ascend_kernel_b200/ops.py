@@ -8,6 +8,9 @@ unchanged) select per-expert counts instead of cumulative sums and the canonical
 """
 from __future__ import annotations
 
+import sys
+import types
+
 import torch
 
 from . import _abi
@@ -15,13 +18,32 @@ from ._abi import CT, LAYOUT
 
 _lib = _abi.lib
 
-# number of this package's kernels launched so far (the benchmark reads and resets it)
-LAUNCHES = 0
+# number of this package's kernels launched so far: ``LAUNCHES`` (the benchmark reads and resets it).  A property of the module, since
+# backward passes launch kernels on threads of torch's, which count in the compiled module.
+_launches = 0
 
 
 def _count(n):
-    global LAUNCHES
-    LAUNCHES += n
+    global _launches
+    _launches += n
+
+
+def _backward_launches():
+    return 0 if _EXT is None else _EXT._mirror_backward_launches()
+
+
+class _Module(types.ModuleType):
+    @property
+    def LAUNCHES(self):
+        return _launches + _backward_launches()
+
+    @LAUNCHES.setter
+    def LAUNCHES(self, n):
+        global _launches
+        _launches = n - _backward_launches()
+
+
+sys.modules[__name__].__class__ = _Module
 
 
 def _ptr(t):
@@ -532,9 +554,9 @@ def fp8_quantize_rows(x, index=None, codes=None, scale=None):
     """x bf16 [T, K] -> (codes uint8 [R, K], scale fp32 [R, ceil(K / 128)]): e4m3 with one scale per 128 elements, a / 448 for
     the block's largest magnitude a (at least 2^-100).  ``index`` int32 [R]: row i of the result is row index[i] of x (R = T and row i
     without it); an index outside x gives zeros.  A block with an infinity or a NaN gets scale NaN.  K % 16 == 0."""
-    out = _ext().fp8_quantize_rows(x, index, codes, scale)
-    _count(int(out[0].numel() > 0))
-    return out
+    codes, scale, launches = _ext()._mirror_fp8_quantize_rows(x, index, codes, scale)
+    _count(launches)
+    return codes, scale
 
 
 def grouped_gemm_fp8_block(x, x_scale, weight, weight_scale, group_list, output, output_scale=None, group_list_type: int = 0,
@@ -544,8 +566,8 @@ def grouped_gemm_fp8_block(x, x_scale, weight, weight_scale, group_list, output,
     format of :func:`grouped_gemm`).  output bf16 [M, N].  ``gate_up_silu``: N = 2I with the gate columns first, output e4m3
     [M, I] and output_scale [M, I / 128] = silu(gate) * up quantised like :func:`fp8_quantize_rows`, which the down projection takes
     as they are.  K and N multiples of 16, with ``gate_up_silu`` N of 256.  Codes are uint8 or float8_e4m3fn tensors."""
-    _ext()._mirror_grouped_gemm_fp8_block(x, x_scale, weight, weight_scale, group_list, output, output_scale, group_list_type, gate_up_silu)
-    _count(int(x.shape[0] > 0))
+    _count(_ext()._mirror_grouped_gemm_fp8_block(x, x_scale, weight, weight_scale, group_list, output, output_scale, group_list_type,
+                                                 gate_up_silu))
 
 
 def moe_balance_loss(logits, idx, seq_list=None, token_mask=None):
