@@ -426,9 +426,16 @@ std::tuple<at::Tensor, at::Tensor, int> QuantizeRows(const at::Tensor& x, const 
     check_e4m3(codes, "codes", 2);
     TORCH_CHECK(codes.size(0) == R && codes.size(1) == K, "codes must be [", R, ", ", K, "]");
     check_f32(scale, "scale", {R, KB});
-    const size_t scratch_bytes = b200moe_fp8_quantize_rows_scratch_bytes(T, R, K, index != nullptr);
-    at::Tensor scratch;  // from the caching allocator and back to it
-    if (scratch_bytes > 0) scratch = at::empty({(int64_t)scratch_bytes}, x.options().dtype(at::kByte));
+    // scratch from the caching allocator and back to it; without it every row of the result is quantised
+    size_t scratch_bytes = b200moe_fp8_quantize_rows_scratch_bytes(T, R, K, index != nullptr);
+    at::Tensor scratch;
+    if (scratch_bytes > 0) {
+        try {
+            scratch = at::empty({(int64_t)scratch_bytes}, x.options().dtype(at::kByte));
+        } catch (const c10::OutOfMemoryError&) {
+            scratch_bytes = 0;
+        }
+    }
     raise_on(b200moe_fp8_quantize_rows(x.data_ptr(), index ? index->data_ptr<int32_t>() : nullptr, codes.data_ptr(),
                                        scale.data_ptr<float>(), T, R, K, scratch_bytes > 0 ? scratch.data_ptr() : nullptr,
                                        scratch_bytes, c10::cuda::getCurrentCUDAStream().stream()),
