@@ -43,7 +43,7 @@ namespace fb {
 constexpr int kWarpLoad = 0, kWarpMma0 = 1, kWarpScale = 3, kWarpEpi0 = 4;
 constexpr int kMaxR = kTileTokens;     // token rows of a tile
 constexpr int kABytes = 128 * 128;     // 128 weight columns of a stage
-constexpr int kMaxSlots = 12, kMaxBufs = 8;
+constexpr int kMaxSlots = 10, kMaxBufs = 8;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kStripBytes = 2048;      // of an epilogue warp
 // The epilogue's warps come in groups of four (128 weight columns), which share the tile's tokens.
@@ -67,6 +67,7 @@ struct Mode {
     static constexpr int kFixedBytes = 1024 + kBarrierBytes + kScaleRingBytes + kEpiWarps * kStripBytes + 2 * kTopBytes + 2 * (kMaxExperts + 4) * 4;
     static constexpr int kRingBytes = kSmemBytes - kFixedBytes;
     static_assert(kRingBytes % 16 == 0 && kRingBytes >= 4 * (HALVES * kABytes + kMaxR * 64), "stages");
+    static_assert(kRingBytes / (HALVES * kABytes + 32 * 64) <= kMaxSlots, "barriers of every stage");
 };
 using One = Mode<1, false>;
 using Two = Mode<2, false>;
@@ -746,7 +747,7 @@ static bool sizes_ok(int64_t M, int64_t K, int64_t N, int64_t G) {
 constexpr int64_t kPairs = 74;  // of a B200's multiprocessors (rules and sizes go by the sizes of a call alone)
 
 // Whether a tile's stage holds two blocks of 128 columns a CTA: a pair then reads 512 contiguous bytes of a weight row and the rows of x
-// half as often, but has three to five stages in flight instead of seven to eleven.  One | two blocks, us (experts, tokens x
+// half as often, but has four or five stages in flight instead of seven to ten.  One | two blocks, us (experts, tokens x
 // top_k, K x N): 256, 37 x 8, 2048 x 7168: 445 | 376; 256, 1024 x 8, 7168 x 4096: 1325 | 1138; 256, 2048 x 8, 2048 x 7168: 851 | 662, of 80 rows
 // an expert 840 | 772, of 96 rows 810 | 924, of 128 rows 966 | 1148.  Where the tiles are a few waves of the pairs, the cut that
 // fills its last wave better: 8 experts of a row, 2048 x 7168: 29.8 | 27.2; 64 experts of 64 rows, 2048 x 2048: 58.6 | 65.5.
