@@ -21,12 +21,15 @@
 //
 // Few tiles: the k range is split into parts whose fp32 sums go to the workspace, and a second kernel adds them in their order.
 //
-// What bounds it.  Few rows: the weights' bytes (256 experts of a row, 2048 x 7168: 524 us, 7.2 TB/s; 8 experts: 28 us, 1.5 waves of the
-// pairs).
-// Many rows: the sums outside the tensor core.  A block of 256 x 160 x 128 is 320 cycles of a pair's MMA and about 610 of an epilogue
-// group's (93 waiting for the commit, 371 tensor-memory loads and fused multiply-adds, 57 handing the buffer back, 89 of loop), and at 990 W
-// the clock is 1.24 to 1.4 GHz: 256 experts of 256 rows, 2048 x 7168: 1.32 ms, 1.46 PFLOP/s; 64 of 128 rows: 187 us (1.28 PFLOP/s, 5.7 TB/s);
-// gate/up of 256 experts of 128 rows, 7168 x 4096: 1.5 ms (1.27 to 1.32 PFLOP/s, 5.1 to 5.4 TB/s).
+// What bounds it.  Few rows: the weights' bytes (256 experts of a row, 2048 x 7168: 523 us, 7.2 TB/s, 549 in a steady loop; 8 experts: 25 us,
+// 1.5 waves of the pairs; gate/up of one token, 7168 x 4096: 45 us, 128 units and their join for 36 us of bytes).
+// Many rows: the way of a block through the epilogue -- wait for the commit, loads from tensor memory, multiply-adds, the buffer handed
+// back -- whose latencies two warps a scheduler do not cover: with the weights in L2 (8 experts of 640 rows) the tensor pipe is active 35 % of the
+// cycles, issue slots 36 to 42 %, and no pipe is near its limit.  A block of 256 x 160 x 128 is 320 cycles of a pair's MMA; a call
+// takes a pair 664 (Zipf rows, 7168 x 4096) to 875 cycles a block, the ends of its tiles included.  Short bursts run at a higher clock than
+// the 1.25 to 1.42 GHz that the power limit leaves a steady loop, burst | steady: 256 experts of 256 rows, 2048 x 7168: 1.39 | 1.65 ms (1.17
+// PFLOP/s); gate/up of 256 experts of 128 rows each, 7168 x 4096: 1.49 | 1.80 ms.  That is the favourable split: of a routed batch of the same
+// mean half the experts have 129 to 160 rows, which cost a tile 160 and the whole call a fourth buffer (1.93 ms steady).
 // Tiles of at most 160 rows leave three buffers of tensor memory: with 256 rows there are two, with 128 four, both slower.  Two groups of
 // four epilogue warps: with four groups 37 tokens x 8 on 256 experts of 2048 x 7168 took 396 us for 372, 4096 x 8 rows 886 for 783.
 #include <algorithm>

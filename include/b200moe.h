@@ -314,7 +314,8 @@ int b200moe_fp8_quantize_rows(const void* x, const int32_t* index, void* codes, 
  * the format's own (0x7F and 0xFF are NaN, which b200moe_grouped_gemm reads as +-480).  Sums in fp32, scales applied in fp32.
  * gate_up_silu == 0: out bf16 [M, N], out_scale unused.  gate_up_silu == 1: N = 2 I with the gate columns first, N % 256 == 0;
  * silu(gate) * up in fp32, quantised as b200moe_fp8_quantize_rows does: out e4m3 [M, I], out_scale fp32 [M, I / 128].
- * K % 16 == 0 and N % 16 == 0; x, weight and out aligned to 16 bytes.  Rows of no expert are left as they were.
+ * K % 16 == 0 and N % 16 == 0; x, weight and out aligned to 16 bytes.  Rows of no expert are left as they were, but how a call is cut goes by
+ * M, which counts them: the same rows in a longer tensor may be summed in another order.
  * The workspace belongs to the call until it has completed on the stream, and calls that overlap have one each; it holds no status
  * words: an invalid group_list (rows were clamped) or an expired wait is kept for b200moe_read_findings, or where `findings` says. */
 size_t b200moe_grouped_gemm_fp8_block_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, int gate_up_silu);
