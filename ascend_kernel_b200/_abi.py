@@ -31,6 +31,9 @@ EXPORTS = [
     "b200moe_fp8_quantize_rows", "b200moe_fp8_quantize_rows_scratch_bytes", "b200moe_grouped_gemm_fp8_block", "b200moe_grouped_gemm_fp8_block_workspace_bytes",
     "b200moe_moe_balance_scratch_bytes", "b200moe_moe_balance_loss", "b200moe_moe_balance_loss_grad", "b200moe_read_findings",
     "b200moe_grouped_gemm_fp8_block_findings", "b200moe_moe_balance_loss_findings", "b200moe_findings_pair", "b200moe_read_findings_at",
+    "b200moe_moe_sort", "b200moe_moe_sort_scratch_bytes", "b200moe_moe_dispatch", "b200moe_moe_dispatch_grad", "b200moe_moe_combine",
+    "b200moe_moe_combine_grad", "b200moe_mxfp4_quantize_rows", "b200moe_mxfp4_quantize_rows_scratch_bytes",
+    "b200moe_grouped_gemm_mxfp4", "b200moe_grouped_gemm_mxfp4_workspace_bytes",
     "b200moe_set_gemm_reserved_sms", "b200moe_ipc_alloc", "b200moe_ipc_open", "b200moe_ipc_close", "b200moe_ipc_free",
 ]
 
@@ -143,6 +146,22 @@ def _load() -> ctypes.CDLL:
     lib.b200moe_read_findings_at.restype = i32
     lib.b200moe_read_findings.argtypes = [ctypes.POINTER(ctypes.c_int32), i32, vp]
     lib.b200moe_read_findings.restype = i32
+    lib.b200moe_moe_sort_scratch_bytes.argtypes = [i64, i64, i64]
+    lib.b200moe_moe_sort_scratch_bytes.restype = sz
+    lib.b200moe_moe_sort.argtypes = [vp, i64, i64, i64, vp, vp, vp, vp, sz, vp]
+    lib.b200moe_moe_dispatch.argtypes = [vp, i32, vp, vp, vp, i64, i64, i64, vp]
+    lib.b200moe_moe_dispatch_grad.argtypes = [vp, i32, vp, vp, i64, i64, i64, vp]
+    lib.b200moe_moe_combine.argtypes = [vp, i32, vp, vp, vp, i64, i64, i64, vp]
+    lib.b200moe_moe_combine_grad.argtypes = [vp, i32, vp, vp, vp, vp, vp, vp, i64, i64, i64, vp]
+    lib.b200moe_mxfp4_quantize_rows_scratch_bytes.argtypes = [i64, i64, i64, i32]
+    lib.b200moe_mxfp4_quantize_rows_scratch_bytes.restype = sz
+    lib.b200moe_mxfp4_quantize_rows.argtypes = [vp, vp, vp, vp, i64, i64, i64, vp, sz, vp]
+    lib.b200moe_grouped_gemm_mxfp4_workspace_bytes.argtypes = [i64, i64, i64, i64, i32]
+    lib.b200moe_grouped_gemm_mxfp4_workspace_bytes.restype = sz
+    lib.b200moe_grouped_gemm_mxfp4.argtypes = [vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i32, i32, vp, sz, vp, vp]
+    for f in (lib.b200moe_grouped_gemm_mxfp4, lib.b200moe_moe_sort, lib.b200moe_moe_dispatch, lib.b200moe_moe_dispatch_grad, lib.b200moe_moe_combine,
+              lib.b200moe_moe_combine_grad, lib.b200moe_mxfp4_quantize_rows):
+        f.restype = i32
     u64, comm = ctypes.c_uint64, ctypes.POINTER(EpComm)
     lib.b200moe_ep_post_counts.argtypes = [comm, vp, u64, vp]
     lib.b200moe_ep_dispatch.argtypes = [comm, vp, vp, i64, u64, vp, vp, vp, vp, vp]

@@ -565,6 +565,213 @@ std::tuple<at::Tensor, at::Tensor> MoeBalanceLoss(const at::Tensor& logits, cons
     return {out[0], out[1]};
 }
 
+// ---- tokens on their way to the experts and back, with gradients ----------------------------------------------------------
+
+// A scratch tensor from the caching allocator, for a call alone: two graphs captured on one stream may be replayed side by side.
+at::Tensor bytes_like(const at::Tensor& like, size_t bytes) { return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)); }
+
+// (counts, token_of, slot, number of kernels launched)
+std::tuple<at::Tensor, at::Tensor, at::Tensor, int> SortPairs(const at::Tensor& idx, int64_t n_experts) {
+    check_tensor(idx, "idx");
+    TORCH_CHECK(idx.scalar_type() == at::kInt && idx.dim() == 2, "idx must be int32 [T, k]");
+    const int64_t T = idx.size(0), k = idx.size(1);
+    TORCH_CHECK(n_experts > 0 && n_experts <= 1024, "n_experts must be 1 .. 1024");
+    c10::cuda::CUDAGuard guard(idx.device());
+    at::Tensor counts = at::empty({n_experts}, idx.options().dtype(at::kLong));
+    at::Tensor token_of = at::empty({T * k}, idx.options()), slot = at::empty({T, k}, idx.options());
+    const size_t bytes = b200moe_moe_sort_scratch_bytes(T, n_experts, k);
+    at::Tensor scratch;
+    if (bytes > 0) scratch = bytes_like(idx, bytes);
+    raise_on(b200moe_moe_sort(idx.data_ptr<int32_t>(), T, n_experts, k, counts.data_ptr<int64_t>(), token_of.data_ptr<int32_t>(),
+                              slot.data_ptr<int32_t>(), bytes > 0 ? scratch.data_ptr() : nullptr, bytes,
+                              c10::cuda::getCurrentCUDAStream().stream()),
+             "moe_sort");
+    return {counts, token_of, slot, bytes > 0 ? 2 : 1};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> MoeSort(const at::Tensor& idx, int64_t n_experts) {
+    const auto out = SortPairs(idx, n_experts);
+    return {std::get<0>(out), std::get<1>(out), std::get<2>(out)};
+}
+
+// Rows of T tokens, or of their T * k pairs, and the two index tensors of a sort.
+void check_rows(const at::Tensor& rows, const char* name, bool pairs, const at::Tensor& token_of, const at::Tensor& slot) {
+    check_tensor(rows, name);
+    check_beside(token_of, "token_of", rows); check_beside(slot, "slot", rows);
+    TORCH_CHECK(rows.dim() == 2 && (rows.scalar_type() == at::kBFloat16 || rows.scalar_type() == at::kFloat), name,
+                " must be bfloat16 or float32 with two dimensions");
+    TORCH_CHECK(rows.size(1) > 0 && rows.size(1) % 8 == 0, "rows must have a multiple of 8 elements");
+    TORCH_CHECK(slot.scalar_type() == at::kInt && slot.dim() == 2 && slot.size(1) > 0, "slot must be int32 [T, k]");
+    TORCH_CHECK(token_of.scalar_type() == at::kInt && token_of.dim() == 1 && token_of.size(0) == slot.numel(), "token_of must be int32 [",
+                slot.numel(), "]");
+    TORCH_CHECK(rows.size(0) == (pairs ? slot.numel() : slot.size(0)), name, " must have ", pairs ? slot.numel() : slot.size(0), " rows");
+}
+
+template <Binding BINDING>
+struct Dispatch : torch::autograd::Function<Dispatch<BINDING>> {
+    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& token_of, const at::Tensor& slot) {
+        c10::cuda::CUDAGuard guard(x.device());
+        at::Tensor rows = at::empty({slot.numel(), x.size(1)}, x.options());
+        raise_on(b200moe_moe_dispatch(x.data_ptr(), x.scalar_type() == at::kFloat ? 1 : 0, token_of.data_ptr<int32_t>(),
+                                      slot.data_ptr<int32_t>(), rows.data_ptr(), x.size(0), slot.size(1), x.size(1),
+                                      c10::cuda::getCurrentCUDAStream().stream()),
+                 "moe_dispatch");
+        ctx->save_for_backward({slot});
+        return rows;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "moe_dispatch is differentiable once");
+        if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor()};
+        const at::Tensor slot = ctx->get_saved_variables()[0], g = grads[0].contiguous();
+        c10::cuda::CUDAGuard guard(g.device());
+        at::Tensor grad_x = at::empty({slot.size(0), g.size(1)}, g.options());
+        raise_on(b200moe_moe_dispatch_grad(g.data_ptr(), g.scalar_type() == at::kFloat ? 1 : 0, slot.data_ptr<int32_t>(), grad_x.data_ptr(),
+                                           slot.size(0), slot.size(1), g.size(1), c10::cuda::getCurrentCUDAStream().stream()),
+                 "moe_dispatch (gradient)");
+        if (slot.size(0) > 0 && BINDING == kMirror) ++g_mirror_backward_launches;
+        return {grad_x, at::Tensor(), at::Tensor()};
+    }
+};
+
+template <Binding BINDING>
+at::Tensor MoeDispatch(const at::Tensor& x, const at::Tensor& token_of, const at::Tensor& slot) {
+    check_rows(x, "x", false, token_of, slot);
+    return Dispatch<BINDING>::apply(x, token_of, slot);
+}
+
+template <Binding BINDING>
+struct Combine : torch::autograd::Function<Combine<BINDING>> {
+    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& y, const at::Tensor& weight, const at::Tensor& token_of,
+                              const at::Tensor& slot) {
+        c10::cuda::CUDAGuard guard(y.device());
+        at::Tensor out = at::empty({slot.size(0), y.size(1)}, y.options());
+        raise_on(b200moe_moe_combine(y.data_ptr(), y.scalar_type() == at::kFloat ? 1 : 0, weight.data_ptr<float>(),
+                                     slot.data_ptr<int32_t>(), out.data_ptr(), slot.size(0), slot.size(1), y.size(1),
+                                     c10::cuda::getCurrentCUDAStream().stream()),
+                 "moe_combine");
+        ctx->save_for_backward({y, weight, token_of, slot});
+        return out;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "moe_combine is differentiable once");
+        const bool need_y = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+        if (!grads[0].defined() || (!need_y && !need_w)) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &y = saved[0], &weight = saved[1], &token_of = saved[2], &slot = saved[3], g = grads[0].contiguous();
+        c10::cuda::CUDAGuard guard(y.device());
+        at::Tensor grad_y, grad_w;
+        if (need_y) grad_y = at::empty_like(y);
+        if (need_w) grad_w = at::empty_like(weight);
+        raise_on(b200moe_moe_combine_grad(y.data_ptr(), y.scalar_type() == at::kFloat ? 1 : 0, weight.data_ptr<float>(),
+                                          token_of.data_ptr<int32_t>(), slot.data_ptr<int32_t>(), g.data_ptr(),
+                                          need_y ? grad_y.data_ptr() : nullptr, need_w ? grad_w.data_ptr<float>() : nullptr, slot.size(0),
+                                          slot.size(1), y.size(1), c10::cuda::getCurrentCUDAStream().stream()),
+                 "moe_combine (gradient)");
+        if (slot.size(0) > 0 && BINDING == kMirror) ++g_mirror_backward_launches;
+        return {grad_y, grad_w, at::Tensor(), at::Tensor()};
+    }
+};
+
+template <Binding BINDING>
+at::Tensor MoeCombine(const at::Tensor& y, const at::Tensor& weight, const at::Tensor& token_of, const at::Tensor& slot) {
+    check_rows(y, "y", true, token_of, slot);
+    check_beside(weight, "weight", y);
+    check_f32(weight, "weight", slot.sizes());
+    return Combine<BINDING>::apply(y, weight, token_of, slot);
+}
+
+// ---- rows and experts in 4-bit floats with a scale per 32 -------------------------------------------------------------------
+
+int64_t mxfp4_width(int64_t K) { return 4 * ((K + 127) / 128); }
+void check_bytes(const at::Tensor& t, const char* name, at::IntArrayRef shape) {
+    TORCH_CHECK(t.scalar_type() == at::kByte && t.sizes() == shape, name, " must be uint8 of shape ", shape, ", got ", t.scalar_type(), " ",
+                t.sizes());
+}
+
+// (codes, scale, number of kernels launched)
+std::tuple<at::Tensor, at::Tensor, int> QuantizeRowsMxfp4(const at::Tensor& x, const OptionalTensor& index_opt,
+                                                          const OptionalTensor& codes_opt, const OptionalTensor& scale_opt) {
+    check_tensor(x, "x");
+    TORCH_CHECK(x.dim() == 2 && x.scalar_type() == at::kBFloat16, "x must be bfloat16 [T, K]");
+    const at::Tensor* index = given(index_opt, "index", x);
+    TORCH_CHECK(!index || (index->scalar_type() == at::kInt && index->dim() == 1), "index must be int32 [R]");
+    const int64_t T = x.size(0), K = x.size(1), R = index ? index->numel() : T, W = mxfp4_width(K);
+    c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor* codes_in = given(codes_opt, "codes", x);
+    const at::Tensor* scale_in = given(scale_opt, "scale", x);
+    at::Tensor codes = codes_in ? *codes_in : at::empty({R, K / 2}, x.options().dtype(at::kByte));
+    at::Tensor scale = scale_in ? *scale_in : at::empty({R, W}, x.options().dtype(at::kByte));
+    check_bytes(codes, "codes", {R, K / 2});
+    check_bytes(scale, "scale", {R, W});
+    // scratch from the caching allocator and back to it; without it every row of the result is quantised
+    size_t scratch_bytes = b200moe_mxfp4_quantize_rows_scratch_bytes(T, R, K, index != nullptr);
+    at::Tensor scratch;
+    if (scratch_bytes > 0) {
+        try {
+            scratch = bytes_like(x, scratch_bytes);
+        } catch (const c10::OutOfMemoryError&) {
+            scratch_bytes = 0;
+        }
+    }
+    raise_on(b200moe_mxfp4_quantize_rows(x.data_ptr(), index ? index->data_ptr<int32_t>() : nullptr, codes.data_ptr(),
+                                         scale.data_ptr<uint8_t>(), T, R, K, scratch_bytes > 0 ? scratch.data_ptr() : nullptr,
+                                         scratch_bytes, c10::cuda::getCurrentCUDAStream().stream()),
+             "mxfp4_quantize_rows");
+    return {codes, scale, R == 0 ? 0 : scratch_bytes > 0 ? 2 : 1};
+}
+
+std::tuple<at::Tensor, at::Tensor> Mxfp4QuantizeRows(const at::Tensor& x, const OptionalTensor& index, const OptionalTensor& codes,
+                                                     const OptionalTensor& scale) {
+    const auto out = QuantizeRowsMxfp4(x, index, codes, scale);
+    return {std::get<0>(out), std::get<1>(out)};
+}
+
+// The number of kernels launched.
+template <Binding BINDING>
+int ProductMxfp4(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& weight, const at::Tensor& weight_scale,
+                 const at::Tensor& group_list, const at::Tensor& output, const OptionalTensor& output_scale_opt, int64_t group_list_type,
+                 bool gate_up_silu) {
+    check_tensor(x, "x");
+    check_beside(x_scale, "x_scale", x); check_beside(weight, "weight", x); check_beside(weight_scale, "weight_scale", x);
+    check_beside(group_list, "group_list", x); check_beside(output, "output", x);
+    const at::Tensor* output_scale = given(output_scale_opt, "output_scale", x);
+    TORCH_CHECK(x.scalar_type() == at::kByte && x.dim() == 2, "x must be uint8 [M, K / 2]");
+    TORCH_CHECK(weight.scalar_type() == at::kByte && weight.dim() == 3, "weight must be uint8 [G, N, K / 2]");
+    TORCH_CHECK(group_list.scalar_type() == at::kLong, "group_list must be int64");
+    const int64_t M = x.size(0), K = 2 * x.size(1), G = weight.size(0), N = weight.size(1), W = mxfp4_width(K);
+    TORCH_CHECK(2 * weight.size(2) == K && group_list.numel() == G, "shape mismatch: x ", x.sizes(), ", weight ", weight.sizes(),
+                ", group_list ", group_list.numel());
+    check_bytes(x_scale, "x_scale", {M, W});
+    check_bytes(weight_scale, "weight_scale", {G, N, W});
+    if (gate_up_silu) {
+        TORCH_CHECK(N % 256 == 0, "gate_up_silu needs N to be a multiple of 256");
+        TORCH_CHECK(output_scale, "gate_up_silu needs an output_scale");
+        check_bytes(output, "output", {M, N / 4});
+        check_bytes(*output_scale, "output_scale", {M, N / 64});
+    } else {
+        TORCH_CHECK(output.scalar_type() == at::kBFloat16 && output.dim() == 2 && output.size(0) == M && output.size(1) == N &&
+                    !output_scale, "output must be bfloat16 [", M, ", ", N, "], without output_scale");
+    }
+    TORCH_CHECK(group_list_type == 0 || group_list_type == 1, "group_list_type must be 0 or 1");
+    c10::cuda::CUDAGuard guard(x.device());
+    const size_t bytes = b200moe_grouped_gemm_mxfp4_workspace_bytes(M, K, N, G, gate_up_silu ? 1 : 0);
+    at::Tensor workspace = bytes_like(x, bytes);
+    const auto stream = c10::cuda::getCurrentCUDAStream().stream();
+    raise_on(b200moe_grouped_gemm_mxfp4(x.data_ptr(), x_scale.data_ptr<uint8_t>(), weight.data_ptr(), weight_scale.data_ptr<uint8_t>(),
+                                        group_list.data_ptr<int64_t>(), output.data_ptr(),
+                                        output_scale ? output_scale->data_ptr<uint8_t>() : nullptr, M, K, N, G, (int)group_list_type,
+                                        gate_up_silu ? 1 : 0, workspace.data_ptr(), bytes, findings_for(BINDING, x.get_device(), stream),
+                                        stream),
+             "grouped_gemm_mxfp4");
+    return M == 0 ? 0 : 1;
+}
+
+void GroupedGemmMxfp4(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& weight, const at::Tensor& weight_scale,
+                      const at::Tensor& group_list, const at::Tensor& output, const OptionalTensor& output_scale, int64_t group_list_type,
+                      bool gate_up_silu) {
+    ProductMxfp4<kDropIn>(x, x_scale, weight, weight_scale, group_list, output, output_scale, group_list_type, gate_up_silu);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -592,10 +799,24 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "GROUP GEMM on e4m3 rows and e4m3 weights with scales per block of 128.");
     m.def("moe_balance_loss", &MoeBalanceLoss<kDropIn>, "logits"_a, "idx"_a, "seq_list"_a = pybind11::none(), "token_mask"_a = pybind11::none(),
           "(balance loss per sequence, pairs per sequence and expert), differentiable in the logits.");
+    m.def("moe_sort", &MoeSort, "idx"_a, "n_experts"_a, "(token, j) pairs by expert, stable: (counts, token_of, slot).");
+    m.def("moe_dispatch", &MoeDispatch<kDropIn>, "x"_a, "token_of"_a, "slot"_a, "Rows of the sorted pairs, differentiable in x.");
+    m.def("moe_combine", &MoeCombine<kDropIn>, "y"_a, "weight"_a, "token_of"_a, "slot"_a,
+          "Weighted sum of each token's rows, differentiable in y and weight.");
+    m.def("mxfp4_quantize_rows", &Mxfp4QuantizeRows, "x"_a, "index"_a = pybind11::none(), "codes"_a = pybind11::none(),
+          "scale"_a = pybind11::none(), "bf16 rows -> (e2m1 codes, e8m0 scale per 32), optionally gathered by an index.");
+    m.def("grouped_gemm_mxfp4", &GroupedGemmMxfp4, "x"_a, "x_scale"_a, "weight"_a, "weight_scale"_a, "group_list"_a, "output"_a,
+          "output_scale"_a = pybind11::none(), "group_list_type"_a = 0, "gate_up_silu"_a = false,
+          "GROUP GEMM on e2m1 rows and e2m1 weights with e8m0 scales per 32 k.");
     // the package's functions of the same names: their findings are read by its status calls, their launches counted there
     m.def("_mirror_fp8_quantize_rows", &QuantizeRows);
     m.def("_mirror_grouped_gemm_fp8_block", &ProductFp8Block<kMirror>);
     m.def("_mirror_moe_balance_loss", &MoeBalanceLoss<kMirror>);
+    m.def("_mirror_moe_sort", &SortPairs);
+    m.def("_mirror_moe_dispatch", &MoeDispatch<kMirror>);
+    m.def("_mirror_moe_combine", &MoeCombine<kMirror>);
+    m.def("_mirror_mxfp4_quantize_rows", &QuantizeRowsMxfp4);
+    m.def("_mirror_grouped_gemm_mxfp4", &ProductMxfp4<kMirror>);
     m.def("_mirror_findings", &MirrorFindings);
     m.def("_mirror_backward_launches", []() { return g_mirror_backward_launches.load(); });
     m.def("last_status", [](bool clear) { return LastStatus(clear); }, "clear"_a = false,

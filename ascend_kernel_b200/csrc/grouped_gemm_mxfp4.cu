@@ -1,0 +1,524 @@
+// Grouped GEMM whose two operands are 4-bit floats with one power-of-two scale per 32 k:
+//
+//   y[m, n] = sum_k x[m, k] * w[g, n, k],  both e2m1 with an e8m0 scale per 32 k along their rows
+//
+// Persistent kernel, tcgen05 kind::mxf4: the tensor core multiplies the codes, applies both scales and keeps the sums of the whole k range in
+// fp32.  The operands are swapped: the 128 lanes of an MMA are weight columns, one or two blocks of them to a tile, and its N extent is the
+// tile's token rows rounded up to 16 (16 .. 192), so an expert's weights pass once where it has up to 192 rows.  Codes enter by TMA as they
+// are stored.  Scales are gathered four bytes (128 k of a row) at a time with cp.async into the order that tensor memory wants them in: word
+// w of row r at 512 w + 16 (r % 32) + 4 (r / 32), which tcgen05.cp copies to the four lane quarters.
+//
+// Gate/up: a tile's two blocks are 128 gate columns and the up columns of the same indices; silu(gate) * up in fp32, a warp's 32 columns
+// are a block of the result: its largest magnitude, its scale and codes are the warp's own business.
+//
+// Warp roles: 0 loads codes, 1 issues MMAs, 4 .. 7 load scales, 8 .. 15 epilogue.  Every wait is bounded.
+#include <algorithm>
+
+#include "common.cuh"
+#include "mxfp4.cuh"
+#include "ptx.cuh"
+
+namespace b200moe {
+namespace mf {
+
+constexpr int kWarpLoad = 0, kWarpMma = 1, kWarpScale0 = 4, kScaleWarps = 4, kWarpEpi0 = 8, kEpiWarps = 8;
+constexpr int kThreads = (kWarpEpi0 + kEpiWarps) * 32;
+constexpr int kMaxR = 192;               // token rows of a tile
+constexpr int kBlockBytes = 128 * 128;   // 128 weight columns x 256 k
+constexpr int kSegK = 256;               // k of a segment: 128 bytes of a row
+constexpr int kScaleBytes = 512;         // the scales of 128 rows and 128 k
+constexpr int kMaxSlots = 10, kMaxBufs = 4;
+constexpr uint32_t kTmemCols = 512;
+constexpr int kStripBytes = 1024;        // of an epilogue warp: 16 tokens x 32 columns in bf16
+constexpr int kBigBox = 64, kSmallBox = 16;
+constexpr int kBarrierBytes = 1024;
+constexpr int kSmemBytes = 227 * 1024;
+constexpr int kAhead = 2;                // stages of scales under way
+
+// What a tile is: the number of blocks of 128 weight columns, whether they are gate and up columns, and the segments of a stage.
+template <int HALVES, bool GATE, int SEGS>
+struct Mode {
+    static constexpr int kHalves = HALVES, kSegs = SEGS, kWords = 2 * SEGS;
+    static constexpr bool kGate = GATE;
+    // columns that a tile advances by (gate/up: of each)
+    static constexpr int kTileColumns = GATE ? 128 : 128 * HALVES;
+    static __device__ __forceinline__ int block_step(int N) { return GATE ? N >> 1 : 128; }
+    static constexpr int kFixedBytes = 1024 + kBarrierBytes + kEpiWarps * kStripBytes + 2 * (kMaxExperts + 4) * 4;
+    static constexpr int kRingBytes = kSmemBytes - kFixedBytes;
+    static __host__ __device__ constexpr int scale_blocks(int width) { return (width + 127) / 128; }
+    static __host__ __device__ constexpr int slot_bytes(int width) {
+        return SEGS * (HALVES * kBlockBytes + width * 128) + kWords * kScaleBytes * (HALVES + scale_blocks(width));
+    }
+    // tensor-memory columns of a stage's scales
+    static __host__ __device__ constexpr int scale_columns(int width) { return kWords * 4 * (HALVES + scale_blocks(width)); }
+    static_assert(kRingBytes % 16 == 0 && kRingBytes / slot_bytes(kMaxR) > kAhead, "stages");
+    static_assert((int)kTmemCols - 2 * scale_columns(kMaxR) >= HALVES * kMaxR, "tensor memory");
+};
+
+struct Args {
+    const uint8_t* x_scale;
+    const uint8_t* w_scale;
+    const int64_t* group_list;
+    void* out;
+    uint8_t* out_scale;
+    int M, K, N, G, gl_type;
+    int words;         // of a row of scales
+    int* findings;
+};
+
+struct Sync {
+    uint64_t full[kMaxSlots];    // the bytes of the stage's codes, and the warps that brought its scales
+    uint64_t empty[kMaxSlots];   // commit of the stage's MMAs
+    uint64_t d_full[kMaxBufs];   // commit of a tile's MMAs
+    uint64_t d_empty[kMaxBufs];  // the epilogue warps have the tile's sums
+    uint64_t drain;
+    uint32_t tmem_base;
+    int abort;
+    int n_units, width;          // width: token rows of the widest tile, rounded up to 16
+};
+static_assert(sizeof(Sync) <= kBarrierBytes, "barrier block");
+
+struct Tile {
+    int g, row0, rows, n, nt;  // n: rows rounded up to 16
+};
+
+// Waits are a whole warp's: it votes at every poll and so leaves them together.
+__device__ __forceinline__ bool all(bool v) { return __all_sync(0xffffffffu, v); }
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Sync* sy, int* findings, int id) {
+    const uint32_t b = ptx::smem_u32(bar);
+    uint64_t t0 = 0;
+    for (uint32_t spins = 0; !all(ptx::mbar_try_wait(b, parity)); ++spins) {
+        if ((spins & 0xFF) != 0) continue;
+        if (spins == 0) {
+            t0 = ptx::globaltimer_ns();
+            continue;
+        }
+        bool out = *reinterpret_cast<volatile int*>(&sy->abort) != 0;
+        if (!out && ptx::globaltimer_ns() - t0 > ptx::kWaitLimitNs) {
+            *reinterpret_cast<volatile int*>(&sy->abort) = 1;
+            keep_finding(findings, kDevWaitExpired, id);
+            out = true;
+        }
+        if (!all(!out)) return false;
+    }
+    return true;
+}
+
+// An expert's rows are cut into the fewest tiles, of equal size rounded up to 16.
+__device__ __forceinline__ int tiles_of(int rows) { return (rows + kMaxR - 1) / kMaxR; }
+__device__ __forceinline__ int tile_rows_of(int rows, int tiles) { return ((rows + tiles - 1) / tiles + 15) & ~15; }
+
+// Inside an expert the row tiles of a weight column run together, so that they share the weights in L2.
+__device__ __forceinline__ Tile locate(int unit, const int* prefix, const int* row_start, int G, int n_nt) {
+    int lo = 0, hi = G;  // largest g with prefix[g] <= unit
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (prefix[mid] <= unit) lo = mid;
+        else hi = mid;
+    }
+    const int j = unit - prefix[lo], mt = (prefix[lo + 1] - prefix[lo]) / n_nt;
+    const int nt = j / mt, m = j - nt * mt;
+    const int rows = row_start[lo + 1] - row_start[lo], tr = tile_rows_of(rows, mt);
+    Tile t;
+    t.g = lo;
+    t.nt = nt;
+    t.row0 = row_start[lo] + m * tr;
+    t.rows = min(tr, rows - m * tr);
+    t.n = (t.rows + 15) & ~15;
+    return t;
+}
+
+__device__ __forceinline__ float silu(float g) {
+    const float e = __expf(-fabsf(g));  // (at most 1: nothing overflows)
+    return g * __fdividef(g < 0.f ? e : 1.f, 1.f + e);
+}
+
+// Sixteen tokens x the warp's 32 columns in bf16 through the warp's strip: the transposing store gives 16-byte pieces of eight columns, 64
+// contiguous bytes of a row.
+__device__ __forceinline__ void store_rows(const uint32_t (&d)[2][8], const Tile& t, int token0, int col, uint8_t* strip, const Args& a) {
+    const int lane = threadIdx.x & 31, g8 = lane >> 2, q = lane & 3;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        // lane (g8, q) has columns g8, g8 + 8, .. and tokens 2q, 2q + 1 of each patch of 8
+        uint32_t o[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+            o[m] = pack_bf16x2(__uint_as_float(d[m >> 1][4 * j + 2 * (m & 1)]), __uint_as_float(d[m >> 1][4 * j + 2 * (m & 1) + 1]));
+        const int token = j * 8 + (lane & 7);  // row lane % 8 of piece lane / 8
+        ptx::stmatrix_x4_trans(ptx::smem_u32(strip) + (uint32_t)(token * 64 + (((lane >> 3) ^ (token >> 1)) & 3) * 16), o[0], o[1], o[2], o[3]);
+    }
+    __syncwarp();
+    const bool inside = col + q * 8 < a.N;
+    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (size_t)(t.row0 + token0) * a.N + col + q * 8;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int token = j * 8 + g8;
+        const uint4 v = *reinterpret_cast<const uint4*>(strip + token * 64 + ((q ^ (token >> 1)) & 3) * 16);
+        if (token0 + token < t.rows && inside) *reinterpret_cast<uint4*>(dst + (size_t)token * a.N) = v;
+    }
+    __syncwarp();
+}
+
+// Nibble i of lane j of every eight lanes becomes nibble j of lane i.
+__device__ __forceinline__ uint32_t transpose_nibbles(uint32_t v) {
+    const int lane = threadIdx.x & 31;
+    uint32_t r = __shfl_xor_sync(0xffffffffu, v, 4);
+    v = (lane & 4) ? (v & 0xFFFF0000u) | (r >> 16) : (v & 0x0000FFFFu) | (r << 16);
+    r = __shfl_xor_sync(0xffffffffu, v, 2);
+    v = (lane & 2) ? (v & 0xFF00FF00u) | ((r >> 8) & 0x00FF00FFu) : (v & 0x00FF00FFu) | ((r & 0x00FF00FFu) << 8);
+    r = __shfl_xor_sync(0xffffffffu, v, 1);
+    return (lane & 1) ? (v & 0xF0F0F0F0u) | ((r >> 4) & 0x0F0F0F0Fu) : (v & 0x0F0F0F0Fu) | ((r & 0x0F0F0F0Fu) << 4);
+}
+
+// silu(gate) * up of the lane's column and sixteen tokens, quantised by the warp's 32 columns.
+__device__ __forceinline__ void store_quantized(const uint32_t (&gate)[16], const uint32_t (&up)[16], const Tile& t, int token0, int col,
+                                                const Args& a) {
+    const int lane = threadIdx.x & 31, inter = a.N >> 1;
+    uint32_t mine = 0;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+        float h[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = silu(__uint_as_float(gate[8 * p + i])) * __uint_as_float(up[8 * p + i]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            // magnitudes order as their bits do, infinities and NaN last
+            const uint32_t byte = mxfp4::scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(h[i]) & 0x7FFFFFFFu));
+            h[i] = byte == mxfp4::kNaN ? 0.f : h[i] * mxfp4::inverse(byte);
+            if (lane == 8 * p + i) mine = byte;
+        }
+        const uint32_t codes = transpose_nibbles(mxfp4::codes8(h));  // lane % 8's token, eight columns
+        const int token = token0 + 8 * p + (lane & 7);
+        if (token < t.rows)
+            *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + (size_t)(t.row0 + token) * (inter >> 1) + (col >> 1) + (lane >> 3) * 4) = codes;
+    }
+    if (lane < 16 && token0 + lane < t.rows) a.out_scale[(size_t)(t.row0 + token0 + lane) * (inter >> 5) + (col >> 5)] = (uint8_t)mine;
+}
+
+template <class M>
+__global__ void __launch_bounds__(kThreads, 1)
+    grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x64,
+                   const __grid_constant__ CUtensorMap map_x16, const Args a) {
+    constexpr int kHalves = M::kHalves, kSegs = M::kSegs, kWords = M::kWords;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* ring = smem_raw + ((1024u - (ptx::smem_u32(smem_raw) & 1023u)) & 1023u);
+    Sync* sy = reinterpret_cast<Sync*>(ring + M::kRingBytes);
+    uint8_t* strips = ring + M::kRingBytes + kBarrierBytes;
+    int* row_start = reinterpret_cast<int*>(strips + kEpiWarps * kStripBytes);
+    int* prefix = row_start + kMaxExperts + 4;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n_nt = ((M::kGate ? a.N >> 1 : a.N) + M::kTileColumns - 1) / M::kTileColumns;
+
+    // what needs nothing from memory comes first: the kernel may have started beside the end of the one before it
+    if (threadIdx.x == kThreads - 32) {
+        sy->abort = 0;
+        const auto init = [](uint64_t* b, int n, uint32_t count) {
+            for (int i = 0; i < n; ++i) ptx::mbar_init(ptx::smem_u32(b + i), count);
+        };
+        init(sy->full, kMaxSlots, 1 + kScaleWarps);
+        init(sy->empty, kMaxSlots, 1);
+        init(sy->d_full, kMaxBufs, 1);
+        init(sy->d_empty, kMaxBufs, kEpiWarps);
+        init(&sy->drain, 1, 1);
+        ptx::fence_mbar_init();
+        ptx::prefetch_tensormap(&map_w);
+        ptx::prefetch_tensormap(&map_x64);
+        ptx::prefetch_tensormap(&map_x16);
+    }
+    if (warp == kWarpMma) {
+        ptx::tmem_alloc(ptx::smem_u32(&sy->tmem_base), kTmemCols);
+        ptx::tmem_relinquish();
+    }
+    grid_dep_wait();
+    grid_dep_launch();
+    load_row_starts(a.group_list, a.G, a.M, a.gl_type, row_start, nullptr, blockIdx.x == 0 ? a.findings : nullptr);
+    if (warp == 0) {
+        int lo, hi, mine = 0, total, wide = 0;
+        lane_experts(a.G, lo, hi);
+        for (int g = lo; g < hi; ++g) {
+            const int rows = row_start[g + 1] - row_start[g], mt = tiles_of(rows);
+            mine += mt;
+            if (mt) wide = max(wide, tile_rows_of(rows, mt));
+        }
+        int at = warp_exclusive_sum(mine, total);
+        wide = __reduce_max_sync(0xffffffffu, wide);
+        for (int g = lo; g < hi; ++g) {
+            prefix[g] = at * n_nt;
+            at += tiles_of(row_start[g + 1] - row_start[g]);
+        }
+        if (lane == 0) {
+            prefix[a.G] = total * n_nt;
+            sy->n_units = total * n_nt;
+            sy->width = max(wide, 16);
+        }
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+
+    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sy->tmem_base);
+    const int n_units = sy->n_units, width = sy->width;
+    const int slot_bytes = M::slot_bytes(width), n_slots = min(kMaxSlots, M::kRingBytes / slot_bytes);
+    const int scale_columns = M::scale_columns(width), scale_blocks = M::scale_blocks(width);
+    const int n_bufs = min(kMaxBufs, ((int)kTmemCols - 2 * scale_columns) / (kHalves * width));
+    // of a stage: codes of the weights, of x, scales of the weights, of x
+    const int x_at = kHalves * kSegs * kBlockBytes, ws_at = x_at + kSegs * width * 128, xs_at = ws_at + kHalves * kWords * kScaleBytes;
+    const int segs = (a.K + kSegK - 1) / kSegK, words = a.words, stages = (segs + kSegs - 1) / kSegs;
+
+    if (warp == kWarpLoad) {
+        // ------------------------------ codes ------------------------------
+        // The warp walks together and one lane issues.
+        const bool leader = ptx::elect_one();
+        uint32_t it = 0, slot = 0, ph = 0;
+        bool ok = true;
+        for (int unit = blockIdx.x; ok && unit < n_units; unit += gridDim.x) {
+            const Tile t = locate(unit, prefix, row_start, a.G, n_nt);
+            const int n_big = t.n / kBigBox, n_small = (t.n % kBigBox) / kSmallBox;
+            for (int kb = 0; kb < stages; ++kb, ++it) {
+                if (it >= (uint32_t)n_slots && !wait(&sy->empty[slot], ph ^ 1, sy, a.findings, 10)) { ok = false; break; }
+                if (leader) {
+                    const uint32_t bar = ptx::smem_u32(&sy->full[slot]), dst = ptx::smem_u32(ring) + slot * (uint32_t)slot_bytes;
+                    const int here = min(kSegs, segs - kb * kSegs);
+                    ptx::mbar_arrive_expect_tx(bar, (uint32_t)(here * (kHalves * kBlockBytes + t.n * 128)));
+#pragma unroll
+                    for (int s = 0; s < kSegs; ++s) {
+                        if (s >= here) break;
+                        const int x = (kb * kSegs + s) * 128;
+#pragma unroll
+                        for (int u = 0; u < kHalves; ++u)
+                            ptx::tma_load_3d(dst + (u * kSegs + s) * kBlockBytes, &map_w, bar, x, t.nt * M::kTileColumns + u * M::block_step(a.N), t.g);
+                        uint32_t at = dst + x_at + s * width * 128;
+                        int r = t.row0;
+                        for (int b = 0; b < n_big; ++b, at += kBigBox * 128, r += kBigBox) ptx::tma_load_2d(at, &map_x64, bar, x, r);
+                        for (int b = 0; b < n_small; ++b, at += kSmallBox * 128, r += kSmallBox) ptx::tma_load_2d(at, &map_x16, bar, x, r);
+                    }
+                }
+                __syncwarp();
+                if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
+            }
+        }
+        // the commits that give the last stages back have arrived before the CTA ends
+        for (uint32_t i = it; ok && i < it + (uint32_t)n_slots; ++i) {
+            if (i >= (uint32_t)n_slots) ok = wait(&sy->empty[slot], ph ^ 1, sy, a.findings, 11);
+            if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
+        }
+        if (leader && *reinterpret_cast<volatile int*>(&sy->abort)) {
+            // copies in flight land before the shared memory goes
+            const uint64_t t0 = ptx::globaltimer_ns();
+            while (ptx::globaltimer_ns() - t0 < 10000000ull) {}
+        }
+        __syncwarp();
+    } else if (warp >= kWarpScale0 && warp < kWarpScale0 + kScaleWarps) {
+        // ------------------------------ scales ------------------------------
+        // A warp has the rows 32 q .. 32 q + 31 of every block.
+        const int q = warp - kWarpScale0, row = q * 32 + lane;
+        uint32_t it = 0, slot = 0, ph = 0, done_slot = 0;
+        bool ok = true;
+        const auto give = [&]() {
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->full[done_slot]));
+            if (++done_slot == (uint32_t)n_slots) done_slot = 0;
+        };
+        for (int unit = blockIdx.x; ok && unit < n_units; unit += gridDim.x) {
+            const Tile t = locate(unit, prefix, row_start, a.G, n_nt);
+            const uint8_t* w_src[kHalves];
+            bool w_some[kHalves];
+#pragma unroll
+            for (int u = 0; u < kHalves; ++u) {
+                const int n = t.nt * M::kTileColumns + u * M::block_step(a.N) + row;
+                w_some[u] = n < a.N;
+                w_src[u] = a.w_scale + ((size_t)t.g * a.N + (w_some[u] ? n : 0)) * ((size_t)words * 4);
+            }
+            const uint8_t* x_src[2];
+            bool x_some[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                x_some[b] = b * 128 + row < t.rows;
+                x_src[b] = a.x_scale + (size_t)(t.row0 + (x_some[b] ? b * 128 + row : 0)) * ((size_t)words * 4);
+            }
+            for (int kb = 0; kb < stages; ++kb, ++it) {
+                if (it >= (uint32_t)n_slots && !wait(&sy->empty[slot], ph ^ 1, sy, a.findings, 20)) { ok = false; break; }
+                const uint32_t dst = ptx::smem_u32(ring) + slot * (uint32_t)slot_bytes + (uint32_t)(lane * 16 + q * 4);
+                const int here = min(kWords, words - kb * kWords);
+#pragma unroll
+                for (int w = 0; w < kWords; ++w) {
+                    if (w >= here) break;
+                    const int at = (kb * kWords + w) * 4;
+#pragma unroll
+                    for (int u = 0; u < kHalves; ++u)
+                        ptx::cp_async_4(dst + ws_at + (u * kWords + w) * kScaleBytes, w_src[u] + at, w_some[u]);
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+                        if (b * 128 + q * 32 < t.n) ptx::cp_async_4(dst + xs_at + (w * scale_blocks + b) * kScaleBytes, x_src[b] + at, x_some[b]);
+                }
+                ptx::cp_async_commit();
+                if (it >= (uint32_t)kAhead) {
+                    ptx::cp_async_wait<kAhead>();
+                    give();
+                }
+                if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
+            }
+        }
+        ptx::cp_async_wait<0>();
+        if (ok)
+            for (uint32_t i = min(it, (uint32_t)kAhead); i > 0; --i) give();
+    } else if (warp == kWarpMma) {
+        // ------------------------------ MMA issue ------------------------------
+        const bool leader = ptx::elect_one();
+        uint32_t slot = 0, ph = 0, buf = 0, bph = 0, it = 0, n = 0;
+        bool ok = true;
+        const uint32_t ring0 = ptx::smem_u32(ring), scale0 = tmem_base + kTmemCols - 2 * (uint32_t)scale_columns;
+        const uint64_t d_sw = ptx::umma_desc_sw128(0, 0, 1024), d_scale = ptx::umma_desc_plain(0, 0, 128);
+        for (int unit = blockIdx.x; ok && unit < n_units; unit += gridDim.x, ++n) {
+            const Tile t = locate(unit, prefix, row_start, a.G, n_nt);
+            const uint32_t idesc = ptx::umma_idesc_mxf4(128, t.n), d0 = tmem_base + buf * (uint32_t)(kHalves * width);
+            const int blocks = M::scale_blocks(t.n);
+            // the epilogue has taken what the buffer held
+            if (n >= (uint32_t)n_bufs && !wait(&sy->d_empty[buf], bph ^ 1, sy, a.findings, 30)) { ok = false; break; }
+            for (int kb = 0; kb < stages; ++kb, ++it) {
+                if (!wait(&sy->full[slot], ph, sy, a.findings, 40)) { ok = false; break; }
+                ptx::tc_fence_after();
+                if (leader) {
+                    const uint32_t at = ring0 + slot * (uint32_t)slot_bytes, ws = scale0 + (it & 1) * (uint32_t)scale_columns;
+                    const uint32_t xs = ws + kHalves * kWords * 4;
+                    const int here = min(kWords, words - kb * kWords);
+#pragma unroll
+                    for (int w = 0; w < kWords; ++w) {
+                        if (w >= here) break;
+#pragma unroll
+                        for (int u = 0; u < kHalves; ++u)
+                            ptx::tmem_copy_scales(ws + (u * kWords + w) * 4, d_scale + ((at + ws_at + (u * kWords + w) * kScaleBytes) >> 4));
+                        for (int b = 0; b < blocks; ++b)
+                            ptx::tmem_copy_scales(xs + (w * scale_blocks + b) * 4, d_scale + ((at + xs_at + (w * scale_blocks + b) * kScaleBytes) >> 4));
+                    }
+#pragma unroll
+                    for (int w = 0; w < kWords; ++w) {
+                        if (w >= here) break;
+#pragma unroll
+                        for (int u = 0; u < kHalves; ++u)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const uint32_t step = (uint32_t)(((w & 1) * 2 + h) * 32);  // bytes of 64 k
+                                ptx::umma_mxf4(d0 + u * width, d_sw + ((at + (u * kSegs + (w >> 1)) * kBlockBytes + step) >> 4),
+                                               d_sw + ((at + x_at + (w >> 1) * width * 128 + step) >> 4), idesc | ptx::umma_scale_half(h),
+                                               ws + (u * kWords + w) * 4, xs + w * scale_blocks * 4, (uint32_t)(kb + w + h != 0));
+                            }
+                    }
+                    ptx::umma_commit(ptx::smem_u32(&sy->empty[slot]));
+                    if (kb + 1 == stages) ptx::umma_commit(ptx::smem_u32(&sy->d_full[buf]));
+                }
+                __syncwarp();
+                if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
+            }
+            if (++buf == (uint32_t)n_bufs) { buf = 0; bph ^= 1; }
+        }
+        // every MMA issued here must have completed before tensor and shared memory go
+        if (leader) {
+            ptx::umma_commit(ptx::smem_u32(&sy->drain));
+            (void)ptx::mbar_wait(ptx::smem_u32(&sy->drain), 0);
+        }
+        __syncwarp();
+    } else if (warp >= kWarpEpi0) {
+        // ------------------------------ epilogue ------------------------------
+        const int e = warp - kWarpEpi0, group = e >> 2, quarter = warp & 3;
+        uint8_t* strip = strips + e * kStripBytes;
+        const uint32_t tmem = tmem_base + ((uint32_t)(quarter * 32) << 16);
+        uint32_t buf = 0, ph = 0;
+        for (int unit = blockIdx.x; unit < n_units; unit += gridDim.x) {
+            const Tile t = locate(unit, prefix, row_start, a.G, n_nt);
+            if (!wait(&sy->d_full[buf], ph, sy, a.findings, 50)) break;
+            ptx::tc_fence_after();
+            const uint32_t d0 = tmem + buf * (uint32_t)(kHalves * width);
+            const int col = t.nt * M::kTileColumns + quarter * 32;
+            if constexpr (M::kGate) {
+                for (int c = group; c < t.n / 16; c += 2) {
+                    uint32_t g[16], u[16];
+                    ptx::tmem_ld_32x16(d0 + c * 16, g);
+                    ptx::tmem_ld_32x16(d0 + width + c * 16, u);
+                    ptx::tmem_ld_wait();
+                    store_quantized(g, u, t, c * 16, col, a);
+                }
+            } else {
+                for (int i = group; i < t.n / 16 * kHalves; i += 2) {
+                    const int c = i / kHalves, u = i % kHalves;
+                    uint32_t d[2][8];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) ptx::tmem_ld_16x16(d0 + u * width + c * 16 + ((uint32_t)(h * 16) << 16), d[h]);
+                    ptx::tmem_ld_wait();
+                    store_rows(d, t, c * 16, col + u * 128, strip, a);
+                }
+            }
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->d_empty[buf]));
+            if (++buf == (uint32_t)n_bufs) { buf = 0; ph ^= 1; }
+        }
+    }
+
+    __syncwarp();
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (warp == kWarpMma) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem_base, kTmemCols);
+    }
+}
+
+using Plain = Mode<2, false, 1>;
+using GateUp = Mode<2, true, 1>;
+
+static bool sizes_ok(int64_t M, int64_t K, int64_t N, int64_t G) {
+    constexpr int64_t kMost = 0x3FFFFFFF;  // (products of two sizes stay in 64 bits)
+    return M >= 0 && M <= kMost && K > 0 && K <= kMost && N > 0 && N <= kMost && G > 0 && G <= kMaxExperts;
+}
+constexpr size_t kWorkspaceBytes = 256;
+
+}  // namespace mf
+}  // namespace b200moe
+
+using namespace b200moe;
+
+extern "C" size_t b200moe_grouped_gemm_mxfp4_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, int gate_up_silu) {
+    (void)M; (void)K; (void)N; (void)G; (void)gate_up_silu;
+    return mf::kWorkspaceBytes;
+}
+
+extern "C" int b200moe_grouped_gemm_mxfp4(const void* x, const uint8_t* x_scale, const void* weight, const uint8_t* weight_scale,
+                                          const int64_t* group_list, void* out, uint8_t* out_scale, int64_t M, int64_t K, int64_t N,
+                                          int64_t G, int group_list_type, int gate_up_silu, void* workspace, size_t workspace_bytes,
+                                          int32_t* findings, void* stream) {
+    if (!mf::sizes_ok(M, K, N, G) || (K % 32) != 0 || (N % 16) != 0 || (gate_up_silu && (N % 256) != 0)) return B200MOE_ERR_SHAPE;
+    if (group_list_type != B200MOE_GROUP_LIST_CUMSUM && group_list_type != B200MOE_GROUP_LIST_COUNTS) return B200MOE_ERR_ARGUMENT;
+    if (gate_up_silu != 0 && gate_up_silu != 1) return B200MOE_ERR_ARGUMENT;
+    if (M == 0) return B200MOE_OK;
+    // (unit numbers)
+    if ((M / mf::kMaxR + G) * ((N + 127) / 128) > 0x3FFFFFFLL) return B200MOE_ERR_SHAPE;
+    if (!x || !x_scale || !weight || !weight_scale || !group_list || !out || (gate_up_silu && !out_scale)) return B200MOE_ERR_NULL_POINTER;
+    const auto aligned4 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; };
+    if (!aligned16(x) || !aligned16(weight) || !aligned16(out) || !aligned4(x_scale) || !aligned4(weight_scale) || !aligned4(out_scale))
+        return B200MOE_ERR_ALIGNMENT;
+    if (!workspace || workspace_bytes < b200moe_grouped_gemm_mxfp4_workspace_bytes(M, K, N, G, gate_up_silu)) return B200MOE_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return B200MOE_ERR_ALIGNMENT;
+    mf::Args a = {};
+    a.x_scale = x_scale;
+    a.w_scale = weight_scale;
+    a.group_list = group_list;
+    a.out = out;
+    a.out_scale = out_scale;
+    a.M = (int)M; a.K = (int)K; a.N = (int)N; a.G = (int)G;
+    a.gl_type = group_list_type;
+    a.words = (int)(mxfp4::scale_width(K) / 4);
+    a.findings = findings != nullptr ? findings : findings_words();
+    CUtensorMap map_w, map_x64, map_x16;
+    int rc = make_tensor_map_3d_u8(&map_w, weight, (uint64_t)G, (uint64_t)N, (uint64_t)(K / 2), 128, 128);
+    if (rc == B200MOE_OK) rc = make_tensor_map_2d(&map_x64, x, 1, (uint64_t)M, (uint64_t)(K / 2), mf::kBigBox, 128, true);
+    if (rc == B200MOE_OK) rc = make_tensor_map_2d(&map_x16, x, 1, (uint64_t)M, (uint64_t)(K / 2), mf::kSmallBox, 128, true);
+    if (rc != B200MOE_OK) return rc;
+    const auto kernel = gate_up_silu ? mf::grouped_kernel<mf::GateUp> : mf::grouped_kernel<mf::Plain>;
+    B200MOE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, mf::kSmemBytes));
+    B200MOE_CUDA_TRY(launch_dependent(kernel, (unsigned)sm_count(), mf::kThreads, mf::kSmemBytes, static_cast<cudaStream_t>(stream), map_w,
+                                      map_x64, map_x16, a));
+    return B200MOE_OK;
+}

@@ -319,5 +319,56 @@ __device__ __forceinline__ uint32_t umma_idesc_e4m3_mn_k(int m, int n) {
     return (1u << 4) | (1u << 15) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+// ---- 4-bit floats with scales in tensor memory ---------------------------------------------------
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+// Four bytes global -> shared by the thread itself; zeros where `some` is false (`src` is not read then).
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src, bool some) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)), "r"(some ? 4 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// Shared-memory descriptor without swizzle: cores of 8 rows x 16 bytes, `sbo_bytes` from one to the next along the rows.
+__device__ __forceinline__ uint64_t umma_desc_plain(uint32_t smem_addr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr & 0x3FFFF) >> 4);
+    d |= (uint64_t)((lbo_bytes >> 4) & 0x3FFF) << 16;
+    d |= (uint64_t)((sbo_bytes >> 4) & 0x3FFF) << 32;
+    d |= (uint64_t)1 << 46;
+    return d;
+}
+// 32 rows x 16 bytes of shared memory -> 32 lanes x 4 columns of tensor memory, the same in each quarter of the lanes.  In order with the
+// MMAs that the thread issues.
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// D[tmem] (+)= A * B, both e2m1 (two to a byte, K-major) with an e8m0 scale per 32 k in tensor memory, fp32 sums; 64 k.  Scales: row r of an
+// operand in lane r % 32 of column r / 32, the four bytes of a column for 128 k of which the instruction descriptor names two.
+__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t tmem_sa, uint32_t tmem_sb,
+                                          uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %6, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
+        "}\n" ::"r"(tmem_d),
+        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
+        : "memory");
+}
+// Instruction descriptor, kind::mxf4: A and B e2m1 and K-major, scales e8m0; and the bits that take the lower (0) or the upper (1) two
+// scales of both operands' columns.
+__device__ __forceinline__ uint32_t umma_idesc_mxf4(int m, int n) {
+    return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 7) << 27);
+}
+__device__ __forceinline__ uint32_t umma_scale_half(int h) { return ((uint32_t)(2 * h) << 4) | ((uint32_t)(2 * h) << 29); }
+
 }  // namespace ptx
 }  // namespace b200moe

@@ -584,6 +584,52 @@ def moe_balance_loss(logits, idx, seq_list=None, token_mask=None):
     return out
 
 
+def moe_sort(idx, n_experts: int):
+    """The (token, j) pairs in expert order, stable: ``idx`` int32 [T, k], the experts of each token as any router chose them (an entry outside 0 ..
+    n_experts - 1 is a dropped pair) -> (counts int64 [E], token_of int32 [T * k], slot int32 [T, k]) like those of :func:`moe_route`;
+    token_of is -1 behind the kept pairs, slot -1 for a dropped one."""
+    counts, token_of, slot, launches = _ext()._mirror_moe_sort(idx, n_experts)
+    _count(launches)
+    return counts, token_of, slot
+
+
+def moe_dispatch(x, token_of, slot):
+    """Rows of the sorted pairs, [T * k, H]: rows[slot[t, j]] = x[t], zero where ``token_of`` is -1; differentiable (once) in ``x`` (bf16 or fp32
+    [T, H], H % 8 == 0).  ``token_of`` and ``slot`` are those of one sort (:func:`moe_sort` or :func:`moe_route`)."""
+    rows = _ext()._mirror_moe_dispatch(x, token_of, slot)
+    _count(int(x.shape[0] > 0))
+    return rows
+
+
+def moe_combine(y, weight, token_of, slot):
+    """Weighted sum of each token's rows, [T, H]: out[t] = sum_j weight[t, j] * y[slot[t, j]] over its kept pairs, in fp32, rounded once;
+    differentiable (once) in ``y`` (bf16 or fp32 [T * k, H], H % 8 == 0) and ``weight`` (fp32 [T, k]).  Rows that no pair has get gradient 0, and so
+    do the weights of dropped pairs.  ``token_of`` and ``slot`` as for :func:`moe_dispatch`."""
+    out = _ext()._mirror_moe_combine(y, weight, token_of, slot)
+    _count(int(slot.shape[0] > 0))
+    return out
+
+
+def mxfp4_quantize_rows(x, index=None, codes=None, scale=None):
+    """x bf16 [T, K] -> (codes uint8 [R, K / 2], scale uint8 [R, 4 * ceil(K / 128)]): e2m1, two to a byte (low nibble = even k), with one e8m0
+    scale per 32 elements, the smallest power of two of which 7 reach the block's largest magnitude (at least 2^-100).  ``index`` int32 [R]: row
+    i of the result is row index[i] of x (R = T and row i without it); an index outside x gives zeros.  A block with an infinity or a NaN gets
+    scale 255 (NaN).  K % 32 == 0; the scale bytes behind K / 32 are 0."""
+    codes, scale, launches = _ext()._mirror_mxfp4_quantize_rows(x, index, codes, scale)
+    _count(launches)
+    return codes, scale
+
+
+def grouped_gemm_mxfp4(x, x_scale, weight, weight_scale, group_list, output, output_scale=None, group_list_type: int = 0,
+                       gate_up_silu: bool = False):
+    """Grouped GEMM on e2m1 rows and e2m1 experts, both with one e8m0 scale per 32 k along their rows: x uint8 [M, K / 2] with x_scale
+    [M, W] (:func:`mxfp4_quantize_rows` makes them, W = 4 * ceil(K / 128)), weight uint8 [G, N, K / 2] with weight_scale [G, N, W].  output
+    bf16 [M, N].  ``gate_up_silu``: N = 2I with the gate columns first, output uint8 [M, I / 2] and output_scale [M, I / 32] = silu(gate) * up
+    quantised like :func:`mxfp4_quantize_rows`, which the down projection takes as they are.  K a multiple of 32 and N of 16, with
+    ``gate_up_silu`` N of 256; scale bytes behind K / 32 are not 255."""
+    _count(_ext()._mirror_grouped_gemm_mxfp4(x, x_scale, weight, weight_scale, group_list, output, output_scale, group_list_type, gate_up_silu))
+
+
 def silu_mul_dyn(h, n_rows, out=None):
     """silu_mul over the first ``n_rows[0]`` rows of h (``n_rows``: int64 device tensor)."""
     _need_cuda(h=h, n_rows=n_rows, out=out)

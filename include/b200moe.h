@@ -350,7 +350,62 @@ int b200moe_moe_balance_loss_grad(const void* logits, int logits_fp32, const int
                                   const float* load, const float* inv_tokens, const float* grad_loss, int64_t n_tokens,
                                   int64_t n_experts, int64_t n_seqs, void* grad_logits, void* stream);
 
-/* A finding (code, detail; those of status words 0 and 1) of b200moe_grouped_gemm_fp8_block or b200moe_moe_balance_loss is kept in two
+/* ---- tokens on their way to the experts and back, with gradients ----------------------------------------------------
+ * (No reference counterpart: it ships the experts' products alone.  b200moe_moe_route sorts what it routes itself, in an arbitrary order
+ * inside an expert; these take any router's choice and are what training it needs.) */
+/* The pairs (t, j) in expert order, stable: idx int32 [T, top_k] the experts of each token (an entry outside 0 .. E - 1 is a pair that was
+ * dropped) -> counts int64 [E] (usable as a counts group_list), token_of int32 [T * top_k] the token of each sorted row, -1 behind the kept ones, slot int32 [T,
+ * top_k] the sorted row of each pair, -1 where it was dropped.  E <= 1024, top_k <= 32, T * top_k < 2^30.  scratch: as much as
+ * scratch_bytes says (0 for short calls), aligned to 16 bytes; it belongs to the call until it has completed on the stream. */
+size_t b200moe_moe_sort_scratch_bytes(int64_t n_tokens, int64_t n_experts, int64_t top_k);
+int b200moe_moe_sort(const int32_t* idx, int64_t n_tokens, int64_t n_experts, int64_t top_k, int64_t* counts, int32_t* token_of,
+                     int32_t* slot, void* scratch, size_t scratch_bytes, void* stream);
+/* The rows of the sorted pairs: rows[slot[t, j]] = x[t], rows that no pair has (token_of -1) zero; and the gradient, grad_x[t] = sum_j
+ * grad_rows[slot[t, j]] (fp32 sums in the order of j).  token_of and slot are those of one sort (b200moe_moe_sort or b200moe_moe_route).
+ * x [T, width] and rows [T * top_k, width] bf16, or fp32 with fp32 = 1; width % 8 == 0; aligned to 16 bytes.  An entry of slot outside
+ * the rows counts as dropped. */
+int b200moe_moe_dispatch(const void* x, int fp32, const int32_t* token_of, const int32_t* slot, void* rows, int64_t n_tokens, int64_t top_k,
+                         int64_t width, void* stream);
+int b200moe_moe_dispatch_grad(const void* grad_rows, int fp32, const int32_t* slot, void* grad_x, int64_t n_tokens, int64_t top_k,
+                              int64_t width, void* stream);
+/* The weighted sum of each token's rows: out[t] = sum_j weight[t, j] y[slot[t, j]], dropped pairs left out (fp32 sums in the order of j,
+ * rounded once); and its gradients, grad_y[slot[t, j]] = weight[t, j] grad_out[t] (zero for rows that no pair has) and grad_weight[t, j] = the sum of
+ * grad_out[t] * y[slot[t, j]] in fp32 (0 for a dropped pair); either may be NULL.  y [T * top_k, width] and out [T, width] as above,
+ * weight fp32 [T, top_k]. */
+int b200moe_moe_combine(const void* y, int fp32, const float* weight, const int32_t* slot, void* out, int64_t n_tokens, int64_t top_k,
+                        int64_t width, void* stream);
+int b200moe_moe_combine_grad(const void* y, int fp32, const float* weight, const int32_t* token_of, const int32_t* slot,
+                             const void* grad_out, void* grad_y, float* grad_weight, int64_t n_tokens, int64_t top_k, int64_t width,
+                             void* stream);
+
+/* ---- experts and rows in 4-bit floats, one power-of-two scale per 32 k ------------------------------------------------
+ * (No reference counterpart: its fp4 format is weight-only.)  Rows run along k: codes e2m1 two to a byte, low nibble = even k, [.., K / 2],
+ * scales e8m0 one byte per 32 k, [.., W] with W = 4 * ceil(K / 128): whole words of four, the bytes behind K / 32 unused (never 255; the
+ * quantisation writes 0).  K % 128 == 0 makes that [.., K / 32], the format of b200moe_fp4_dequant. */
+/* Rows of bf16 -> that format.  Row i of the result is row index[i] of x [n_src, K], or row i where index is NULL (then n_rows <= n_src);
+ * an index outside x gives a row of zeros.  Per 32 elements with largest magnitude a:
+ *   2^e the smallest power of two with a <= 7 * 2^e (the nearest code is then 6 at most), e >= -100, scale = e + 127, code = e2m1(x / 2^e),
+ * round to nearest even; a block that holds an infinity or a NaN gets scale 255 (NaN) and codes 0.  K % 32 == 0; x and codes aligned to 16
+ * bytes, scale to 4.  scratch (16-byte aligned, or NULL): with scratch_bytes of it, where that is not 0, a long call quantises every row of x
+ * once and gathers the bytes; without it every row of the result is quantised.  Same bits. */
+size_t b200moe_mxfp4_quantize_rows_scratch_bytes(int64_t n_src, int64_t n_rows, int64_t K, int has_index);
+int b200moe_mxfp4_quantize_rows(const void* x, const int32_t* index, void* codes, uint8_t* scale, int64_t n_src, int64_t n_rows, int64_t K,
+                                void* scratch, size_t scratch_bytes, void* stream);
+
+/* Grouped GEMM on such rows and weights: y[m, n] = sum_k x[m, k] w[g, n, k], x [M, K / 2] with x_scale [M, W], weight [G, N, K / 2] with
+ * weight_scale [G, N, W]; products exact, sums in fp32.  gate_up_silu == 0: out bf16 [M, N], out_scale unused.  gate_up_silu == 1: N = 2 I with
+ * the gate columns first, N % 256 == 0; silu(gate) * up in fp32, quantised as b200moe_mxfp4_quantize_rows does: out [M, I / 2], out_scale
+ * [M, I / 32], which the down projection takes as they are.  K % 32 == 0 and N % 16 == 0; x, weight and out aligned to 16 bytes, the scales
+ * to 4.  Rows of no expert are left as they were.  The workspace belongs to the call until it has completed on the stream, and calls that overlap have one
+ * each; it holds no status words: an invalid group_list (rows were clamped) or an expired wait is kept for b200moe_read_findings, or
+ * where `findings` says. */
+size_t b200moe_grouped_gemm_mxfp4_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, int gate_up_silu);
+int b200moe_grouped_gemm_mxfp4(const void* x, const uint8_t* x_scale, const void* weight, const uint8_t* weight_scale,
+                               const int64_t* group_list, void* out, uint8_t* out_scale, int64_t M, int64_t K, int64_t N, int64_t G,
+                               int group_list_type, int gate_up_silu, void* workspace, size_t workspace_bytes, int32_t* findings,
+                               void* stream);
+
+/* A finding (code, detail; those of status words 0 and 1) of b200moe_grouped_gemm_fp8_block, b200moe_grouped_gemm_mxfp4 or b200moe_moe_balance_loss is kept in two
  * words on the device, which hold the first one until they are cleared.  The `_findings` entries take them (zeroed device memory that
  * outlives the call and its replays); NULL, and the entries without, stand for one pair of a device that all such calls share.
  * b200moe_findings_pair: the address, on the current device, of one of the B200MOE_FINDINGS_PAIRS pairs that the library has, zero at the
