@@ -5,8 +5,8 @@
 // Persistent kernel, tcgen05 kind::mxf4: the tensor core multiplies the codes, applies both scales and keeps the sums of the whole k range in
 // fp32.  The operands are swapped: the 128 lanes of an MMA are weight columns, one or two blocks of them to a tile, and its N extent is the
 // tile's token rows rounded up to 16 (16 .. 192), so an expert's weights pass once where it has up to 192 rows.  Codes enter by TMA as they
-// are stored.  Scales are gathered four bytes (128 k of a row) at a time with cp.async into the order that tensor memory wants them in: word
-// w of row r at 512 w + 16 (r % 32) + 4 (r / 32), which tcgen05.cp copies to the four lane quarters.
+// are stored.  Scales come through registers, 16 bytes (512 k of a row) at a time, into the order that tensor memory wants them in: word (128 k) w
+// of row r at 512 w + 16 (r % 32) + 4 (r / 32), which tcgen05.cp copies to the four lane quarters.
 //
 // Gate/up: a tile's two blocks are 128 gate columns and the up columns of the same indices; silu(gate) * up in fp32, a warp's 32 columns
 // are a block of the result: its largest magnitude, its scale and codes are the warp's own business.
@@ -33,7 +33,6 @@ constexpr int kStripBytes = 1024;        // of an epilogue warp: 16 tokens x 32 
 constexpr int kBigBox = 64, kSmallBox = 16;
 constexpr int kBarrierBytes = 1024;
 constexpr int kSmemBytes = 227 * 1024;
-constexpr int kAhead = 2;                // stages of scales under way
 
 // What a tile is: the number of blocks of 128 weight columns, whether they are gate and up columns, and the segments of a stage.
 template <int HALVES, bool GATE, int SEGS>
@@ -51,7 +50,7 @@ struct Mode {
     }
     // tensor-memory columns of a stage's scales
     static __host__ __device__ constexpr int scale_columns(int width) { return kWords * 4 * (HALVES + scale_blocks(width)); }
-    static_assert(kRingBytes % 16 == 0 && kRingBytes / slot_bytes(kMaxR) > kAhead, "stages");
+    static_assert(kRingBytes % 16 == 0 && kRingBytes / slot_bytes(kMaxR) >= 3, "stages");
     static_assert((int)kTmemCols - 2 * scale_columns(kMaxR) >= HALVES * kMaxR, "tensor memory");
 };
 
@@ -311,59 +310,96 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
     } else if (warp >= kWarpScale0 && warp < kWarpScale0 + kScaleWarps) {
         // ------------------------------ scales ------------------------------
-        // A warp has the rows 32 q .. 32 q + 31 of every block.
-        const int q = warp - kWarpScale0, row = q * 32 + lane;
-        uint32_t it = 0, slot = 0, ph = 0, done_slot = 0;
-        bool ok = true;
-        const auto give = [&]() {
-            ptx::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->full[done_slot]));
-            if (++done_slot == (uint32_t)n_slots) done_slot = 0;
+        // A thread has a row of every block of 128: 16 bytes, 512 k, of each on their way while the two before them are stored.
+        const int q = warp - kWarpScale0, row = q * 32 + lane, chunks = (words + 3) / 4;
+        const bool whole = (words & 3) == 0 && ((reinterpret_cast<uintptr_t>(a.w_scale) | reinterpret_cast<uintptr_t>(a.x_scale)) & 15) == 0;
+        struct Chunk {
+            uint4 v[kHalves + 2];  // of the weights' blocks and the two of x
+            int words;             // 0: the schedule has ended
+            bool last;             // of its tile
         };
-        for (int unit = blockIdx.x; ok && unit < n_units; unit += gridDim.x) {
-            const Tile t = locate(unit, prefix, row_start, a.G, n_nt);
-            const uint8_t* w_src[kHalves];
-            bool w_some[kHalves];
-#pragma unroll
-            for (int u = 0; u < kHalves; ++u) {
-                const int n = t.nt * M::kTileColumns + u * M::block_step(a.N) + row;
-                w_some[u] = n < a.N;
-                w_src[u] = a.w_scale + ((size_t)t.g * a.N + (w_some[u] ? n : 0)) * ((size_t)words * 4);
-            }
-            const uint8_t* x_src[2];
-            bool x_some[2];
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                x_some[b] = b * 128 + row < t.rows;
-                x_src[b] = a.x_scale + (size_t)(t.row0 + (x_some[b] ? b * 128 + row : 0)) * ((size_t)words * 4);
-            }
-            for (int kb = 0; kb < stages; ++kb, ++it) {
-                if (it >= (uint32_t)n_slots && !wait(&sy->empty[slot], ph ^ 1, sy, a.findings, 20)) { ok = false; break; }
-                const uint32_t dst = ptx::smem_u32(ring) + slot * (uint32_t)slot_bytes + (uint32_t)(lane * 16 + q * 4);
-                const int here = min(kWords, words - kb * kWords);
-#pragma unroll
-                for (int w = 0; w < kWords; ++w) {
-                    if (w >= here) break;
-                    const int at = (kb * kWords + w) * 4;
-#pragma unroll
-                    for (int u = 0; u < kHalves; ++u)
-                        ptx::cp_async_4(dst + ws_at + (u * kWords + w) * kScaleBytes, w_src[u] + at, w_some[u]);
-#pragma unroll
-                    for (int b = 0; b < 2; ++b)
-                        if (b * 128 + q * 32 < t.n) ptx::cp_async_4(dst + xs_at + (w * scale_blocks + b) * kScaleBytes, x_src[b] + at, x_some[b]);
+        int unit = (int)blockIdx.x - (int)gridDim.x, at = chunks;
+        const uint32_t* src[kHalves + 2];  // NULL: no row there, zeros
+        const auto fetch = [&](Chunk& c) {
+            if (at == chunks) {
+                unit += (int)gridDim.x;
+                if (unit >= n_units) {
+                    unit -= (int)gridDim.x;
+                    c.words = 0;
+                    return;
                 }
-                ptx::cp_async_commit();
-                if (it >= (uint32_t)kAhead) {
-                    ptx::cp_async_wait<kAhead>();
-                    give();
+                const Tile t = locate(unit, prefix, row_start, a.G, n_nt);
+#pragma unroll
+                for (int u = 0; u < kHalves; ++u) {
+                    const int n = t.nt * M::kTileColumns + u * M::block_step(a.N) + row;
+                    src[u] = n < a.N ? reinterpret_cast<const uint32_t*>(a.w_scale) + ((size_t)t.g * a.N + n) * (size_t)words : nullptr;
                 }
-                if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+                    src[kHalves + b] = b * 128 + row < t.rows
+                                           ? reinterpret_cast<const uint32_t*>(a.x_scale) + (size_t)(t.row0 + b * 128 + row) * (size_t)words
+                                           : nullptr;
+                at = 0;
             }
+            c.words = min(4, words - 4 * at);
+            c.last = at + 1 == chunks;
+#pragma unroll
+            for (int b = 0; b < kHalves + 2; ++b) {
+                const uint32_t* p = src[b] + 4 * at;
+                c.v[b] = make_uint4(0u, 0u, 0u, 0u);
+                if (src[b] != nullptr) {
+                    // (ordinary loads: the kernel ahead may have written either operand's scales)
+                    if (whole) {
+                        c.v[b] = __ldca(reinterpret_cast<const uint4*>(p));
+                    } else {
+                        c.v[b].x = __ldca(p);
+                        if (c.words > 1) c.v[b].y = __ldca(p + 1);
+                        if (c.words > 2) c.v[b].z = __ldca(p + 2);
+                        if (c.words > 3) c.v[b].w = __ldca(p + 3);
+                    }
+                }
+            }
+            ++at;
+        };
+        uint32_t it = 0, slot = 0, ph = 0, stage_word = 0;
+        bool ok = true;
+        const auto put = [&](const Chunk& c) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (i >= c.words || !ok) break;
+                if (stage_word == 0 && it >= (uint32_t)n_slots && !wait(&sy->empty[slot], ph ^ 1, sy, a.findings, 20)) { ok = false; break; }
+                uint8_t* dst = ring + slot * (uint32_t)slot_bytes + lane * 16 + q * 4;
+#pragma unroll
+                for (int b = 0; b < kHalves + 2; ++b) {
+                    const uint32_t v = i == 0 ? c.v[b].x : i == 1 ? c.v[b].y : i == 2 ? c.v[b].z : c.v[b].w;
+                    if (b < kHalves) *reinterpret_cast<uint32_t*>(dst + ws_at + (b * kWords + stage_word) * kScaleBytes) = v;
+                    else if (b - kHalves < scale_blocks)
+                        *reinterpret_cast<uint32_t*>(dst + xs_at + (stage_word * scale_blocks + (b - kHalves)) * kScaleBytes) = v;
+                }
+                if (++stage_word == (uint32_t)kWords || (c.last && i + 1 == c.words)) {
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->full[slot]));
+                    stage_word = 0;
+                    ++it;
+                    if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
+                }
+            }
+        };
+        Chunk c0, c1, c2;
+        fetch(c0);
+        fetch(c1);
+        while (ok) {
+            fetch(c2);
+            if (c0.words == 0) break;
+            put(c0);
+            fetch(c0);
+            if (c1.words == 0) break;
+            put(c1);
+            fetch(c1);
+            if (c2.words == 0) break;
+            put(c2);
         }
-        ptx::cp_async_wait<0>();
-        if (ok)
-            for (uint32_t i = min(it, (uint32_t)kAhead); i > 0; --i) give();
     } else if (warp == kWarpMma) {
         // ------------------------------ MMA issue ------------------------------
         const bool leader = ptx::elect_one();
