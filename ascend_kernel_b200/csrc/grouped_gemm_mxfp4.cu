@@ -127,24 +127,44 @@ __device__ __forceinline__ Tile locate(int unit, const int* prefix, const int* r
     return t;
 }
 
-__device__ __forceinline__ float silu(float g) {
-    const float e = __expf(-fabsf(g));  // (at most 1: nothing overflows)
-    return g * __fdividef(g < 0.f ? e : 1.f, 1.f + e);
+// 2^v and 1 / v; what is below 2^-126 as 0 (the first of these is then added to 1, the second multiplies what it divides)
+__device__ __forceinline__ float exp2_flushed(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float reciprocal_flushed(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+// g / (1 + e^-g); an e^-g that overflows makes it 0, which it is to 2^-120
+__device__ __forceinline__ float silu(float g) { return g * reciprocal_flushed(1.f + exp2_flushed(-1.44269504f * g)); }
+
+// What an epilogue warp works on: its 32 columns from `col` on (tensor-memory lanes) of the tile's sums at `tmem`.
+struct Share {
+    Tile t;
+    uint32_t tmem, width;
+    int group, col;
+    uint64_t* d_empty;
+    uint8_t* strip;
+};
+// The sums are in registers: the buffer goes back.
+__device__ __forceinline__ void release(const Share& e) {
+    ptx::tc_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(ptx::smem_u32(e.d_empty));
 }
 
 // Sixteen tokens x the warp's 32 columns in bf16 through the warp's strip: the transposing store gives 16-byte pieces of eight columns, 64
-// contiguous bytes of a row.
-__device__ __forceinline__ void store_rows(const uint32_t (&d)[2][8], const Tile& t, int token0, int col, uint8_t* strip, const Args& a) {
+// contiguous bytes of a row.  d[4 j + 2 h + i]: columns 16 h + 8 i + g8 and tokens 8 j + 2 q, + 1 of lane (g8, q).
+__device__ __forceinline__ void store_rows(const uint32_t (&d)[8], const Tile& t, int token0, int col, uint8_t* strip, const Args& a) {
     const int lane = threadIdx.x & 31, g8 = lane >> 2, q = lane & 3;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        // lane (g8, q) has columns g8, g8 + 8, .. and tokens 2q, 2q + 1 of each patch of 8
-        uint32_t o[4];
-#pragma unroll
-        for (int m = 0; m < 4; ++m)
-            o[m] = pack_bf16x2(__uint_as_float(d[m >> 1][4 * j + 2 * (m & 1)]), __uint_as_float(d[m >> 1][4 * j + 2 * (m & 1) + 1]));
         const int token = j * 8 + (lane & 7);  // row lane % 8 of piece lane / 8
-        ptx::stmatrix_x4_trans(ptx::smem_u32(strip) + (uint32_t)(token * 64 + (((lane >> 3) ^ (token >> 1)) & 3) * 16), o[0], o[1], o[2], o[3]);
+        ptx::stmatrix_x4_trans(ptx::smem_u32(strip) + (uint32_t)(token * 64 + (((lane >> 3) ^ (token >> 1)) & 3) * 16), d[4 * j], d[4 * j + 1],
+                               d[4 * j + 2], d[4 * j + 3]);
     }
     __syncwarp();
     const bool inside = col + q * 8 < a.N;
@@ -158,6 +178,33 @@ __device__ __forceinline__ void store_rows(const uint32_t (&d)[2][8], const Tile
     __syncwarp();
 }
 
+// Block `group` of the tile's 128 columns in bf16: NC pieces of 16 tokens at most, all in registers before the first is stored.
+template <int NC>
+__device__ __forceinline__ void finish_rows(const Share& e, const Args& a) {
+    const uint32_t td = e.tmem + e.group * e.width;
+    uint32_t v[2][2][8], o[NC][8];
+    const auto fetch = [&](int c, uint32_t(&d)[2][8]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) ptx::tmem_ld_16x16(td + (uint32_t)(c * 16) + ((uint32_t)(h * 16) << 16), d[h]);
+    };
+    fetch(0, v[0]);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        ptx::tmem_ld_wait();
+        if (c + 1 < NC) fetch(c + 1, v[(c + 1) & 1]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const uint32_t(&d)[8] = v[c & 1][m >> 1];
+                o[c][4 * j + m] = pack_bf16x2(__uint_as_float(d[4 * j + 2 * (m & 1)]), __uint_as_float(d[4 * j + 2 * (m & 1) + 1]));
+            }
+    }
+    release(e);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) store_rows(o[c], e.t, c * 16, e.col + e.group * 128, e.strip, a);
+}
+
 // Nibble i of lane j of every eight lanes becomes nibble j of lane i.
 __device__ __forceinline__ uint32_t transpose_nibbles(uint32_t v) {
     const int lane = threadIdx.x & 31;
@@ -169,29 +216,56 @@ __device__ __forceinline__ uint32_t transpose_nibbles(uint32_t v) {
     return (lane & 1) ? (v & 0xF0F0F0F0u) | ((r >> 4) & 0x0F0F0F0Fu) : (v & 0x0F0F0F0Fu) | ((r & 0x0F0F0F0Fu) << 4);
 }
 
-// silu(gate) * up of the lane's column and sixteen tokens, quantised by the warp's 32 columns.
-__device__ __forceinline__ void store_quantized(const uint32_t (&gate)[16], const uint32_t (&up)[16], const Tile& t, int token0, int col,
-                                                const Args& a) {
+// The lane's column of sixteen tokens, quantised by the warp's 32 columns.
+__device__ __forceinline__ void store_quantized(float (&h)[16], const Tile& t, int token0, int col, const Args& a) {
     const int lane = threadIdx.x & 31, inter = a.N >> 1;
-    uint32_t mine = 0;
+    uint32_t top = 0;  // lane i: the largest magnitude of token i (magnitudes order as their bits do, infinities and NaN last)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(h[i]) & 0x7FFFFFFFu);
+        if (lane == i) top = m;
+    }
+    const uint32_t byte = mxfp4::scale_byte(top);
+    const float inv = mxfp4::inverse(byte);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) h[i] *= __shfl_sync(0xffffffffu, inv, i);
+    const uint32_t bad = __ballot_sync(0xffffffffu, byte == mxfp4::kNaN);
+    if (bad != 0) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if ((bad >> i) & 1) h[i] = 0.f;
+    }
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-        float h[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] = silu(__uint_as_float(gate[8 * p + i])) * __uint_as_float(up[8 * p + i]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            // magnitudes order as their bits do, infinities and NaN last
-            const uint32_t byte = mxfp4::scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(h[i]) & 0x7FFFFFFFu));
-            h[i] = byte == mxfp4::kNaN ? 0.f : h[i] * mxfp4::inverse(byte);
-            if (lane == 8 * p + i) mine = byte;
-        }
-        const uint32_t codes = transpose_nibbles(mxfp4::codes8(h));  // lane % 8's token, eight columns
+        const float v[8] = {h[8 * p], h[8 * p + 1], h[8 * p + 2], h[8 * p + 3], h[8 * p + 4], h[8 * p + 5], h[8 * p + 6], h[8 * p + 7]};
+        const uint32_t codes = transpose_nibbles(mxfp4::codes8(v));  // lane % 8's token, eight columns
         const int token = token0 + 8 * p + (lane & 7);
         if (token < t.rows)
             *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + (size_t)(t.row0 + token) * (inter >> 1) + (col >> 1) + (lane >> 3) * 4) = codes;
     }
-    if (lane < 16 && token0 + lane < t.rows) a.out_scale[(size_t)(t.row0 + token0 + lane) * (inter >> 5) + (col >> 5)] = (uint8_t)mine;
+    if (lane < 16 && token0 + lane < t.rows) a.out_scale[(size_t)(t.row0 + token0 + lane) * (inter >> 5) + (col >> 5)] = (uint8_t)byte;
+}
+
+// silu(gate) * up of every other piece of 16 tokens, NC at most, in registers before the first is quantised.
+template <int NC>
+__device__ __forceinline__ void finish_quantized(const Share& e, const Args& a) {
+    uint32_t v[2][2][16];
+    float h[NC][16];
+    const auto fetch = [&](int c, uint32_t(&d)[2][16]) {
+        ptx::tmem_ld_32x16(e.tmem + (uint32_t)((2 * c + e.group) * 16), d[0]);
+        ptx::tmem_ld_32x16(e.tmem + e.width + (uint32_t)((2 * c + e.group) * 16), d[1]);
+    };
+    fetch(0, v[0]);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        ptx::tmem_ld_wait();
+        if (c + 1 < NC) fetch(c + 1, v[(c + 1) & 1]);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) h[c][i] = silu(__uint_as_float(v[c & 1][0][i])) * __uint_as_float(v[c & 1][1][i]);
+    }
+    release(e);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) store_quantized(h[c], e.t, (2 * c + e.group) * 16, e.col, a);
 }
 
 template <class M>
@@ -265,50 +339,111 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int x_at = kHalves * kSegs * kBlockBytes, ws_at = x_at + kSegs * width * 128, xs_at = ws_at + kHalves * kWords * kScaleBytes;
     const int segs = (a.K + kSegK - 1) / kSegK, words = a.words, stages = (segs + kSegs - 1) / kSegs;
 
-    if (warp == kWarpLoad) {
-        // ------------------------------ codes ------------------------------
-        // The warp walks together and one lane issues.
-        const bool leader = ptx::elect_one();
-        uint32_t it = 0, slot = 0, ph = 0;
-        bool ok = true;
-        for (int unit = blockIdx.x; ok && unit < n_units; unit += gridDim.x) {
-            const Tile t = locate(unit, prefix, row_start, a.G, n_nt);
-            const int n_big = t.n / kBigBox, n_small = (t.n % kBigBox) / kSmallBox;
-            for (int kb = 0; kb < stages; ++kb, ++it) {
-                if (it >= (uint32_t)n_slots && !wait(&sy->empty[slot], ph ^ 1, sy, a.findings, 10)) { ok = false; break; }
-                if (leader) {
-                    const uint32_t bar = ptx::smem_u32(&sy->full[slot]), dst = ptx::smem_u32(ring) + slot * (uint32_t)slot_bytes;
-                    const int here = min(kSegs, segs - kb * kSegs);
-                    ptx::mbar_arrive_expect_tx(bar, (uint32_t)(here * (kHalves * kBlockBytes + t.n * 128)));
-#pragma unroll
-                    for (int s = 0; s < kSegs; ++s) {
-                        if (s >= here) break;
-                        const int x = (kb * kSegs + s) * 128;
-#pragma unroll
-                        for (int u = 0; u < kHalves; ++u)
-                            ptx::tma_load_3d(dst + (u * kSegs + s) * kBlockBytes, &map_w, bar, x, t.nt * M::kTileColumns + u * M::block_step(a.N), t.g);
-                        uint32_t at = dst + x_at + s * width * 128;
-                        int r = t.row0;
-                        for (int b = 0; b < n_big; ++b, at += kBigBox * 128, r += kBigBox) ptx::tma_load_2d(at, &map_x64, bar, x, r);
-                        for (int b = 0; b < n_small; ++b, at += kSmallBox * 128, r += kSmallBox) ptx::tma_load_2d(at, &map_x16, bar, x, r);
+    // registers of a lane: 56, 88 and twice 184 for the four warps of each kind, together as many as the launch has
+    if (warp < kWarpScale0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == kWarpLoad) {
+            // ------------------------------ codes ------------------------------
+            // The warp walks together and one lane issues.
+            const bool leader = ptx::elect_one();
+            uint32_t it = 0, slot = 0, ph = 0;
+            bool ok = true;
+            for (int unit = blockIdx.x; ok && unit < n_units; unit += gridDim.x) {
+                const Tile t = locate(unit, prefix, row_start, a.G, n_nt);
+                const int n_big = t.n / kBigBox, n_small = (t.n % kBigBox) / kSmallBox;
+                for (int kb = 0; kb < stages; ++kb, ++it) {
+                    if (it >= (uint32_t)n_slots && !wait(&sy->empty[slot], ph ^ 1, sy, a.findings, 10)) { ok = false; break; }
+                    if (leader) {
+                        const uint32_t bar = ptx::smem_u32(&sy->full[slot]), dst = ptx::smem_u32(ring) + slot * (uint32_t)slot_bytes;
+                        const int here = min(kSegs, segs - kb * kSegs);
+                        ptx::mbar_arrive_expect_tx(bar, (uint32_t)(here * (kHalves * kBlockBytes + t.n * 128)));
+    #pragma unroll
+                        for (int s = 0; s < kSegs; ++s) {
+                            if (s >= here) break;
+                            const int x = (kb * kSegs + s) * 128;
+    #pragma unroll
+                            for (int u = 0; u < kHalves; ++u)
+                                ptx::tma_load_3d(dst + (u * kSegs + s) * kBlockBytes, &map_w, bar, x, t.nt * M::kTileColumns + u * M::block_step(a.N), t.g);
+                            uint32_t at = dst + x_at + s * width * 128;
+                            int r = t.row0;
+                            for (int b = 0; b < n_big; ++b, at += kBigBox * 128, r += kBigBox) ptx::tma_load_2d(at, &map_x64, bar, x, r);
+                            for (int b = 0; b < n_small; ++b, at += kSmallBox * 128, r += kSmallBox) ptx::tma_load_2d(at, &map_x16, bar, x, r);
+                        }
                     }
+                    __syncwarp();
+                    if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
                 }
-                __syncwarp();
+            }
+            // the commits that give the last stages back have arrived before the CTA ends
+            for (uint32_t i = it; ok && i < it + (uint32_t)n_slots; ++i) {
+                if (i >= (uint32_t)n_slots) ok = wait(&sy->empty[slot], ph ^ 1, sy, a.findings, 11);
                 if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
             }
+            if (leader && *reinterpret_cast<volatile int*>(&sy->abort)) {
+                // copies in flight land before the shared memory goes
+                const uint64_t t0 = ptx::globaltimer_ns();
+                while (ptx::globaltimer_ns() - t0 < 10000000ull) {}
+            }
+            __syncwarp();
+        } else if (warp == kWarpMma) {
+            // ------------------------------ MMA issue ------------------------------
+            const bool leader = ptx::elect_one();
+            uint32_t slot = 0, ph = 0, buf = 0, bph = 0, it = 0, n = 0;
+            bool ok = true;
+            const uint32_t ring0 = ptx::smem_u32(ring), scale0 = tmem_base + kTmemCols - 2 * (uint32_t)scale_columns;
+            const uint64_t d_sw = ptx::umma_desc_sw128(0, 0, 1024), d_scale = ptx::umma_desc_plain(0, 0, 128);
+            for (int unit = blockIdx.x; ok && unit < n_units; unit += gridDim.x, ++n) {
+                const Tile t = locate(unit, prefix, row_start, a.G, n_nt);
+                const uint32_t idesc = ptx::umma_idesc_mxf4(128, t.n), d0 = tmem_base + buf * (uint32_t)(kHalves * width);
+                const int blocks = M::scale_blocks(t.n);
+                // the epilogue has taken what the buffer held
+                if (n >= (uint32_t)n_bufs && !wait(&sy->d_empty[buf], bph ^ 1, sy, a.findings, 30)) { ok = false; break; }
+                for (int kb = 0; kb < stages; ++kb, ++it) {
+                    if (!wait(&sy->full[slot], ph, sy, a.findings, 40)) { ok = false; break; }
+                    ptx::tc_fence_after();
+                    if (leader) {
+                        const uint32_t at = ring0 + slot * (uint32_t)slot_bytes, ws = scale0 + (it & 1) * (uint32_t)scale_columns;
+                        const uint32_t xs = ws + kHalves * kWords * 4;
+                        const int here = min(kWords, words - kb * kWords);
+    #pragma unroll
+                        for (int w = 0; w < kWords; ++w) {
+                            if (w >= here) break;
+    #pragma unroll
+                            for (int u = 0; u < kHalves; ++u)
+                                ptx::tmem_copy_scales(ws + (u * kWords + w) * 4, d_scale + ((at + ws_at + (u * kWords + w) * kScaleBytes) >> 4));
+                            for (int b = 0; b < blocks; ++b)
+                                ptx::tmem_copy_scales(xs + (w * scale_blocks + b) * 4, d_scale + ((at + xs_at + (w * scale_blocks + b) * kScaleBytes) >> 4));
+                        }
+    #pragma unroll
+                        for (int w = 0; w < kWords; ++w) {
+                            if (w >= here) break;
+    #pragma unroll
+                            for (int u = 0; u < kHalves; ++u)
+    #pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const uint32_t step = (uint32_t)(((w & 1) * 2 + h) * 32);  // bytes of 64 k
+                                    ptx::umma_mxf4(d0 + u * width, d_sw + ((at + (u * kSegs + (w >> 1)) * kBlockBytes + step) >> 4),
+                                                   d_sw + ((at + x_at + (w >> 1) * width * 128 + step) >> 4), idesc | ptx::umma_scale_half(h),
+                                                   ws + (u * kWords + w) * 4, xs + w * scale_blocks * 4, (uint32_t)(kb + w + h != 0));
+                                }
+                        }
+                        ptx::umma_commit(ptx::smem_u32(&sy->empty[slot]));
+                        if (kb + 1 == stages) ptx::umma_commit(ptx::smem_u32(&sy->d_full[buf]));
+                    }
+                    __syncwarp();
+                    if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
+                }
+                if (++buf == (uint32_t)n_bufs) { buf = 0; bph ^= 1; }
+            }
+            // every MMA issued here must have completed before tensor and shared memory go
+            if (leader) {
+                ptx::umma_commit(ptx::smem_u32(&sy->drain));
+                (void)ptx::mbar_wait(ptx::smem_u32(&sy->drain), 0);
+            }
+            __syncwarp();
         }
-        // the commits that give the last stages back have arrived before the CTA ends
-        for (uint32_t i = it; ok && i < it + (uint32_t)n_slots; ++i) {
-            if (i >= (uint32_t)n_slots) ok = wait(&sy->empty[slot], ph ^ 1, sy, a.findings, 11);
-            if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
-        }
-        if (leader && *reinterpret_cast<volatile int*>(&sy->abort)) {
-            // copies in flight land before the shared memory goes
-            const uint64_t t0 = ptx::globaltimer_ns();
-            while (ptx::globaltimer_ns() - t0 < 10000000ull) {}
-        }
-        __syncwarp();
-    } else if (warp >= kWarpScale0 && warp < kWarpScale0 + kScaleWarps) {
+    } else if (warp < kWarpEpi0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         // ------------------------------ scales ------------------------------
         // A thread has a row of every block of 128: 16 bytes, 512 k, of each on their way while the two before them are stored.
         const int q = warp - kWarpScale0, row = q * 32 + lane, chunks = (words + 3) / 4;
@@ -400,95 +535,42 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (c2.words == 0) break;
             put(c2);
         }
-    } else if (warp == kWarpMma) {
-        // ------------------------------ MMA issue ------------------------------
-        const bool leader = ptx::elect_one();
-        uint32_t slot = 0, ph = 0, buf = 0, bph = 0, it = 0, n = 0;
-        bool ok = true;
-        const uint32_t ring0 = ptx::smem_u32(ring), scale0 = tmem_base + kTmemCols - 2 * (uint32_t)scale_columns;
-        const uint64_t d_sw = ptx::umma_desc_sw128(0, 0, 1024), d_scale = ptx::umma_desc_plain(0, 0, 128);
-        for (int unit = blockIdx.x; ok && unit < n_units; unit += gridDim.x, ++n) {
-            const Tile t = locate(unit, prefix, row_start, a.G, n_nt);
-            const uint32_t idesc = ptx::umma_idesc_mxf4(128, t.n), d0 = tmem_base + buf * (uint32_t)(kHalves * width);
-            const int blocks = M::scale_blocks(t.n);
-            // the epilogue has taken what the buffer held
-            if (n >= (uint32_t)n_bufs && !wait(&sy->d_empty[buf], bph ^ 1, sy, a.findings, 30)) { ok = false; break; }
-            for (int kb = 0; kb < stages; ++kb, ++it) {
-                if (!wait(&sy->full[slot], ph, sy, a.findings, 40)) { ok = false; break; }
-                ptx::tc_fence_after();
-                if (leader) {
-                    const uint32_t at = ring0 + slot * (uint32_t)slot_bytes, ws = scale0 + (it & 1) * (uint32_t)scale_columns;
-                    const uint32_t xs = ws + kHalves * kWords * 4;
-                    const int here = min(kWords, words - kb * kWords);
-#pragma unroll
-                    for (int w = 0; w < kWords; ++w) {
-                        if (w >= here) break;
-#pragma unroll
-                        for (int u = 0; u < kHalves; ++u)
-                            ptx::tmem_copy_scales(ws + (u * kWords + w) * 4, d_scale + ((at + ws_at + (u * kWords + w) * kScaleBytes) >> 4));
-                        for (int b = 0; b < blocks; ++b)
-                            ptx::tmem_copy_scales(xs + (w * scale_blocks + b) * 4, d_scale + ((at + xs_at + (w * scale_blocks + b) * kScaleBytes) >> 4));
-                    }
-#pragma unroll
-                    for (int w = 0; w < kWords; ++w) {
-                        if (w >= here) break;
-#pragma unroll
-                        for (int u = 0; u < kHalves; ++u)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const uint32_t step = (uint32_t)(((w & 1) * 2 + h) * 32);  // bytes of 64 k
-                                ptx::umma_mxf4(d0 + u * width, d_sw + ((at + (u * kSegs + (w >> 1)) * kBlockBytes + step) >> 4),
-                                               d_sw + ((at + x_at + (w >> 1) * width * 128 + step) >> 4), idesc | ptx::umma_scale_half(h),
-                                               ws + (u * kWords + w) * 4, xs + w * scale_blocks * 4, (uint32_t)(kb + w + h != 0));
-                            }
-                    }
-                    ptx::umma_commit(ptx::smem_u32(&sy->empty[slot]));
-                    if (kb + 1 == stages) ptx::umma_commit(ptx::smem_u32(&sy->d_full[buf]));
-                }
-                __syncwarp();
-                if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
-            }
-            if (++buf == (uint32_t)n_bufs) { buf = 0; bph ^= 1; }
-        }
-        // every MMA issued here must have completed before tensor and shared memory go
-        if (leader) {
-            ptx::umma_commit(ptx::smem_u32(&sy->drain));
-            (void)ptx::mbar_wait(ptx::smem_u32(&sy->drain), 0);
-        }
-        __syncwarp();
-    } else if (warp >= kWarpEpi0) {
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
         // ------------------------------ epilogue ------------------------------
-        const int e = warp - kWarpEpi0, group = e >> 2, quarter = warp & 3;
-        uint8_t* strip = strips + e * kStripBytes;
-        const uint32_t tmem = tmem_base + ((uint32_t)(quarter * 32) << 16);
+        Share e;
+        e.group = (warp - kWarpEpi0) >> 2;
+        e.strip = strips + (warp - kWarpEpi0) * kStripBytes;
+        e.width = (uint32_t)width;
+        const int quarter = warp & 3;
         uint32_t buf = 0, ph = 0;
         for (int unit = blockIdx.x; unit < n_units; unit += gridDim.x) {
-            const Tile t = locate(unit, prefix, row_start, a.G, n_nt);
+            e.t = locate(unit, prefix, row_start, a.G, n_nt);
+            e.tmem = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * (uint32_t)(kHalves * width);
+            e.col = e.t.nt * M::kTileColumns + quarter * 32;
+            e.d_empty = &sy->d_empty[buf];
             if (!wait(&sy->d_full[buf], ph, sy, a.findings, 50)) break;
             ptx::tc_fence_after();
-            const uint32_t d0 = tmem + buf * (uint32_t)(kHalves * width);
-            const int col = t.nt * M::kTileColumns + quarter * 32;
+            // (the number of pieces is a constant, so that they stay in registers)
             if constexpr (M::kGate) {
-                for (int c = group; c < t.n / 16; c += 2) {
-                    uint32_t g[16], u[16];
-                    ptx::tmem_ld_32x16(d0 + c * 16, g);
-                    ptx::tmem_ld_32x16(d0 + width + c * 16, u);
-                    ptx::tmem_ld_wait();
-                    store_quantized(g, u, t, c * 16, col, a);
+                switch ((e.t.n + 31) / 32) {
+                    case 1: finish_quantized<1>(e, a); break;
+                    case 2: finish_quantized<2>(e, a); break;
+                    case 3: finish_quantized<3>(e, a); break;
+                    case 4: finish_quantized<4>(e, a); break;
+                    case 5: finish_quantized<5>(e, a); break;
+                    default: finish_quantized<6>(e, a); break;
                 }
             } else {
-                for (int i = group; i < t.n / 16 * kHalves; i += 2) {
-                    const int c = i / kHalves, u = i % kHalves;
-                    uint32_t d[2][8];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) ptx::tmem_ld_16x16(d0 + u * width + c * 16 + ((uint32_t)(h * 16) << 16), d[h]);
-                    ptx::tmem_ld_wait();
-                    store_rows(d, t, c * 16, col + u * 128, strip, a);
+                switch ((e.t.n + 31) / 32) {
+                    case 1: finish_rows<2>(e, a); break;
+                    case 2: finish_rows<4>(e, a); break;
+                    case 3: finish_rows<6>(e, a); break;
+                    case 4: finish_rows<8>(e, a); break;
+                    case 5: finish_rows<10>(e, a); break;
+                    default: finish_rows<12>(e, a); break;
                 }
             }
-            ptx::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->d_empty[buf]));
             if (++buf == (uint32_t)n_bufs) { buf = 0; ph ^= 1; }
         }
     }
