@@ -5,13 +5,12 @@
 // Persistent kernel, tcgen05 kind::mxf4: the tensor core multiplies the codes, applies both scales and keeps the sums of the whole k range in
 // fp32.  The operands are swapped: the 128 lanes of an MMA are weight columns, one or two blocks of them to a tile, and its N extent is the
 // tile's token rows rounded up to 16 (16 .. 192), so an expert's weights pass once where it has up to 192 rows.  Codes enter by TMA as they
-// are stored.  Scales come through registers, 16 bytes (512 k of a row) at a time, into the order that tensor memory wants them in: word (128 k) w
-// of row r at 512 w + 16 (r % 32) + 4 (r / 32), which tcgen05.cp copies to the four lane quarters.
+// are stored.  Scales come through registers, 16 bytes (512 k of a row) at a time, and are written to tensor memory by the warps that fetch them.
 //
 // Gate/up: a tile's two blocks are 128 gate columns and the up columns of the same indices; silu(gate) * up in fp32, a warp's 32 columns
 // are a block of the result: its largest magnitude, its scale and codes are the warp's own business.
 //
-// Warp roles: 0 loads codes, 1 issues MMAs, 4 .. 7 load scales, 8 .. 15 epilogue.  Every wait is bounded.
+// Warp roles: 0 loads codes, 1 and 2 issue the MMAs of a block of columns each, 4 .. 7 bring scales, 8 .. 15 epilogue.  Every wait is bounded.
 #include <algorithm>
 
 #include "common.cuh"
@@ -21,37 +20,37 @@
 namespace b200moe {
 namespace mf {
 
-constexpr int kWarpLoad = 0, kWarpMma = 1, kWarpScale0 = 4, kScaleWarps = 4, kWarpEpi0 = 8, kEpiWarps = 8;
+constexpr int kWarpLoad = 0, kWarpMma0 = 1, kWarpScale0 = 4, kScaleWarps = 4, kWarpEpi0 = 8, kEpiWarps = 8;
 constexpr int kThreads = (kWarpEpi0 + kEpiWarps) * 32;
 constexpr int kMaxR = 192;               // token rows of a tile
 constexpr int kBlockBytes = 128 * 128;   // 128 weight columns x 256 k
 constexpr int kSegK = 256;               // k of a segment: 128 bytes of a row
-constexpr int kScaleBytes = 512;         // the scales of 128 rows and 128 k
+constexpr int kChunkWords = 4;           // of scales: 16 bytes, 512 k of a row
 constexpr int kMaxSlots = 10, kMaxBufs = 4;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kStripBytes = 1024;        // of an epilogue warp: 16 tokens x 32 columns in bf16
 constexpr int kBigBox = 64, kSmallBox = 16;
+constexpr int kScaleRows = 2 * 128 + kMaxR;
+constexpr int kExchangeBytes = 2 * kScaleRows * 16;
 constexpr int kBarrierBytes = 1024;
 constexpr int kSmemBytes = 227 * 1024;
 
 // What a tile is: the number of blocks of 128 weight columns, whether they are gate and up columns, and the segments of a stage.
 template <int HALVES, bool GATE, int SEGS>
 struct Mode {
-    static constexpr int kHalves = HALVES, kSegs = SEGS, kWords = 2 * SEGS;
+    static constexpr int kHalves = HALVES, kSegs = SEGS, kWords = 2 * SEGS;  // (a word of scales: 128 k)
     static constexpr bool kGate = GATE;
     // columns that a tile advances by (gate/up: of each)
     static constexpr int kTileColumns = GATE ? 128 : 128 * HALVES;
     static __device__ __forceinline__ int block_step(int N) { return GATE ? N >> 1 : 128; }
-    static constexpr int kFixedBytes = 1024 + kBarrierBytes + kEpiWarps * kStripBytes + 2 * (kMaxExperts + 4) * 4;
+    static constexpr int kFixedBytes = 1024 + kBarrierBytes + kEpiWarps * kStripBytes + kExchangeBytes + 2 * (kMaxExperts + 4) * 4;
     static constexpr int kRingBytes = kSmemBytes - kFixedBytes;
-    static __host__ __device__ constexpr int scale_blocks(int width) { return (width + 127) / 128; }
-    static __host__ __device__ constexpr int slot_bytes(int width) {
-        return SEGS * (HALVES * kBlockBytes + width * 128) + kWords * kScaleBytes * (HALVES + scale_blocks(width));
-    }
-    // tensor-memory columns of a stage's scales
-    static __host__ __device__ constexpr int scale_columns(int width) { return kWords * 4 * (HALVES + scale_blocks(width)); }
+    static __host__ __device__ constexpr int slot_bytes(int width) { return SEGS * (HALVES * kBlockBytes + width * 128); }
+    // tensor-memory columns of a chunk of scales
+    static constexpr int kScaleColumns = kChunkWords * 4 * (HALVES + 2);
     static_assert(kRingBytes % 16 == 0 && kRingBytes / slot_bytes(kMaxR) >= 3, "stages");
-    static_assert((int)kTmemCols - 2 * scale_columns(kMaxR) >= HALVES * kMaxR, "tensor memory");
+    static_assert(HALVES * kMaxR + 2 * kScaleColumns <= (int)kTmemCols, "tensor memory");
+    static_assert(kChunkWords % kWords == 0 || kWords % kChunkWords == 0, "chunks");
 };
 
 struct Args {
@@ -66,11 +65,14 @@ struct Args {
 };
 
 struct Sync {
-    uint64_t full[kMaxSlots];    // the bytes of the stage's codes, and the warps that brought its scales
-    uint64_t empty[kMaxSlots];   // commit of the stage's MMAs
-    uint64_t d_full[kMaxBufs];   // commit of a tile's MMAs
+    uint64_t full[kMaxSlots];    // the bytes of the stage's codes
+    uint64_t empty[kMaxSlots];   // commits of the stage's MMAs, one for each block of columns
+    uint64_t s_full[2];          // the scale warps have written their lanes' copy of a chunk
+    uint64_t s_empty[2];         // commits of its last MMAs
+    uint64_t exchange;           // the scale warps among themselves
+    uint64_t d_full[kMaxBufs];   // commits of a tile's MMAs
     uint64_t d_empty[kMaxBufs];  // the epilogue warps have the tile's sums
-    uint64_t drain;
+    uint64_t drain[2];
     uint32_t tmem_base;
     int abort;
     int n_units, width;          // width: token rows of the widest tile, rounded up to 16
@@ -83,6 +85,8 @@ struct Tile {
 
 // Waits are a whole warp's: it votes at every poll and so leaves them together.
 __device__ __forceinline__ bool all(bool v) { return __all_sync(0xffffffffu, v); }
+// A value that every lane has, in a form that shows it.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Sync* sy, int* findings, int id) {
     const uint32_t b = ptx::smem_u32(bar);
     uint64_t t0 = 0;
@@ -277,10 +281,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* ring = smem_raw + ((1024u - (ptx::smem_u32(smem_raw) & 1023u)) & 1023u);
     Sync* sy = reinterpret_cast<Sync*>(ring + M::kRingBytes);
     uint8_t* strips = ring + M::kRingBytes + kBarrierBytes;
-    int* row_start = reinterpret_cast<int*>(strips + kEpiWarps * kStripBytes);
+    uint8_t* exchange = strips + kEpiWarps * kStripBytes;
+    int* row_start = reinterpret_cast<int*>(exchange + kExchangeBytes);
     int* prefix = row_start + kMaxExperts + 4;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int n_nt = ((M::kGate ? a.N >> 1 : a.N) + M::kTileColumns - 1) / M::kTileColumns;
 
     // what needs nothing from memory comes first: the kernel may have started beside the end of the one before it
@@ -289,17 +294,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         const auto init = [](uint64_t* b, int n, uint32_t count) {
             for (int i = 0; i < n; ++i) ptx::mbar_init(ptx::smem_u32(b + i), count);
         };
-        init(sy->full, kMaxSlots, 1 + kScaleWarps);
-        init(sy->empty, kMaxSlots, 1);
-        init(sy->d_full, kMaxBufs, 1);
+        init(sy->full, kMaxSlots, 1);
+        init(sy->empty, kMaxSlots, kHalves);
+        init(sy->s_full, 2, kScaleWarps);
+        init(sy->s_empty, 2, kHalves);
+        init(&sy->exchange, 1, kScaleWarps);
+        init(sy->d_full, kMaxBufs, kHalves);
         init(sy->d_empty, kMaxBufs, kEpiWarps);
-        init(&sy->drain, 1, 1);
+        init(sy->drain, 2, 1);
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&map_w);
         ptx::prefetch_tensormap(&map_x64);
         ptx::prefetch_tensormap(&map_x16);
     }
-    if (warp == kWarpMma) {
+    if (warp == kWarpMma0) {
         ptx::tmem_alloc(ptx::smem_u32(&sy->tmem_base), kTmemCols);
         ptx::tmem_relinquish();
     }
@@ -330,18 +338,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     ptx::tc_fence_after();
 
-    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sy->tmem_base);
-    const int n_units = sy->n_units, width = sy->width;
+    const uint32_t tmem_base = (uint32_t)uniform((int)*reinterpret_cast<volatile uint32_t*>(&sy->tmem_base));
+    const int n_units = uniform(sy->n_units), width = uniform(sy->width);
     const int slot_bytes = M::slot_bytes(width), n_slots = min(kMaxSlots, M::kRingBytes / slot_bytes);
-    const int scale_columns = M::scale_columns(width), scale_blocks = M::scale_blocks(width);
-    const int n_bufs = min(kMaxBufs, ((int)kTmemCols - 2 * scale_columns) / (kHalves * width));
-    // of a stage: codes of the weights, of x, scales of the weights, of x
-    const int x_at = kHalves * kSegs * kBlockBytes, ws_at = x_at + kSegs * width * 128, xs_at = ws_at + kHalves * kWords * kScaleBytes;
+    // tensor memory: the sums of one to four tiles from the start, two chunks of scales at the end
+    constexpr int kScaleColumns = M::kScaleColumns, kXScaleAt = kChunkWords * 4 * kHalves;
+    const int n_bufs = min(kMaxBufs, ((int)kTmemCols - 2 * kScaleColumns) / (kHalves * width));
+    const uint32_t scale0 = tmem_base + kTmemCols - 2 * kScaleColumns;
+    const int x_at = kHalves * kSegs * kBlockBytes;  // of a stage: the codes of the weights, then those of x
     const int segs = (a.K + kSegK - 1) / kSegK, words = a.words, stages = (segs + kSegs - 1) / kSegs;
 
-    // registers of a lane: 56, 88 and twice 184 for the four warps of each kind, together as many as the launch has
+    // registers of a lane: 72, 120 and twice 160 for the four warps of each kind, together as many as the launch has
     if (warp < kWarpScale0) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == kWarpLoad) {
             // ------------------------------ codes ------------------------------
             // The warp walks together and one lane issues.
@@ -385,85 +394,92 @@ __global__ void __launch_bounds__(kThreads, 1)
                 while (ptx::globaltimer_ns() - t0 < 10000000ull) {}
             }
             __syncwarp();
-        } else if (warp == kWarpMma) {
+        } else if (warp < kWarpMma0 + kHalves) {
             // ------------------------------ MMA issue ------------------------------
+            // A warp for each block of columns: it walks together and one lane issues.  Of the descriptors only the address, in the low
+            // word, changes.
+            const int u = warp - kWarpMma0;
             const bool leader = ptx::elect_one();
-            uint32_t slot = 0, ph = 0, buf = 0, bph = 0, it = 0, n = 0;
+            uint32_t slot = 0, ph = 0, buf = 0, bph = 0, n = 0, cb = 0, cph = 0;
             bool ok = true;
-            const uint32_t ring0 = ptx::smem_u32(ring), scale0 = tmem_base + kTmemCols - 2 * (uint32_t)scale_columns;
-            const uint64_t d_sw = ptx::umma_desc_sw128(0, 0, 1024), d_scale = ptx::umma_desc_plain(0, 0, 128);
+            const uint64_t desc = ptx::umma_desc_sw128(0, 0, 1024);
+            const uint32_t desc_hi = (uint32_t)(desc >> 32);
+            const uint32_t a0 = (uint32_t)desc + ((ptx::smem_u32(ring) + (uint32_t)(u * kSegs * kBlockBytes)) >> 4);
+            const uint32_t x0 = (uint32_t)desc + ((ptx::smem_u32(ring) + (uint32_t)x_at) >> 4);
+            const uint32_t slot_step = (uint32_t)slot_bytes >> 4, seg_step = (uint32_t)width * 8;
             for (int unit = blockIdx.x; ok && unit < n_units; unit += gridDim.x, ++n) {
-                const Tile t = locate(unit, prefix, row_start, a.G, n_nt);
-                const uint32_t idesc = ptx::umma_idesc_mxf4(128, t.n), d0 = tmem_base + buf * (uint32_t)(kHalves * width);
-                const int blocks = M::scale_blocks(t.n);
+                const int cols = uniform(locate(unit, prefix, row_start, a.G, n_nt).n), x_words = cols > 128 ? 8 : 4;
+                const uint32_t idesc = ptx::umma_idesc_mxf4(128, cols), d = tmem_base + (buf * kHalves + u) * (uint32_t)width;
                 // the epilogue has taken what the buffer held
-                if (n >= (uint32_t)n_bufs && !wait(&sy->d_empty[buf], bph ^ 1, sy, a.findings, 30)) { ok = false; break; }
-                for (int kb = 0; kb < stages; ++kb, ++it) {
+                if (n >= (uint32_t)n_bufs && !wait(&sy->d_empty[buf], bph ^ 1, sy, a.findings, 30)) break;
+                uint32_t more = 0;
+                for (int kb = 0; kb < stages; ++kb) {
                     if (!wait(&sy->full[slot], ph, sy, a.findings, 40)) { ok = false; break; }
-                    ptx::tc_fence_after();
-                    if (leader) {
-                        const uint32_t at = ring0 + slot * (uint32_t)slot_bytes, ws = scale0 + (it & 1) * (uint32_t)scale_columns;
-                        const uint32_t xs = ws + kHalves * kWords * 4;
-                        const int here = min(kWords, words - kb * kWords);
-    #pragma unroll
-                        for (int w = 0; w < kWords; ++w) {
-                            if (w >= here) break;
-    #pragma unroll
-                            for (int u = 0; u < kHalves; ++u)
-                                ptx::tmem_copy_scales(ws + (u * kWords + w) * 4, d_scale + ((at + ws_at + (u * kWords + w) * kScaleBytes) >> 4));
-                            for (int b = 0; b < blocks; ++b)
-                                ptx::tmem_copy_scales(xs + (w * scale_blocks + b) * 4, d_scale + ((at + xs_at + (w * scale_blocks + b) * kScaleBytes) >> 4));
+                    const uint32_t al = a0 + slot * slot_step, xl = x0 + slot * slot_step;
+                    const int here = min(kWords, words - kb * kWords);
+#pragma unroll
+                    for (int w = 0; w < kWords; ++w) {
+                        if (w >= here) break;
+                        const int cw = (kb * kWords + w) & (kChunkWords - 1);  // the word's place in its chunk
+                        if (cw == 0 && !wait(&sy->s_full[cb], cph, sy, a.findings, 41)) { ok = false; break; }
+                        if (w == 0 || cw == 0) ptx::tc_fence_after();
+                        if (leader) {
+                            const uint32_t ws = scale0 + cb * kScaleColumns + (uint32_t)((u * kChunkWords + cw) * 4);
+                            const uint32_t xs = scale0 + cb * kScaleColumns + (uint32_t)(kXScaleAt + cw * x_words);
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const uint32_t step = (uint32_t)(((w & 1) * 2 + h) * 2);  // 64 k
+                                ptx::umma_mxf4(d, al + (uint32_t)((w >> 1) * (kBlockBytes >> 4)) + step, xl + (w >> 1) * seg_step + step, desc_hi,
+                                               idesc | ptx::umma_scale_half(h), ws, xs, h == 0 ? more : 1u);
+                            }
                         }
-    #pragma unroll
-                        for (int w = 0; w < kWords; ++w) {
-                            if (w >= here) break;
-    #pragma unroll
-                            for (int u = 0; u < kHalves; ++u)
-    #pragma unroll
-                                for (int h = 0; h < 2; ++h) {
-                                    const uint32_t step = (uint32_t)(((w & 1) * 2 + h) * 32);  // bytes of 64 k
-                                    ptx::umma_mxf4(d0 + u * width, d_sw + ((at + (u * kSegs + (w >> 1)) * kBlockBytes + step) >> 4),
-                                                   d_sw + ((at + x_at + (w >> 1) * width * 128 + step) >> 4), idesc | ptx::umma_scale_half(h),
-                                                   ws + (u * kWords + w) * 4, xs + w * scale_blocks * 4, (uint32_t)(kb + w + h != 0));
-                                }
+                        more = 1;
+                        if (cw == kChunkWords - 1 || kb * kWords + w + 1 == words) {
+                            if (leader) ptx::umma_commit(ptx::smem_u32(&sy->s_empty[cb]));
+                            cb ^= 1;
+                            cph ^= cb == 0;
                         }
+                    }
+                    if (leader && ok) {
                         ptx::umma_commit(ptx::smem_u32(&sy->empty[slot]));
                         if (kb + 1 == stages) ptx::umma_commit(ptx::smem_u32(&sy->d_full[buf]));
                     }
                     __syncwarp();
+                    if (!ok) break;
                     if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
                 }
                 if (++buf == (uint32_t)n_bufs) { buf = 0; bph ^= 1; }
             }
             // every MMA issued here must have completed before tensor and shared memory go
             if (leader) {
-                ptx::umma_commit(ptx::smem_u32(&sy->drain));
-                (void)ptx::mbar_wait(ptx::smem_u32(&sy->drain), 0);
+                ptx::umma_commit(ptx::smem_u32(&sy->drain[u]));
+                (void)ptx::mbar_wait(ptx::smem_u32(&sy->drain[u]), 0);
             }
             __syncwarp();
         }
     } else if (warp < kWarpEpi0) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
         // ------------------------------ scales ------------------------------
-        // A thread has a row of every block of 128: 16 bytes, 512 k, of each on their way while the two before them are stored.
-        const int q = warp - kWarpScale0, row = q * 32 + lane, chunks = (words + 3) / 4;
+        // A thread fetches a row of every block of 128, 16 bytes (512 k) of each; the warps exchange them through shared memory, since each
+        // writes all rows to its quarter of the lanes: row r in lane r % 32 of column r / 32, four columns for a word (128 k) of 128 rows.
+        const int q = warp - kWarpScale0, row = q * 32 + lane, chunks = (words + kChunkWords - 1) / kChunkWords;
         const bool whole = (words & 3) == 0 && ((reinterpret_cast<uintptr_t>(a.w_scale) | reinterpret_cast<uintptr_t>(a.x_scale)) & 15) == 0;
         struct Chunk {
             uint4 v[kHalves + 2];  // of the weights' blocks and the two of x
-            int words;             // 0: the schedule has ended
-            bool last;             // of its tile
+            int cols;              // token rows of the tile rounded up; 0: the schedule has ended
         };
-        int unit = (int)blockIdx.x - (int)gridDim.x, at = chunks;
+        int unit = (int)blockIdx.x - (int)gridDim.x, at = chunks, cols = 0;
         const uint32_t* src[kHalves + 2];  // NULL: no row there, zeros
         const auto fetch = [&](Chunk& c) {
             if (at == chunks) {
                 unit += (int)gridDim.x;
                 if (unit >= n_units) {
                     unit -= (int)gridDim.x;
-                    c.words = 0;
+                    c.cols = 0;
                     return;
                 }
                 const Tile t = locate(unit, prefix, row_start, a.G, n_nt);
+                cols = t.n;
 #pragma unroll
                 for (int u = 0; u < kHalves; ++u) {
                     const int n = t.nt * M::kTileColumns + u * M::block_step(a.N) + row;
@@ -476,11 +492,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                                            : nullptr;
                 at = 0;
             }
-            c.words = min(4, words - 4 * at);
-            c.last = at + 1 == chunks;
+            c.cols = cols;
+            const int here = words - kChunkWords * at;
 #pragma unroll
             for (int b = 0; b < kHalves + 2; ++b) {
-                const uint32_t* p = src[b] + 4 * at;
+                const uint32_t* p = src[b] + kChunkWords * at;
                 c.v[b] = make_uint4(0u, 0u, 0u, 0u);
                 if (src[b] != nullptr) {
                     // (ordinary loads: the kernel ahead may have written either operand's scales)
@@ -488,55 +504,78 @@ __global__ void __launch_bounds__(kThreads, 1)
                         c.v[b] = __ldca(reinterpret_cast<const uint4*>(p));
                     } else {
                         c.v[b].x = __ldca(p);
-                        if (c.words > 1) c.v[b].y = __ldca(p + 1);
-                        if (c.words > 2) c.v[b].z = __ldca(p + 2);
-                        if (c.words > 3) c.v[b].w = __ldca(p + 3);
+                        if (here > 1) c.v[b].y = __ldca(p + 1);
+                        if (here > 2) c.v[b].z = __ldca(p + 2);
+                        if (here > 3) c.v[b].w = __ldca(p + 3);
                     }
                 }
             }
             ++at;
         };
-        uint32_t it = 0, slot = 0, ph = 0, stage_word = 0;
-        bool ok = true;
+        uint32_t n = 0, cb = 0, cph = 0;
+        const uint32_t quarter = scale0 + ((uint32_t)(q * 32) << 16);
         const auto put = [&](const Chunk& c) {
+            uint4* room = reinterpret_cast<uint4*>(exchange) + cb * kScaleRows;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (i >= c.words || !ok) break;
-                if (stage_word == 0 && it >= (uint32_t)n_slots && !wait(&sy->empty[slot], ph ^ 1, sy, a.findings, 20)) { ok = false; break; }
-                uint8_t* dst = ring + slot * (uint32_t)slot_bytes + lane * 16 + q * 4;
+            for (int b = 0; b < kHalves; ++b) room[b * 128 + row] = c.v[b];
+            room[kHalves * 128 + row] = c.v[kHalves];
+            if (128 + row < kMaxR) room[kHalves * 128 + 128 + row] = c.v[kHalves + 1];
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->exchange));
+            if (!wait(&sy->exchange, n & 1, sy, a.findings, 21)) return false;
+            if (n >= 2 && !wait(&sy->s_empty[cb], cph ^ 1, sy, a.findings, 20)) return false;
+            ptx::tc_fence_after();
+            const uint32_t to = quarter + cb * kScaleColumns;
+            // four rows of a block, word by word
+            const auto rows4 = [&](const uint4* r, uint32_t(&o)[16]) {
 #pragma unroll
-                for (int b = 0; b < kHalves + 2; ++b) {
-                    const uint32_t v = i == 0 ? c.v[b].x : i == 1 ? c.v[b].y : i == 2 ? c.v[b].z : c.v[b].w;
-                    if (b < kHalves) *reinterpret_cast<uint32_t*>(dst + ws_at + (b * kWords + stage_word) * kScaleBytes) = v;
-                    else if (b - kHalves < scale_blocks)
-                        *reinterpret_cast<uint32_t*>(dst + xs_at + (stage_word * scale_blocks + (b - kHalves)) * kScaleBytes) = v;
+                for (int i = 0; i < 4; ++i) {
+                    const uint4 v = r[i * 32 + lane];
+                    o[i] = v.x; o[4 + i] = v.y; o[8 + i] = v.z; o[12 + i] = v.w;
                 }
-                if (++stage_word == (uint32_t)kWords || (c.last && i + 1 == c.words)) {
-                    ptx::fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->full[slot]));
-                    stage_word = 0;
-                    ++it;
-                    if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
+            };
+            uint32_t o[16];
+#pragma unroll
+            for (int u = 0; u < kHalves; ++u) {
+                rows4(room + u * 128, o);
+                ptx::tmem_st_32x16(to + u * (kChunkWords * 4), o);
+            }
+            rows4(room + kHalves * 128, o);
+            if (c.cols <= 128) {
+                ptx::tmem_st_32x16(to + kXScaleAt, o);
+            } else {
+                uint32_t p[8];
+#pragma unroll
+                for (int i = 0; i < (kMaxR - 128) / 32; ++i) {
+                    const uint4 v = room[kHalves * 128 + 128 + i * 32 + lane];
+                    p[i] = v.x; p[2 + i] = v.y; p[4 + i] = v.z; p[6 + i] = v.w;
+                }
+#pragma unroll
+                for (int w = 0; w < kChunkWords; ++w) {
+                    const uint32_t r[8] = {o[4 * w], o[4 * w + 1], o[4 * w + 2], o[4 * w + 3], p[2 * w], p[2 * w + 1], 0u, 0u};
+                    ptx::tmem_st_32x8(to + kXScaleAt + w * 8, r);
                 }
             }
+            ptx::tmem_st_wait();
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->s_full[cb]));
+            ++n;
+            cb ^= 1;
+            cph ^= cb == 0;
+            return true;
         };
-        Chunk c0, c1, c2;
+        static_assert(kMaxR == 192, "two rows of the second block of x");
+        Chunk c0, c1;
         fetch(c0);
-        fetch(c1);
-        while (ok) {
-            fetch(c2);
-            if (c0.words == 0) break;
-            put(c0);
-            fetch(c0);
-            if (c1.words == 0) break;
-            put(c1);
+        while (true) {
             fetch(c1);
-            if (c2.words == 0) break;
-            put(c2);
+            if (c0.cols == 0 || !put(c0)) break;
+            fetch(c0);
+            if (c1.cols == 0 || !put(c1)) break;
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
         // ------------------------------ epilogue ------------------------------
         Share e;
         e.group = (warp - kWarpEpi0) >> 2;
@@ -578,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     ptx::tc_fence_before();
     __syncthreads();
-    if (warp == kWarpMma) {
+    if (warp == kWarpMma0) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc(tmem_base, kTmemCols);
     }

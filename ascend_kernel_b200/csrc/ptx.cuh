@@ -326,31 +326,28 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* m, 
         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(z)
         : "memory");
 }
-// Shared-memory descriptor without swizzle: cores of 8 rows x 16 bytes, `sbo_bytes` from one to the next along the rows.
-__device__ __forceinline__ uint64_t umma_desc_plain(uint32_t smem_addr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
-    uint64_t d = 0;
-    d |= (uint64_t)((smem_addr & 0x3FFFF) >> 4);
-    d |= (uint64_t)((lbo_bytes >> 4) & 0x3FFF) << 16;
-    d |= (uint64_t)((sbo_bytes >> 4) & 0x3FFF) << 32;
-    d |= (uint64_t)1 << 46;
-    return d;
-}
-// 32 rows x 16 bytes of shared memory -> 32 lanes x 4 columns of tensor memory, the same in each quarter of the lanes.  In order with the
-// MMAs that the thread issues.
-__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+// 32 lanes x 16 consecutive 32-bit columns, registers -> tensor memory (see tmem_st_32x8).
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+                 "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
 }
 // D[tmem] (+)= A * B, both e2m1 (two to a byte, K-major) with an e8m0 scale per 32 k in tensor memory, fp32 sums; 64 k.  Scales: row r of an
 // operand in lane r % 32 of column r / 32, the four bytes of a column for 128 k of which the instruction descriptor names two.
-__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t tmem_sa, uint32_t tmem_sb,
-                                          uint32_t accumulate) {
+// The same in each quarter of the lanes.  Both descriptors have the upper word `desc_hi`.
+__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint32_t desc_a, uint32_t desc_b, uint32_t desc_hi, uint32_t idesc, uint32_t tmem_sa,
+                                          uint32_t tmem_sb, uint32_t accumulate) {
     asm volatile(
         "{\n"
         ".reg .pred p;\n"
-        "setp.ne.b32 p, %6, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
+        ".reg .b64 a, b;\n"
+        "mov.b64 a, {%1, %3};\n"
+        "mov.b64 b, {%2, %3};\n"
+        "setp.ne.b32 p, %7, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %4, [%5], [%6], p;\n"
         "}\n" ::"r"(tmem_d),
-        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
+        "r"(desc_a), "r"(desc_b), "r"(desc_hi), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
         : "memory");
 }
 // Instruction descriptor, kind::mxf4: A and B e2m1 and K-major, scales e8m0; and the bits that take the lower (0) or the upper (1) two
