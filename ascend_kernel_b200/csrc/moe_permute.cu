@@ -21,188 +21,233 @@ constexpr int kMaxTopK = 32;
 //
 // A CTA takes a range of pairs, each of its warps a part of that.  Two passes over the ids: count per warp and expert
 // in shared memory, then, with every warp's first position of every expert in the counts' place, hand the positions out.  In a
-// warp, lanes of the same expert find one another (match) and take positions in the order of their lanes.  Up to 8 CTAs are
-// one cluster and read one another's counts from shared memory, in one launch; more CTAs leave their counts in scratch memory for a second kernel
-// whose first pass runs beside the first kernel.
+// warp, lanes of the same expert find one another by a vote on each bit of its number, and take positions in the order of their lanes.  Short calls
+// are one CTA's; where there are more, a first kernel leaves each CTA's counts in scratch memory, and every CTA of the second adds up those before it,
+// its own counting done beside the first kernel.
+//
+// Measured, one call after the other, us (256 experts): 37 x 8 pairs 4.2, 512 x 8 10, 65536 x 8 16.4 (of its 6.3 MB the memory takes 1): launches and the chains
+// of shared-memory latencies in between.  Tried and not kept: the match instruction (22.6), clusters that add up their counts in
+// distributed shared memory (18 in clusters of 4, 31 of 8, which do not all fit at once), stores put in order in shared memory first (16.4).
 
-constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
-constexpr int kCtaPairs = 4096;    // of a CTA where the call has few
-constexpr int kClusterCtas = 8, kMostCtas = 128;
-constexpr int kBatch = 4;          // ids a lane has under way
+constexpr int kWarps = 32, kFewWarps = 8;
+constexpr int kOnePairs = 4096;    // of a call that is one CTA's
+constexpr int kMostCtas = 128;
+constexpr int kBatch = 4;          // ids a lane has at a time
 
 struct SortArgs {
     const int32_t* idx;
     long long* counts;
     int32_t* token_of;
     int32_t* slot;
-    int32_t* totals;   // [CTAs][E]
+    int32_t* totals;   // [E][kMostCtas]
     int P, E, k, cta_pairs, warp_pairs;
+    int bits;          // of an expert's number
+    unsigned long long per_k;  // ceil(2^35 / k)
 };
 
-// fn(pair, expert or -1, lanes of the same expert) over the warp's pairs, in their order; the whole warp calls it.
-template <class F>
-__device__ __forceinline__ void each_pair(const SortArgs& a, F&& fn) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// p / k: with p < 2^30 and k <= 32 the rounding of per_k adds less than 31 * 2^30 < 2^35
+__device__ __forceinline__ int token_of_pair(const SortArgs& a, int p) {
+    return a.k == 1 ? p : (int)(((unsigned long long)(unsigned)p * a.per_k) >> 35);
+}
+
+// The lanes whose expert is the same; for a lane without one (-1) it means nothing.  (A vote for each bit: the match instruction takes as many
+// steps as there are different numbers.)
+__device__ __forceinline__ unsigned same_expert(int e, int bits) {
+    unsigned same = __ballot_sync(0xffffffffu, e >= 0);
+#pragma unroll
+    for (int b = 0; b < 10; ++b) {
+        if (b >= bits) break;
+        const bool mine = (e >> b) & 1;
+        const unsigned set = __ballot_sync(0xffffffffu, mine);
+        same &= mine ? set : ~set;
+    }
+    return same;
+}
+
+// A warp's pairs, 32 * kBatch at a time: [first, end) and the ids of a batch (-1: none).
+struct WarpRange {
+    long long first;
+    int end;
+};
+__device__ __forceinline__ WarpRange warp_range(const SortArgs& a) {
     const long long cta_end = min((long long)a.P, ((long long)blockIdx.x + 1) * a.cta_pairs);
-    const long long first = (long long)blockIdx.x * a.cta_pairs + (long long)warp * a.warp_pairs;
-    const int end = (int)min(cta_end, first + a.warp_pairs);
-    for (long long p0 = first; p0 < end; p0 += 32 * kBatch) {
-        int e[kBatch];
+    const long long first = (long long)blockIdx.x * a.cta_pairs + (long long)(threadIdx.x >> 5) * a.warp_pairs;
+    return {first, (int)min(cta_end, first + a.warp_pairs)};
+}
+__device__ __forceinline__ void load_batch(const SortArgs& a, long long p0, int end, int (&e)[kBatch]) {
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const long long p = p0 + 32 * i + lane;
-            e[i] = p < end ? __ldg(a.idx + p) : -1;
-            if ((unsigned)e[i] >= (unsigned)a.E) e[i] = -1;
-        }
+    for (int i = 0; i < kBatch; ++i) {
+        const long long p = p0 + 32 * i + (threadIdx.x & 31);
+        e[i] = p < end ? __ldg(a.idx + p) : -1;
+        if ((unsigned)e[i] >= (unsigned)a.E) e[i] = -1;
+    }
+}
+// Counts a batch on top of `mine`, the warp's counts by expert, in the order of the pairs; rank[i]: the pairs of the same expert before.
+__device__ __forceinline__ void count_batch(const SortArgs& a, const int (&e)[kBatch], int* mine, int (&rank)[kBatch]) {
+    unsigned peers[kBatch];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            if (p0 + 32 * i >= end) break;
-            const unsigned peers = __match_any_sync(0xffffffffu, e[i]);
-            const long long p = p0 + 32 * i + lane;
-            fn((int)p, p < end, e[i], peers);
-            __syncwarp();
-        }
+    for (int i = 0; i < kBatch; ++i) peers[i] = same_expert(e[i], a.bits);
+    const unsigned lower = (1u << (threadIdx.x & 31)) - 1;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+        const int below = __popc(peers[i] & lower);
+        int before = 0;
+        if (e[i] >= 0) before = mine[e[i]];
+        __syncwarp();
+        if (e[i] >= 0 && below == 0) mine[e[i]] = before + __popc(peers[i]);
+        __syncwarp();
+        rank[i] = before + below;
     }
 }
 
-// hist[warp][e] = the warp's pairs of expert e
-__device__ __forceinline__ void count_pairs(const SortArgs& a, int* hist) {
-    for (int i = threadIdx.x; i < kSortWarps * a.E; i += kSortThreads) hist[i] = 0;
+// The first pass: hist[warp][e] = the warp's pairs of expert e; e and rank are those of its last batch.
+template <int WARPS>
+__device__ __forceinline__ void count_pairs(const SortArgs& a, int* hist, int (&e)[kBatch], int (&rank)[kBatch]) {
+    const WarpRange w = warp_range(a);
+    load_batch(a, w.first, w.end, e);
+    for (int i = threadIdx.x; i < WARPS * a.E; i += WARPS * 32) hist[i] = 0;
     __syncthreads();
     int* mine = hist + (threadIdx.x >> 5) * a.E;
-    each_pair(a, [&](int, bool, int e, unsigned peers) {
-        if (e >= 0 && (peers & ((1u << (threadIdx.x & 31)) - 1)) == 0) mine[e] += __popc(peers);
-    });
+    for (long long p0 = w.first; p0 < w.end; p0 += 32 * kBatch) {
+        if (p0 != w.first) load_batch(a, p0, w.end, e);
+        count_batch(a, e, mine, rank);
+    }
     __syncthreads();
 }
 
 // hist -> the sums over the warps before each; returns expert threadIdx.x's pairs in the CTA.
+template <int WARPS>
 __device__ __forceinline__ int scan_warps(const SortArgs& a, int* hist) {
     int total = 0;
     if ((int)threadIdx.x < a.E) {
-#pragma unroll 8
-        for (int w = 0; w < kSortWarps; ++w) {
-            const int c = hist[w * a.E + threadIdx.x];
+        int c[WARPS];
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) c[w] = hist[w * a.E + threadIdx.x];
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
             hist[w * a.E + threadIdx.x] = total;
-            total += c;
+            total += c[w];
         }
     }
     return total;
 }
 
 // Sum over the threads below and, in `all`, over all of the CTA.
+template <int WARPS>
 __device__ __forceinline__ int cta_exclusive_sum(int v, int& all, int* room) {
     int sum;
     const int below = warp_exclusive_sum(v, sum);
     if ((threadIdx.x & 31) == 31) room[threadIdx.x >> 5] = sum;
     __syncthreads();
-    int w = room[threadIdx.x & 31], total;
-    const int before = warp_exclusive_sum(w, total);
-    all = total;
+    const int lane = threadIdx.x & 31;
+    const int before = warp_exclusive_sum(lane < WARPS ? room[lane] : 0, all);
     return below + __shfl_sync(0xffffffffu, before, threadIdx.x >> 5);
 }
 
-// Second pass: base[e] is where the CTA's pairs of expert e begin.
-__device__ __forceinline__ void place_pairs(const SortArgs& a, int* hist, const int* base, int kept, int cta, int ctas) {
+// The second pass: base[e] is where the CTA's pairs of expert e begin.  A warp with one batch still has its ranks.
+__device__ __forceinline__ void place_pairs(const SortArgs& a, int* hist, const int* base, int kept, int (&e)[kBatch], int (&rank)[kBatch]) {
+    const WarpRange w = warp_range(a);
     int* mine = hist + (threadIdx.x >> 5) * a.E;
-    each_pair(a, [&](int p, bool inside, int e, unsigned peers) {
-        const int lane = threadIdx.x & 31, below = __popc(peers & ((1u << lane) - 1));
-        int at = -1;
-        if (e >= 0) at = base[e] + mine[e] + below;
-        __syncwarp();
-        if (e >= 0 && below == 0) mine[e] += __popc(peers);
-        if (inside) a.slot[p] = at;
-        if (at >= 0) a.token_of[at] = p / a.k;
-    });
-    for (long long r = (long long)kept + cta * kSortThreads + threadIdx.x; r < a.P; r += (long long)ctas * kSortThreads) a.token_of[r] = -1;
-}
-
-__global__ void __launch_bounds__(kSortThreads, 1) sort_cluster_kernel(const SortArgs a) {
-    extern __shared__ int smem[];  // [warps][E], [E] the CTA's pairs, [E] base
-    __shared__ int s_room[32];
-    int *hist = smem, *total = hist + kSortWarps * a.E, *base = total + a.E;
-    const int e = threadIdx.x, ctas = gridDim.x, cta = blockIdx.x;
-    count_pairs(a, hist);
-    int all = scan_warps(a, hist), before = 0;
-    if (e < a.E) total[e] = all;
-    if (ctas > 1) {
-        ptx::cluster_sync();
-        if (e < a.E) {
-            int v[kClusterCtas];
+    const bool once = a.warp_pairs <= 32 * kBatch;
+    for (long long p0 = w.first; p0 < w.end; p0 += 32 * kBatch) {
+        if (!once) {
+            load_batch(a, p0, w.end, e);
+            count_batch(a, e, mine, rank);
+        }
 #pragma unroll
-            for (int c = 0; c < kClusterCtas; ++c)
-                v[c] = c < ctas ? __float_as_int(ptx::ld_cluster_f32(ptx::map_rank(ptx::smem_u32(total + e), (uint32_t)c))) : 0;
-            all = 0;
-#pragma unroll
-            for (int c = 0; c < kClusterCtas; ++c) {
-                if (c == cta) before = all;
-                all += v[c];
-            }
+        for (int i = 0; i < kBatch; ++i) {
+            const int p = (int)p0 + 32 * i + (int)(threadIdx.x & 31);
+            const int at = e[i] < 0 ? -1 : base[e[i]] + rank[i] + (once ? mine[e[i]] : 0);
+            if (p < w.end) a.slot[p] = at;
+            if (at >= 0) a.token_of[at] = token_of_pair(a, p);
         }
     }
-    int kept;
-    const int start = cta_exclusive_sum(all, kept, s_room);
-    if (e < a.E) {
-        base[e] = start + before;
-        if (cta == 0) a.counts[e] = all;
-    }
-    __syncthreads();
-    place_pairs(a, hist, base, kept, cta, ctas);
-    if (ctas > 1) ptx::cluster_sync();  // (the others have read this CTA's counts)
+    for (long long r = (long long)kept + blockIdx.x * blockDim.x + threadIdx.x; r < a.P; r += (long long)gridDim.x * blockDim.x) a.token_of[r] = -1;
 }
 
-__global__ void __launch_bounds__(kSortThreads, 1) sort_count_kernel(const SortArgs a) {
-    extern __shared__ int smem[];
-    count_pairs(a, smem);
-    const int total = scan_warps(a, smem);
-    if ((int)threadIdx.x < a.E) a.totals[(size_t)blockIdx.x * a.E + threadIdx.x] = total;
+// A call that is one CTA's; E <= 32 WARPS.
+template <int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 1) sort_one_kernel(const SortArgs a) {
+    extern __shared__ int smem[];  // [WARPS][E], [E]
+    __shared__ int s_room[32];
+    int *hist = smem, *base = hist + WARPS * a.E;
+    int id[kBatch], rank[kBatch], kept;
+    count_pairs<WARPS>(a, hist, id, rank);
+    const int total = scan_warps<WARPS>(a, hist);
+    const int start = cta_exclusive_sum<WARPS>(total, kept, s_room);
+    if ((int)threadIdx.x < a.E) {
+        base[threadIdx.x] = start;
+        a.counts[threadIdx.x] = total;
+    }
+    __syncthreads();
+    place_pairs(a, hist, base, kept, id, rank);
+}
+
+__global__ void __launch_bounds__(kWarps * 32, 1) sort_count_kernel(const SortArgs a) {
+    extern __shared__ int smem[];  // [kWarps][E]
+    int id[kBatch], rank[kBatch];
+    count_pairs<kWarps>(a, smem, id, rank);
+    if ((int)threadIdx.x < a.E) {
+        int total = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) total += smem[w * a.E + threadIdx.x];
+        a.totals[threadIdx.x * kMostCtas + blockIdx.x] = total;
+    }
     grid_dep_launch();
 }
 
-__global__ void __launch_bounds__(kSortThreads, 1) sort_place_kernel(const SortArgs a) {
-    extern __shared__ int smem[];  // [warps][E], [2 E]
+__global__ void __launch_bounds__(kWarps * 32, 1) sort_place_kernel(const SortArgs a) {
+    extern __shared__ int smem[];  // [kWarps][E], twice [E]
     __shared__ int s_room[32];
-    int *hist = smem, *base = hist + kSortWarps * a.E, *alls = base + a.E;
+    int *hist = smem, *base = hist + kWarps * a.E, *alls = base + a.E;
     const int e = threadIdx.x;
-    count_pairs(a, hist);
-    scan_warps(a, hist);
-    for (int i = threadIdx.x; i < a.E; i += kSortThreads) base[i] = alls[i] = 0;
-    __syncthreads();
-    // every expert's pairs in the CTAs before this one and in all: several threads share an expert's CTAs where experts are few
-    const int share = max(1, kSortThreads / a.E), part = threadIdx.x / a.E, mine = threadIdx.x - part * a.E;
+    int id[kBatch], rank[kBatch], kept;
+    count_pairs<kWarps>(a, hist, id, rank);
+    scan_warps<kWarps>(a, hist);
+    // every expert's pairs in the CTAs before this one and in all: a warp an expert, a lane four CTAs
+    const int lane = threadIdx.x & 31;
     grid_dep_wait();
-    if (part < share) {
+#pragma unroll 4
+    for (int x = threadIdx.x >> 5; x < a.E; x += kWarps) {
+        static_assert(kMostCtas == 4 * 32, "CTAs of a lane");
+        const int4 v = __ldcg(reinterpret_cast<const int4*>(a.totals + x * kMostCtas) + lane);
+        const int c[4] = {v.x, v.y, v.z, v.w};
         int before = 0, all = 0;
-#pragma unroll 8
-        for (int c = part; c < (int)gridDim.x; c += share) {
-            const int v = __ldcg(a.totals + (size_t)c * a.E + mine);
-            all += v;
-            if (c < (int)blockIdx.x) before += v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (4 * lane + i < (int)gridDim.x) all += c[i];
+            if (4 * lane + i < (int)blockIdx.x) before += c[i];
         }
-        atomicAdd(base + mine, before);  // (whole numbers: any order gives the same sum)
-        atomicAdd(alls + mine, all);
+        before = __reduce_add_sync(0xffffffffu, before);
+        all = __reduce_add_sync(0xffffffffu, all);
+        if (lane == 0) {
+            base[x] = before;
+            alls[x] = all;
+        }
     }
     __syncthreads();
-    int kept;
     const int all = e < a.E ? alls[e] : 0;
-    const int start = cta_exclusive_sum(all, kept, s_room);
+    const int start = cta_exclusive_sum<kWarps>(all, kept, s_room);
     if (e < a.E) {
         base[e] += start;
         if (blockIdx.x == 0) a.counts[e] = all;
     }
     __syncthreads();
-    place_pairs(a, hist, base, kept, blockIdx.x, gridDim.x);
+    place_pairs(a, hist, base, kept, id, rank);
 }
 
 static bool sort_sizes_ok(int64_t T, int64_t E, int64_t k) {
     return T >= 0 && E > 0 && E <= kMaxExperts && k > 0 && k <= kMaxTopK && T <= 0x3FFFFFFF / k;
 }
-// Pairs of a CTA and the number of CTAs.
-static int cta_pairs_of(int64_t P) {
-    const int64_t n = (P + kMostCtas - 1) / kMostCtas;
-    return (int)std::max<int64_t>(kCtaPairs, (n + 1023) / 1024 * 1024);
+// The number of CTAs and the pairs of each.
+static int ctas_of(int64_t P) {
+    if (P <= kOnePairs) return 1;
+    return (int)std::min<int64_t>(kMostCtas, (P + 1023) / 1024);
 }
-static int ctas_of(int64_t P) { return (int)std::max<int64_t>(1, (P + cta_pairs_of(P) - 1) / cta_pairs_of(P)); }
+static int cta_pairs_of(int64_t P) {
+    const int64_t n = (P + ctas_of(P) - 1) / ctas_of(P);
+    return (int)((n + 1023) / 1024 * 1024);
+}
 
 // ---- rows ---------------------------------------------------------------------------------------------------------------
 
@@ -308,10 +353,10 @@ __global__ void __launch_bounds__(kRowThreads) combine_grad_kernel(const uint4* 
                                                                    const int32_t* __restrict__ token_of, const int32_t* __restrict__ slot,
                                                                    const uint4* __restrict__ grad, uint4* __restrict__ grad_y,
                                                                    float* __restrict__ grad_w, int k, int width16) {
-    constexpr int N = Piece<T>::N, kWarps = kRowThreads / 32;
+    constexpr int N = Piece<T>::N, kRowWarps = kRowThreads / 32;
     __shared__ int s_slot[kMaxTopK];
     __shared__ float s_w[kMaxTopK];
-    __shared__ float s_dot[kWarps][8];
+    __shared__ float s_dot[kRowWarps][8];
     const long long t = blockIdx.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     load_slots(slot, t, k, (long long)gridDim.x * k, s_slot);
@@ -359,7 +404,7 @@ __global__ void __launch_bounds__(kRowThreads) combine_grad_kernel(const uint4* 
             if (threadIdx.x < 8 && j0 + (int)threadIdx.x < k) {
                 float sum = 0.f;
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) sum += s_dot[w][threadIdx.x];
+                for (int w = 0; w < kRowWarps; ++w) sum += s_dot[w][threadIdx.x];
                 grad_w[t * k + j0 + threadIdx.x] = sum;
             }
             __syncthreads();
@@ -386,7 +431,7 @@ using namespace b200moe;
 extern "C" size_t b200moe_moe_sort_scratch_bytes(int64_t n_tokens, int64_t n_experts, int64_t top_k) {
     if (!mp::sort_sizes_ok(n_tokens, n_experts, top_k)) return 0;
     const int ctas = mp::ctas_of(n_tokens * top_k);
-    return ctas <= mp::kClusterCtas ? 0 : (size_t)ctas * (size_t)n_experts * 4;
+    return ctas == 1 ? 0 : (size_t)mp::kMostCtas * (size_t)n_experts * 4;
 }
 
 extern "C" int b200moe_moe_sort(const int32_t* idx, int64_t n_tokens, int64_t n_experts, int64_t top_k, int64_t* counts,
@@ -404,37 +449,31 @@ extern "C" int b200moe_moe_sort(const int32_t* idx, int64_t n_tokens, int64_t n_
     a.slot = slot;
     a.totals = static_cast<int32_t*>(scratch);
     a.P = (int)(n_tokens * top_k); a.E = (int)n_experts; a.k = (int)top_k;
+    while ((1 << a.bits) < a.E) ++a.bits;
+    a.per_k = ((1ull << 35) + (unsigned)a.k - 1) / (unsigned)a.k;
     const int ctas = mp::ctas_of(a.P);
+    // Eight warps where the call has pairs for no more: less to clear and to add up.
+    const bool few = ctas == 1 && a.E <= mp::kFewWarps * 32 && a.P <= 32 * mp::kBatch * mp::kFewWarps;
+    const int warps = few ? mp::kFewWarps : mp::kWarps;
     a.cta_pairs = mp::cta_pairs_of(a.P);
-    // (the warps of a call with few pairs share them)
-    const int most = (int)std::min<int64_t>(a.P, a.cta_pairs);
-    a.warp_pairs = std::max(1, ((most + mp::kSortWarps - 1) / mp::kSortWarps + 31) / 32) * 32;
-    const size_t smem = (size_t)(mp::kSortWarps + 2) * (size_t)a.E * 4;
-    const auto opt_in = [&](auto* kernel) {
-        return smem > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (mp::kSortWarps + 2) * kMaxExperts * 4)
+    a.warp_pairs = std::max(1, ((std::min(a.P, a.cta_pairs) + warps - 1) / warps + 31) / 32) * 32;
+    const size_t smem = (size_t)(warps + 2) * (size_t)a.E * 4;
+    const auto opt_in = [&](void (*kernel)(mp::SortArgs)) {
+        return smem > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (mp::kWarps + 2) * kMaxExperts * 4)
                                 : cudaSuccess;
     };
     if (need == 0) {
-        B200MOE_CUDA_TRY(opt_in(mp::sort_cluster_kernel));
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)ctas);
-        cfg.blockDim = dim3(mp::kSortThreads);
-        cfg.dynamicSmemBytes = smem;
-        cfg.stream = st;
-        cudaLaunchAttribute attr = {};
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = (unsigned)ctas;
-        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
-        B200MOE_CUDA_TRY(cudaLaunchKernelEx(&cfg, mp::sort_cluster_kernel, a));
+        const auto kernel = few ? mp::sort_one_kernel<mp::kFewWarps> : mp::sort_one_kernel<mp::kWarps>;
+        B200MOE_CUDA_TRY(opt_in(kernel));
+        kernel<<<1, warps * 32, smem, st>>>(a);
+        B200MOE_CUDA_TRY(cudaGetLastError());
         return B200MOE_OK;
     }
     B200MOE_CUDA_TRY(opt_in(mp::sort_count_kernel));
     B200MOE_CUDA_TRY(opt_in(mp::sort_place_kernel));
-    mp::sort_count_kernel<<<(unsigned)ctas, mp::kSortThreads, smem, st>>>(a);
+    mp::sort_count_kernel<<<(unsigned)ctas, warps * 32, smem, st>>>(a);
     B200MOE_CUDA_TRY(cudaGetLastError());
-    B200MOE_CUDA_TRY(launch_dependent(mp::sort_place_kernel, (unsigned)ctas, mp::kSortThreads, smem, st, a));
+    B200MOE_CUDA_TRY(launch_dependent(mp::sort_place_kernel, (unsigned)ctas, (unsigned)(warps * 32), smem, st, a));
     return B200MOE_OK;
 }
 

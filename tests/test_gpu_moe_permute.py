@@ -34,7 +34,7 @@ def _same(got, want):
                                            (509, 64, 2, 1.0), (4096, 60, 1, 0), (513, 8, 8, 0.5), (8192, 257, 8, 0), (8200, 1024, 8, 0.03),
                                            (9000, 1, 1, 0.3), (40001, 16, 1, 0.0), (20011, 384, 4, 0.05), (40000, 1000, 8, 0.0)])
 def test_sort_is_stable(T, E, k, dropped):
-    """One block, several in a cluster (over 4096 pairs), more of them (over 32768)."""
+    """One block of few warps or many, and several (over 4096 pairs)."""
     idx = _idx(T, E, k, _gen(T + E), dropped)
     _same(ak.moe_sort(idx, E), R.sort(idx, E))
 

@@ -32,12 +32,10 @@ def test_sort_scratch_of_absurd_sizes(big):
 
 
 def test_sort_scratch_holds_the_counts_of_every_block():
-    for T, E, k in ((1, 1, 1), (4096, 256, 8), (4097, 256, 8), (65536, 1024, 8), (1 << 25, 7, 31)):
+    for T, E, k in ((1, 1, 1), (512, 256, 8), (513, 256, 8), (4096, 256, 8), (4097, 256, 8), (65536, 1024, 8), (1 << 25, 7, 31)):
         pairs = T * k
-        per = max(4096, (-(-pairs // 128) + 1023) // 1024 * 1024)
-        blocks = -(-pairs // per)
-        assert lib.b200moe_moe_sort_scratch_bytes(T, E, k) == (0 if blocks <= 8 else 4 * E * blocks)
-        assert blocks <= 128
+        blocks = 1 if pairs <= 4096 else min(128, -(-pairs // 1024))
+        assert lib.b200moe_moe_sort_scratch_bytes(T, E, k) == (0 if blocks == 1 else 4 * E * 128)
 
 
 def _rows(name, **change):
