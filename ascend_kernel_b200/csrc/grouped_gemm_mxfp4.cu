@@ -40,12 +40,13 @@ template <int HALVES, bool GATE, int SEGS>
 struct Mode {
     static constexpr int kHalves = HALVES, kSegs = SEGS, kWords = 2 * SEGS;  // (a word of scales: 128 k)
     static constexpr bool kGate = GATE;
-    // columns that a tile advances by (gate/up: of each)
-    static constexpr int kTileColumns = GATE ? 128 : 128 * HALVES;
+    // columns that a tile advances by (gate/up: of each), and the CTA's first
+    static constexpr int kTileColumns = GATE ? 256 : 256 * HALVES;
+    static __device__ __forceinline__ int first_column(int nt, uint32_t rank) { return nt * kTileColumns + (int)rank * (kTileColumns / 2); }
     static __device__ __forceinline__ int block_step(int N) { return GATE ? N >> 1 : 128; }
     static constexpr int kFixedBytes = 1024 + kBarrierBytes + kEpiWarps * kStripBytes + kExchangeBytes + 2 * (kMaxExperts + 4) * 4;
     static constexpr int kRingBytes = kSmemBytes - kFixedBytes;
-    static __host__ __device__ constexpr int slot_bytes(int width) { return SEGS * (HALVES * kBlockBytes + width * 128); }
+    static __host__ __device__ constexpr int slot_bytes(int width) { return SEGS * (HALVES * kBlockBytes + width * 64); }
     // tensor-memory columns of a chunk of scales
     static constexpr int kScaleColumns = kChunkWords * 4 * (HALVES + 2);
     static_assert(kRingBytes % 16 == 0 && kRingBytes / slot_bytes(kMaxR) >= 3, "stages");
@@ -65,22 +66,22 @@ struct Args {
 };
 
 struct Sync {
-    uint64_t full[kMaxSlots];    // the bytes of the stage's codes
-    uint64_t empty[kMaxSlots];   // commits of the stage's MMAs, one for each block of columns
-    uint64_t s_full[2];          // the scale warps have written their lanes' copy of a chunk
-    uint64_t s_empty[2];         // commits of its last MMAs
-    uint64_t exchange;           // the scale warps among themselves
-    uint64_t d_full[kMaxBufs];   // commits of a tile's MMAs
-    uint64_t d_empty[kMaxBufs];  // the epilogue warps have the tile's sums
+    uint64_t full[kMaxSlots];    // first CTA: the bytes of both CTAs' codes
+    uint64_t empty[kMaxSlots];   // each CTA: commits of the stage's MMAs, one for each block of columns
+    uint64_t s_full[2];          // first CTA: the scale warps of both have written their lanes' copy of a chunk
+    uint64_t s_empty[2];         // each CTA: commits of its last MMAs
+    uint64_t exchange;           // the CTA's scale warps among themselves
+    uint64_t d_full[kMaxBufs];   // each CTA: commits of a tile's MMAs
+    uint64_t d_empty[kMaxBufs];  // first CTA: the epilogue warps of both have the tile's sums
     uint64_t drain[2];
     uint32_t tmem_base;
     int abort;
-    int n_units, width;          // width: token rows of the widest tile, rounded up to 16
+    int n_units, width;          // width: token rows of the widest tile, rounded up to 32
 };
 static_assert(sizeof(Sync) <= kBarrierBytes, "barrier block");
 
 struct Tile {
-    int g, row0, rows, n, nt;  // n: rows rounded up to 16
+    int g, row0, rows, n, nt;  // n: rows rounded up to 32
 };
 
 // Waits are a whole warp's: it votes at every poll and so leaves them together.
@@ -107,9 +108,9 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Sync* sy, i
     return true;
 }
 
-// An expert's rows are cut into the fewest tiles, of equal size rounded up to 16.
+// An expert's rows are cut into the fewest tiles, of equal size rounded up to 32.
 __device__ __forceinline__ int tiles_of(int rows) { return (rows + kMaxR - 1) / kMaxR; }
-__device__ __forceinline__ int tile_rows_of(int rows, int tiles) { return ((rows + tiles - 1) / tiles + 15) & ~15; }
+__device__ __forceinline__ int tile_rows_of(int rows, int tiles) { return ((rows + tiles - 1) / tiles + 31) & ~31; }
 
 // Inside an expert the row tiles of a weight column run together, so that they share the weights in L2.
 __device__ __forceinline__ Tile locate(int unit, const int* prefix, const int* row_start, int G, int n_nt) {
@@ -127,7 +128,7 @@ __device__ __forceinline__ Tile locate(int unit, const int* prefix, const int* r
     t.nt = nt;
     t.row0 = row_start[lo] + m * tr;
     t.rows = min(tr, rows - m * tr);
-    t.n = (t.rows + 15) & ~15;
+    t.n = (t.rows + 31) & ~31;
     return t;
 }
 
@@ -150,14 +151,14 @@ struct Share {
     Tile t;
     uint32_t tmem, width;
     int group, col;
-    uint64_t* d_empty;
+    uint32_t d_empty;  // in the first CTA
     uint8_t* strip;
 };
 // The sums are in registers: the buffer goes back.
 __device__ __forceinline__ void release(const Share& e) {
     ptx::tc_fence_before();
     __syncwarp();
-    if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(ptx::smem_u32(e.d_empty));
+    if ((threadIdx.x & 31) == 0) ptx::mbar_arrive_remote(e.d_empty);
 }
 
 // Sixteen tokens x the warp's 32 columns in bf16 through the warp's strip: the transposing store gives 16-byte pieces of eight columns, 64
@@ -223,6 +224,7 @@ __device__ __forceinline__ uint32_t transpose_nibbles(uint32_t v) {
 // The lane's column of sixteen tokens, quantised by the warp's 32 columns.
 __device__ __forceinline__ void store_quantized(float (&h)[16], const Tile& t, int token0, int col, const Args& a) {
     const int lane = threadIdx.x & 31, inter = a.N >> 1;
+    const bool inside = col < inter;  // (an odd number of blocks leaves the pair's last CTA without one)
     uint32_t top = 0;  // lane i: the largest magnitude of token i (magnitudes order as their bits do, infinities and NaN last)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -244,10 +246,10 @@ __device__ __forceinline__ void store_quantized(float (&h)[16], const Tile& t, i
         const float v[8] = {h[8 * p], h[8 * p + 1], h[8 * p + 2], h[8 * p + 3], h[8 * p + 4], h[8 * p + 5], h[8 * p + 6], h[8 * p + 7]};
         const uint32_t codes = transpose_nibbles(mxfp4::codes8(v));  // lane % 8's token, eight columns
         const int token = token0 + 8 * p + (lane & 7);
-        if (token < t.rows)
+        if (token < t.rows && inside)
             *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + (size_t)(t.row0 + token) * (inter >> 1) + (col >> 1) + (lane >> 3) * 4) = codes;
     }
-    if (lane < 16 && token0 + lane < t.rows) a.out_scale[(size_t)(t.row0 + token0 + lane) * (inter >> 5) + (col >> 5)] = (uint8_t)byte;
+    if (lane < 16 && token0 + lane < t.rows && inside) a.out_scale[(size_t)(t.row0 + token0 + lane) * (inter >> 5) + (col >> 5)] = (uint8_t)byte;
 }
 
 // silu(gate) * up of every other piece of 16 tokens, NC at most, in registers before the first is quantised.
@@ -273,7 +275,7 @@ __device__ __forceinline__ void finish_quantized(const Share& e, const Args& a) 
 }
 
 template <class M>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x64,
                    const __grid_constant__ CUtensorMap map_x16, const Args a) {
     constexpr int kHalves = M::kHalves, kSegs = M::kSegs, kWords = M::kWords;
@@ -286,6 +288,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int* prefix = row_start + kMaxExperts + 4;
 
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const uint32_t rank = ptx::cluster_rank();
+    const int pairs = (int)gridDim.x / 2, pair = (int)blockIdx.x / 2;
     const int n_nt = ((M::kGate ? a.N >> 1 : a.N) + M::kTileColumns - 1) / M::kTileColumns;
 
     // what needs nothing from memory comes first: the kernel may have started beside the end of the one before it
@@ -296,11 +300,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         init(sy->full, kMaxSlots, 1);
         init(sy->empty, kMaxSlots, kHalves);
-        init(sy->s_full, 2, kScaleWarps);
+        init(sy->s_full, 2, 2 * kScaleWarps);
         init(sy->s_empty, 2, kHalves);
         init(&sy->exchange, 1, kScaleWarps);
         init(sy->d_full, kMaxBufs, kHalves);
-        init(sy->d_empty, kMaxBufs, kEpiWarps);
+        init(sy->d_empty, kMaxBufs, 2 * kEpiWarps);
         init(sy->drain, 2, 1);
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&map_w);
@@ -308,8 +312,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         ptx::prefetch_tensormap(&map_x16);
     }
     if (warp == kWarpMma0) {
-        ptx::tmem_alloc(ptx::smem_u32(&sy->tmem_base), kTmemCols);
-        ptx::tmem_relinquish();
+        ptx::tmem_alloc_pair(ptx::smem_u32(&sy->tmem_base), kTmemCols);
+        ptx::tmem_relinquish_pair();
     }
     grid_dep_wait();
     grid_dep_launch();
@@ -331,11 +335,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) {
             prefix[a.G] = total * n_nt;
             sy->n_units = total * n_nt;
-            sy->width = max(wide, 16);
+            sy->width = max(wide, 32);
         }
     }
     ptx::tc_fence_before();
     __syncthreads();
+    ptx::cluster_sync();
     ptx::tc_fence_after();
 
     const uint32_t tmem_base = (uint32_t)uniform((int)*reinterpret_cast<volatile uint32_t*>(&sy->tmem_base));
@@ -357,33 +362,35 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool leader = ptx::elect_one();
             uint32_t it = 0, slot = 0, ph = 0;
             bool ok = true;
-            for (int unit = blockIdx.x; ok && unit < n_units; unit += gridDim.x) {
+            const uint32_t full0 = ptx::map_rank(ptx::smem_u32(sy->full), 0);
+            for (int unit = pair; ok && unit < n_units; unit += pairs) {
                 const Tile t = locate(unit, prefix, row_start, a.G, n_nt);
-                const int n_big = t.n / kBigBox, n_small = (t.n % kBigBox) / kSmallBox;
+                const int half = t.n >> 1, n_big = half / kBigBox, n_small = (half % kBigBox) / kSmallBox;
+                const int col = M::first_column(t.nt, rank), row = t.row0 + (int)rank * half;
                 for (int kb = 0; kb < stages; ++kb, ++it) {
                     if (it >= (uint32_t)n_slots && !wait(&sy->empty[slot], ph ^ 1, sy, a.findings, 10)) { ok = false; break; }
                     if (leader) {
-                        const uint32_t bar = ptx::smem_u32(&sy->full[slot]), dst = ptx::smem_u32(ring) + slot * (uint32_t)slot_bytes;
+                        const uint32_t bar0 = full0 + slot * 8, dst = ptx::smem_u32(ring) + slot * (uint32_t)slot_bytes;
                         const int here = min(kSegs, segs - kb * kSegs);
-                        ptx::mbar_arrive_expect_tx(bar, (uint32_t)(here * (kHalves * kBlockBytes + t.n * 128)));
-    #pragma unroll
+                        if (rank == 0) ptx::mbar_arrive_expect_tx(ptx::smem_u32(&sy->full[slot]), 2u * (uint32_t)(here * (kHalves * kBlockBytes + half * 128)));
+#pragma unroll
                         for (int s = 0; s < kSegs; ++s) {
                             if (s >= here) break;
                             const int x = (kb * kSegs + s) * 128;
-    #pragma unroll
+#pragma unroll
                             for (int u = 0; u < kHalves; ++u)
-                                ptx::tma_load_3d(dst + (u * kSegs + s) * kBlockBytes, &map_w, bar, x, t.nt * M::kTileColumns + u * M::block_step(a.N), t.g);
-                            uint32_t at = dst + x_at + s * width * 128;
-                            int r = t.row0;
-                            for (int b = 0; b < n_big; ++b, at += kBigBox * 128, r += kBigBox) ptx::tma_load_2d(at, &map_x64, bar, x, r);
-                            for (int b = 0; b < n_small; ++b, at += kSmallBox * 128, r += kSmallBox) ptx::tma_load_2d(at, &map_x16, bar, x, r);
+                                ptx::tma_load_3d_pair(dst + (u * kSegs + s) * kBlockBytes, &map_w, bar0, x, col + u * M::block_step(a.N), t.g);
+                            uint32_t at = dst + x_at + s * width * 64;
+                            int r = row;
+                            for (int b = 0; b < n_big; ++b, at += kBigBox * 128, r += kBigBox) ptx::tma_load_2d_pair(at, &map_x64, bar0, x, r);
+                            for (int b = 0; b < n_small; ++b, at += kSmallBox * 128, r += kSmallBox) ptx::tma_load_2d_pair(at, &map_x16, bar0, x, r);
                         }
                     }
                     __syncwarp();
                     if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
                 }
             }
-            // the commits that give the last stages back have arrived before the CTA ends
+            // the commits that give the last stages back have arrived before the CTA ends (the second CTA's come from the first one)
             for (uint32_t i = it; ok && i < it + (uint32_t)n_slots; ++i) {
                 if (i >= (uint32_t)n_slots) ok = wait(&sy->empty[slot], ph ^ 1, sy, a.findings, 11);
                 if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
@@ -394,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 while (ptx::globaltimer_ns() - t0 < 10000000ull) {}
             }
             __syncwarp();
-        } else if (warp < kWarpMma0 + kHalves) {
+        } else if (warp < kWarpMma0 + kHalves && rank == 0) {
             // ------------------------------ MMA issue ------------------------------
             // A warp for each block of columns: it walks together and one lane issues.  Of the descriptors only the address, in the low
             // word, changes.
@@ -406,10 +413,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t desc_hi = (uint32_t)(desc >> 32);
             const uint32_t a0 = (uint32_t)desc + ((ptx::smem_u32(ring) + (uint32_t)(u * kSegs * kBlockBytes)) >> 4);
             const uint32_t x0 = (uint32_t)desc + ((ptx::smem_u32(ring) + (uint32_t)x_at) >> 4);
-            const uint32_t slot_step = (uint32_t)slot_bytes >> 4, seg_step = (uint32_t)width * 8;
-            for (int unit = blockIdx.x; ok && unit < n_units; unit += gridDim.x, ++n) {
+            const uint32_t slot_step = (uint32_t)slot_bytes >> 4, seg_step = (uint32_t)width * 4;
+            for (int unit = pair; ok && unit < n_units; unit += pairs, ++n) {
                 const int cols = uniform(locate(unit, prefix, row_start, a.G, n_nt).n), x_words = cols > 128 ? 8 : 4;
-                const uint32_t idesc = ptx::umma_idesc_mxf4(128, cols), d = tmem_base + (buf * kHalves + u) * (uint32_t)width;
+                const uint32_t idesc = ptx::umma_idesc_mxf4(256, cols), d = tmem_base + (buf * kHalves + u) * (uint32_t)width;
                 // the epilogue has taken what the buffer held
                 if (n >= (uint32_t)n_bufs && !wait(&sy->d_empty[buf], bph ^ 1, sy, a.findings, 30)) break;
                 uint32_t more = 0;
@@ -429,20 +436,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
                                 const uint32_t step = (uint32_t)(((w & 1) * 2 + h) * 2);  // 64 k
-                                ptx::umma_mxf4(d, al + (uint32_t)((w >> 1) * (kBlockBytes >> 4)) + step, xl + (w >> 1) * seg_step + step, desc_hi,
+                                ptx::umma_mxf4_pair(d, al + (uint32_t)((w >> 1) * (kBlockBytes >> 4)) + step, xl + (w >> 1) * seg_step + step, desc_hi,
                                                idesc | ptx::umma_scale_half(h), ws, xs, h == 0 ? more : 1u);
                             }
                         }
                         more = 1;
                         if (cw == kChunkWords - 1 || kb * kWords + w + 1 == words) {
-                            if (leader) ptx::umma_commit(ptx::smem_u32(&sy->s_empty[cb]));
+                            if (leader) ptx::umma_commit_pair(ptx::smem_u32(&sy->s_empty[cb]));
                             cb ^= 1;
                             cph ^= cb == 0;
                         }
                     }
                     if (leader && ok) {
-                        ptx::umma_commit(ptx::smem_u32(&sy->empty[slot]));
-                        if (kb + 1 == stages) ptx::umma_commit(ptx::smem_u32(&sy->d_full[buf]));
+                        ptx::umma_commit_pair(ptx::smem_u32(&sy->empty[slot]));
+                        if (kb + 1 == stages) ptx::umma_commit_pair(ptx::smem_u32(&sy->d_full[buf]));
                     }
                     __syncwarp();
                     if (!ok) break;
@@ -452,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             // every MMA issued here must have completed before tensor and shared memory go
             if (leader) {
-                ptx::umma_commit(ptx::smem_u32(&sy->drain[u]));
+                ptx::umma_commit_pair(ptx::smem_u32(&sy->drain[u]));
                 (void)ptx::mbar_wait(ptx::smem_u32(&sy->drain[u]), 0);
             }
             __syncwarp();
@@ -468,13 +475,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint4 v[kHalves + 2];  // of the weights' blocks and the two of x
             int cols;              // token rows of the tile rounded up; 0: the schedule has ended
         };
-        int unit = (int)blockIdx.x - (int)gridDim.x, at = chunks, cols = 0;
+        int unit = pair - pairs, at = chunks, cols = 0;
         const uint32_t* src[kHalves + 2];  // NULL: no row there, zeros
         const auto fetch = [&](Chunk& c) {
             if (at == chunks) {
-                unit += (int)gridDim.x;
+                unit += pairs;
                 if (unit >= n_units) {
-                    unit -= (int)gridDim.x;
+                    unit -= pairs;
                     c.cols = 0;
                     return;
                 }
@@ -482,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 cols = t.n;
 #pragma unroll
                 for (int u = 0; u < kHalves; ++u) {
-                    const int n = t.nt * M::kTileColumns + u * M::block_step(a.N) + row;
+                    const int n = M::first_column(t.nt, rank) + u * M::block_step(a.N) + row;
                     src[u] = n < a.N ? reinterpret_cast<const uint32_t*>(a.w_scale) + ((size_t)t.g * a.N + n) * (size_t)words : nullptr;
                 }
 #pragma unroll
@@ -513,6 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ++at;
         };
         uint32_t n = 0, cb = 0, cph = 0;
+        const uint32_t s_full0 = ptx::map_rank(ptx::smem_u32(sy->s_full), 0);
         const uint32_t quarter = scale0 + ((uint32_t)(q * 32) << 16);
         const auto put = [&](const Chunk& c) {
             uint4* room = reinterpret_cast<uint4*>(exchange) + cb * kScaleRows;
@@ -559,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ptx::tmem_st_wait();
             ptx::tc_fence_before();
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->s_full[cb]));
+            if (lane == 0) ptx::mbar_arrive_remote(s_full0 + cb * 8);
             ++n;
             cb ^= 1;
             cph ^= cb == 0;
@@ -567,12 +575,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         static_assert(kMaxR == 192, "two rows of the second block of x");
         Chunk c0, c1;
+        bool ok = true;
         fetch(c0);
         while (true) {
             fetch(c1);
-            if (c0.cols == 0 || !put(c0)) break;
+            if (c0.cols == 0 || !(ok = put(c0))) break;
             fetch(c0);
-            if (c1.cols == 0 || !put(c1)) break;
+            if (c1.cols == 0 || !(ok = put(c1))) break;
+        }
+        // (the commits of the last chunks have arrived before the CTA ends)
+        for (uint32_t i = n < 2 ? n : 2; ok && i > 0; --i) {
+            if (n < 2 && i == n) cb = 0, cph = 1;  // (one chunk alone: the first buffer's first phase)
+            ok = wait(&sy->s_empty[cb], cph ^ 1, sy, a.findings, 22);
+            cb ^= 1;
+            cph ^= cb == 0;
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
@@ -582,17 +598,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         e.strip = strips + (warp - kWarpEpi0) * kStripBytes;
         e.width = (uint32_t)width;
         const int quarter = warp & 3;
+        const uint32_t d_empty0 = ptx::map_rank(ptx::smem_u32(sy->d_empty), 0);
         uint32_t buf = 0, ph = 0;
-        for (int unit = blockIdx.x; unit < n_units; unit += gridDim.x) {
+        for (int unit = pair; unit < n_units; unit += pairs) {
             e.t = locate(unit, prefix, row_start, a.G, n_nt);
             e.tmem = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * (uint32_t)(kHalves * width);
-            e.col = e.t.nt * M::kTileColumns + quarter * 32;
-            e.d_empty = &sy->d_empty[buf];
+            e.col = M::first_column(e.t.nt, rank) + quarter * 32;
+            e.d_empty = d_empty0 + buf * 8;
             if (!wait(&sy->d_full[buf], ph, sy, a.findings, 50)) break;
             ptx::tc_fence_after();
             // (the number of pieces is a constant, so that they stay in registers)
             if constexpr (M::kGate) {
-                switch ((e.t.n + 31) / 32) {
+                switch (e.t.n / 32) {
                     case 1: finish_quantized<1>(e, a); break;
                     case 2: finish_quantized<2>(e, a); break;
                     case 3: finish_quantized<3>(e, a); break;
@@ -601,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     default: finish_quantized<6>(e, a); break;
                 }
             } else {
-                switch ((e.t.n + 31) / 32) {
+                switch (e.t.n / 32) {
                     case 1: finish_rows<2>(e, a); break;
                     case 2: finish_rows<4>(e, a); break;
                     case 3: finish_rows<6>(e, a); break;
@@ -617,9 +634,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     ptx::tc_fence_before();
     __syncthreads();
+    // (so have the last commits of the MMA warps, which arrive here too; the first CTA's warps waited for theirs)
+    if (rank != 0 && warp >= kWarpMma0 && warp < kWarpMma0 + kHalves) (void)ptx::mbar_wait(ptx::smem_u32(&sy->drain[warp - kWarpMma0]), 0);
+    __syncwarp();
+    ptx::cluster_sync();  // (what one CTA sends the other, loads and MMAs of the pair among it, has arrived)
     if (warp == kWarpMma0) {
         ptx::tc_fence_after();
-        ptx::tmem_dealloc(tmem_base, kTmemCols);
+        ptx::tmem_dealloc_pair(tmem_base, kTmemCols);
     }
 }
 
@@ -651,7 +672,7 @@ extern "C" int b200moe_grouped_gemm_mxfp4(const void* x, const uint8_t* x_scale,
     if (gate_up_silu != 0 && gate_up_silu != 1) return B200MOE_ERR_ARGUMENT;
     if (M == 0) return B200MOE_OK;
     // (unit numbers)
-    if ((M / mf::kMaxR + G) * ((N + 127) / 128) > 0x3FFFFFFLL) return B200MOE_ERR_SHAPE;
+    if ((M / mf::kMaxR + G) * ((N + 255) / 256) > 0x3FFFFFFLL) return B200MOE_ERR_SHAPE;
     if (!x || !x_scale || !weight || !weight_scale || !group_list || !out || (gate_up_silu && !out_scale)) return B200MOE_ERR_NULL_POINTER;
     const auto aligned4 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; };
     if (!aligned16(x) || !aligned16(weight) || !aligned16(out) || !aligned4(x_scale) || !aligned4(weight_scale) || !aligned4(out_scale))
@@ -675,7 +696,7 @@ extern "C" int b200moe_grouped_gemm_mxfp4(const void* x, const uint8_t* x_scale,
     if (rc != B200MOE_OK) return rc;
     const auto kernel = gate_up_silu ? mf::grouped_kernel<mf::GateUp> : mf::grouped_kernel<mf::Plain>;
     B200MOE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, mf::kSmemBytes));
-    B200MOE_CUDA_TRY(launch_dependent(kernel, (unsigned)sm_count(), mf::kThreads, mf::kSmemBytes, static_cast<cudaStream_t>(stream), map_w,
+    B200MOE_CUDA_TRY(launch_dependent(kernel, (unsigned)(sm_count() / 2 * 2), mf::kThreads, mf::kSmemBytes, static_cast<cudaStream_t>(stream), map_w,
                                       map_x64, map_x16, a));
     return B200MOE_OK;
 }

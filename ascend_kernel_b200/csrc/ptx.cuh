@@ -336,7 +336,7 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r
 // D[tmem] (+)= A * B, both e2m1 (two to a byte, K-major) with an e8m0 scale per 32 k in tensor memory, fp32 sums; 64 k.  Scales: row r of an
 // operand in lane r % 32 of column r / 32, the four bytes of a column for 128 k of which the instruction descriptor names two.
 // The same in each quarter of the lanes.  Both descriptors have the upper word `desc_hi`.
-__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint32_t desc_a, uint32_t desc_b, uint32_t desc_hi, uint32_t idesc, uint32_t tmem_sa,
+__device__ __forceinline__ void umma_mxf4_pair(uint32_t tmem_d, uint32_t desc_a, uint32_t desc_b, uint32_t desc_hi, uint32_t idesc, uint32_t tmem_sa,
                                           uint32_t tmem_sb, uint32_t accumulate) {
     asm volatile(
         "{\n"
@@ -345,7 +345,7 @@ __device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint32_t desc_a, uint
         "mov.b64 a, {%1, %3};\n"
         "mov.b64 b, {%2, %3};\n"
         "setp.ne.b32 p, %7, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %4, [%5], [%6], p;\n"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %4, [%5], [%6], p;\n"
         "}\n" ::"r"(tmem_d),
         "r"(desc_a), "r"(desc_b), "r"(desc_hi), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
         : "memory");
