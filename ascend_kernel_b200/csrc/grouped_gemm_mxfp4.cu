@@ -353,9 +353,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int x_at = kHalves * kSegs * kBlockBytes;  // of a stage: the codes of the weights, then those of x
     const int segs = (a.K + kSegK - 1) / kSegK, words = a.words, stages = (segs + kSegs - 1) / kSegs;
 
-    // registers of a lane: 72, 120 and twice 160 for the four warps of each kind, together as many as the launch has
+    // registers of a lane: 56, 104 and twice 176 for the four warps of each kind, together as many as the launch has
     if (warp < kWarpScale0) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == kWarpLoad) {
             // ------------------------------ codes ------------------------------
             // The warp walks together and one lane issues.
@@ -465,7 +465,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             __syncwarp();
         }
     } else if (warp < kWarpEpi0) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         // ------------------------------ scales ------------------------------
         // A thread fetches a row of every block of 128, 16 bytes (512 k) of each; the warps exchange them through shared memory, since each
         // writes all rows to its quarter of the lanes: row r in lane r % 32 of column r / 32, four columns for a word (128 k) of 128 rows.
@@ -591,7 +591,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             cph ^= cb == 0;
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
         // ------------------------------ epilogue ------------------------------
         Share e;
         e.group = (warp - kWarpEpi0) >> 2;
