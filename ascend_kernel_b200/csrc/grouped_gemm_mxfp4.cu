@@ -16,6 +16,7 @@
 #include "common.cuh"
 #include "mxfp4.cuh"
 #include "ptx.cuh"
+#include "tile_ring.h"
 
 namespace b200moe {
 namespace mf {
@@ -29,17 +30,19 @@ constexpr int kChunkWords = 4;           // of scales: 16 bytes, 512 k of a row
 constexpr int kMaxSlots = 10, kMaxBufs = 4;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kStripBytes = 1024;        // of an epilogue warp: 16 tokens x 32 columns in bf16
-constexpr int kBigBox = 64, kSmallBox = 16;
+constexpr int kBoxes[3] = {64, 32, 16};  // rows of x that a load takes
 constexpr int kScaleRows = 2 * 128 + kMaxR;
 constexpr int kExchangeBytes = 2 * kScaleRows * 16;
-constexpr int kBarrierBytes = 1024;
+constexpr int kBarrierBytes = 2048;
 constexpr int kSmemBytes = 227 * 1024;
 
 // What a tile is: the number of blocks of 128 weight columns, whether they are gate and up columns, and the segments of a stage.
 template <int HALVES, bool GATE, int SEGS>
 struct Mode {
     static constexpr int kHalves = HALVES, kSegs = SEGS, kWords = 2 * SEGS;  // (a word of scales: 128 k)
-    static constexpr bool kGate = GATE;
+    static constexpr bool kGate = GATE, kDrawn = !GATE;
+    // loads of a segment of the weights: blocks of 128 columns that are neighbours, and their segments too, come together
+    static constexpr int kWeightBoxes = GATE || SEGS > 1 ? HALVES : 1, kBoxColumns = 128 * HALVES / kWeightBoxes;
     // columns that a tile advances by (gate/up: of each), and the CTA's first
     static constexpr int kTileColumns = GATE ? 256 : 256 * HALVES;
     static __device__ __forceinline__ int first_column(int nt, uint32_t rank) { return nt * kTileColumns + (int)rank * (kTileColumns / 2); }
@@ -62,6 +65,8 @@ struct Args {
     uint8_t* out_scale;
     int M, K, N, G, gl_type;
     int words;         // of a row of scales
+    int dynamic;       // whether the pairs draw their tiles (from the workspace's first word) or take every n-th
+    int* ticket;
     int* findings;
 };
 
@@ -76,7 +81,8 @@ struct Sync {
     uint64_t drain[2];
     uint32_t tmem_base;
     int abort;
-    int n_units, width;          // width: token rows of the widest tile, rounded up to 32
+    int n_tiles, width;          // width: token rows of the widest tile, rounded up to 32
+    alignas(16) TileEntry ring[kTileRing];
 };
 static_assert(sizeof(Sync) <= kBarrierBytes, "barrier block");
 
@@ -84,27 +90,30 @@ struct Tile {
     int g, row0, rows, n, nt;  // n: rows rounded up to 32
 };
 
-// Waits are a whole warp's: it votes at every poll and so leaves them together.
+// Waits and tile look-ups are a whole warp's: it votes at every poll and so leaves them together.
 __device__ __forceinline__ bool all(bool v) { return __all_sync(0xffffffffu, v); }
 // A value that every lane has, in a form that shows it.
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+// Whether a poll that has failed `spins` times gives up: the other roles have, or the time is over.
+__device__ __forceinline__ bool give_up(uint32_t spins, uint64_t& t0, Sync* sy, int* findings, int id) {
+    if ((spins & 0xFF) != 0xFF) return false;  // (the clock is not read in a wait that ends soon)
+    if (t0 == 0) {
+        t0 = ptx::globaltimer_ns();
+        return false;
+    }
+    bool out = *reinterpret_cast<volatile int*>(&sy->abort) != 0;
+    if (!out && ptx::globaltimer_ns() - t0 > ptx::kWaitLimitNs) {
+        *reinterpret_cast<volatile int*>(&sy->abort) = 1;
+        keep_finding(findings, kDevWaitExpired, id);
+        out = true;
+    }
+    return !all(!out);
+}
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Sync* sy, int* findings, int id) {
     const uint32_t b = ptx::smem_u32(bar);
     uint64_t t0 = 0;
-    for (uint32_t spins = 0; !all(ptx::mbar_try_wait(b, parity)); ++spins) {
-        if ((spins & 0xFF) != 0) continue;
-        if (spins == 0) {
-            t0 = ptx::globaltimer_ns();
-            continue;
-        }
-        bool out = *reinterpret_cast<volatile int*>(&sy->abort) != 0;
-        if (!out && ptx::globaltimer_ns() - t0 > ptx::kWaitLimitNs) {
-            *reinterpret_cast<volatile int*>(&sy->abort) = 1;
-            keep_finding(findings, kDevWaitExpired, id);
-            out = true;
-        }
-        if (!all(!out)) return false;
-    }
+    for (uint32_t spins = 0; !all(ptx::mbar_try_wait(b, parity)); ++spins)
+        if (give_up(spins, t0, sy, findings, id)) return false;
     return true;
 }
 
@@ -113,23 +122,57 @@ __device__ __forceinline__ int tiles_of(int rows) { return (rows + kMaxR - 1) / 
 __device__ __forceinline__ int tile_rows_of(int rows, int tiles) { return ((rows + tiles - 1) / tiles + 31) & ~31; }
 
 // Inside an expert the row tiles of a weight column run together, so that they share the weights in L2.
-__device__ __forceinline__ Tile locate(int unit, const int* prefix, const int* row_start, int G, int n_nt) {
-    int lo = 0, hi = G;  // largest g with prefix[g] <= unit
+struct Tiles {
+    const int *prefix, *row_start;
+    int G, n_nt, n, pair, pairs;
+};
+__device__ __forceinline__ Tile locate(const Tiles& all, int tile) {
+    int lo = 0, hi = all.G;  // largest g with prefix[g] <= tile
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (prefix[mid] <= unit) lo = mid;
+        if (all.prefix[mid] <= tile) lo = mid;
         else hi = mid;
     }
-    const int j = unit - prefix[lo], mt = (prefix[lo + 1] - prefix[lo]) / n_nt;
+    const int j = tile - all.prefix[lo], mt = (all.prefix[lo + 1] - all.prefix[lo]) / all.n_nt;
     const int nt = j / mt, m = j - nt * mt;
-    const int rows = row_start[lo + 1] - row_start[lo], tr = tile_rows_of(rows, mt);
+    const int rows = all.row_start[lo + 1] - all.row_start[lo], tr = tile_rows_of(rows, mt);
     Tile t;
     t.g = lo;
     t.nt = nt;
-    t.row0 = row_start[lo] + m * tr;
+    t.row0 = all.row_start[lo] + m * tr;
     t.rows = min(tr, rows - m * tr);
     t.n = (t.rows + 31) & ~31;
     return t;
+}
+
+// The pair's next tile; false when the schedule has ended, a wait expired or another role aborted.
+//
+// Gate/up: every n-th tile, which each role finds by itself (seq: its number).  Otherwise the pairs draw their tiles, and the loading warp of the first
+// CTA hands them to the other roles through a ring, a tile ahead (seq: the tile's place there).  Every n-th | drawn, us: 256 experts, 4096 x 8 rows,
+// 2048 x 7168: 386 | 377; 37 x 8 rows 229 | 219; gate/up of 4096 x 8 rows, 7168 x 4096: 683 | 690, of 8192 x 8 Zipf rows 1107 | 1141.
+template <class M>
+__device__ __forceinline__ bool next_tile(const Tiles& tiles, Sync* sy, uint32_t& seq, Tile& t, const Args& a) {
+    if constexpr (!M::kDrawn) {
+        if ((int)seq >= tiles.n) return false;
+        t = locate(tiles, (int)seq);
+        seq += (uint32_t)tiles.pairs;
+        return true;
+    } else {
+        const TileEntry* e = &sy->ring[seq % kTileRing];
+        const uint32_t want = seq + 1;
+        TileEntry v;
+        uint64_t t0 = 0;
+        for (uint32_t spins = 0; !all(tile_entry_is(v = ring_load(e), want)); ++spins)
+            if (give_up(spins, t0, sy, a.findings, 90)) return false;
+        ++seq;
+        t.rows = tile_entry_rows(v);
+        if (t.rows == 0) return false;
+        t.row0 = tile_entry_row0(v);
+        t.g = tile_entry_expert(v);
+        t.nt = tile_entry_column(v);
+        t.n = (t.rows + 31) & ~31;
+        return true;
+    }
 }
 
 // 2^v and 1 / v; what is below 2^-126 as 0 (the first of these is then added to 1, the second multiplies what it divides)
@@ -255,19 +298,20 @@ __device__ __forceinline__ void store_quantized(float (&h)[16], const Tile& t, i
 // silu(gate) * up of every other piece of 16 tokens, NC at most, in registers before the first is quantised.
 template <int NC>
 __device__ __forceinline__ void finish_quantized(const Share& e, const Args& a) {
-    uint32_t v[2][2][16];
+    uint32_t v[2][2][8];
     float h[NC][16];
-    const auto fetch = [&](int c, uint32_t(&d)[2][16]) {
-        ptx::tmem_ld_32x16(e.tmem + (uint32_t)((2 * c + e.group) * 16), d[0]);
-        ptx::tmem_ld_32x16(e.tmem + e.width + (uint32_t)((2 * c + e.group) * 16), d[1]);
+    const auto fetch = [&](int s, uint32_t(&d)[2][8]) {  // half a piece
+        const uint32_t at = e.tmem + (uint32_t)(((s & ~1) + e.group) * 16 + (s & 1) * 8);
+        ptx::tmem_ld_32x8(at, d[0]);
+        ptx::tmem_ld_32x8(at + e.width, d[1]);
     };
     fetch(0, v[0]);
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
+    for (int s = 0; s < 2 * NC; ++s) {
         ptx::tmem_ld_wait();
-        if (c + 1 < NC) fetch(c + 1, v[(c + 1) & 1]);
+        if (s + 1 < 2 * NC) fetch(s + 1, v[(s + 1) & 1]);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) h[c][i] = silu(__uint_as_float(v[c & 1][0][i])) * __uint_as_float(v[c & 1][1][i]);
+        for (int i = 0; i < 8; ++i) h[s >> 1][(s & 1) * 8 + i] = silu(__uint_as_float(v[s & 1][0][i])) * __uint_as_float(v[s & 1][1][i]);
     }
     release(e);
 #pragma unroll
@@ -277,7 +321,7 @@ __device__ __forceinline__ void finish_quantized(const Share& e, const Args& a) 
 template <class M>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x64,
-                   const __grid_constant__ CUtensorMap map_x16, const Args a) {
+                   const __grid_constant__ CUtensorMap map_x32, const __grid_constant__ CUtensorMap map_x16, const Args a) {
     constexpr int kHalves = M::kHalves, kSegs = M::kSegs, kWords = M::kWords;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = smem_raw + ((1024u - (ptx::smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -295,6 +339,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // what needs nothing from memory comes first: the kernel may have started beside the end of the one before it
     if (threadIdx.x == kThreads - 32) {
         sy->abort = 0;
+        for (int i = 0; i < kTileRing; ++i) sy->ring[i] = tile_entry(0u, 0u, 0u, 0u, 0u);
         const auto init = [](uint64_t* b, int n, uint32_t count) {
             for (int i = 0; i < n; ++i) ptx::mbar_init(ptx::smem_u32(b + i), count);
         };
@@ -309,6 +354,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&map_w);
         ptx::prefetch_tensormap(&map_x64);
+        ptx::prefetch_tensormap(&map_x32);
         ptx::prefetch_tensormap(&map_x16);
     }
     if (warp == kWarpMma0) {
@@ -334,7 +380,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         if (lane == 0) {
             prefix[a.G] = total * n_nt;
-            sy->n_units = total * n_nt;
+            sy->n_tiles = total * n_nt;
             sy->width = max(wide, 32);
         }
     }
@@ -344,13 +390,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ptx::tc_fence_after();
 
     const uint32_t tmem_base = (uint32_t)uniform((int)*reinterpret_cast<volatile uint32_t*>(&sy->tmem_base));
-    const int n_units = uniform(sy->n_units), width = uniform(sy->width);
+    const int n_tiles = uniform(sy->n_tiles), width = uniform(sy->width);
     const int slot_bytes = M::slot_bytes(width), n_slots = min(kMaxSlots, M::kRingBytes / slot_bytes);
     // tensor memory: the sums of one to four tiles from the start, two chunks of scales at the end
     constexpr int kScaleColumns = M::kScaleColumns, kXScaleAt = kChunkWords * 4 * kHalves;
     const int n_bufs = min(kMaxBufs, ((int)kTmemCols - 2 * kScaleColumns) / (kHalves * width));
     const uint32_t scale0 = tmem_base + kTmemCols - 2 * kScaleColumns;
     const int x_at = kHalves * kSegs * kBlockBytes;  // of a stage: the codes of the weights, then those of x
+    const Tiles tiles = {prefix, row_start, a.G, n_nt, n_tiles, pair, pairs};
     const int segs = (a.K + kSegK - 1) / kSegK, words = a.words, stages = (segs + kSegs - 1) / kSegs;
 
     // registers of a lane: 56, 104 and twice 176 for the four warps of each kind, together as many as the launch has
@@ -360,12 +407,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             // ------------------------------ codes ------------------------------
             // The warp walks together and one lane issues.
             const bool leader = ptx::elect_one();
-            uint32_t it = 0, slot = 0, ph = 0;
-            bool ok = true;
-            const uint32_t full0 = ptx::map_rank(ptx::smem_u32(sy->full), 0);
-            for (int unit = pair; ok && unit < n_units; unit += pairs) {
-                const Tile t = locate(unit, prefix, row_start, a.G, n_nt);
-                const int half = t.n >> 1, n_big = half / kBigBox, n_small = (half % kBigBox) / kSmallBox;
+            uint32_t it = 0, slot = 0, ph = 0, seq = M::kDrawn ? 0u : (uint32_t)pair, published = 0;
+            int tile = pair, drawn = 0;
+            bool live = true, ok = true;
+            const uint32_t full0 = ptx::map_rank(ptx::smem_u32(sy->full), 0), ring_there = ptx::map_rank(ptx::smem_u32(sy->ring), 1);
+            const auto publish = [&]() {
+                if (!M::kDrawn || rank != 0 || !live) return;
+                if (published > 0) tile = a.dynamic ? pairs + __reduce_add_sync(0xffffffffu, drawn) : tile + pairs;
+                live = tile < n_tiles;
+                TileEntry e = tile_entry(published + 1, 0u, 0u, 0u, 0u);  // rows 0: the schedule has ended
+                if (live) {
+                    const Tile f = locate(tiles, tile);
+                    e = tile_entry(published + 1, (uint32_t)f.row0, (uint32_t)f.rows, (uint32_t)f.g, (uint32_t)f.nt);
+                }
+                if (leader) {
+                    const uint32_t at = (published % kTileRing) * (uint32_t)sizeof(TileEntry);
+                    ring_store(&sy->ring[published % kTileRing], e);
+                    ptx::st_cluster_u64(ring_there + at, e.a);
+                    ptx::st_cluster_u64(ring_there + at + 8, e.b);
+                    if (live && a.dynamic) drawn = atomicAdd(a.ticket, 1);  // (needed a tile later)
+                }
+                ++published;
+            };
+            publish();
+            Tile t;
+            while (ok) {
+                publish();  // (a tile ahead: the other roles find it there)
+                if (!next_tile<M>(tiles, sy, seq, t, a)) break;
+                const int half = t.n >> 1;
                 const int col = M::first_column(t.nt, rank), row = t.row0 + (int)rank * half;
                 for (int kb = 0; kb < stages; ++kb, ++it) {
                     if (it >= (uint32_t)n_slots && !wait(&sy->empty[slot], ph ^ 1, sy, a.findings, 10)) { ok = false; break; }
@@ -378,12 +447,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             if (s >= here) break;
                             const int x = (kb * kSegs + s) * 128;
 #pragma unroll
-                            for (int u = 0; u < kHalves; ++u)
+                            for (int u = 0; u < M::kWeightBoxes; ++u)
                                 ptx::tma_load_3d_pair(dst + (u * kSegs + s) * kBlockBytes, &map_w, bar0, x, col + u * M::block_step(a.N), t.g);
                             uint32_t at = dst + x_at + s * width * 64;
                             int r = row;
-                            for (int b = 0; b < n_big; ++b, at += kBigBox * 128, r += kBigBox) ptx::tma_load_2d_pair(at, &map_x64, bar0, x, r);
-                            for (int b = 0; b < n_small; ++b, at += kSmallBox * 128, r += kSmallBox) ptx::tma_load_2d_pair(at, &map_x16, bar0, x, r);
+                            if (half & 64) ptx::tma_load_2d_pair(at, &map_x64, bar0, x, r), at += 64 * 128, r += 64;
+                            if (half & 32) ptx::tma_load_2d_pair(at, &map_x32, bar0, x, r), at += 32 * 128, r += 32;
+                            if (half & 16) ptx::tma_load_2d_pair(at, &map_x16, bar0, x, r);
                         }
                     }
                     __syncwarp();
@@ -414,8 +484,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const uint32_t a0 = (uint32_t)desc + ((ptx::smem_u32(ring) + (uint32_t)(u * kSegs * kBlockBytes)) >> 4);
             const uint32_t x0 = (uint32_t)desc + ((ptx::smem_u32(ring) + (uint32_t)x_at) >> 4);
             const uint32_t slot_step = (uint32_t)slot_bytes >> 4, seg_step = (uint32_t)width * 4;
-            for (int unit = pair; ok && unit < n_units; unit += pairs, ++n) {
-                const int cols = uniform(locate(unit, prefix, row_start, a.G, n_nt).n), x_words = cols > 128 ? 8 : 4;
+            uint32_t seq = M::kDrawn ? 0u : (uint32_t)pair;
+            Tile t;
+            for (; ok && next_tile<M>(tiles, sy, seq, t, a); ++n) {
+                const int cols = uniform(t.n), x_words = cols > 128 ? 8 : 4;
                 const uint32_t idesc = ptx::umma_idesc_mxf4(256, cols), d = tmem_base + (buf * kHalves + u) * (uint32_t)width;
                 // the epilogue has taken what the buffer held
                 if (n >= (uint32_t)n_bufs && !wait(&sy->d_empty[buf], bph ^ 1, sy, a.findings, 30)) break;
@@ -475,17 +547,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             uint4 v[kHalves + 2];  // of the weights' blocks and the two of x
             int cols;              // token rows of the tile rounded up; 0: the schedule has ended
         };
-        int unit = pair - pairs, at = chunks, cols = 0;
+        int at = chunks, cols = 0;
+        uint32_t seq = M::kDrawn ? 0u : (uint32_t)pair;
+        bool live = true;
         const uint32_t* src[kHalves + 2];  // NULL: no row there, zeros
         const auto fetch = [&](Chunk& c) {
             if (at == chunks) {
-                unit += pairs;
-                if (unit >= n_units) {
-                    unit -= pairs;
+                Tile t;
+                if (live) live = next_tile<M>(tiles, sy, seq, t, a);
+                if (!live) {
                     c.cols = 0;
                     return;
                 }
-                const Tile t = locate(unit, prefix, row_start, a.G, n_nt);
                 cols = t.n;
 #pragma unroll
                 for (int u = 0; u < kHalves; ++u) {
@@ -600,8 +673,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int quarter = warp & 3;
         const uint32_t d_empty0 = ptx::map_rank(ptx::smem_u32(sy->d_empty), 0);
         uint32_t buf = 0, ph = 0;
-        for (int unit = pair; unit < n_units; unit += pairs) {
-            e.t = locate(unit, prefix, row_start, a.G, n_nt);
+        uint32_t seq = M::kDrawn ? 0u : (uint32_t)pair;
+        while (next_tile<M>(tiles, sy, seq, e.t, a)) {
             e.tmem = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * (uint32_t)(kHalves * width);
             e.col = M::first_column(e.t.nt, rank) + quarter * 32;
             e.d_empty = d_empty0 + buf * 8;
@@ -652,6 +725,7 @@ static bool sizes_ok(int64_t M, int64_t K, int64_t N, int64_t G) {
     return M >= 0 && M <= kMost && K > 0 && K <= kMost && N > 0 && N <= kMost && G > 0 && G <= kMaxExperts;
 }
 constexpr size_t kWorkspaceBytes = 256;
+constexpr int64_t kPairs = 74;  // of a B200's multiprocessors (rules go by the sizes of a call alone)
 
 }  // namespace mf
 }  // namespace b200moe
@@ -689,14 +763,18 @@ extern "C" int b200moe_grouped_gemm_mxfp4(const void* x, const uint8_t* x_scale,
     a.gl_type = group_list_type;
     a.words = (int)(mxfp4::scale_width(K) / 4);
     a.findings = findings != nullptr ? findings : findings_words();
-    CUtensorMap map_w, map_x64, map_x16;
-    int rc = make_tensor_map_3d_u8(&map_w, weight, (uint64_t)G, (uint64_t)N, (uint64_t)(K / 2), 128, 128);
-    if (rc == B200MOE_OK) rc = make_tensor_map_2d(&map_x64, x, 1, (uint64_t)M, (uint64_t)(K / 2), mf::kBigBox, 128, true);
-    if (rc == B200MOE_OK) rc = make_tensor_map_2d(&map_x16, x, 1, (uint64_t)M, (uint64_t)(K / 2), mf::kSmallBox, 128, true);
+    a.ticket = static_cast<int*>(workspace);
+    // (few tiles are dealt out in turn: the ticket would have to be cleared first)
+    a.dynamic = !gate_up_silu && (N + mf::Plain::kTileColumns - 1) / mf::Plain::kTileColumns * std::min(G, M) >= 16 * mf::kPairs;
+    CUtensorMap map_w, map_x[3];
+    int rc = make_tensor_map_3d_u8(&map_w, weight, (uint64_t)G, (uint64_t)N, (uint64_t)(K / 2), gate_up_silu ? mf::GateUp::kBoxColumns : mf::Plain::kBoxColumns, 128);
+    for (int i = 0; i < 3 && rc == B200MOE_OK; ++i)
+        rc = make_tensor_map_2d(&map_x[i], x, 1, (uint64_t)M, (uint64_t)(K / 2), mf::kBoxes[i], 128, true);
     if (rc != B200MOE_OK) return rc;
     const auto kernel = gate_up_silu ? mf::grouped_kernel<mf::GateUp> : mf::grouped_kernel<mf::Plain>;
     B200MOE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, mf::kSmemBytes));
+    if (a.dynamic) B200MOE_CUDA_TRY(cudaMemsetAsync(workspace, 0, mf::kWorkspaceBytes, static_cast<cudaStream_t>(stream)));
     B200MOE_CUDA_TRY(launch_dependent(kernel, (unsigned)(sm_count() / 2 * 2), mf::kThreads, mf::kSmemBytes, static_cast<cudaStream_t>(stream), map_w,
-                                      map_x64, map_x16, a));
+                                      map_x[0], map_x[1], map_x[2], a));
     return B200MOE_OK;
 }
