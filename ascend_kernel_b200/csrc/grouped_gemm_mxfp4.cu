@@ -16,7 +16,6 @@
 #include "common.cuh"
 #include "mxfp4.cuh"
 #include "ptx.cuh"
-#include "tile_ring.h"
 
 namespace b200moe {
 namespace mf {
@@ -30,17 +29,17 @@ constexpr int kChunkWords = 4;           // of scales: 16 bytes, 512 k of a row
 constexpr int kMaxSlots = 10, kMaxBufs = 4;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kStripBytes = 1024;        // of an epilogue warp: 16 tokens x 32 columns in bf16
-constexpr int kBoxes[3] = {64, 32, 16};  // rows of x that a load takes
+constexpr int kBoxes[4] = {64, 32, 16, 8};  // rows of x that a load takes
 constexpr int kScaleRows = 2 * 128 + kMaxR;
 constexpr int kExchangeBytes = 2 * kScaleRows * 16;
-constexpr int kBarrierBytes = 2048;
+constexpr int kBarrierBytes = 1024;
 constexpr int kSmemBytes = 227 * 1024;
 
 // What a tile is: the number of blocks of 128 weight columns, whether they are gate and up columns, and the segments of a stage.
 template <int HALVES, bool GATE, int SEGS>
 struct Mode {
     static constexpr int kHalves = HALVES, kSegs = SEGS, kWords = 2 * SEGS;  // (a word of scales: 128 k)
-    static constexpr bool kGate = GATE, kDrawn = !GATE;
+    static constexpr bool kGate = GATE;
     // loads of a segment of the weights: blocks of 128 columns that are neighbours, and their segments too, come together
     static constexpr int kWeightBoxes = GATE || SEGS > 1 ? HALVES : 1, kBoxColumns = 128 * HALVES / kWeightBoxes;
     // columns that a tile advances by (gate/up: of each), and the CTA's first
@@ -65,8 +64,6 @@ struct Args {
     uint8_t* out_scale;
     int M, K, N, G, gl_type;
     int words;         // of a row of scales
-    int dynamic;       // whether the pairs draw their tiles (from the workspace's first word) or take every n-th
-    int* ticket;
     int* findings;
 };
 
@@ -81,13 +78,12 @@ struct Sync {
     uint64_t drain[2];
     uint32_t tmem_base;
     int abort;
-    int n_tiles, width;          // width: token rows of the widest tile, rounded up to 32
-    alignas(16) TileEntry ring[kTileRing];
+    int n_tiles, width;          // width: token rows of the widest tile, rounded up to 16
 };
 static_assert(sizeof(Sync) <= kBarrierBytes, "barrier block");
 
 struct Tile {
-    int g, row0, rows, n, nt;  // n: rows rounded up to 32
+    int g, row0, rows, n, nt;  // n: rows rounded up to 16
 };
 
 // Waits and tile look-ups are a whole warp's: it votes at every poll and so leaves them together.
@@ -117,9 +113,9 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Sync* sy, i
     return true;
 }
 
-// An expert's rows are cut into the fewest tiles, of equal size rounded up to 32.
+// An expert's rows are cut into the fewest tiles, of equal size rounded up to 16.
 __device__ __forceinline__ int tiles_of(int rows) { return (rows + kMaxR - 1) / kMaxR; }
-__device__ __forceinline__ int tile_rows_of(int rows, int tiles) { return ((rows + tiles - 1) / tiles + 31) & ~31; }
+__device__ __forceinline__ int tile_rows_of(int rows, int tiles) { return ((rows + tiles - 1) / tiles + 15) & ~15; }
 
 // Inside an expert the row tiles of a weight column run together, so that they share the weights in L2.
 struct Tiles {
@@ -141,38 +137,18 @@ __device__ __forceinline__ Tile locate(const Tiles& all, int tile) {
     t.nt = nt;
     t.row0 = all.row_start[lo] + m * tr;
     t.rows = min(tr, rows - m * tr);
-    t.n = (t.rows + 31) & ~31;
+    t.n = (t.rows + 15) & ~15;
     return t;
 }
 
-// The pair's next tile; false when the schedule has ended, a wait expired or another role aborted.
-//
-// Gate/up: every n-th tile, which each role finds by itself (seq: its number).  Otherwise the pairs draw their tiles, and the loading warp of the first
-// CTA hands them to the other roles through a ring, a tile ahead (seq: the tile's place there).  Every n-th | drawn, us: 256 experts, 4096 x 8 rows,
-// 2048 x 7168: 386 | 377; 37 x 8 rows 229 | 219; gate/up of 4096 x 8 rows, 7168 x 4096: 683 | 690, of 8192 x 8 Zipf rows 1107 | 1141.
-template <class M>
-__device__ __forceinline__ bool next_tile(const Tiles& tiles, Sync* sy, uint32_t& seq, Tile& t, const Args& a) {
-    if constexpr (!M::kDrawn) {
-        if ((int)seq >= tiles.n) return false;
-        t = locate(tiles, (int)seq);
-        seq += (uint32_t)tiles.pairs;
-        return true;
-    } else {
-        const TileEntry* e = &sy->ring[seq % kTileRing];
-        const uint32_t want = seq + 1;
-        TileEntry v;
-        uint64_t t0 = 0;
-        for (uint32_t spins = 0; !all(tile_entry_is(v = ring_load(e), want)); ++spins)
-            if (give_up(spins, t0, sy, a.findings, 90)) return false;
-        ++seq;
-        t.rows = tile_entry_rows(v);
-        if (t.rows == 0) return false;
-        t.row0 = tile_entry_row0(v);
-        t.g = tile_entry_expert(v);
-        t.nt = tile_entry_column(v);
-        t.n = (t.rows + 31) & ~31;
-        return true;
-    }
+// The pair's next tile, every n-th of all, which each role finds by itself; false at the end.  (Drawing tiles from a counter costs a call that clears it
+// and a ring between the roles, and a steady loop, which the power limit bounds, gains nothing: 256 experts, 4096 x 8 rows, 2048 x
+// 7168: alone 386 | drawn 377, in a loop 416 | 430.)
+__device__ __forceinline__ bool next_tile(const Tiles& all, int& tile, Tile& t) {
+    if (tile >= all.n) return false;
+    t = locate(all, tile);
+    tile += all.pairs;
+    return true;
 }
 
 // 2^v and 1 / v; what is below 2^-126 as 0 (the first of these is then added to 1, the second multiplies what it divides)
@@ -321,7 +297,7 @@ __device__ __forceinline__ void finish_quantized(const Share& e, const Args& a) 
 template <class M>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x64,
-                   const __grid_constant__ CUtensorMap map_x32, const __grid_constant__ CUtensorMap map_x16, const Args a) {
+                   const __grid_constant__ CUtensorMap map_x32, const __grid_constant__ CUtensorMap map_x16, const __grid_constant__ CUtensorMap map_x8, const Args a) {
     constexpr int kHalves = M::kHalves, kSegs = M::kSegs, kWords = M::kWords;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = smem_raw + ((1024u - (ptx::smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -339,7 +315,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // what needs nothing from memory comes first: the kernel may have started beside the end of the one before it
     if (threadIdx.x == kThreads - 32) {
         sy->abort = 0;
-        for (int i = 0; i < kTileRing; ++i) sy->ring[i] = tile_entry(0u, 0u, 0u, 0u, 0u);
         const auto init = [](uint64_t* b, int n, uint32_t count) {
             for (int i = 0; i < n; ++i) ptx::mbar_init(ptx::smem_u32(b + i), count);
         };
@@ -356,6 +331,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ptx::prefetch_tensormap(&map_x64);
         ptx::prefetch_tensormap(&map_x32);
         ptx::prefetch_tensormap(&map_x16);
+        ptx::prefetch_tensormap(&map_x8);
     }
     if (warp == kWarpMma0) {
         ptx::tmem_alloc_pair(ptx::smem_u32(&sy->tmem_base), kTmemCols);
@@ -381,7 +357,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (lane == 0) {
             prefix[a.G] = total * n_nt;
             sy->n_tiles = total * n_nt;
-            sy->width = max(wide, 32);
+            sy->width = max(wide, 16);
         }
     }
     ptx::tc_fence_before();
@@ -407,33 +383,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             // ------------------------------ codes ------------------------------
             // The warp walks together and one lane issues.
             const bool leader = ptx::elect_one();
-            uint32_t it = 0, slot = 0, ph = 0, seq = M::kDrawn ? 0u : (uint32_t)pair, published = 0;
-            int tile = pair, drawn = 0;
-            bool live = true, ok = true;
-            const uint32_t full0 = ptx::map_rank(ptx::smem_u32(sy->full), 0), ring_there = ptx::map_rank(ptx::smem_u32(sy->ring), 1);
-            const auto publish = [&]() {
-                if (!M::kDrawn || rank != 0 || !live) return;
-                if (published > 0) tile = a.dynamic ? pairs + __reduce_add_sync(0xffffffffu, drawn) : tile + pairs;
-                live = tile < n_tiles;
-                TileEntry e = tile_entry(published + 1, 0u, 0u, 0u, 0u);  // rows 0: the schedule has ended
-                if (live) {
-                    const Tile f = locate(tiles, tile);
-                    e = tile_entry(published + 1, (uint32_t)f.row0, (uint32_t)f.rows, (uint32_t)f.g, (uint32_t)f.nt);
-                }
-                if (leader) {
-                    const uint32_t at = (published % kTileRing) * (uint32_t)sizeof(TileEntry);
-                    ring_store(&sy->ring[published % kTileRing], e);
-                    ptx::st_cluster_u64(ring_there + at, e.a);
-                    ptx::st_cluster_u64(ring_there + at + 8, e.b);
-                    if (live && a.dynamic) drawn = atomicAdd(a.ticket, 1);  // (needed a tile later)
-                }
-                ++published;
-            };
-            publish();
+            uint32_t it = 0, slot = 0, ph = 0;
+            int tile = pair;
+            bool ok = true;
+            const uint32_t full0 = ptx::map_rank(ptx::smem_u32(sy->full), 0);
             Tile t;
-            while (ok) {
-                publish();  // (a tile ahead: the other roles find it there)
-                if (!next_tile<M>(tiles, sy, seq, t, a)) break;
+            while (ok && next_tile(tiles, tile, t)) {
                 const int half = t.n >> 1;
                 const int col = M::first_column(t.nt, rank), row = t.row0 + (int)rank * half;
                 for (int kb = 0; kb < stages; ++kb, ++it) {
@@ -453,7 +408,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             int r = row;
                             if (half & 64) ptx::tma_load_2d_pair(at, &map_x64, bar0, x, r), at += 64 * 128, r += 64;
                             if (half & 32) ptx::tma_load_2d_pair(at, &map_x32, bar0, x, r), at += 32 * 128, r += 32;
-                            if (half & 16) ptx::tma_load_2d_pair(at, &map_x16, bar0, x, r);
+                            if (half & 16) ptx::tma_load_2d_pair(at, &map_x16, bar0, x, r), at += 16 * 128, r += 16;
+                            if (half & 8) ptx::tma_load_2d_pair(at, &map_x8, bar0, x, r);
                         }
                     }
                     __syncwarp();
@@ -484,9 +440,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const uint32_t a0 = (uint32_t)desc + ((ptx::smem_u32(ring) + (uint32_t)(u * kSegs * kBlockBytes)) >> 4);
             const uint32_t x0 = (uint32_t)desc + ((ptx::smem_u32(ring) + (uint32_t)x_at) >> 4);
             const uint32_t slot_step = (uint32_t)slot_bytes >> 4, seg_step = (uint32_t)width * 4;
-            uint32_t seq = M::kDrawn ? 0u : (uint32_t)pair;
+            int tile = pair;
             Tile t;
-            for (; ok && next_tile<M>(tiles, sy, seq, t, a); ++n) {
+            for (; ok && next_tile(tiles, tile, t); ++n) {
                 const int cols = uniform(t.n), x_words = cols > 128 ? 8 : 4;
                 const uint32_t idesc = ptx::umma_idesc_mxf4(256, cols), d = tmem_base + (buf * kHalves + u) * (uint32_t)width;
                 // the epilogue has taken what the buffer held
@@ -548,13 +504,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             int cols;              // token rows of the tile rounded up; 0: the schedule has ended
         };
         int at = chunks, cols = 0;
-        uint32_t seq = M::kDrawn ? 0u : (uint32_t)pair;
+        int tile = pair;
         bool live = true;
         const uint32_t* src[kHalves + 2];  // NULL: no row there, zeros
         const auto fetch = [&](Chunk& c) {
             if (at == chunks) {
                 Tile t;
-                if (live) live = next_tile<M>(tiles, sy, seq, t, a);
+                if (live) live = next_tile(tiles, tile, t);
                 if (!live) {
                     c.cols = 0;
                     return;
@@ -673,8 +629,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int quarter = warp & 3;
         const uint32_t d_empty0 = ptx::map_rank(ptx::smem_u32(sy->d_empty), 0);
         uint32_t buf = 0, ph = 0;
-        uint32_t seq = M::kDrawn ? 0u : (uint32_t)pair;
-        while (next_tile<M>(tiles, sy, seq, e.t, a)) {
+        int tile = pair;
+        while (next_tile(tiles, tile, e.t)) {
             e.tmem = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * (uint32_t)(kHalves * width);
             e.col = M::first_column(e.t.nt, rank) + quarter * 32;
             e.d_empty = d_empty0 + buf * 8;
@@ -682,7 +638,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             ptx::tc_fence_after();
             // (the number of pieces is a constant, so that they stay in registers)
             if constexpr (M::kGate) {
-                switch (e.t.n / 32) {
+                switch ((e.t.n + 31) / 32) {
                     case 1: finish_quantized<1>(e, a); break;
                     case 2: finish_quantized<2>(e, a); break;
                     case 3: finish_quantized<3>(e, a); break;
@@ -691,7 +647,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     default: finish_quantized<6>(e, a); break;
                 }
             } else {
-                switch (e.t.n / 32) {
+                switch ((e.t.n + 31) / 32) {
                     case 1: finish_rows<2>(e, a); break;
                     case 2: finish_rows<4>(e, a); break;
                     case 3: finish_rows<6>(e, a); break;
@@ -725,7 +681,6 @@ static bool sizes_ok(int64_t M, int64_t K, int64_t N, int64_t G) {
     return M >= 0 && M <= kMost && K > 0 && K <= kMost && N > 0 && N <= kMost && G > 0 && G <= kMaxExperts;
 }
 constexpr size_t kWorkspaceBytes = 256;
-constexpr int64_t kPairs = 74;  // of a B200's multiprocessors (rules go by the sizes of a call alone)
 
 }  // namespace mf
 }  // namespace b200moe
@@ -763,18 +718,14 @@ extern "C" int b200moe_grouped_gemm_mxfp4(const void* x, const uint8_t* x_scale,
     a.gl_type = group_list_type;
     a.words = (int)(mxfp4::scale_width(K) / 4);
     a.findings = findings != nullptr ? findings : findings_words();
-    a.ticket = static_cast<int*>(workspace);
-    // (few tiles are dealt out in turn: the ticket would have to be cleared first)
-    a.dynamic = !gate_up_silu && (N + mf::Plain::kTileColumns - 1) / mf::Plain::kTileColumns * std::min(G, M) >= 16 * mf::kPairs;
-    CUtensorMap map_w, map_x[3];
+    CUtensorMap map_w, map_x[4];
     int rc = make_tensor_map_3d_u8(&map_w, weight, (uint64_t)G, (uint64_t)N, (uint64_t)(K / 2), gate_up_silu ? mf::GateUp::kBoxColumns : mf::Plain::kBoxColumns, 128);
-    for (int i = 0; i < 3 && rc == B200MOE_OK; ++i)
+    for (int i = 0; i < 4 && rc == B200MOE_OK; ++i)
         rc = make_tensor_map_2d(&map_x[i], x, 1, (uint64_t)M, (uint64_t)(K / 2), mf::kBoxes[i], 128, true);
     if (rc != B200MOE_OK) return rc;
     const auto kernel = gate_up_silu ? mf::grouped_kernel<mf::GateUp> : mf::grouped_kernel<mf::Plain>;
     B200MOE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, mf::kSmemBytes));
-    if (a.dynamic) B200MOE_CUDA_TRY(cudaMemsetAsync(workspace, 0, mf::kWorkspaceBytes, static_cast<cudaStream_t>(stream)));
     B200MOE_CUDA_TRY(launch_dependent(kernel, (unsigned)(sm_count() / 2 * 2), mf::kThreads, mf::kSmemBytes, static_cast<cudaStream_t>(stream), map_w,
-                                      map_x[0], map_x[1], map_x[2], a));
+                                      map_x[0], map_x[1], map_x[2], map_x[3], a));
     return B200MOE_OK;
 }
