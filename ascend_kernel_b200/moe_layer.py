@@ -75,6 +75,9 @@ class MoELayer:
         [E_local, H/128, 2I/128], w2 uint8 [E_local, I, H], s2 [E_local, I/128, H/128], o13 / o2 None, H and I multiples of 128 -- and a
         pass multiplies in 8 bits: the rows are quantised to e4m3 per 128 elements on their way to the experts, the gate/up
         GEMM's epilogue quantises silu(gate) * up, and the down projection takes that as it is.
+        ``weight_format="mxfp4"``: the experts are e2m1 with one e8m0 byte per 32 k along their rows -- w13 uint8 [E_local, 2I, H/2] (gate
+        columns first), s13 [E_local, 2I, H/32], w2 uint8 [E_local, H, I/2], s2 [E_local, H, I/32], o13 / o2 None, H and I multiples of 128
+        -- and a pass multiplies in 4 bits, its rows quantised per 32 elements at the same two places.
         ``exchange_buffers=2`` (p2p exchange only) doubles the exchange buffers, which ``OverlappedSteps``
         needs to run one step's token exchange beside the expert GEMMs of the step before."""
         self.ops = row_ops
@@ -89,10 +92,11 @@ class MoELayer:
             self.world, self.rank = 1, 0
         self.e_local = w13.shape[0]
         assert self.e_local * self.world == n_experts
-        self.hidden, self.inter = w13.shape[1], w2.shape[1]
+        if weight_format not in ("int8", "fp4", "fp8", "mxfp4"):
+            raise ValueError("weight_format must be 'int8', 'fp4', 'fp8' or 'mxfp4'")
+        # (4-bit rows run along k, two codes to a byte)
+        self.hidden, self.inter = (2 * w13.shape[2], 2 * w2.shape[2]) if weight_format == "mxfp4" else (w13.shape[1], w2.shape[1])
         self.device = w13.device
-        if weight_format not in ("int8", "fp4", "fp8"):
-            raise ValueError("weight_format must be 'int8', 'fp4' or 'fp8'")
         self.weight_format = weight_format
         if weight_format == "fp4":
             if o13 is not None or o2 is not None or row_ops is not CudaRowOps:
@@ -106,6 +110,15 @@ class MoELayer:
             if (self.hidden % 128 or self.inter % 128 or w13.shape[2] != 2 * self.inter or w2.shape[2] != self.hidden
                     or w13.element_size() != 1 or w2.element_size() != 1):
                 raise ValueError("expected w13 [E, H, 2I] and w2 [E, I, H] e4m3 codes, H and I multiples of 128")
+            fuse_silu, gemm = False, "generic"
+        elif weight_format == "mxfp4":
+            if o13 is not None or o2 is not None or row_ops is not CudaRowOps:
+                raise ValueError("4-bit floating-point experts take no offsets and run on the CUDA row operations only")
+            E, H, I = self.e_local, self.hidden, self.inter
+            if (H % 128 or I % 128 or tuple(w13.shape) != (E, 2 * I, H // 2) or tuple(w2.shape) != (E, H, I // 2)
+                    or tuple(s13.shape) != (E, 2 * I, H // 32) or tuple(s2.shape) != (E, H, I // 32)):
+                raise ValueError("expected w13 [E, 2I, H/2] with s13 [E, 2I, H/32] and w2 [E, H, I/2] with s2 [E, H, I/32], H and I "
+                                 "multiples of 128")
             fuse_silu, gemm = False, "generic"
         self.fuse_silu = (row_ops is CudaRowOps) if fuse_silu is None else bool(fuse_silu)
         if gemm is None:
@@ -180,7 +193,7 @@ class MoELayer:
         each result row where its code says (the return buffer of the rank the token came from) instead
         of into ``y``; packed GEMMs only.  ``rows_sum``: fp32 sums of the rows when the caller has them (the
         packed gate/up GEMM then skips its own pass over the rows).  ``max_rows``: rows an expert has at most,
-        where that is known.  ``row_scale``: the rows are e4m3 already, with these scales."""
+        where that is known.  ``row_scale``: the rows are quantised already, with these scales."""
         R = rows.shape[0]
         if y is None:
             y = torch.empty(R, self.hidden, dtype=torch.bfloat16, device=self.device)
@@ -212,6 +225,21 @@ class MoELayer:
                 ev[1].record()
                 ev[2].record()
             ops.grouped_gemm_fp8_block(act, act_scale, self.w2, self.s2, counts, y, group_list_type=1)
+            if ev:
+                ev[3].record()
+                self.timing = ev
+            return y
+        if self.weight_format == "mxfp4":
+            if row_scale is None:
+                rows, row_scale = ops.mxfp4_quantize_rows(rows)
+            act = torch.empty(R, self.inter // 2, dtype=torch.uint8, device=self.device)
+            act_scale = torch.empty(R, self.inter // 32, dtype=torch.uint8, device=self.device)
+            ops.grouped_gemm_mxfp4(rows, row_scale, self.w13, self.s13, counts, act, output_scale=act_scale, group_list_type=1,
+                                   gate_up_silu=True)
+            if ev:
+                ev[1].record()
+                ev[2].record()
+            ops.grouped_gemm_mxfp4(act, act_scale, self.w2, self.s2, counts, y, group_list_type=1)
             if ev:
                 ev[3].record()
                 self.timing = ev
@@ -307,6 +335,8 @@ class MoELayer:
         sums = row_scale = None
         if self.world == 1 and self.weight_format == "fp8":
             send, row_scale = ops.fp8_quantize_rows(x, token_of)  # gathered and quantised in one operator
+        elif self.world == 1 and self.weight_format == "mxfp4":
+            send, row_scale = ops.mxfp4_quantize_rows(x, token_of)
         elif (self.gather_sums and self.world == 1 and self.gemm == "packed" and self.o13 is not None
                 and self.ops is CudaRowOps):
             send, sums = ops.gather_rows(x, token_of, with_sums=True)
@@ -353,6 +383,23 @@ class MoELayer:
         mark("combine")
         self.phases = marks
         return out
+
+    @torch.no_grad()
+    def forward_routed(self, x, idx, weight):
+        """The pass on another router's choice: ``idx`` int32 [T, k] the experts of each token (an entry outside 0 .. n_experts - 1 is
+        a dropped pair) and ``weight`` fp32 [T, k]; x bf16 [T, H] -> bf16 [T, H].  For one rank without an exchange."""
+        if self.world != 1 or self.px is not None:
+            raise RuntimeError("forward_routed runs on one rank, without an exchange")
+        counts, token_of, slot = ops.moe_sort(idx, self.n_experts)
+        row_scale = None
+        if self.weight_format == "fp8":
+            send, row_scale = ops.fp8_quantize_rows(x, token_of)
+        elif self.weight_format == "mxfp4":
+            send, row_scale = ops.mxfp4_quantize_rows(x, token_of)
+        else:
+            send = ops.moe_dispatch(x, token_of, slot)
+        y = self._experts(send, counts, False, max_rows=x.shape[0], row_scale=row_scale)
+        return ops.moe_combine(y, weight, token_of, slot)
 
     def forward_host(self, x_host, logits_host, out_host=None):
         """End-to-end call with host buffers: pinned host -> device copies of this step's inputs,

@@ -95,3 +95,15 @@ def test_python_refuses_host_tensors():
                  lambda: ops.moe_combine(x, torch.zeros(2, 2), i.view(-1), i)):
         with pytest.raises(RuntimeError):
             call()
+
+
+def test_routed_pass_is_for_one_rank():
+    from ascend_kernel_b200.moe_layer import MoELayer
+
+    layer = object.__new__(MoELayer)
+    layer.world, layer.px = 2, None
+    with pytest.raises(RuntimeError, match="one rank"):
+        layer.forward_routed(None, None, None)
+    layer.world, layer.px = 1, object()
+    with pytest.raises(RuntimeError, match="one rank"):
+        layer.forward_routed(None, None, None)
