@@ -33,7 +33,7 @@ EXPORTS = [
     "b200moe_grouped_gemm_fp8_block_findings", "b200moe_moe_balance_loss_findings", "b200moe_findings_pair", "b200moe_read_findings_at",
     "b200moe_moe_sort", "b200moe_moe_sort_scratch_bytes", "b200moe_moe_dispatch", "b200moe_moe_dispatch_grad", "b200moe_moe_combine",
     "b200moe_moe_combine_grad", "b200moe_mxfp4_quantize_rows", "b200moe_mxfp4_quantize_rows_scratch_bytes",
-    "b200moe_grouped_gemm_mxfp4", "b200moe_grouped_gemm_mxfp4_workspace_bytes",
+    "b200moe_grouped_gemm_mxfp4",
     "b200moe_set_gemm_reserved_sms", "b200moe_ipc_alloc", "b200moe_ipc_open", "b200moe_ipc_close", "b200moe_ipc_free",
 ]
 
@@ -156,9 +156,7 @@ def _load() -> ctypes.CDLL:
     lib.b200moe_mxfp4_quantize_rows_scratch_bytes.argtypes = [i64, i64, i64, i32]
     lib.b200moe_mxfp4_quantize_rows_scratch_bytes.restype = sz
     lib.b200moe_mxfp4_quantize_rows.argtypes = [vp, vp, vp, vp, i64, i64, i64, vp, sz, vp]
-    lib.b200moe_grouped_gemm_mxfp4_workspace_bytes.argtypes = [i64, i64, i64, i64, i32]
-    lib.b200moe_grouped_gemm_mxfp4_workspace_bytes.restype = sz
-    lib.b200moe_grouped_gemm_mxfp4.argtypes = [vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i32, i32, vp, sz, vp, vp]
+    lib.b200moe_grouped_gemm_mxfp4.argtypes = [vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i32, i32, vp, vp]
     for f in (lib.b200moe_grouped_gemm_mxfp4, lib.b200moe_moe_sort, lib.b200moe_moe_dispatch, lib.b200moe_moe_dispatch_grad, lib.b200moe_moe_combine,
               lib.b200moe_moe_combine_grad, lib.b200moe_mxfp4_quantize_rows):
         f.restype = i32

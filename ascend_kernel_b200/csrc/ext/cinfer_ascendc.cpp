@@ -607,6 +607,12 @@ void check_rows(const at::Tensor& rows, const char* name, bool pairs, const at::
     TORCH_CHECK(rows.size(0) == (pairs ? slot.numel() : slot.size(0)), name, " must have ", pairs ? slot.numel() : slot.size(0), " rows");
 }
 
+// A gradient as the kernels take it: contiguous and aligned (it may be a part of something larger).
+at::Tensor whole_rows(const at::Tensor& grad) {
+    const at::Tensor g = grad.contiguous();
+    return (reinterpret_cast<uintptr_t>(g.data_ptr()) & 15) != 0 ? g.clone() : g;
+}
+
 template <Binding BINDING>
 struct Dispatch : torch::autograd::Function<Dispatch<BINDING>> {
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& token_of, const at::Tensor& slot) {
@@ -622,7 +628,7 @@ struct Dispatch : torch::autograd::Function<Dispatch<BINDING>> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "moe_dispatch is differentiable once");
         if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor()};
-        const at::Tensor slot = ctx->get_saved_variables()[0], g = grads[0].contiguous();
+        const at::Tensor slot = ctx->get_saved_variables()[0], g = whole_rows(grads[0]);
         c10::cuda::CUDAGuard guard(g.device());
         at::Tensor grad_x = at::empty({slot.size(0), g.size(1)}, g.options());
         raise_on(b200moe_moe_dispatch_grad(g.data_ptr(), g.scalar_type() == at::kFloat ? 1 : 0, slot.data_ptr<int32_t>(), grad_x.data_ptr(),
@@ -657,7 +663,7 @@ struct Combine : torch::autograd::Function<Combine<BINDING>> {
         const bool need_y = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
         if (!grads[0].defined() || (!need_y && !need_w)) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
         const auto saved = ctx->get_saved_variables();
-        const at::Tensor &y = saved[0], &weight = saved[1], &token_of = saved[2], &slot = saved[3], g = grads[0].contiguous();
+        const at::Tensor &y = saved[0], &weight = saved[1], &token_of = saved[2], &slot = saved[3], g = whole_rows(grads[0]);
         c10::cuda::CUDAGuard guard(y.device());
         at::Tensor grad_y, grad_w;
         if (need_y) grad_y = at::empty_like(y);
@@ -754,14 +760,11 @@ int ProductMxfp4(const at::Tensor& x, const at::Tensor& x_scale, const at::Tenso
     }
     TORCH_CHECK(group_list_type == 0 || group_list_type == 1, "group_list_type must be 0 or 1");
     c10::cuda::CUDAGuard guard(x.device());
-    const size_t bytes = b200moe_grouped_gemm_mxfp4_workspace_bytes(M, K, N, G, gate_up_silu ? 1 : 0);
-    at::Tensor workspace = bytes_like(x, bytes);
     const auto stream = c10::cuda::getCurrentCUDAStream().stream();
     raise_on(b200moe_grouped_gemm_mxfp4(x.data_ptr(), x_scale.data_ptr<uint8_t>(), weight.data_ptr(), weight_scale.data_ptr<uint8_t>(),
                                         group_list.data_ptr<int64_t>(), output.data_ptr(),
                                         output_scale ? output_scale->data_ptr<uint8_t>() : nullptr, M, K, N, G, (int)group_list_type,
-                                        gate_up_silu ? 1 : 0, workspace.data_ptr(), bytes, findings_for(BINDING, x.get_device(), stream),
-                                        stream),
+                                        gate_up_silu ? 1 : 0, findings_for(BINDING, x.get_device(), stream), stream),
              "grouped_gemm_mxfp4");
     return M == 0 ? 0 : 1;
 }

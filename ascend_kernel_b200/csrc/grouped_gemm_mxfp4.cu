@@ -2,15 +2,29 @@
 //
 //   y[m, n] = sum_k x[m, k] * w[g, n, k],  both e2m1 with an e8m0 scale per 32 k along their rows
 //
-// Persistent kernel, tcgen05 kind::mxf4: the tensor core multiplies the codes, applies both scales and keeps the sums of the whole k range in
-// fp32.  The operands are swapped: the 128 lanes of an MMA are weight columns, one or two blocks of them to a tile, and its N extent is the
-// tile's token rows rounded up to 16 (16 .. 192), so an expert's weights pass once where it has up to 192 rows.  Codes enter by TMA as they
-// are stored.  Scales come through registers, 16 bytes (512 k of a row) at a time, and are written to tensor memory by the warps that fetch them.
+// Persistent kernel on pairs of CTAs, tcgen05 kind::mxf4: the tensor core multiplies the codes, applies both scales and keeps the sums of the whole k
+// range in fp32.  The operands are swapped: the 256 lanes of a pair's MMA are weight columns, two blocks of 128 to a CTA's tile, and its N extent
+// is the tile's token rows rounded up to 16 (16 .. 192), so an expert's weights pass once where it has up to 192 rows.  The rows of x are split
+// between the two CTAs' shared memory and read by both.  Codes enter by TMA as they are stored.  Scales come through registers, 16 bytes (512 k of a
+// row) at a time, and are written to tensor memory by the warps that fetch them.
 //
-// Gate/up: a tile's two blocks are 128 gate columns and the up columns of the same indices; silu(gate) * up in fp32, a warp's 32 columns
+// Gate/up: a CTA's two blocks are 128 gate columns and the up columns of the same indices; silu(gate) * up in fp32, a warp's 32 columns
 // are a block of the result: its largest magnitude, its scale and codes are the warp's own business.
 //
-// Warp roles: 0 loads codes, 1 and 2 issue the MMAs of a block of columns each, 4 .. 7 bring scales, 8 .. 15 epilogue.  Every wait is bounded.
+// Warp roles: 0 loads codes, 1 and 2 issue the MMAs of a block of columns each (first CTA), 4 .. 7 bring scales, 8 .. 15 epilogue.  Every wait
+// is bounded.  A tile's sums are single in tensor memory where it has more than 96 rows, so the epilogue takes them to registers (silu and the product
+// made on the way) before it quantises or stores.
+//
+// What bounds it, measured alone | in a steady loop (which runs at 1.2 to 1.45 GHz, at the power limit), us: 256 experts, 4096 x 8 rows: 2048 x
+// 7168 386 | 416, of 381 for its 2.5 GB; gate/up 7168 x 4096 683 | 766, of 634; 8192 x 8 Zipf rows, gate/up 1107 | 1260, of 658 for its bytes and 450 of
+// MMA at the peak rate; 37 x 8 rows, 2048 x 7168 229 of 213; 32 x 8 rows, gate/up 395 of 388; one token's 8 experts 25 (2048 x 7168) and 41 (gate/up, of
+// 19: 64 tiles on 74 pairs, set-up and first loads).  So: memory, then power; Zipf rows, whose experts with thousands of rows read the
+// weights from L2 again and again: loads into the multiprocessors (without the epilogue 1069, with MMAs of 16 columns 1050, of both 978, without loads 647).
+//
+// Steps, us (gate/up 4096 x 8 | Zipf rows): scales gathered by cp.async, handed over two stages late 3137 Zipf; on arrival 1063 | 1872; through registers
+// 795 | 1405; sums to registers first 739 | 1296; scales written to tensor memory instead of copied there (tcgen05.cp goes in turn with the
+// MMAs) and an MMA warp for each block 684 | 1149; pairs 683 | 1107.  Tried and not kept: copies of the next stage's scales ahead of the
+// MMAs (813), weight scales prefetched to L2 a tile ahead (833), one reciprocal for two values of silu (706 | 1152), tiles drawn from a counter (below).
 #include <algorithm>
 
 #include "common.cuh"
@@ -23,8 +37,10 @@ namespace mf {
 constexpr int kWarpLoad = 0, kWarpMma0 = 1, kWarpScale0 = 4, kScaleWarps = 4, kWarpEpi0 = 8, kEpiWarps = 8;
 constexpr int kThreads = (kWarpEpi0 + kEpiWarps) * 32;
 constexpr int kMaxR = 192;               // token rows of a tile
+constexpr int kBlocks = 2;               // of 128 weight columns, of a CTA's tile
 constexpr int kBlockBytes = 128 * 128;   // 128 weight columns x 256 k
-constexpr int kSegK = 256;               // k of a segment: 128 bytes of a row
+constexpr int kStageK = 256;             // 128 bytes of a row
+constexpr int kWords = 2;                // of scales of a stage (a word: 128 k)
 constexpr int kChunkWords = 4;           // of scales: 16 bytes, 512 k of a row
 constexpr int kMaxSlots = 10, kMaxBufs = 4;
 constexpr uint32_t kTmemCols = 512;
@@ -35,26 +51,26 @@ constexpr int kExchangeBytes = 2 * kScaleRows * 16;
 constexpr int kBarrierBytes = 1024;
 constexpr int kSmemBytes = 227 * 1024;
 
-// What a tile is: the number of blocks of 128 weight columns, whether they are gate and up columns, and the segments of a stage.
-template <int HALVES, bool GATE, int SEGS>
+// What a tile is: two blocks of 128 weight columns to a CTA, neighbours, or gate columns and the up columns of the same indices.
+template <bool GATE>
 struct Mode {
-    static constexpr int kHalves = HALVES, kSegs = SEGS, kWords = 2 * SEGS;  // (a word of scales: 128 k)
     static constexpr bool kGate = GATE;
-    // loads of a segment of the weights: blocks of 128 columns that are neighbours, and their segments too, come together
-    static constexpr int kWeightBoxes = GATE || SEGS > 1 ? HALVES : 1, kBoxColumns = 128 * HALVES / kWeightBoxes;
-    // columns that a tile advances by (gate/up: of each), and the CTA's first
-    static constexpr int kTileColumns = GATE ? 256 : 256 * HALVES;
+    // columns that a tile advances by (gate/up: of each), the CTA's first, and how far its second block is
+    static constexpr int kTileColumns = GATE ? 256 : 512;
     static __device__ __forceinline__ int first_column(int nt, uint32_t rank) { return nt * kTileColumns + (int)rank * (kTileColumns / 2); }
     static __device__ __forceinline__ int block_step(int N) { return GATE ? N >> 1 : 128; }
-    static constexpr int kFixedBytes = 1024 + kBarrierBytes + kEpiWarps * kStripBytes + kExchangeBytes + 2 * (kMaxExperts + 4) * 4;
-    static constexpr int kRingBytes = kSmemBytes - kFixedBytes;
-    static __host__ __device__ constexpr int slot_bytes(int width) { return SEGS * (HALVES * kBlockBytes + width * 64); }
-    // tensor-memory columns of a chunk of scales
-    static constexpr int kScaleColumns = kChunkWords * 4 * (HALVES + 2);
-    static_assert(kRingBytes % 16 == 0 && kRingBytes / slot_bytes(kMaxR) >= 3, "stages");
-    static_assert(HALVES * kMaxR + 2 * kScaleColumns <= (int)kTmemCols, "tensor memory");
-    static_assert(kChunkWords % kWords == 0 || kWords % kChunkWords == 0, "chunks");
+    // neighbours come in one load
+    static constexpr int kLoads = GATE ? 2 : 1, kLoadColumns = 256 / kLoads;
 };
+using Plain = Mode<false>;
+using GateUp = Mode<true>;
+constexpr int kFixedBytes = 1024 + kBarrierBytes + kEpiWarps * kStripBytes + kExchangeBytes + 2 * (kMaxExperts + 4) * 4;
+constexpr int kRingBytes = kSmemBytes - kFixedBytes;
+// A stage: the CTA's two blocks, and its half of the tile's rows.
+__host__ __device__ constexpr int slot_bytes_of(int width) { return kBlocks * kBlockBytes + width * 64; }
+constexpr int kScaleColumns = kChunkWords * 4 * (kBlocks + 2);  // tensor-memory columns of a chunk of scales
+static_assert(kRingBytes % 16 == 0 && kRingBytes / slot_bytes_of(kMaxR) >= 3, "stages");
+static_assert(kBlocks * kMaxR + 2 * kScaleColumns <= (int)kTmemCols, "tensor memory");
 
 struct Args {
     const uint8_t* x_scale;
@@ -120,22 +136,22 @@ __device__ __forceinline__ int tile_rows_of(int rows, int tiles) { return ((rows
 // Inside an expert the row tiles of a weight column run together, so that they share the weights in L2.
 struct Tiles {
     const int *prefix, *row_start;
-    int G, n_nt, n, pair, pairs;
+    int G, n_nt, n, pairs;
 };
-__device__ __forceinline__ Tile locate(const Tiles& all, int tile) {
-    int lo = 0, hi = all.G;  // largest g with prefix[g] <= tile
+__device__ __forceinline__ Tile locate(const Tiles& s, int tile) {
+    int lo = 0, hi = s.G;  // largest g with prefix[g] <= tile
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (all.prefix[mid] <= tile) lo = mid;
+        if (s.prefix[mid] <= tile) lo = mid;
         else hi = mid;
     }
-    const int j = tile - all.prefix[lo], mt = (all.prefix[lo + 1] - all.prefix[lo]) / all.n_nt;
+    const int j = tile - s.prefix[lo], mt = (s.prefix[lo + 1] - s.prefix[lo]) / s.n_nt;
     const int nt = j / mt, m = j - nt * mt;
-    const int rows = all.row_start[lo + 1] - all.row_start[lo], tr = tile_rows_of(rows, mt);
+    const int rows = s.row_start[lo + 1] - s.row_start[lo], tr = tile_rows_of(rows, mt);
     Tile t;
     t.g = lo;
     t.nt = nt;
-    t.row0 = all.row_start[lo] + m * tr;
+    t.row0 = s.row_start[lo] + m * tr;
     t.rows = min(tr, rows - m * tr);
     t.n = (t.rows + 15) & ~15;
     return t;
@@ -144,10 +160,10 @@ __device__ __forceinline__ Tile locate(const Tiles& all, int tile) {
 // The pair's next tile, every n-th of all, which each role finds by itself; false at the end.  (Drawing tiles from a counter costs a call that clears it
 // and a ring between the roles, and a steady loop, which the power limit bounds, gains nothing: 256 experts, 4096 x 8 rows, 2048 x
 // 7168: alone 386 | drawn 377, in a loop 416 | 430.)
-__device__ __forceinline__ bool next_tile(const Tiles& all, int& tile, Tile& t) {
-    if (tile >= all.n) return false;
-    t = locate(all, tile);
-    tile += all.pairs;
+__device__ __forceinline__ bool next_tile(const Tiles& s, int& tile, Tile& t) {
+    if (tile >= s.n) return false;
+    t = locate(s, tile);
+    tile += s.pairs;
     return true;
 }
 
@@ -298,11 +314,10 @@ template <class M>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x64,
                    const __grid_constant__ CUtensorMap map_x32, const __grid_constant__ CUtensorMap map_x16, const __grid_constant__ CUtensorMap map_x8, const Args a) {
-    constexpr int kHalves = M::kHalves, kSegs = M::kSegs, kWords = M::kWords;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = smem_raw + ((1024u - (ptx::smem_u32(smem_raw) & 1023u)) & 1023u);
-    Sync* sy = reinterpret_cast<Sync*>(ring + M::kRingBytes);
-    uint8_t* strips = ring + M::kRingBytes + kBarrierBytes;
+    Sync* sy = reinterpret_cast<Sync*>(ring + kRingBytes);
+    uint8_t* strips = ring + kRingBytes + kBarrierBytes;
     uint8_t* exchange = strips + kEpiWarps * kStripBytes;
     int* row_start = reinterpret_cast<int*>(exchange + kExchangeBytes);
     int* prefix = row_start + kMaxExperts + 4;
@@ -319,11 +334,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             for (int i = 0; i < n; ++i) ptx::mbar_init(ptx::smem_u32(b + i), count);
         };
         init(sy->full, kMaxSlots, 1);
-        init(sy->empty, kMaxSlots, kHalves);
+        init(sy->empty, kMaxSlots, kBlocks);
         init(sy->s_full, 2, 2 * kScaleWarps);
-        init(sy->s_empty, 2, kHalves);
+        init(sy->s_empty, 2, kBlocks);
         init(&sy->exchange, 1, kScaleWarps);
-        init(sy->d_full, kMaxBufs, kHalves);
+        init(sy->d_full, kMaxBufs, kBlocks);
         init(sy->d_empty, kMaxBufs, 2 * kEpiWarps);
         init(sy->drain, 2, 1);
         ptx::fence_mbar_init();
@@ -367,14 +382,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
     const uint32_t tmem_base = (uint32_t)uniform((int)*reinterpret_cast<volatile uint32_t*>(&sy->tmem_base));
     const int n_tiles = uniform(sy->n_tiles), width = uniform(sy->width);
-    const int slot_bytes = M::slot_bytes(width), n_slots = min(kMaxSlots, M::kRingBytes / slot_bytes);
+    const int slot_bytes = slot_bytes_of(width), n_slots = min(kMaxSlots, kRingBytes / slot_bytes);
     // tensor memory: the sums of one to four tiles from the start, two chunks of scales at the end
-    constexpr int kScaleColumns = M::kScaleColumns, kXScaleAt = kChunkWords * 4 * kHalves;
-    const int n_bufs = min(kMaxBufs, ((int)kTmemCols - 2 * kScaleColumns) / (kHalves * width));
+    constexpr int kXScaleAt = kChunkWords * 4 * kBlocks;
+    const int n_bufs = min(kMaxBufs, ((int)kTmemCols - 2 * kScaleColumns) / (kBlocks * width));
     const uint32_t scale0 = tmem_base + kTmemCols - 2 * kScaleColumns;
-    const int x_at = kHalves * kSegs * kBlockBytes;  // of a stage: the codes of the weights, then those of x
-    const Tiles tiles = {prefix, row_start, a.G, n_nt, n_tiles, pair, pairs};
-    const int segs = (a.K + kSegK - 1) / kSegK, words = a.words, stages = (segs + kSegs - 1) / kSegs;
+    constexpr int x_at = kBlocks * kBlockBytes;  // of a stage: the codes of the weights, then those of x
+    const Tiles tiles = {prefix, row_start, a.G, n_nt, n_tiles, pairs};
+    const int words = a.words, stages = (a.K + kStageK - 1) / kStageK;
 
     // registers of a lane: 56, 104 and twice 176 for the four warps of each kind, together as many as the launch has
     if (warp < kWarpScale0) {
@@ -395,22 +410,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     if (it >= (uint32_t)n_slots && !wait(&sy->empty[slot], ph ^ 1, sy, a.findings, 10)) { ok = false; break; }
                     if (leader) {
                         const uint32_t bar0 = full0 + slot * 8, dst = ptx::smem_u32(ring) + slot * (uint32_t)slot_bytes;
-                        const int here = min(kSegs, segs - kb * kSegs);
-                        if (rank == 0) ptx::mbar_arrive_expect_tx(ptx::smem_u32(&sy->full[slot]), 2u * (uint32_t)(here * (kHalves * kBlockBytes + half * 128)));
+                        if (rank == 0) ptx::mbar_arrive_expect_tx(ptx::smem_u32(&sy->full[slot]), 2u * (uint32_t)(kBlocks * kBlockBytes + half * 128));
+                        const int x = kb * 128;
 #pragma unroll
-                        for (int s = 0; s < kSegs; ++s) {
-                            if (s >= here) break;
-                            const int x = (kb * kSegs + s) * 128;
-#pragma unroll
-                            for (int u = 0; u < M::kWeightBoxes; ++u)
-                                ptx::tma_load_3d_pair(dst + (u * kSegs + s) * kBlockBytes, &map_w, bar0, x, col + u * M::block_step(a.N), t.g);
-                            uint32_t at = dst + x_at + s * width * 64;
-                            int r = row;
-                            if (half & 64) ptx::tma_load_2d_pair(at, &map_x64, bar0, x, r), at += 64 * 128, r += 64;
-                            if (half & 32) ptx::tma_load_2d_pair(at, &map_x32, bar0, x, r), at += 32 * 128, r += 32;
-                            if (half & 16) ptx::tma_load_2d_pair(at, &map_x16, bar0, x, r), at += 16 * 128, r += 16;
-                            if (half & 8) ptx::tma_load_2d_pair(at, &map_x8, bar0, x, r);
-                        }
+                        for (int u = 0; u < M::kLoads; ++u)
+                            ptx::tma_load_3d_pair(dst + u * kBlockBytes, &map_w, bar0, x, col + u * M::block_step(a.N), t.g);
+                        uint32_t at = dst + x_at;
+                        int r = row;
+                        if (half & 64) ptx::tma_load_2d_pair(at, &map_x64, bar0, x, r), at += 64 * 128, r += 64;
+                        if (half & 32) ptx::tma_load_2d_pair(at, &map_x32, bar0, x, r), at += 32 * 128, r += 32;
+                        if (half & 16) ptx::tma_load_2d_pair(at, &map_x16, bar0, x, r), at += 16 * 128, r += 16;
+                        if (half & 8) ptx::tma_load_2d_pair(at, &map_x8, bar0, x, r);
                     }
                     __syncwarp();
                     if (++slot == (uint32_t)n_slots) { slot = 0; ph ^= 1; }
@@ -427,7 +437,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 while (ptx::globaltimer_ns() - t0 < 10000000ull) {}
             }
             __syncwarp();
-        } else if (warp < kWarpMma0 + kHalves && rank == 0) {
+        } else if (warp < kWarpMma0 + kBlocks && rank == 0) {
             // ------------------------------ MMA issue ------------------------------
             // A warp for each block of columns: it walks together and one lane issues.  Of the descriptors only the address, in the low
             // word, changes.
@@ -437,14 +447,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             bool ok = true;
             const uint64_t desc = ptx::umma_desc_sw128(0, 0, 1024);
             const uint32_t desc_hi = (uint32_t)(desc >> 32);
-            const uint32_t a0 = (uint32_t)desc + ((ptx::smem_u32(ring) + (uint32_t)(u * kSegs * kBlockBytes)) >> 4);
+            const uint32_t a0 = (uint32_t)desc + ((ptx::smem_u32(ring) + (uint32_t)(u * kBlockBytes)) >> 4);
             const uint32_t x0 = (uint32_t)desc + ((ptx::smem_u32(ring) + (uint32_t)x_at) >> 4);
-            const uint32_t slot_step = (uint32_t)slot_bytes >> 4, seg_step = (uint32_t)width * 4;
+            const uint32_t slot_step = (uint32_t)slot_bytes >> 4;
             int tile = pair;
             Tile t;
             for (; ok && next_tile(tiles, tile, t); ++n) {
                 const int cols = uniform(t.n), x_words = cols > 128 ? 8 : 4;
-                const uint32_t idesc = ptx::umma_idesc_mxf4(256, cols), d = tmem_base + (buf * kHalves + u) * (uint32_t)width;
+                const uint32_t idesc = ptx::umma_idesc_mxf4(256, cols), d = tmem_base + (buf * kBlocks + u) * (uint32_t)width;
                 // the epilogue has taken what the buffer held
                 if (n >= (uint32_t)n_bufs && !wait(&sy->d_empty[buf], bph ^ 1, sy, a.findings, 30)) break;
                 uint32_t more = 0;
@@ -463,9 +473,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             const uint32_t xs = scale0 + cb * kScaleColumns + (uint32_t)(kXScaleAt + cw * x_words);
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                const uint32_t step = (uint32_t)(((w & 1) * 2 + h) * 2);  // 64 k
-                                ptx::umma_mxf4_pair(d, al + (uint32_t)((w >> 1) * (kBlockBytes >> 4)) + step, xl + (w >> 1) * seg_step + step, desc_hi,
-                                               idesc | ptx::umma_scale_half(h), ws, xs, h == 0 ? more : 1u);
+                                const uint32_t step = (uint32_t)((w * 2 + h) * 2);  // 64 k: 32 bytes
+                                ptx::umma_mxf4_pair(d, al + step, xl + step, desc_hi, idesc | ptx::umma_scale_half(h), ws, xs, h == 0 ? more : 1u);
                             }
                         }
                         more = 1;
@@ -500,13 +509,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int q = warp - kWarpScale0, row = q * 32 + lane, chunks = (words + kChunkWords - 1) / kChunkWords;
         const bool whole = (words & 3) == 0 && ((reinterpret_cast<uintptr_t>(a.w_scale) | reinterpret_cast<uintptr_t>(a.x_scale)) & 15) == 0;
         struct Chunk {
-            uint4 v[kHalves + 2];  // of the weights' blocks and the two of x
+            uint4 v[kBlocks + 2];  // of the weights' blocks and the two of x
             int cols;              // token rows of the tile rounded up; 0: the schedule has ended
         };
         int at = chunks, cols = 0;
         int tile = pair;
         bool live = true;
-        const uint32_t* src[kHalves + 2];  // NULL: no row there, zeros
+        const uint32_t* src[kBlocks + 2];  // NULL: no row there, zeros
         const auto fetch = [&](Chunk& c) {
             if (at == chunks) {
                 Tile t;
@@ -517,13 +526,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 }
                 cols = t.n;
 #pragma unroll
-                for (int u = 0; u < kHalves; ++u) {
+                for (int u = 0; u < kBlocks; ++u) {
                     const int n = M::first_column(t.nt, rank) + u * M::block_step(a.N) + row;
                     src[u] = n < a.N ? reinterpret_cast<const uint32_t*>(a.w_scale) + ((size_t)t.g * a.N + n) * (size_t)words : nullptr;
                 }
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
-                    src[kHalves + b] = b * 128 + row < t.rows
+                    src[kBlocks + b] = b * 128 + row < t.rows
                                            ? reinterpret_cast<const uint32_t*>(a.x_scale) + (size_t)(t.row0 + b * 128 + row) * (size_t)words
                                            : nullptr;
                 at = 0;
@@ -531,7 +540,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             c.cols = cols;
             const int here = words - kChunkWords * at;
 #pragma unroll
-            for (int b = 0; b < kHalves + 2; ++b) {
+            for (int b = 0; b < kBlocks + 2; ++b) {
                 const uint32_t* p = src[b] + kChunkWords * at;
                 c.v[b] = make_uint4(0u, 0u, 0u, 0u);
                 if (src[b] != nullptr) {
@@ -554,9 +563,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const auto put = [&](const Chunk& c) {
             uint4* room = reinterpret_cast<uint4*>(exchange) + cb * kScaleRows;
 #pragma unroll
-            for (int b = 0; b < kHalves; ++b) room[b * 128 + row] = c.v[b];
-            room[kHalves * 128 + row] = c.v[kHalves];
-            if (128 + row < kMaxR) room[kHalves * 128 + 128 + row] = c.v[kHalves + 1];
+            for (int b = 0; b < kBlocks; ++b) room[b * 128 + row] = c.v[b];
+            room[kBlocks * 128 + row] = c.v[kBlocks];
+            if (128 + row < kMaxR) room[kBlocks * 128 + 128 + row] = c.v[kBlocks + 1];
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sy->exchange));
             if (!wait(&sy->exchange, n & 1, sy, a.findings, 21)) return false;
@@ -573,18 +582,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             };
             uint32_t o[16];
 #pragma unroll
-            for (int u = 0; u < kHalves; ++u) {
+            for (int u = 0; u < kBlocks; ++u) {
                 rows4(room + u * 128, o);
                 ptx::tmem_st_32x16(to + u * (kChunkWords * 4), o);
             }
-            rows4(room + kHalves * 128, o);
+            rows4(room + kBlocks * 128, o);
             if (c.cols <= 128) {
                 ptx::tmem_st_32x16(to + kXScaleAt, o);
             } else {
                 uint32_t p[8];
 #pragma unroll
                 for (int i = 0; i < (kMaxR - 128) / 32; ++i) {
-                    const uint4 v = room[kHalves * 128 + 128 + i * 32 + lane];
+                    const uint4 v = room[kBlocks * 128 + 128 + i * 32 + lane];
                     p[i] = v.x; p[2 + i] = v.y; p[4 + i] = v.z; p[6 + i] = v.w;
                 }
 #pragma unroll
@@ -631,7 +640,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         uint32_t buf = 0, ph = 0;
         int tile = pair;
         while (next_tile(tiles, tile, e.t)) {
-            e.tmem = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * (uint32_t)(kHalves * width);
+            e.tmem = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * (uint32_t)(kBlocks * width);
             e.col = M::first_column(e.t.nt, rank) + quarter * 32;
             e.d_empty = d_empty0 + buf * 8;
             if (!wait(&sy->d_full[buf], ph, sy, a.findings, 50)) break;
@@ -664,7 +673,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ptx::tc_fence_before();
     __syncthreads();
     // (so have the last commits of the MMA warps, which arrive here too; the first CTA's warps waited for theirs)
-    if (rank != 0 && warp >= kWarpMma0 && warp < kWarpMma0 + kHalves) (void)ptx::mbar_wait(ptx::smem_u32(&sy->drain[warp - kWarpMma0]), 0);
+    if (rank != 0 && warp >= kWarpMma0 && warp < kWarpMma0 + kBlocks) (void)ptx::mbar_wait(ptx::smem_u32(&sy->drain[warp - kWarpMma0]), 0);
     __syncwarp();
     ptx::cluster_sync();  // (what one CTA sends the other, loads and MMAs of the pair among it, has arrived)
     if (warp == kWarpMma0) {
@@ -673,29 +682,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
 }
 
-using Plain = Mode<2, false, 1>;
-using GateUp = Mode<2, true, 1>;
-
 static bool sizes_ok(int64_t M, int64_t K, int64_t N, int64_t G) {
     constexpr int64_t kMost = 0x3FFFFFFF;  // (products of two sizes stay in 64 bits)
     return M >= 0 && M <= kMost && K > 0 && K <= kMost && N > 0 && N <= kMost && G > 0 && G <= kMaxExperts;
 }
-constexpr size_t kWorkspaceBytes = 256;
 
 }  // namespace mf
 }  // namespace b200moe
 
 using namespace b200moe;
 
-extern "C" size_t b200moe_grouped_gemm_mxfp4_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, int gate_up_silu) {
-    (void)M; (void)K; (void)N; (void)G; (void)gate_up_silu;
-    return mf::kWorkspaceBytes;
-}
-
 extern "C" int b200moe_grouped_gemm_mxfp4(const void* x, const uint8_t* x_scale, const void* weight, const uint8_t* weight_scale,
                                           const int64_t* group_list, void* out, uint8_t* out_scale, int64_t M, int64_t K, int64_t N,
-                                          int64_t G, int group_list_type, int gate_up_silu, void* workspace, size_t workspace_bytes,
-                                          int32_t* findings, void* stream) {
+                                          int64_t G, int group_list_type, int gate_up_silu, int32_t* findings, void* stream) {
     if (!mf::sizes_ok(M, K, N, G) || (K % 32) != 0 || (N % 16) != 0 || (gate_up_silu && (N % 256) != 0)) return B200MOE_ERR_SHAPE;
     if (group_list_type != B200MOE_GROUP_LIST_CUMSUM && group_list_type != B200MOE_GROUP_LIST_COUNTS) return B200MOE_ERR_ARGUMENT;
     if (gate_up_silu != 0 && gate_up_silu != 1) return B200MOE_ERR_ARGUMENT;
@@ -706,8 +705,6 @@ extern "C" int b200moe_grouped_gemm_mxfp4(const void* x, const uint8_t* x_scale,
     const auto aligned4 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; };
     if (!aligned16(x) || !aligned16(weight) || !aligned16(out) || !aligned4(x_scale) || !aligned4(weight_scale) || !aligned4(out_scale))
         return B200MOE_ERR_ALIGNMENT;
-    if (!workspace || workspace_bytes < b200moe_grouped_gemm_mxfp4_workspace_bytes(M, K, N, G, gate_up_silu)) return B200MOE_ERR_WORKSPACE;
-    if (!aligned16(workspace)) return B200MOE_ERR_ALIGNMENT;
     mf::Args a = {};
     a.x_scale = x_scale;
     a.w_scale = weight_scale;
@@ -719,7 +716,7 @@ extern "C" int b200moe_grouped_gemm_mxfp4(const void* x, const uint8_t* x_scale,
     a.words = (int)(mxfp4::scale_width(K) / 4);
     a.findings = findings != nullptr ? findings : findings_words();
     CUtensorMap map_w, map_x[4];
-    int rc = make_tensor_map_3d_u8(&map_w, weight, (uint64_t)G, (uint64_t)N, (uint64_t)(K / 2), gate_up_silu ? mf::GateUp::kBoxColumns : mf::Plain::kBoxColumns, 128);
+    int rc = make_tensor_map_3d_u8(&map_w, weight, (uint64_t)G, (uint64_t)N, (uint64_t)(K / 2), gate_up_silu ? mf::GateUp::kLoadColumns : mf::Plain::kLoadColumns, 128);
     for (int i = 0; i < 4 && rc == B200MOE_OK; ++i)
         rc = make_tensor_map_2d(&map_x[i], x, 1, (uint64_t)M, (uint64_t)(K / 2), mf::kBoxes[i], 128, true);
     if (rc != B200MOE_OK) return rc;

@@ -396,17 +396,14 @@ int b200moe_mxfp4_quantize_rows(const void* x, const int32_t* index, void* codes
  * weight_scale [G, N, W]; products exact, sums in fp32.  gate_up_silu == 0: out bf16 [M, N], out_scale unused.  gate_up_silu == 1: N = 2 I with
  * the gate columns first, N % 256 == 0; silu(gate) * up in fp32, quantised as b200moe_mxfp4_quantize_rows does: out [M, I / 2], out_scale
  * [M, I / 32], which the down projection takes as they are.  K % 32 == 0 and N % 16 == 0; x, weight and out aligned to 16 bytes, the scales
- * to 4.  Rows of no expert are left as they were.  The workspace belongs to the call until it has completed on the stream, and calls that overlap have one
- * each; it holds no status words: an invalid group_list (rows were clamped) or an expired wait is kept for b200moe_read_findings, or
- * where `findings` says. */
-size_t b200moe_grouped_gemm_mxfp4_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, int gate_up_silu);
+ * to 4.  Rows of no expert are left as they were.  The call needs no workspace; an invalid group_list (rows were clamped) or an expired wait
+ * is kept where `findings` says (NULL: for b200moe_read_findings). */
 int b200moe_grouped_gemm_mxfp4(const void* x, const uint8_t* x_scale, const void* weight, const uint8_t* weight_scale,
                                const int64_t* group_list, void* out, uint8_t* out_scale, int64_t M, int64_t K, int64_t N, int64_t G,
-                               int group_list_type, int gate_up_silu, void* workspace, size_t workspace_bytes, int32_t* findings,
-                               void* stream);
+                               int group_list_type, int gate_up_silu, int32_t* findings, void* stream);
 
 /* A finding (code, detail; those of status words 0 and 1) of b200moe_grouped_gemm_fp8_block, b200moe_grouped_gemm_mxfp4 or b200moe_moe_balance_loss is kept in two
- * words on the device, which hold the first one until they are cleared.  The `_findings` entries take them (zeroed device memory that
+ * words on the device, which hold the first one until they are cleared.  The `_findings` entries (and the 4-bit product's) take them (zeroed device memory that
  * outlives the call and its replays); NULL, and the entries without, stand for one pair of a device that all such calls share.
  * b200moe_findings_pair: the address, on the current device, of one of the B200MOE_FINDINGS_PAIRS pairs that the library has, zero at the
  * start; pair 0 is the shared one.  b200moe_read_findings_at: what a pair holds, (0, 0) if nothing; b200moe_read_findings: the shared one.

@@ -320,3 +320,17 @@ def test_rows_behind_31_bits():
         assert bool((rows[r:r + step] == (token_of[r:r + step] % 251).to(torch.bfloat16).unsqueeze(1)).all())
     w = torch.full((T, k), 0.125, device=DEV)
     assert torch.equal(ak.moe_combine(rows, w, token_of, slot), x)
+
+
+def test_a_gradient_that_is_not_aligned():
+    gen = _gen(11)
+    _, token_of, slot = ak.moe_sort(_idx(30, 8, 2, gen), 8)
+    x = torch.randn(30, 64, generator=gen, device=DEV).requires_grad_()
+    w = torch.rand(30, 2, generator=gen, device=DEV).requires_grad_()
+    rows = ak.moe_dispatch(x, token_of, slot)
+    g = torch.randn(60 * 64 + 1, generator=gen, device=DEV)[1:].view(60, 64)
+    assert g.data_ptr() % 16 != 0
+    assert torch.equal(torch.autograd.grad(rows, x, g, retain_graph=True)[0], torch.autograd.grad(rows, x, g.clone())[0])
+    out = ak.moe_combine(rows.detach(), w, token_of, slot)
+    g = torch.randn(30 * 64 + 1, generator=gen, device=DEV)[1:].view(30, 64)
+    assert torch.equal(torch.autograd.grad(out, w, g, retain_graph=True)[0], torch.autograd.grad(out, w, g.clone())[0])
