@@ -391,9 +391,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const Tiles tiles = {prefix, row_start, a.G, n_nt, n_tiles, pairs};
     const int words = a.words, stages = (a.K + kStageK - 1) / kStageK;
 
-    // registers of a lane: 56, 104 and twice 176 for the four warps of each kind, together as many as the launch has
+    // registers of a lane: 48, 112 and twice 176 for the four warps of each kind, together as many as the launch has (with 56 and 104 the
+    // down projection spills in a loop: 386 -> 428 us)
     if (warp < kWarpScale0) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         if (warp == kWarpLoad) {
             // ------------------------------ codes ------------------------------
             // The warp walks together and one lane issues.
@@ -502,7 +503,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             __syncwarp();
         }
     } else if (warp < kWarpEpi0) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
         // ------------------------------ scales ------------------------------
         // A thread fetches a row of every block of 128, 16 bytes (512 k) of each; the warps exchange them through shared memory, since each
         // writes all rows to its quarter of the lanes: row r in lane r % 32 of column r / 32, four columns for a word (128 k) of 128 rows.

@@ -288,3 +288,50 @@ def test_the_operators_together():
     terms = R.values(h, hs).abs().sum(dim=1).max() * R.values(w2, s2).abs().max()
     assert bool(((out.double() - want).abs() <= 2.0 ** -8 * (mag + want.abs() * 1.01) + (I + 64) * 2.0 ** -23 * k * terms).all())
     ak.check_status()
+
+
+def test_rows_that_come_through_a_prefix_of_other_kernels():
+    """Quantisation, product and quantised product right behind one another on a stream, again and again: each starts beside the end of the one before
+    it and may not read what that has not written."""
+    gen = _gen(13)
+    T, E, k, H, I = 300, 16, 4, 1024, 512
+    w13, s13 = _bytes((E, 2 * I, H // 2), gen), _scales((E, 2 * I), H, 119, 121, gen)
+    w2, s2 = _bytes((E, H, I // 2), gen), _scales((E, H), I, 120, 122, gen)
+    h, hs = torch.zeros(T * k, I // 2, dtype=torch.uint8, device=DEV), torch.zeros(T * k, I // 32, dtype=torch.uint8, device=DEV)
+    q, qs = torch.zeros(T * k, H // 2, dtype=torch.uint8, device=DEV), torch.zeros(T * k, H // 32, dtype=torch.uint8, device=DEV)
+    y = torch.zeros(T * k, H, dtype=torch.bfloat16, device=DEV)
+    xs = [torch.randn(T, H, generator=gen, device=DEV).to(torch.bfloat16) for _ in range(6)]
+    idx = [torch.rand(T, E, generator=gen, device=DEV).topk(k, dim=1).indices.to(torch.int32) for _ in range(6)]
+    wts = torch.rand(T, k, generator=gen, device=DEV)
+
+    def run(i):
+        counts, token_of, slot = ak.moe_sort(idx[i], E)
+        ak.mxfp4_quantize_rows(xs[i], token_of, codes=q, scale=qs)
+        ak.grouped_gemm_mxfp4(q, qs, w13, s13, counts, h, output_scale=hs, group_list_type=1, gate_up_silu=True)
+        ak.grouped_gemm_mxfp4(h, hs, w2, s2, counts, y, group_list_type=1)
+        return ak.moe_combine(y, wts, token_of, slot)
+
+    alone = []
+    for i in range(6):
+        alone.append(run(i))
+        torch.cuda.synchronize()
+    for _ in range(5):
+        got = [run(i) for i in range(6)]
+        torch.cuda.synchronize()
+        for a, b in zip(got, alone):
+            assert torch.equal(a, b)
+    ak.check_status()
+
+
+@pytest.mark.parametrize("G", [1, 300, 1024])
+def test_one_expert_and_as_many_as_there_can_be(G):
+    gen = _gen(G)
+    K, N = 64, 32
+    counts = [0] * G
+    for g in torch.randint(0, G, (40,), generator=gen, device=DEV).tolist():
+        counts[g] += 1
+    counts[0] += 200
+    x, xs, w, ws, gl = _problem(counts, K, N, seed=G)
+    out = torch.zeros(sum(counts), N, dtype=torch.bfloat16, device=DEV)
+    ak.grouped_gemm_mxfp4(x, xs, w, ws, gl, out, group_list_type=1)
+    assert torch.equal(out, _product(x, xs, w, ws, _ranges(counts)).float().to(torch.bfloat16))
