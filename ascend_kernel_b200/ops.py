@@ -136,9 +136,9 @@ def last_status(device=None, clear: bool = False):
     """(code, detail) of the first device-side finding of any operator call on ``device`` (default: the
     current one) since the status was last cleared; (0, 0) if none.  code 1: a group_list was invalid and
     rows were clamped (detail = expert index); 2: a bounded wait inside a kernel expired and the output
-    is incomplete.  Synchronises the streams the operators ran on (and the caller's, where 8-bit products or balance losses are
+    is incomplete.  Synchronises the streams the operators ran on (and the caller's, where 8-bit or 4-bit products or balance losses are
     among them: replays of captured ones run there); a stream that is being captured is left alone.  ``clear`` leaves a finding of these
-    two that is not the one returned to the next call, on whichever stream it was made."""
+    that is not the one returned to the next call, on whichever stream it was made."""
     import ctypes
 
     if device is not None and torch.device(device).type != "cuda":
