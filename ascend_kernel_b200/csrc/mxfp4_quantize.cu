@@ -100,9 +100,9 @@ static bool sizes_ok(int64_t n_src, int64_t n_rows, int64_t K) {
 
 // Whether the rows of x are quantised once, into scratch, and their bytes gathered: where an index names every row of x four times or
 // more and the second launch does not matter.  Every row of the result quantised | two passes, us (rows of x, times each is named, K): 4096 x 8,
-// 7168: 66.1 | 40.3; 1024 x 8, 7168: 18.6 | 12.3; 512 x 8, 7168: 11.1 | 11.1; 256 x 8, 7168: 7.6 | 7.8; 4096 x 8, 2048: 36.9 | 16.4;
-// 4096 x 4, 7168: 35.4 | 28.7; 4096 x 2, 7168: 20.5 | 24.
-static bool two_passes(int64_t n_src, int64_t n_rows, int64_t K) { return n_rows >= 4 * n_src && n_rows * K >= (32ll << 20); }
+// 7168: 66.0 | 40.5; 1024 x 8, 7168: 18.5 | 12.3; 512 x 8, 7168: 11.1 | 8.2; 256 x 8, 7168: 7.5 | 6.2; 128 x 8, 7168: 6.2 | 6.2; 4096 x 8, 2048:
+// 36.9 | 16.4; 4096 x 4, 7168: 35.5 | 28.7; 4096 x 2, 7168: 20.5 | 21.3.
+static bool two_passes(int64_t n_src, int64_t n_rows, int64_t K) { return n_rows >= 4 * n_src && n_rows * K >= (12ll << 20); }
 
 static int launch_quantize(const void* x, const int32_t* index, void* codes, uint8_t* scale, int64_t n_src, int64_t n_rows, int64_t K,
                            cudaStream_t st) {
