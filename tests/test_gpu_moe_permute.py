@@ -166,7 +166,7 @@ def test_gradients_against_differences():
             d = d.view_as(leaf)
             args = [(x + s * d, w) if leaf is x else (x, w + s * d) for s in (1, -1)]
             diff = ((f(*args[0]).double() - f(*args[1]).double()) * g.double()).sum() / 2
-            assert abs(float(diff - grad.view(-1)[i])) <= (2 * k + H) * 2.0 ** -24 * 64 * 8
+            assert abs(float(diff.detach() - grad.view(-1)[i])) <= (2 * k + H) * 2.0 ** -24 * 64 * 8
 
 
 def test_non_finite_values_stay_with_their_rows():
