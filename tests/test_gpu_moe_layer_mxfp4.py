@@ -136,3 +136,52 @@ def test_launches():
     before = ops.LAUNCHES
     layer.forward_routed(x, idx, wts)
     assert ops.LAUNCHES - before == 5  # sort, quantisation, two products, combine
+
+
+def test_rows_that_come_through_the_exchange():
+    """exchange="p2p" with one rank: the rows are quantised where they arrive, in a buffer with room for more.  How an expert's rows are cut goes by their number
+    alone, so the results have the same bits."""
+    E, H, I, k = 8, 256, 128, 2
+    layer, gen = _layer(E, H, I, k, seed=4)
+    p2p = MoELayer(layer.w13, layer.s13, None, layer.w2, layer.s2, None, E, k, weight_format="mxfp4", exchange="p2p", max_tokens=64)
+    try:
+        for T in (64, 7, 50):
+            x = torch.randn(T, H, generator=gen, device=DEV).to(torch.bfloat16)
+            logits = torch.randn(T, E, generator=gen, device=DEV).to(torch.bfloat16)
+            assert torch.equal(layer.forward(x, logits), p2p.forward(x, logits))
+        p2p.read_status()
+    finally:
+        p2p.px.close()
+
+
+def test_trained_beside_the_pass():
+    """A step as it would be used: the sort of a router's choice, the rows to plain experts and back, and the gradients of all of them, beside
+    the balance loss of the same choice."""
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    T, E, H, k = 60, 6, 64, 2
+    x = torch.randn(T, H, generator=gen, device=DEV).requires_grad_()
+    router = (torch.randn(H, E, generator=gen, device=DEV) * 0.2).requires_grad_()
+    experts = (torch.randn(E, H, H, generator=gen, device=DEV) * H ** -0.5).requires_grad_()
+    logits = x @ router
+    prob, chosen = torch.softmax(logits, dim=1).topk(k, dim=1)
+    idx = chosen.to(torch.int32)
+    counts, token_of, slot = ak.moe_sort(idx, E)
+    rows = ak.moe_dispatch(x, token_of, slot)
+    y = torch.cat([r @ w for r, w in zip(rows.split(counts.tolist()), experts)])
+    out = ak.moe_combine(y, prob, token_of, slot)
+    loss, pairs = ak.moe_balance_loss(logits, idx)
+    assert torch.equal(pairs[0], counts)
+    g = torch.randn(T, H, generator=gen, device=DEV)
+    got = torch.autograd.grad((out * g).sum() + 0.1 * loss.sum(), (x, router, experts))
+    # the same in 64 bits, every expert on every token
+    x64, r64, e64 = [t.detach().double().requires_grad_() for t in (x, router, experts)]
+    lg = x64 @ r64
+    p = torch.softmax(lg, dim=1)
+    on = torch.zeros(T, E, dtype=torch.float64, device=DEV).scatter_(1, chosen, 1.0)
+    out64 = torch.einsum("te,teh->th", p * on, torch.einsum("th,ehj->tej", x64, e64))
+    loss64 = E / (k * T * T) * (counts.double() * p.sum(dim=0)).sum()
+    want = torch.autograd.grad((out64 * g.double()).sum() + 0.1 * loss64, (x64, r64, e64))
+    assert float((out.detach().double() - out64.detach()).norm() / out64.detach().norm()) <= 1e-3
+    for a, b in zip(got, want):
+        # (torch's own products may run in tf32: 2^-11 a factor, of some ten in a row)
+        assert float((a.double() - b).norm() / b.norm()) <= 10 * 2.0 ** -11
