@@ -30,6 +30,7 @@ constexpr int kMaxTopK = 32;
 // distributed shared memory (18 in clusters of 4, 31 of 8, which do not all fit at once), stores put in order in shared memory first (16.4).
 
 constexpr int kWarps = 32, kFewWarps = 8;
+constexpr int kRoom = 32;          // sums of the warps, in static shared memory
 constexpr int kOnePairs = 4096;    // of a call that is one CTA's
 constexpr int kMostCtas = 128;
 constexpr int kBatch = 4;          // ids a lane has at a time
@@ -169,7 +170,7 @@ __device__ __forceinline__ void place_pairs(const SortArgs& a, int* hist, const 
 template <int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, 1) sort_one_kernel(const SortArgs a) {
     extern __shared__ int smem[];  // [WARPS][E], [E]
-    __shared__ int s_room[32];
+    __shared__ int s_room[kRoom];
     int *hist = smem, *base = hist + WARPS * a.E;
     int id[kBatch], rank[kBatch], kept;
     count_pairs<WARPS>(a, hist, id, rank);
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) sort_count_kernel(const SortAr
 
 __global__ void __launch_bounds__(kWarps * 32, 1) sort_place_kernel(const SortArgs a) {
     extern __shared__ int smem[];  // [kWarps][E], twice [E]
-    __shared__ int s_room[32];
+    __shared__ int s_room[kRoom];
     int *hist = smem, *base = hist + kWarps * a.E, *alls = base + a.E;
     const int e = threadIdx.x;
     int id[kBatch], rank[kBatch], kept;
@@ -462,9 +463,10 @@ extern "C" int b200moe_moe_sort(const int32_t* idx, int64_t n_tokens, int64_t n_
     a.cta_pairs = mp::cta_pairs_of(a.P);
     a.warp_pairs = std::max(1, ((std::min(a.P, a.cta_pairs) + warps - 1) / warps + 31) / 32) * 32;
     const size_t smem = (size_t)(warps + 2) * (size_t)a.E * 4;
+    // (what a launch has without asking for more holds the static part too)
     const auto opt_in = [&](void (*kernel)(mp::SortArgs)) {
-        return smem > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (mp::kWarps + 2) * kMaxExperts * 4)
-                                : cudaSuccess;
+        if (smem + mp::kRoom * sizeof(int) <= 48 * 1024) return cudaSuccess;
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (mp::kWarps + 2) * kMaxExperts * 4);
     };
     if (need == 0) {
         const auto kernel = few ? mp::sort_one_kernel<mp::kFewWarps> : mp::sort_one_kernel<mp::kWarps>;
