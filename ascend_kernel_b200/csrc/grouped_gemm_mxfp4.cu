@@ -178,8 +178,16 @@ __device__ __forceinline__ float reciprocal_flushed(float v) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-// g / (1 + e^-g); an e^-g that overflows makes it 0, which it is to 2^-120
+// g / (1 + e^-g), for g down to kTail: from -87 on the reciprocal would be below the smallest normal number, and up, which multiplies it, may be large
+constexpr float kTail = -80.f;
 __device__ __forceinline__ float silu(float g) { return g * reciprocal_flushed(1.f + exp2_flushed(-1.44269504f * g)); }
+// silu(g) * up for every g.  Under kTail silu is g e^g (to 2^-115), and either factor takes half of the exponent.  e^(g / 2) is 0 from g = -174 on, where
+// what it stands for is below 2^-116 for every up; half of the smallest code of the smallest scale is 2^-102.
+__device__ __forceinline__ float silu_times(float g, float up) {
+    if (!(g < kTail)) return silu(g) * up;
+    const float r = exp2_flushed(0.72134752f * g);
+    return (g * r) * (up * r);
+}
 
 // What an epilogue warp works on: its 32 columns from `col` on (tensor-memory lanes) of the tile's sums at `tmem`.
 struct Share {
@@ -189,11 +197,11 @@ struct Share {
     uint32_t d_empty;  // in the first CTA
     uint8_t* strip;
 };
-// The sums are in registers: the buffer goes back.
-__device__ __forceinline__ void release(const Share& e) {
+// The sums are in registers: the buffer goes back, unless they are needed once more.
+__device__ __forceinline__ void release(const Share& e, bool now = true) {
     ptx::tc_fence_before();
     __syncwarp();
-    if ((threadIdx.x & 31) == 0) ptx::mbar_arrive_remote(e.d_empty);
+    if ((threadIdx.x & 31) == 0 && now) ptx::mbar_arrive_remote(e.d_empty);
 }
 
 // Sixteen tokens x the warp's 32 columns in bf16 through the warp's strip: the transposing store gives 16-byte pieces of eight columns, 64
@@ -287,11 +295,13 @@ __device__ __forceinline__ void store_quantized(float (&h)[16], const Tile& t, i
     if (lane < 16 && token0 + lane < t.rows && inside) a.out_scale[(size_t)(t.row0 + token0 + lane) * (inter >> 5) + (col >> 5)] = (uint8_t)byte;
 }
 
-// silu(gate) * up of every other piece of 16 tokens, NC at most, in registers before the first is quantised.
+// silu(gate) * up of every other piece of 16 tokens, NC at most, in registers before the first is quantised.  false: a gate is under kTail, and the buffer
+// is kept for finish_tail.  (A piece behind the tile's rows counts too: whatever it holds costs time alone.  To leave here in that case, before the
+// buffer goes back, costs every tile: Zipf rows 1081 us without a look at the gates, 1085 so, 1105 with a branch.)
 template <int NC>
-__device__ __forceinline__ void finish_quantized(const Share& e, const Args& a) {
+__device__ __forceinline__ bool finish_quantized(const Share& e, const Args& a) {
     uint32_t v[2][2][8];
-    float h[NC][16];
+    float h[NC][16], low = 0.f;
     const auto fetch = [&](int s, uint32_t(&d)[2][8]) {  // half a piece
         const uint32_t at = e.tmem + (uint32_t)(((s & ~1) + e.group) * 16 + (s & 1) * 8);
         ptx::tmem_ld_32x8(at, d[0]);
@@ -303,11 +313,36 @@ __device__ __forceinline__ void finish_quantized(const Share& e, const Args& a) 
         ptx::tmem_ld_wait();
         if (s + 1 < 2 * NC) fetch(s + 1, v[(s + 1) & 1]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) h[s >> 1][(s & 1) * 8 + i] = silu(__uint_as_float(v[s & 1][0][i])) * __uint_as_float(v[s & 1][1][i]);
+        for (int i = 0; i < 8; ++i) {
+            const float g = __uint_as_float(v[s & 1][0][i]);
+            low = fminf(low, g);
+            h[s >> 1][(s & 1) * 8 + i] = silu(g) * __uint_as_float(v[s & 1][1][i]);
+        }
     }
-    release(e);
+    const bool done = all(!(low < kTail));
+    release(e, done);
 #pragma unroll
     for (int c = 0; c < NC; ++c) store_quantized(h[c], e.t, (2 * c + e.group) * 16, e.col, a);
+    return done;
+}
+
+// The same, piece by piece, whatever the gates are; every thread stores over what it has stored.
+__device__ __forceinline__ void finish_tail(const Share& e, const Args& a) {
+#pragma unroll 1
+    for (int token0 = e.group * 16; token0 < e.t.n; token0 += 32) {
+        float h[16];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            uint32_t g[8], up[8];
+            ptx::tmem_ld_32x8(e.tmem + (uint32_t)(token0 + 8 * s), g);
+            ptx::tmem_ld_32x8(e.tmem + (uint32_t)(token0 + 8 * s) + e.width, up);
+            ptx::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[8 * s + i] = silu_times(__uint_as_float(g[i]), __uint_as_float(up[i]));
+        }
+        store_quantized(h, e.t, token0, e.col, a);
+    }
+    release(e);
 }
 
 template <class M>
@@ -648,14 +683,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             ptx::tc_fence_after();
             // (the number of pieces is a constant, so that they stay in registers)
             if constexpr (M::kGate) {
+                bool done;
                 switch ((e.t.n + 31) / 32) {
-                    case 1: finish_quantized<1>(e, a); break;
-                    case 2: finish_quantized<2>(e, a); break;
-                    case 3: finish_quantized<3>(e, a); break;
-                    case 4: finish_quantized<4>(e, a); break;
-                    case 5: finish_quantized<5>(e, a); break;
-                    default: finish_quantized<6>(e, a); break;
+                    case 1: done = finish_quantized<1>(e, a); break;
+                    case 2: done = finish_quantized<2>(e, a); break;
+                    case 3: done = finish_quantized<3>(e, a); break;
+                    case 4: done = finish_quantized<4>(e, a); break;
+                    case 5: done = finish_quantized<5>(e, a); break;
+                    default: done = finish_quantized<6>(e, a); break;
                 }
+                if (!done) finish_tail(e, a);
             } else {
                 switch ((e.t.n + 31) / 32) {
                     case 1: finish_rows<2>(e, a); break;
