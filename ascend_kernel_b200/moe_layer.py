@@ -390,6 +390,9 @@ class MoELayer:
         a dropped pair) and ``weight`` fp32 [T, k]; x bf16 [T, H] -> bf16 [T, H].  For one rank without an exchange."""
         if self.world != 1 or self.px is not None:
             raise RuntimeError("forward_routed runs on one rank, without an exchange")
+        if x.shape[:1] != idx.shape[:1] or weight.shape != idx.shape:
+            raise RuntimeError(f"idx and weight must be [T, k] for the tokens of x, {tuple(x.shape)}: got {tuple(idx.shape)} and "
+                               f"{tuple(weight.shape)}")
         counts, token_of, slot = ops.moe_sort(idx, self.n_experts)
         row_scale = None
         if self.weight_format == "fp8":
