@@ -387,7 +387,8 @@ class MoELayer:
     @torch.no_grad()
     def forward_routed(self, x, idx, weight):
         """The pass on another router's choice: ``idx`` int32 [T, k] the experts of each token (an entry outside 0 .. n_experts - 1 is
-        a dropped pair) and ``weight`` fp32 [T, k]; x bf16 [T, H] -> bf16 [T, H].  For one rank without an exchange."""
+        a dropped pair; an expert may be named twice) and ``weight`` fp32 [T, k]; x bf16 [T, H] -> bf16 [T, H].  For one rank without
+        an exchange."""
         if self.world != 1 or self.px is not None:
             raise RuntimeError("forward_routed runs on one rank, without an exchange")
         if x.shape[:1] != idx.shape[:1] or weight.shape != idx.shape:
@@ -401,7 +402,7 @@ class MoELayer:
             send, row_scale = ops.mxfp4_quantize_rows(x, token_of)
         else:
             send = ops.moe_dispatch(x, token_of, slot)
-        y = self._experts(send, counts, False, max_rows=x.shape[0], row_scale=row_scale)
+        y = self._experts(send, counts, False, row_scale=row_scale)  # (a token may name an expert twice: no bound on its rows)
         return ops.moe_combine(y, weight, token_of, slot)
 
     def forward_host(self, x_host, logits_host, out_host=None):

@@ -46,3 +46,14 @@ def test_a_choice_for_other_tokens_is_refused(monkeypatch, fmt, tokens):
     with pytest.raises(RuntimeError, match="tokens"):
         layer.forward_routed(x, good, torch.ones(tokens, 2))
     assert len(calls) == 1
+
+
+def test_rows_an_expert_has_at_most(monkeypatch):
+    """A token may name an expert more than once, so that an expert has more rows than there are tokens: no such bound is handed on."""
+    calls = []
+    _stand_ins(monkeypatch, calls)
+    layer = _layer("int8")
+    layer.forward_routed(torch.zeros(5, 8, dtype=torch.bfloat16), torch.full((5, 3), 2, dtype=torch.int32), torch.ones(5, 3))
+    _, counts, kw = calls[0]
+    assert int(counts.max()) == 15
+    assert kw.get("max_rows") is None or kw["max_rows"] >= 15
