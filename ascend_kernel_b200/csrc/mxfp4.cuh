@@ -6,7 +6,6 @@
 namespace b200moe {
 namespace mxfp4 {
 
-constexpr int kBlock = 32;
 constexpr uint32_t kLowest = 127 - 100;  // smallest scale byte of a block that is finite
 constexpr uint32_t kNaN = 255;
 
