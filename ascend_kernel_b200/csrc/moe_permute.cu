@@ -424,7 +424,7 @@ static bool row_sizes_ok(int64_t T, int64_t k, int64_t width) {
 static int width16_of(int64_t width, int fp32) { return (int)(width / (fp32 ? 4 : 8)); }
 // CTAs that share a token's row where tokens are few.
 static unsigned row_parts(int64_t T, int width16) {
-    const int64_t want = 4 * 148 / std::max<int64_t>(T, 1), most = (width16 + kRowThreads - 1) / kRowThreads;
+    const int64_t want = 4 * sm_count() / std::max<int64_t>(T, 1), most = (width16 + kRowThreads - 1) / kRowThreads;
     return (unsigned)std::max<int64_t>(1, std::min(want, most));
 }
 
