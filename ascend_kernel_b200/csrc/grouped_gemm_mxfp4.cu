@@ -16,10 +16,11 @@
 // made on the way) before it quantises or stores.
 //
 // What bounds it, measured alone | in a steady loop (which runs at 1.2 to 1.45 GHz, at the power limit), us: 256 experts, 4096 x 8 rows: 2048 x
-// 7168 386 | 416, of 381 for its 2.5 GB; gate/up 7168 x 4096 683 | 766, of 634; 8192 x 8 Zipf rows, gate/up 1107 | 1260, of 658 for its bytes and 450 of
-// MMA at the peak rate; 37 x 8 rows, 2048 x 7168 229 of 213; 32 x 8 rows, gate/up 395 of 388; one token's 8 experts 25 (2048 x 7168) and 41 (gate/up, of
-// 19: 64 tiles on 74 pairs, set-up and first loads).  So: memory, then power; Zipf rows, whose experts with thousands of rows read the
-// weights from L2 again and again: loads into the multiprocessors (without the epilogue 1069, with MMAs of 16 columns 1050, of both 978, without loads 647).
+// 7168 386 | 416, of 381 for its 2.5 GB; gate/up 7168 x 4096 683 | 766, of 634; 8192 x 8 Zipf rows, gate/up 1085 to 1111 | 1260, of 658 for its bytes and 450 of
+// MMA at the nominal rate; 37 x 8 rows, 2048 x 7168 229 of 213; 32 x 8 rows, gate/up 395 of 388; one token's 8 experts 25 (2048 x 7168) and 41 (gate/up, of
+// 19: 64 tiles on 74 pairs, each a walk over all of k; 8 are launch and set-up, and the 128 CTAs in use could read the bytes in 22: the rest is not
+// explained).  So: memory, then power; Zipf rows, whose experts with thousands of rows read the weights from L2 again and again: loads into the
+// multiprocessors (without the epilogue 1069, with MMAs of 16 columns 1050, of both 978), and behind them the MMAs (without loads 647).
 //
 // Steps, us (gate/up 4096 x 8 | Zipf rows): scales gathered by cp.async, handed over two stages late 3137 Zipf; on arrival 1063 | 1872; through registers
 // 795 | 1405; sums to registers first 739 | 1296; scales written to tensor memory instead of copied there (tcgen05.cp goes in turn with the

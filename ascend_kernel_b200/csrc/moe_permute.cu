@@ -31,7 +31,9 @@ constexpr int kMaxTopK = 32;
 
 constexpr int kWarps = 32, kFewWarps = 8;
 constexpr int kRoom = 32;          // sums of the warps, in static shared memory
-constexpr int kOnePairs = 4096;    // of a call that is one CTA's
+// Pairs of a call that is one CTA's.  One CTA | two kernels, us (256 experts; 1024): 2048 pairs 8.2 | 14.3; 11.3 | 22.5, 4096 pairs 10.3 | 14.3; 12.3 | 22.5, 6144
+// pairs 16.4 | 13.8; 20.5 | 22.5, 8192 pairs 18.4 | 13.8; 22.5 | 22.5.
+constexpr int kOnePairs = 4096;
 constexpr int kMostCtas = 128;
 constexpr int kBatch = 4;          // ids a lane has at a time
 
@@ -254,7 +256,9 @@ static int cta_pairs_of(int64_t P) {
 //
 // A CTA of 256 threads takes a token, 16 bytes a thread at a time, and where tokens are few several CTAs share its columns (not those that add up the
 // products for a weight's gradient).  Memory bounds all of them.  4096 tokens x 8 rows of 7168 bf16, us: dispatch 92 (529 MB, 5.7 TB/s: nine
-// tenths of it written), its gradient 82 (6.5 TB/s), combine 83, its gradients 160 (6.2 TB/s; of the rows alone 93); 509 x 2 rows of 2048 fp32: 4.2, 4.1, 4.1, 6.2.
+// tenths of it written), its gradient 82 (6.5 TB/s), combine 83, its gradients 160 (6.2 TB/s; of the rows alone 93); 509 x 2 rows of 2048 fp32: 4.2, 4.1, 4.1, 6.2.  Tried and not kept: streaming loads and stores, with which 8 x 4096 rows of
+// 2048 bf16 gain (dispatch 28.7 -> 23.9, its gradient 27.0 -> 22.5, combine 28.7 -> 23.9) and the joint gradients of rows of 7168 lose (160 -> 171): of
+// calls right behind one another, where a part of that is what the call before has left in L2.
 
 // 16 bytes of a row as fp32 and back.
 template <class T>
